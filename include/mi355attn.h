@@ -386,6 +386,78 @@ int mi355_block_head(int dtype, const void* X, int64_t ldx, const void* gamma, c
                      float eps, const void* W_qkv, const float* b_qkv, void* Y, int64_t ldy,
                      int64_t M, int64_t d_model, void* stream);
 
+/*
+ * Attention over packed sequences of different lengths with grouped query heads (a whole batch of
+ * prompts without padding):
+ *   O[i, h] = sum_j softmax_j(scale Q[i, h] · K[j, h / G]) V[j, h / G],  G = heads / kv_heads,
+ * j over the keys of token i's own sequence; causal != 0: only j <= i + (k_len - q_len), positions
+ * counted within the sequence (the last query sees the last key). A token that sees no key gives
+ * zeros. Keys a token does not see do not reach its output, whatever their K and V hold (infinities
+ * and NaN too); a row whose every visible score is -inf is NaN, as softmax's.
+ * Scores and softmax statistics are fp32, probabilities are rounded to the input type before P·V,
+ * outputs once. dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256.
+ *
+ * mi355_attn_packed_plan runs on the host: from the lengths it writes the tiles of rows (32-bit
+ * words, 8 a tile, longest first) that mi355_attn_packed walks. With tiles == NULL it only gives
+ * *n_tiles and *tile_rows; otherwise capacity (in tiles) must hold them. Copy the tiles to the
+ * device and pass them with the same heads, kv_heads, head_dim, causal and tile_rows; they hold for
+ * every call (layer) with these lengths. Sequences follow each other in Q / O (q_lens) and in
+ * K / V (k_lens); tokens behind the last one are not touched. Lengths may be 0; tokens in all
+ * below 2^30.
+ * Strides are {token, head} in elements, the head_dim stride is 1: Q, K, V multiples of 8 with
+ * 16-byte aligned bases, O of 4 with an 8-byte aligned base; token strides of K and V at least
+ * head_dim. scale must be positive and finite.
+ */
+int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t n_seqs,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim, int causal,
+                           int32_t* tiles, int64_t capacity, int64_t* n_tiles, int32_t* tile_rows);
+int mi355_attn_packed(int dtype, const void* Q, const void* K, const void* V, void* O,
+                      int64_t heads, int64_t kv_heads, int64_t head_dim, const int64_t* q_strides,
+                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                      float scale, int causal, const int32_t* tiles, int64_t n_tiles,
+                      int32_t tile_rows, void* stream);
+
+/*
+ * Attention of B sequences' n_q newest tokens (1 when generating) against a prefix of prefix_len
+ * tokens that all of them share and their own caches (room for `room` tokens each, own_lens[b] of
+ * them filled, the n_q newest among them, last): the softmax of mi355_attn_packed over
+ * prefix ++ own[: own_lens[b]]; token i of the n_q sees own keys j <= own_lens[b] - n_q + i.
+ * The prefix is read once for the whole batch. own_lens is read on the device (a captured graph
+ * follows its values) and clamped to [0, room]; what a cache holds behind it does not matter. A token
+ * that sees no key gives zeros. Types, head dims and roundings as mi355_attn_packed, partial results
+ * in fp32.
+ * Strides: Q, O, K_own, V_own {batch, token, head}, K_prefix, V_prefix {token, head}; the same
+ * multiples and alignments. workspace (16-byte aligned) holds
+ * mi355_attn_shared_prefix_workspace_bytes(...) bytes (negative: that argument error); calls that
+ * share one must be stream-ordered.
+ */
+int64_t mi355_attn_shared_prefix_workspace_bytes(int64_t B, int64_t n_q, int64_t heads,
+                                                 int64_t kv_heads, int64_t head_dim,
+                                                 int64_t prefix_len, int64_t room);
+int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_prefix, const void* V_prefix,
+                             const void* K_own, const void* V_own, const int32_t* own_lens, void* O,
+                             int64_t B, int64_t n_q, int64_t heads, int64_t kv_heads,
+                             int64_t head_dim, int64_t prefix_len, int64_t room,
+                             const int64_t* q_strides, const int64_t* kp_strides,
+                             const int64_t* vp_strides, const int64_t* ko_strides,
+                             const int64_t* vo_strides, const int64_t* o_strides, float scale,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Projection of a few rows (single tokens) with 4-bit weights and group scales:
+ *   Y[m, n] = out_dtype( sum_k X[m, k] W[n, k] + bias[n] ),
+ *   W[n, k] = scale[n, k / group] (q[n, k] - zero[n, k / group]).
+ * Wq [N, K / 2] holds q (0 .. 15), the even k in the low half of a byte; scale [N, K / group] is of X's
+ * type; zero [N, K / group] bytes, NULL = 8 everywhere; bias fp32 [N] or NULL; all contiguous. Sums
+ * are fp32, scales are applied to them in fp32, Y is rounded once. dtype F16 or BF16, out_dtype the
+ * same or F32; group 32, 64 or 128, K a multiple of it. Any M, but the weights are read again for
+ * every 64 rows. bf16: |x| below 2^119 (infinities give NaN).
+ * X and Wq 16-byte aligned, ldx a multiple of 8.
+ */
+int mi355_linear_i4(int dtype, int out_dtype, const void* X, int64_t ldx, const uint8_t* Wq,
+                    const void* scale, const uint8_t* zero, const float* bias, void* Y, int64_t ldy,
+                    int64_t M, int64_t N, int64_t K, int64_t group, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

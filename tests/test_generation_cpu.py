@@ -1,0 +1,170 @@
+"""Refusals and host-side work of the token-generation operators, without a GPU: the C entry points
+reject bad arguments before they launch anything, the packed plan covers every row once, and the
+Python wrappers name what is wrong."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tiktok_techjam_2026_track3_amd import _lib, ops
+
+F32, F16, BF16 = 0, 1, 2
+BAD_SIZE, NULL, DTYPE, ALIGN, HEAD, UNSUP = -2, -1, -3, -4, -5, -6
+
+
+def plan(q_lens, k_lens, heads=4, kv_heads=2, head_dim=64, causal=1):
+    n = len(q_lens)
+    arr = C.c_int32 * max(1, n)
+    count, rows = C.c_int64(0), C.c_int32(0)
+    args = (arr(*q_lens), arr(*k_lens), n, heads, kv_heads, head_dim, causal)
+    st = _lib.lib().mi355_attn_packed_plan(*args, 0, 0, C.byref(count), C.byref(rows))
+    if st:
+        return st, None, 0
+    tiles = torch.empty(count.value, 8, dtype=torch.int32)
+    if count.value:
+        assert _lib.lib().mi355_attn_packed_plan(*args, tiles.data_ptr(), count.value - 1, C.byref(count),
+                                                 C.byref(rows)) == BAD_SIZE  # too small a buffer
+        st = _lib.lib().mi355_attn_packed_plan(*args, tiles.data_ptr(), count.value, C.byref(count), C.byref(rows))
+    return st, tiles, rows.value
+
+
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads", [
+    ([5], [5], 4, 2), ([0, 3, 0, 900, 1], [4, 3, 0, 900, 77], 12, 4), ([4096] * 3, [5000, 4096, 100], 32, 8), ([], [], 1, 1),
+    ([1] * 200, list(range(200)), 8, 8)])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_plan_covers_every_row_once_longest_first(q_lens, k_lens, heads, kv_heads, causal):
+    st, tiles, rows = plan(q_lens, k_lens, heads, kv_heads, causal=causal)
+    assert st == 0
+    g = heads // kv_heads
+    want, q0, k0 = set(), 0, 0
+    for n, m in zip(q_lens, k_lens):
+        want |= {(q0, n, k0, m, r) for r in range(0, n * g, rows)}
+        q0, k0 = q0 + n, k0 + m
+    got = [tuple(t[:5]) for t in tiles.tolist()]
+    assert len(got) == len(want) and set(got) == want
+
+    def keys(t):
+        last = (min(t[4] + rows, t[1] * g) - 1) // g
+        return max(0, min(t[3], last + t[3] - t[1] + 1)) if causal else t[3]
+    order = [keys(t) for t in got]
+    assert order == sorted(order, reverse=True)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(heads=3), BAD_SIZE), (dict(heads=0), BAD_SIZE), (dict(kv_heads=0), BAD_SIZE), (dict(head_dim=8), HEAD),
+    (dict(head_dim=0), HEAD), (dict(q_lens=[-1]), BAD_SIZE), (dict(k_lens=[-1]), BAD_SIZE),
+    (dict(q_lens=[1 << 29], heads=8, kv_heads=1), BAD_SIZE), (dict(q_lens=[1 << 29, 1 << 29], k_lens=[1, 1]), BAD_SIZE)])
+def test_plan_refusals(kw, status):
+    kw = {"q_lens": [4], "k_lens": [4], **kw}
+    assert plan(**kw)[0] == status
+
+
+def test_plan_null_pointers():
+    count, rows = C.c_int64(0), C.c_int32(0)
+    f = _lib.lib().mi355_attn_packed_plan
+    assert f(None, None, 1, 4, 2, 64, 1, 0, 0, C.byref(count), C.byref(rows)) == NULL
+    assert f(None, None, 0, 4, 2, 64, 1, 0, 0, None, C.byref(rows)) == NULL
+
+
+PACKED = dict(dtype=F16, Q=64, K=64, V=64, O=64, heads=4, kv_heads=2, head_dim=64, qs=(256, 64), ks=(128, 64),
+              vs=(128, 64), os=(256, 64), scale=0.125, causal=1, tiles=64, n_tiles=3, tile_rows=32)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=F32), DTYPE), (dict(dtype=9), DTYPE), (dict(heads=3), BAD_SIZE), (dict(kv_heads=0), BAD_SIZE),
+    (dict(n_tiles=-1), BAD_SIZE), (dict(n_tiles=1 << 31), BAD_SIZE), (dict(head_dim=40), HEAD), (dict(tile_rows=48), UNSUP),
+    (dict(scale=0.0), UNSUP), (dict(scale=-1.0), UNSUP), (dict(scale=float("inf")), UNSUP), (dict(scale=float("nan")), UNSUP),
+    (dict(Q=0), NULL), (dict(O=0), NULL), (dict(tiles=0), NULL), (dict(Q=72), ALIGN), (dict(K=68), ALIGN), (dict(V=8), ALIGN),
+    (dict(O=68), ALIGN), (dict(qs=(257, 64)), ALIGN), (dict(ks=(132, 64)), ALIGN), (dict(vs=(128, 4)), ALIGN),
+    (dict(os=(256, 62)), ALIGN), (dict(ks=(56, 64)), BAD_SIZE), (dict(vs=(0, 64)), BAD_SIZE), (dict(ks=(1 << 25, 64)), BAD_SIZE)])
+def test_packed_entry_refusals(kw, status):
+    a = {**PACKED, **kw}
+    i64 = _lib.i64_array
+    assert _lib.lib().mi355_attn_packed(
+        a["dtype"], a["Q"], a["K"], a["V"], a["O"], a["heads"], a["kv_heads"], a["head_dim"], i64(a["qs"]), i64(a["ks"]),
+        i64(a["vs"]), i64(a["os"]), a["scale"], a["causal"], a["tiles"], a["n_tiles"], a["tile_rows"], None) == status
+
+
+PREFIX = dict(dtype=F16, ptrs=[64] * 7, B=2, n=1, heads=4, kv_heads=2, head_dim=64, P=100, room=50, qs=(256, 256, 64),
+              kps=(128, 64), vps=(128, 64), kos=(6400, 128, 64), vos=(6400, 128, 64), os=(256, 256, 64), scale=0.125, ws=64,
+              ws_bytes=1 << 30)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=F32), DTYPE), (dict(heads=5), BAD_SIZE), (dict(B=-1), BAD_SIZE), (dict(n=-1), BAD_SIZE), (dict(P=-1), BAD_SIZE),
+    (dict(room=1 << 30), BAD_SIZE), (dict(head_dim=24), HEAD), (dict(scale=0.0), UNSUP), (dict(scale=float("nan")), UNSUP),
+    (dict(ws=0), NULL), (dict(ws_bytes=16), BAD_SIZE), (dict(ws=72), ALIGN), (dict(kps=(56, 64)), BAD_SIZE),
+    (dict(vos=(6400, 64, 64), kv_heads=2, head_dim=128), BAD_SIZE), (dict(qs=(256, 256, 63)), ALIGN),
+    (dict(kos=(6401, 128, 64)), ALIGN), (dict(os=(256, 256, 2)), ALIGN),
+    *[(dict(ptrs=[0 if j == i else 64 for j in range(7)]), NULL) for i in range(7)],
+    *[(dict(ptrs=[72 if j == i else 64 for j in range(7)]), ALIGN) for i in range(5)]])
+def test_prefix_entry_refusals(kw, status):
+    a = {**PREFIX, **kw}
+    i64 = _lib.i64_array
+    q, kp, vp, ko, vo, lens, out = a["ptrs"]
+    assert _lib.lib().mi355_attn_shared_prefix(
+        a["dtype"], q, kp, vp, ko, vo, lens, out, a["B"], a["n"], a["heads"], a["kv_heads"], a["head_dim"], a["P"], a["room"],
+        i64(a["qs"]), i64(a["kps"]), i64(a["vps"]), i64(a["kos"]), i64(a["vos"]), i64(a["os"]), a["scale"], a["ws"],
+        a["ws_bytes"], None) == status
+
+
+def test_prefix_workspace_size():
+    f = _lib.lib().mi355_attn_shared_prefix_workspace_bytes
+    assert f(2, 1, 4, 2, 64, 0, 0) == 0
+    assert f(2, 1, 4, 2, 64, 100, 50) == 2 * 2 * 4 * (64 + 2) * 4  # one range of keys each
+    assert f(2, 1, 4, 3, 64, 100, 50) == BAD_SIZE and f(2, 1, 4, 2, 65, 100, 50) == HEAD
+    assert f(64, 1, 32, 8, 128, 1 << 20, 4096) > 0
+
+
+I4 = dict(dtype=F16, odt=F16, X=64, ldx=256, W=64, s=64, Y=64, ldy=100, M=3, N=100, K=256, group=64)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=F32), DTYPE), (dict(odt=BF16), DTYPE), (dict(odt=7), DTYPE), (dict(group=16), UNSUP), (dict(group=0), UNSUP),
+    (dict(K=224), BAD_SIZE), (dict(M=-1), BAD_SIZE), (dict(N=-1), BAD_SIZE), (dict(ldx=248), BAD_SIZE), (dict(ldy=99), BAD_SIZE),
+    (dict(ldx=260), ALIGN), (dict(X=72), ALIGN), (dict(W=68), ALIGN), (dict(X=0), NULL), (dict(W=0), NULL), (dict(s=0), NULL),
+    (dict(Y=0), NULL)])
+def test_i4_entry_refusals(kw, status):
+    a = {**I4, **kw}
+    assert _lib.lib().mi355_linear_i4(a["dtype"], a["odt"], a["X"], a["ldx"], a["W"], a["s"], 0, 0, a["Y"], a["ldy"], a["M"],
+                                      a["N"], a["K"], a["group"], None) == status
+
+
+def test_wrappers_refuse_cpu_tensors():
+    q, k = torch.zeros(4, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 64, dtype=torch.float16)
+    p = ops.PackedPlan(4, 4, 4, 2, 64, True, 32, 0, torch.zeros(0, 8, dtype=torch.int32))
+    with pytest.raises(ValueError, match="GPU"):
+        ops.attention_packed(q, k, k, p)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.attention_shared_prefix(q[None], k, k, k[None], k[None], torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="GPU"):
+        ops.linear_i4(torch.zeros(1, 64).half(), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1).half())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_lens=[1], k_lens=[1, 2]), dict(q_lens=[-1]), dict(q_lens=[1 << 30]), dict(q_lens=[4], kv_heads=3),
+    dict(q_lens=[4], heads=0), dict(q_lens=[4], head_dim=8), dict(q_lens=[4], device="cpu")])
+def test_packed_plan_wrapper_refusals(kw):
+    kw = {"heads": 4, "kv_heads": 2, "head_dim": 64, **kw}
+    with pytest.raises(ValueError):
+        ops.packed_plan(kw.pop("q_lens"), kw.pop("k_lens", None), **kw)
+
+
+@pytest.mark.parametrize("w,group", [(torch.zeros(4, 64), 64), (torch.zeros(4, 64).half(), 48), (torch.zeros(4, 96).half(), 64),
+                                     (torch.zeros(64).half(), 64)])
+def test_quant_groups_i4_refusals(w, group):
+    with pytest.raises(ValueError):
+        ops.quant_groups_i4(w, group)
+
+
+def test_quant_groups_i4_values():
+    """Two-level groups come back exactly; the even k is in the low half of a byte."""
+    w = torch.zeros(2, 64, dtype=torch.float16)
+    w[0, ::2], w[0, 1::2], w[1] = 0.0, 15.0, -7.0
+    q, s, z = ops.quant_groups_i4(w, 32)
+    assert q.shape == (2, 32) and s.shape == z.shape == (2, 2)
+    assert bool((q[0] == 0xF0).all()) and bool((s[0] == 1).all()) and bool((z[0] == 0).all())
+    values = torch.stack((q & 15, q >> 4), -1).reshape(2, 64).float()
+    assert bool((((values - z.repeat_interleave(32, 1)) * s.float().repeat_interleave(32, 1))[1] + 7).abs().max() < 0.01)
+    q, s, z = ops.quant_groups_i4(w, 32, symmetric=True)
+    assert z is None and bool((q[1] == 0x11).all()) and bool((s[1] == 1).all())

@@ -104,6 +104,26 @@ _SIGNATURES = {
         C.c_int,
         [_P, _P, _P, _P, _P, C.c_int, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, C.c_int, _P],
     ),
+    "mi355_attn_packed_plan": (
+        C.c_int,
+        [C.POINTER(C.c_int32), C.POINTER(C.c_int32), _I64, _I64, _I64, _I64, C.c_int, _P, _I64,
+         C.POINTER(_I64), C.POINTER(C.c_int32)],
+    ),
+    "mi355_attn_packed": (
+        C.c_int,
+        [C.c_int, _P, _P, _P, _P, _I64, _I64, _I64, C.POINTER(_I64), C.POINTER(_I64),
+         C.POINTER(_I64), C.POINTER(_I64), C.c_float, C.c_int, _P, _I64, C.c_int32, _P],
+    ),
+    "mi355_attn_shared_prefix_workspace_bytes": (_I64, [_I64] * 7),
+    "mi355_attn_shared_prefix": (
+        C.c_int,
+        [C.c_int, _P, _P, _P, _P, _P, _P, _P, *[_I64] * 7, *[C.POINTER(_I64)] * 6, C.c_float, _P,
+         _I64, _P],
+    ),
+    "mi355_linear_i4": (
+        C.c_int,
+        [C.c_int, C.c_int, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P],
+    ),
 }
 
 # epilogue flags of mi355_gemm_i8_epilogue (MI355_EPI_*)

@@ -1,0 +1,477 @@
+// Attention over rows = (token, query head of a K/V head's group): what packed prompts
+// (attn_packed.hip) and a batch's new tokens behind a shared prefix (attn_prefix.hip) have in common.
+//
+// For one K/V head and a range of keys, each row i keeps the running maximum mu and sum of its
+// softmax and the output O = sum_j 2^(c s_ij - mu) v_j, c = scale * log2 e:
+//   S^T = K · Q^T and O^T += V^T · P^T on 16x16x32 MFMAs, keys in BN-key tiles through a ring of LDS
+//   tiles filled by LDS-DMA, V^T fragments by transpose reads of the key-major tile. A lane holds
+//   one row (lane % 16) and 4 keys of every 16, so the scores of a 32-key unit are its P^T operand
+//   as they are: keys 4 g + i and 16 + 4 g + i (g = lane / 16), the order of the V^T reads.
+//   The heads of a group are rows of one tile: K and V are read once for all of them.
+//   The maximum moves only when a score exceeds it by more than 8 (log2 units), and only then do
+//   the four lanes of a row exchange anything; sums are exchanged once at the end.
+#pragma once
+
+#include "attn.h"
+
+namespace rows {
+
+enum Mode { PACKED = 0, PREFIX = 1, OWN = 2 };
+
+// One tile of rows of one packed sequence (mi355_attn_packed_plan writes them).
+struct PackedTile {
+  int32_t q0, q_len;  // the sequence's first token in q and its tokens
+  int32_t k0, k_len;  // ... in k / v
+  int32_t row0;       // first row of the tile: token row0 / G, head row0 % G of the group
+  int32_t pad[3];
+};
+static_assert(sizeof(PackedTile) == 32, "plan entry");
+
+struct Args {
+  const void *q, *k, *v;
+  void* o;                // PACKED: output
+  int64_t qb, qt, qh;     // strides in elements: batch (not PACKED), token, head
+  int64_t kb, kt, kh;     // batch (OWN), token, head
+  int64_t vb, vt, vh;
+  int64_t ob, ot, oh;
+  float c;                // scale * log2(e)
+  int32_t G, H, Hkv;      // query heads of a K/V head, query heads, K/V heads
+  // PACKED
+  const PackedTile* tiles;
+  int32_t causal;
+  // PREFIX / OWN: rows of a sequence are its n_q tokens' heads
+  int32_t B, n_q;
+  int32_t keys;           // PREFIX: prefix keys; OWN: keys a cache has room for
+  const int32_t* lens;    // OWN: keys in each cache (clamped to [0, keys])
+  int32_t chunk;          // keys of a split
+  int32_t splits, row_tiles;
+  int32_t part0;          // first split's index in part / ml
+  float* part;            // [splits][B n_q H][HD], unnormalised
+  float* ml;              // [splits][B n_q H][2]: mu (-inf: no key seen), sum
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+MI355_DEVINL f32x4 mma32(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+MI355_DEVINL f32x4 mma32(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+MI355_DEVINL f32x4 mma16(f16x4 a, f16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+MI355_DEVINL f32x4 mma16(bf16x4 a, bf16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+// sum of a fragment's probabilities, as rounded
+MI355_DEVINL float prob_sum(f16x8 f, float acc) {
+  const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_fdot2(f16x2{f[2 * r], f[2 * r + 1]}, one, acc, false);
+  return acc;
+}
+MI355_DEVINL float prob_sum(bf16x8 f, float acc) {
+  const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{f[2 * r], f[2 * r + 1]}, one, acc, false);
+  return acc;
+}
+// reductions over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a row
+MI355_DEVINL float row_maximum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return pair_maximum(vmax(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+MI355_DEVINL float row_sum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// XOR of a row's 16-byte chunks (NCH per row) by its low 4 bits. 16 lanes are served together: of a
+// K fragment read (16 rows, 4 neighbouring chunks) rows 0-3 and 12-15 at one chunk with rows 4-11 at
+// the next, of a V transpose read 4 rows at 2 neighbouring chunks. Row pitches of 2, 6 and 10 chunks
+// keep those apart by themselves.
+template <int NCH>
+MI355_DEVINL int swz(int r) {
+  const int r0 = r & 1, r1 = (r >> 1) & 1, r2 = (r >> 2) & 1, r3 = (r >> 3) & 1;
+  if constexpr (NCH % 16 == 0)
+    return r2 | (r0 << 1) | (r1 << 2) | ((r2 ^ r3) << 3);
+  else if constexpr (NCH % 8 == 0)
+    return r2 | ((r0 ^ r2 ^ r3) << 1) | (r1 << 2);
+  else if constexpr (NCH % 4 == 0)
+    return r2 | ((r1 ^ r2 ^ r3) << 1);
+  else
+    return 0;
+}
+
+// NW waves of QG groups of 16 rows; EU: waves a SIMD shall hold; TERMS: the probabilities enter
+// P · V as that many terms of the input type.
+template <typename T, int HD, int NW, int QG, int BN, int RING, int EU, int TERMS, int MODE>
+__global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
+  using frag = typename Mfma<T>::frag;
+  typedef T frag4 __attribute__((ext_vector_type(4)));
+  static_assert(HD % 16 == 0 && BN % 32 == 0, "shape");
+  constexpr int QW = 16 * QG, BM = NW * QW;
+  constexpr int NCH = HD / 8, ROWB = HD * 2;
+  constexpr int KS = HD / 32;              // 32-element MFMA steps of S^T
+  constexpr bool HALF = HD % 32 != 0;      // and one of 16
+  constexpr int DT = HD / 16, KT = BN / 16;
+  static_assert(BN * NCH % 64 == 0, "whole blocks of loads");
+  constexpr int BLK = BN * NCH / 64, LPW = (BLK + NW - 1) / NW, TILE = BN * NCH;
+  __shared__ u32x4 lds[2 * RING * TILE];   // K ring, V ring
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, l16 = lane & 15;
+
+  // the work-group's rows [row0, nrows) of a sequence (or of the batch), its K/V head and keys
+  int h, row0, nrows, k_begin, k_end, k_off, split = 0, b = 0;
+  const T *Qb, *Kb, *Vb;
+  int64_t out_tok = 0;
+  if constexpr (MODE == PACKED) {
+    h = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.Hkv));
+    const PackedTile t = p.tiles[blockIdx.x / static_cast<unsigned>(p.Hkv)];
+    row0 = t.row0;
+    nrows = t.q_len * p.G;
+    k_begin = 0;
+    // key j is seen by token i when j < i + k_off (causal), j < k_len
+    k_off = p.causal ? t.k_len - t.q_len + 1 : 0x40000000;
+    const int last = (row0 + BM < nrows ? row0 + BM : nrows) - 1;
+    const int lim = last / p.G + k_off;
+    k_end = lim < t.k_len ? (lim > 0 ? lim : 0) : t.k_len;
+    Qb = static_cast<const T*>(p.q) + t.q0 * p.qt;
+    Kb = static_cast<const T*>(p.k) + t.k0 * p.kt + h * p.kh;
+    Vb = static_cast<const T*>(p.v) + t.k0 * p.vt + h * p.vh;
+    out_tok = t.q0;
+  } else {
+    unsigned x = blockIdx.x;
+    h = static_cast<int>(x % static_cast<unsigned>(p.Hkv));
+    x /= static_cast<unsigned>(p.Hkv);
+    split = static_cast<int>(x % static_cast<unsigned>(p.splits));
+    x /= static_cast<unsigned>(p.splits);
+    row0 = static_cast<int>(x % static_cast<unsigned>(p.row_tiles)) * BM;
+    b = static_cast<int>(x / static_cast<unsigned>(p.row_tiles));
+    k_begin = split * p.chunk;
+    Qb = static_cast<const T*>(p.q);
+    Kb = static_cast<const T*>(p.k) + h * p.kh;
+    Vb = static_cast<const T*>(p.v) + h * p.vh;
+    int len = p.keys;
+    if constexpr (MODE == OWN) {
+      nrows = p.n_q * p.G;
+      const int given = p.lens[b];
+      len = given < 0 ? 0 : (given < p.keys ? given : p.keys);
+      k_off = len - p.n_q + 1;
+      Qb += b * p.qb;
+      Kb += b * p.kb;
+      Vb += b * p.vb;
+    } else {
+      nrows = p.B * p.n_q * p.G;
+      k_off = 0x40000000;
+    }
+    if (k_begin >= len) return;  // (the combining kernel does not read this split)
+    k_end = k_begin + p.chunk < len ? k_begin + p.chunk : len;
+  }
+  Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
+  Vb = uniform_ptr(Vb + static_cast<int64_t>(k_begin) * p.vt);
+  const int n_keys = k_end - k_begin;  // keys from here on are counted from k_begin
+  const int row_w = row0 + wave * QW;
+  const bool idle = row_w >= nrows;    // no row of this wave is real: it only loads
+
+  // token (of the batch in PREFIX) of a row, and its offset in q
+  const auto q_of = [&](int r) MI355_LAMBDA_INLINE {
+    const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+    if constexpr (MODE == PREFIX) {
+      const int bb = t / p.n_q;
+      return bb * p.qb + (t - bb * p.n_q) * p.qt + hh * p.qh;
+    } else {
+      return t * p.qt + hh * p.qh;
+    }
+  };
+  // keys [0, lim) of the work-group's range are seen by row r
+  const auto lim_of = [&](int r) MI355_LAMBDA_INLINE {
+    const int lim = r / p.G + k_off - k_begin;
+    return lim < n_keys ? lim : n_keys;
+  };
+
+  // Q^T fragments: lane (row l16 of group n, slice g) holds elements 32 s + 8 g ..
+  frag qf[QG][KS > 0 ? KS : 1];
+  frag4 qh[QG];
+  int lim[QG];
+#pragma unroll
+  for (int n = 0; n < QG; ++n) {
+    const int r = row_w + 16 * n + l16;
+    const bool real = r < nrows;
+    const T* src = Qb + q_of(real ? r : nrows - 1);
+    lim[n] = lim_of(real ? r : nrows - 1);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[n][s] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * g));
+    if constexpr (HALF) qh[n] = __builtin_bit_cast(frag4, *reinterpret_cast<const u32x2*>(src + 32 * KS + 4 * g));
+  }
+  const int lim_first = MODE == PREFIX ? n_keys : __builtin_amdgcn_readfirstlane(lim[0]);
+  const int lim_last = MODE == PREFIX ? n_keys : lim_of(row_w + QW - 1 < nrows ? row_w + QW - 1 : nrows - 1);
+
+  // loads: lane i of block blk lands at chunk 64 blk + i of the tile, so it fetches the logical
+  // chunk that the swizzle places there; rows past the last key read as zeros
+  const uint32_t kstride = static_cast<uint32_t>(p.kt) * sizeof(T), vstride = static_cast<uint32_t>(p.vt) * sizeof(T);
+  const uint32_t kcap = 0xffffffffu / kstride, vcap = 0xffffffffu / vstride;
+  uint32_t koff[LPW], voff[LPW];
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int at = (wave + i * NW) * 64 + lane, row = at / NCH, ch = (at % NCH) ^ swz<NCH>(row);
+    koff[i] = static_cast<uint32_t>(row) * kstride + ch * 16;
+    voff[i] = static_cast<uint32_t>(row) * vstride + ch * 16;
+  }
+  auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
+    const uint32_t key = static_cast<uint32_t>(j) * BN, rem = static_cast<uint32_t>(n_keys) - key;
+    const u32x4 kr = buffer_rsrc(reinterpret_cast<const char*>(Kb) + static_cast<uint64_t>(key) * kstride,
+                                 rem > kcap ? 0xffffffffu : rem * kstride);
+    const u32x4 vr = buffer_rsrc(reinterpret_cast<const char*>(Vb) + static_cast<uint64_t>(key) * vstride,
+                                 rem > vcap ? 0xffffffffu : rem * vstride);
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int blk = wave + i * NW;
+      if (BLK % NW != 0 && blk >= BLK) break;
+      buffer_dma_lds16(kr, koff[i], 0, lds_addr_of(&lds[st * TILE + blk * 64]));
+      buffer_dma_lds16(vr, voff[i], 0, lds_addr_of(&lds[(RING + st) * TILE + blk * 64]));
+    }
+  };
+
+  // byte offsets of a lane's fragments in a tile; what the swizzle makes non-additive in registers
+  constexpr int KV = NCH % 16 == 0 ? 4 : NCH % 8 == 0 ? 2 : 1;
+  constexpr int VV = NCH % 16 == 0 ? 8 : NCH % 8 == 0 ? 4 : NCH % 4 == 0 ? 2 : 1;
+  const char* const ldsb = reinterpret_cast<const char*>(lds);
+  uint32_t k_at[KV], v_at[VV];
+  const int ve = (lane >> 2) & 3, vq = lane & 3;
+#pragma unroll
+  for (int i = 0; i < KV; ++i) k_at[i] = l16 * ROWB + ((4 * i + g) ^ swz<NCH>(l16)) * 16;
+#pragma unroll
+  for (int i = 0; i < VV; ++i)
+    v_at[i] = (4 * g + ve) * ROWB + ((2 * i + (vq >> 1)) ^ swz<NCH>(4 * g + ve)) * 16 + (vq & 1) * 8;
+  auto kfrag = [&](int st, int kt, int s) MI355_LAMBDA_INLINE {
+    return __builtin_bit_cast(frag, *reinterpret_cast<const u32x4*>(
+        ldsb + st * TILE * 16 + 16 * kt * ROWB + s / KV * (KV * 64) + k_at[s % KV]));
+  };
+  auto khalf = [&](int st, int kt) MI355_LAMBDA_INLINE {  // (rows of 2, 6, 10 chunks: no swizzle)
+    return __builtin_bit_cast(frag4, *reinterpret_cast<const u32x2*>(
+        ldsb + st * TILE * 16 + (16 * kt + l16) * ROWB + KS * 64 + g * 8));
+  };
+  auto vfrag = [&](int st, int t, int dt) MI355_LAMBDA_INLINE {
+    const char* base = ldsb + (RING + st) * TILE * 16 + 32 * t * ROWB + dt / VV * (VV * 32) + v_at[dt % VV];
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + 16 * ROWB));
+    return __builtin_bit_cast(frag, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  };
+
+  f32x4 o[QG][DT];
+  float mu[QG], gate[QG], lsum[QG];  // running max (log2 domain), the score that moves it, row sum
+#pragma unroll
+  for (int n = 0; n < QG; ++n) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    mu[n] = 0.f;
+    gate[n] = NEG_INF;
+    lsum[n] = 0.f;
+  }
+
+  auto tile = [&](const int j, const int st) MI355_LAMBDA_INLINE {
+    const int k0 = j * BN;
+    f32x4 s[QG][KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int n = 0; n < QG; ++n) s[n][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const frag kf = kfrag(st, kt, x);
+#pragma unroll
+        for (int n = 0; n < QG; ++n) s[n][kt] = mma32(kf, qf[n][x], s[n][kt]);
+      }
+      if constexpr (HALF) {
+        const frag4 kf = khalf(st, kt);
+#pragma unroll
+        for (int n = 0; n < QG; ++n) s[n][kt] = mma16(kf, qh[n], s[n][kt]);
+      }
+    }
+    if (k0 + BN > lim_first) {  // the tile crosses a row's last key
+#pragma unroll
+      for (int n = 0; n < QG; ++n) {
+        const int rel = lim[n] - k0 - 4 * g;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * kt + i >= rel) s[n][kt][i] = NEG_INF;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < QG; ++n) {
+      float mx = s[n][0][0];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = vmax(mx, s[n][kt][i]);
+      if (__builtin_amdgcn_ballot_w64(mx * p.c > gate[n]) != 0) {
+        mx = row_maximum(mx) * p.c;
+        const bool grow = mx > gate[n];
+        const float m2 = grow ? mx : mu[n];
+        const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(mu[n] - m2);
+        lsum[n] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][t][i] *= alpha;
+        mu[n] = m2;
+        gate[n] = grow ? mx + 8.f : gate[n];
+      }
+    }
+    frag pf[TERMS][QG][KT / 2];
+#pragma unroll
+    for (int t = 0; t < KT / 2; ++t)
+#pragma unroll
+      for (int n = 0; n < QG; ++n) {
+        float e[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          e[r] = fast_exp2(__builtin_fmaf(s[n][2 * t + r / 4][r % 4], p.c, -mu[n]));
+          pf[0][n][t][r] = from_f32<T>(e[r]);
+        }
+        if constexpr (TERMS == 2) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) pf[1][n][t][r] = from_f32<T>(e[r] - to_f32(pf[0][n][t][r]));
+          lsum[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        } else {
+          lsum[n] = prob_sum(pf[0][n][t], lsum[n]);
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < KT / 2; ++t)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const frag vf = vfrag(st, t, dt);
+#pragma unroll
+        for (int n = 0; n < QG; ++n)
+#pragma unroll
+          for (int x = 0; x < TERMS; ++x) o[n][dt] = mma32(vf, pf[x][n][t], o[n][dt]);
+      }
+  };
+
+  const int n_kt = (n_keys + BN - 1) / BN;
+  if (n_kt > 0) issue(0, 0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
+    if (j + 1 < n_kt) issue(j + 1, st ^ 1);
+    if (!idle && j * BN < lim_last) tile(j, st);
+    // this wave's loads of tile j + 1 have landed and its reads of tile j are done
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  };
+  static_assert(RING == 2, "double buffering");
+  int j = 0;
+  for (; j + 2 <= n_kt; j += 2) {
+    step(j, 0);
+    step(j + 1, 1);
+  }
+  if (j < n_kt) step(j, 0);
+
+  // rows out: each lane holds runs of 4 of its row's elements
+  uint64_t nan_rows[QG];
+#pragma unroll
+  for (int n = 0; n < QG; ++n) {
+    const int r = row_w + 16 * n + l16;
+    const float sum = row_sum(lsum[n]);
+    bool bad = false;
+    if (r < nrows) {
+      if constexpr (MODE == PACKED) {
+        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+        T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
+        // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          frag4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = lim[n] > 0 ? o[n][dt][e] * inv : 0.f;
+            bad |= x != x;
+            w[e] = from_f32<T>(x);
+          }
+          *reinterpret_cast<frag4*>(dst + 16 * dt + 4 * g) = w;
+        }
+      } else {
+        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+        const int64_t at = static_cast<int64_t>(p.part0 + split) * p.B * p.n_q * p.H +
+                           (static_cast<int64_t>(MODE == OWN ? b * p.n_q : 0) + t) * p.H + hh;
+        float* dst = p.part + at * HD;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad |= o[n][dt][e] != o[n][dt][e];
+          *reinterpret_cast<f32x4*>(dst + 16 * dt + 4 * g) = o[n][dt];
+        }
+        if (g == 0) {
+          // (a sum that is not 0 without a maximum is NaN's)
+          p.ml[2 * at] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
+          p.ml[2 * at + 1] = sum;
+        }
+      }
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(bad);
+    nan_rows[n] = (m | (m >> 16) | (m >> 32) | (m >> 48)) & 0xffffu;
+  }
+
+  // A key behind a row's last one has probability 0, but its v row is in the tile: 0 · inf and
+  // 0 · NaN leave NaN in rows that do not see it. Rows with NaN whose tile held such keys are
+  // computed again, one key at a time over the keys they see (a row that sees a NaN gets it again).
+  if constexpr (MODE != PREFIX) {
+#pragma unroll
+    for (int n = 0; n < QG; ++n) {
+      if (nan_rows[n] == 0) continue;
+      __builtin_amdgcn_s_waitcnt(0);  // the stores above are done
+      constexpr int DL = (HD + 63) / 64;
+      for (int x = 0; x < 16; ++x) {
+        const int r = row_w + 16 * n + x, keys = lim_of(r < nrows ? r : nrows - 1);
+        if (!((nan_rows[n] >> x) & 1) || r >= nrows || keys <= 0 || keys >= n_keys) continue;
+        const T* src = Qb + q_of(r);
+        float q[DL], acc[DL], m = NEG_INF, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < DL; ++i) {
+          q[i] = lane + 64 * i < HD ? to_f32(src[lane + 64 * i]) : 0.f;
+          acc[i] = 0.f;
+        }
+        for (int key = 0; key < keys; ++key) {
+          const T* kr = Kb + static_cast<int64_t>(key) * p.kt;
+          const T* vr = Vb + static_cast<int64_t>(key) * p.vt;
+          float s = 0.f;
+#pragma unroll
+          for (int i = 0; i < DL; ++i)
+            if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
+          for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+          s *= p.c;
+          const float m2 = vmax(m, s);
+          const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
+          const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
+          l = __builtin_fmaf(l, a, e);
+#pragma unroll
+          for (int i = 0; i < DL; ++i)
+            if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
+          m = m2;
+        }
+        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+        if constexpr (MODE == PACKED) {
+          T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
+#pragma unroll
+          for (int i = 0; i < DL; ++i)
+            if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
+        } else {
+          const int64_t at = static_cast<int64_t>(p.part0 + split) * p.B * p.n_q * p.H +
+                             (static_cast<int64_t>(b) * p.n_q + t) * p.H + hh;
+#pragma unroll
+          for (int i = 0; i < DL; ++i)
+            if (lane + 64 * i < HD) p.part[at * HD + lane + 64 * i] = acc[i];
+          if (lane == 0) {
+            p.ml[2 * at] = m;
+            p.ml[2 * at + 1] = l;
+          }
+        }
+      }
+    }
+  }
+}
+
+}  // namespace rows

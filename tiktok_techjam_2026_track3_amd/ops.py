@@ -6,8 +6,10 @@ device. Nothing here synchronises the host, so the calls are hipGraph-capturable
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -540,4 +542,321 @@ def linear_i8(a: torch.Tensor, w: torch.Tensor, s_a: torch.Tensor, s_w: torch.Te
         acc_out.data_ptr() if acc_out is not None else 0, M, N, K,
         mask, _stream(a))
     _lib.check("mi355_gemm_i8", st)
+    return out
+
+
+# head dims of attention_packed and attention_shared_prefix
+GROUPED_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 192, 256)
+
+
+def _on_device(dev: torch.device):
+    """Makes ``dev`` current for a launch, where it is not."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
+                                 "or with detached tensors")
+
+
+def _rows_view(name: str, t: torch.Tensor, dims: int, dtype: torch.dtype, align: int) -> None:
+    """Checks a [..., token, head, head_dim] view: 16-bit, unit last stride, strides of whole vectors."""
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, q is {dtype}")
+    if t.numel() == 0:
+        return
+    if t.stride(-1) != 1:
+        raise ValueError(f"head_dim must be the unit-stride dimension of {name}")
+    if any(n > 1 and s % align for n, s in zip(t.shape[:-1], t.stride()[:-1])) or t.data_ptr() % (2 * align):
+        raise ValueError(f"{name} needs strides that are multiples of {align} elements and a "
+                         f"{2 * align}-byte aligned start")
+
+
+def _kv_strides(name: str, t: torch.Tensor, axis: int) -> Tuple[int, ...]:
+    """Strides but the last; a token stride that no second token uses is the row itself."""
+    st = list(t.stride()[:-1])
+    if t.shape[axis] <= 1:
+        st[axis] = t.shape[-1]
+    elif t.numel() and not t.shape[-1] <= st[axis] <= 1 << 24:
+        raise ValueError(f"the tokens of {name} overlap or are too far apart (stride {st[axis]})")
+    return _whole(t, st)
+
+
+def _whole(t: torch.Tensor, strides) -> Tuple[int, ...]:
+    """Strides for the library: those of axes of one element do not matter and become 0."""
+    return tuple(0 if n == 1 and s % 8 else s for n, s in zip(t.shape[:-1], strides))
+
+
+def _scale(scale: Optional[float], head_dim: int) -> float:
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
+
+
+def _overlaps(out: torch.Tensor, *others: torch.Tensor) -> bool:
+    """Whether out's bytes may meet another tensor's (by their storages' ranges)."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if out.numel() == 0:
+        return False
+    a, b = span(out)
+    return any(t is not None and t.numel() and span(t)[0] < b and a < span(t)[1] for t in others)
+
+
+@dataclass(frozen=True, eq=False)
+class PackedPlan:
+    """How ``attention_packed`` walks one batch of packed sequences (``packed_plan``). It holds for
+    every call with these lengths (all layers of a model), on any stream of its device."""
+    q_tokens: int
+    k_tokens: int
+    heads: int
+    kv_heads: int
+    head_dim: int
+    causal: bool
+    tile_rows: int
+    n_tiles: int
+    tiles: torch.Tensor
+
+
+def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, heads: int,
+                kv_heads: Optional[int] = None, head_dim: int, causal: bool = True,
+                device="cuda") -> PackedPlan:
+    """Plans ``attention_packed`` over sequences of ``q_lens`` new tokens against ``k_lens`` keys
+    each (default: the same lengths). Lengths are host integers (0 included). Made once per batch,
+    outside a graph capture: it copies the tiles to ``device``."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    q_lens = [int(n) for n in q_lens]
+    k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+    if len(q_lens) != len(k_lens):
+        raise ValueError(f"{len(q_lens)} query lengths and {len(k_lens)} key lengths")
+    if any(not 0 <= n < 1 << 30 for n in q_lens + k_lens):
+        raise ValueError("lengths must be between 0 and 2^30")
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} K/V heads evenly")
+    if head_dim not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"head_dim {head_dim} is not one of {GROUPED_HEAD_DIMS}")
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"expected a GPU device, got {device}")
+    n = len(q_lens)
+    arr = ctypes.c_int32 * max(n, 1)
+    ql, kl = arr(*q_lens), arr(*k_lens)
+    count, rows = ctypes.c_int64(0), ctypes.c_int32(0)
+
+    def plan(tiles: int, capacity: int) -> None:
+        st = _lib.lib().mi355_attn_packed_plan(ql, kl, n, heads, kv_heads, head_dim, int(causal), tiles,
+                                               capacity, ctypes.byref(count), ctypes.byref(rows))
+        _lib.check("mi355_attn_packed_plan", st)
+
+    plan(0, 0)
+    tiles = torch.empty((count.value, 8), dtype=torch.int32)
+    if count.value:
+        plan(tiles.data_ptr(), count.value)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    on_gpu = tiles.to(device)  # (from pageable memory: there when this returns, for every stream)
+    return PackedPlan(sum(q_lens), sum(k_lens), heads, kv_heads, head_dim, bool(causal), rows.value,
+                      count.value, on_gpu)
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Softmax attention of packed sequences with grouped heads: ``q`` ``[q_tokens, heads, head_dim]``,
+    ``k`` and ``v`` ``[k_tokens, kv_heads, head_dim]`` (fp16 or bf16), sequence after sequence with
+    the lengths of ``plan``; query head h reads K/V head ``h // (heads // kv_heads)``.
+
+    With a causal plan, token i of a sequence's n sees its first ``k_len - n + i + 1`` keys (the last
+    token sees them all); otherwise every token sees all keys of its sequence. A token that sees no
+    key gives zeros, and a key that a token does not see never reaches it, NaN and infinities in its
+    K or V included. ``out`` (default: a new contiguous tensor) must not share memory with the inputs;
+    rows behind the plan's tokens (``q`` and ``out`` may have more) are left as they are. fp32
+    statistics, probabilities rounded to the input type. No backward pass."""
+    dev = _on_gpu(q, k, v, plan.tiles, out)
+    _no_grad(q, k, v)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    for name, t, tokens, heads in (("q", q, plan.q_tokens, plan.heads), ("k", k, plan.k_tokens, plan.kv_heads),
+                                   ("v", v, plan.k_tokens, plan.kv_heads)):
+        _rows_view(name, t, 3, q.dtype, 8)
+        if t.shape[0] < tokens or t.shape[1:] != (heads, plan.head_dim):
+            raise ValueError(f"the plan needs {name} [{tokens} or more, {heads}, {plan.head_dim}], got {tuple(t.shape)}")
+    scale = _scale(scale, plan.head_dim)
+    if out is None:
+        if q.shape[0] == plan.q_tokens:
+            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        else:  # rows behind the last token have no value
+            out = torch.zeros(q.shape, device=dev, dtype=q.dtype)
+    else:
+        _rows_view("out", out, 3, q.dtype, 4)
+        if out.shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
+        if _overlaps(out, q, k, v):
+            raise ValueError("out shares memory with an input")
+    if plan.n_tiles == 0:
+        return out
+    i64 = _lib.i64_array
+    with _on_device(dev):
+        st = _lib.lib().mi355_attn_packed(
+            _lib.dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), plan.heads,
+            plan.kv_heads, plan.head_dim, i64(_whole(q, q.stride()[:2])), i64(_kv_strides("k", k, 0)),
+            i64(_kv_strides("v", v, 0)), i64(_whole(out, out.stride()[:2])), scale, int(plan.causal),
+            plan.tiles.data_ptr(), plan.n_tiles, plan.tile_rows, _stream(q))
+    _lib.check("mi355_attn_packed", st)
+    return out
+
+
+def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
+                            k_own: torch.Tensor, v_own: torch.Tensor, own_lens: torch.Tensor,
+                            scale: Optional[float] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a batch's newest tokens when all its sequences start with the same prefix, which
+    is read once for all of them: ``q`` ``[B, n, heads, head_dim]`` (n = 1 when generating) against
+    ``k_prefix`` / ``v_prefix`` ``[P, kv_heads, head_dim]`` and each sequence's own cache ``k_own`` /
+    ``v_own`` ``[B, room, kv_heads, head_dim]``, of which the first ``own_lens[b]`` tokens (int32, on
+    the GPU) are filled, the n newest at their end. Token i of the n sees the whole prefix and the
+    first ``own_lens[b] - n + i + 1`` own keys; a token that sees no key gives zeros.
+
+    ``own_lens`` is read by the kernels, so a captured graph follows its values; it is clamped to
+    [0, room], and what a cache holds behind it does not matter. Types, head dims and roundings as
+    ``attention_packed``. ``out`` must not share memory with the inputs. No backward pass."""
+    dev = _on_gpu(q, k_prefix, v_prefix, k_own, v_own, own_lens, out)
+    _no_grad(q, k_prefix, v_prefix, k_own, v_own)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
+    for name, t, dims in (("q", q, 4), ("k_prefix", k_prefix, 3), ("v_prefix", v_prefix, 3),
+                          ("k_own", k_own, 4), ("v_own", v_own, 4)):
+        _rows_view(name, t, dims, q.dtype, 8)
+    B, n, H, D = q.shape
+    P, Hkv = k_prefix.shape[:2]
+    room = k_own.shape[1]
+    if D not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"head_dim {D} is not one of {GROUPED_HEAD_DIMS}")
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} K/V heads evenly")
+    if (tuple(k_prefix.shape) != (P, Hkv, D) or v_prefix.shape != k_prefix.shape
+            or tuple(k_own.shape) != (B, room, Hkv, D) or v_own.shape != k_own.shape):
+        raise ValueError(f"shape mismatch q={tuple(q.shape)} prefix={tuple(k_prefix.shape)}, "
+                         f"{tuple(v_prefix.shape)} own={tuple(k_own.shape)}, {tuple(v_own.shape)}")
+    if own_lens.dtype != torch.int32 or tuple(own_lens.shape) != (B,) or not own_lens.is_contiguous():
+        raise ValueError(f"own_lens must be a contiguous int32 tensor of shape ({B},)")
+    scale = _scale(scale, D)
+    if out is None:
+        out = torch.empty((B, n, H, D), device=dev, dtype=q.dtype)
+    else:
+        _rows_view("out", out, 4, q.dtype, 4)
+        if out.shape != q.shape:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
+        if _overlaps(out, q, k_prefix, v_prefix, k_own, v_own):
+            raise ValueError("out shares memory with an input")
+    if out.numel() == 0:
+        return out
+    L = _lib.lib()
+    need = L.mi355_attn_shared_prefix_workspace_bytes(B, n, H, Hkv, D, P, room)
+    if need < 0:
+        _lib.check("mi355_attn_shared_prefix_workspace_bytes", need)
+    i64 = _lib.i64_array
+    with _on_device(dev):
+        ws = torch.empty((max(need, 16),), device=dev, dtype=torch.uint8)
+        st = L.mi355_attn_shared_prefix(
+            _lib.dtype_code(q.dtype), q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(),
+            k_own.data_ptr(), v_own.data_ptr(), own_lens.data_ptr(), out.data_ptr(), B, n, H, Hkv, D, P,
+            room, i64(_whole(q, q.stride()[:3])), i64(_kv_strides("k_prefix", k_prefix, 0)),
+            i64(_kv_strides("v_prefix", v_prefix, 0)), i64(_kv_strides("k_own", k_own, 1)),
+            i64(_kv_strides("v_own", v_own, 1)), i64(_whole(out, out.stride()[:3])), scale,
+            ws.data_ptr(), need, _stream(q))
+    _lib.check("mi355_attn_shared_prefix", st)
+    return out
+
+
+# group sizes of linear_i4
+I4_GROUPS = (32, 64, 128)
+
+
+def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
+                    ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """4-bit weights for ``linear_i4`` from ``w`` ``[N, K]`` (fp16 or bf16): ``(q, scale, zero)`` with
+    ``w ~ scale[n, k / group] (q[n, k] - zero[n, k / group])``, q two to a byte (even k in the low
+    half) ``[N, K / 2]`` uint8, scale of w's type. Each group's range (0 included) goes to 0 .. 15, or with
+    ``symmetric`` its largest magnitude to +-7 around 8 (zero is None). Run once per weight."""
+    if w.dim() != 2 or w.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("quant_groups_i4 expects a 2-D fp16 or bf16 weight")
+    if group not in I4_GROUPS or w.shape[1] % group:
+        raise ValueError(f"group must be one of {I4_GROUPS} and divide K = {w.shape[1]}")
+    with torch.no_grad():
+        x = w.detach().float().reshape(w.shape[0], -1, group)
+        tiny = torch.finfo(w.dtype).tiny  # an all-zero group's scale
+        if symmetric:
+            scale = (x.abs().amax(2) / 7).clamp_min(tiny).to(w.dtype)
+            zero, z = None, 8.0
+        else:
+            lo, hi = x.amin(2).clamp_max(0), x.amax(2).clamp_min(0)
+            scale = ((hi - lo) / 15).clamp_min(tiny).to(w.dtype)
+            z = (-lo / scale.float()).round().clamp(0, 15)
+            zero, z = z.to(torch.uint8), z[..., None]
+        q = ((x / scale.float()[..., None]).round() + z).clamp(0, 15).to(torch.uint8).reshape(w.shape)
+        return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scale, zero
+
+
+def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
+              zero: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+              out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Projection of a few rows with 4-bit weights: ``x @ W^T + bias`` with
+    ``W[n, k] = scale[n, k / group] (q[n, k] - zero[n, k / group])``.
+
+    ``x`` is ``[M, K]`` fp16 or bf16 (row-strided, unit column stride); ``w`` ``[N, K / 2]`` uint8 holds
+    q two to a byte, the even k in the low half; ``scale`` ``[N, K / group]`` is of x's type, group 32,
+    64 or 128; ``zero`` uint8 of scale's shape (None: 8); ``bias`` fp32 ``[N]``. Made for M of a few
+    rows (the weights are read again for every 64). fp32 sums, the output (x's type, or fp32 with
+    ``out_dtype``) rounded once. bf16: |x| below 2^119. ``out`` must not share memory with ``x``.
+    No backward pass."""
+    dev = _on_gpu(x, w, scale, zero, bias, out)
+    _no_grad(x, scale, bias)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"x must be fp16 or bf16, got {x.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or scale.dim() != 2:
+        raise ValueError("linear_i4 expects 2-D x, w and scale")
+    M, K = x.shape
+    N = w.shape[0]
+    if w.dtype != torch.uint8 or w.shape[1] * 2 != K or not w.is_contiguous():
+        raise ValueError(f"w must be a contiguous uint8 tensor of shape (N, {K // 2}) for K = {K}")
+    group = K // scale.shape[1] if scale.shape[1] else 0
+    if group not in I4_GROUPS or scale.shape != (N, K // group) or K % group:
+        raise ValueError(f"scale must be [N, K / group] with a group of {I4_GROUPS}, got {tuple(scale.shape)}")
+    if scale.dtype != x.dtype or not scale.is_contiguous():
+        raise ValueError("scale must be contiguous and of x's dtype")
+    if zero is not None and (zero.dtype != torch.uint8 or zero.shape != scale.shape or not zero.is_contiguous()):
+        raise ValueError("zero must be a contiguous uint8 tensor of scale's shape")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous fp32 tensor of shape ({N},)")
+    ldx = x.stride(0) if M > 1 else (K + 7) // 8 * 8
+    if M and (x.stride(1) != 1 or ldx < K or ldx % 8 or x.data_ptr() % 16 or w.data_ptr() % 16):
+        raise ValueError("x needs unit column stride, a row stride of a multiple of 8 that holds a row, "
+                         "and x and w 16-byte aligned starts")
+    odt = out_dtype or (out.dtype if out is not None else x.dtype)
+    if odt not in (x.dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {x.dtype} or float32")
+    if out is None:
+        out = torch.empty((M, N), device=dev, dtype=odt)
+    elif out.shape != (M, N) or out.dtype != odt or (out.numel() and out.stride(1) != 1) \
+            or (M > 1 and out.stride(0) < N):
+        raise ValueError("out must be [M, N] of out_dtype with unit column stride")
+    elif _overlaps(out, x, w, scale, zero, bias):
+        raise ValueError("out shares memory with an input")
+    if out.numel() == 0:
+        return out
+    with _on_device(dev):
+        st = _lib.lib().mi355_linear_i4(
+            _lib.dtype_code(x.dtype), _lib.dtype_code(odt), x.data_ptr(), ldx, w.data_ptr(), scale.data_ptr(),
+            zero.data_ptr() if zero is not None else 0, bias.data_ptr() if bias is not None else 0,
+            out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, group, _stream(x))
+    _lib.check("mi355_linear_i4", st)
     return out
