@@ -50,8 +50,9 @@ MI355_DEVINL typename Nib<T>::vec nibbles(uint32_t w, f16x2 zz) {
   u32x4 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    r[i] = ((w >> (4 * i)) & 0x000f000fu) | Nib<T>::MAGIC;
-    if constexpr (__is_same(T, _Float16)) r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, r[i]) - zz);
+    uint32_t two = ((w >> (4 * i)) & 0x000f000fu) | Nib<T>::MAGIC;
+    if constexpr (__is_same(T, _Float16)) two = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, two) - zz);
+    r[i] = two;
   }
   return __builtin_bit_cast(typename Nib<T>::vec, r);
 }
