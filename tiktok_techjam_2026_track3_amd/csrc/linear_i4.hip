@@ -4,13 +4,13 @@
 // Bound by the weights' bytes: every 4-bit value is read once, straight into the registers of the
 // lane that multiplies it, and rows of x ride along as the other operand of 16x16x32 MFMAs (A = x:
 // 16 rows, B = weights: 16 features; a lane holds one feature, lane % 16, so its scale and zero are
-// one scalar each, and D[m][n] of 4 rows of x). A work-group takes 16 features; its waves take
-// contiguous ranges of k and add up through LDS.
-//   Nibbles become operands without conversions: (w >> 4 i) & 0x000f000f put into the mantissa of
-//   1024 (fp16) or 128 (bf16) is the number 1024 + q or 128 + q. fp16 subtracts 1024 + z, exactly
-//   (packed); bf16 has no packed subtraction, so its sum over a group is corrected in fp32 by
-//   (128 + z) sum x, with sum x from MFMAs against ones. x up to 2^119 is safe there (143 x GROUP
-//   products are added up before the correction).
+// one scalar each, and D[m][n] of 4 rows of x). A wave takes R tiles of 16 features, for which it
+// loads x once; the waves of a work-group take contiguous ranges of k and add up through LDS.
+//   Nibbles become operands without conversions: put into the top mantissa bits of 16 (shift, and-or),
+//   q is the number 16 + q. A group's sum is then corrected in fp32, sum x q' - (16 + z) sum x, with
+//   sum x from MFMAs against ones (shared by the R tiles); at most 31 : 15 + z in size, so that nothing is lost
+//   to the larger operands. Subtracting in 16 bits before the product (packed, fp16 only) took 11 vector
+//   instructions for 8 weights, this takes 8, which is what a CU can spend on them at 5 TB/s.
 //   A lane's 16 bytes are 32 neighbouring k. For GROUP 128 the four lanes of a feature hold the
 //   whole group and each word is one MFMA's operand as it is; for 32 and 64 the words change
 //   places between the four lanes (4 lane swaps) so that one MFMA's 32 k are neighbours.
@@ -34,26 +34,26 @@ struct Nib;
 template <>
 struct Nib<_Float16> {
   using vec = f16x8;
-  static constexpr uint32_t MAGIC = 0x64006400u;
+  static constexpr uint32_t SIXTEEN = 0x4c004c00u;
+  static constexpr int SHIFT = 6;  // of a nibble's lowest bit, 16's mantissa is 10 bits long
 };
 template <>
 struct Nib<__bf16> {
   using vec = bf16x8;
-  static constexpr uint32_t MAGIC = 0x43004300u;
+  static constexpr uint32_t SIXTEEN = 0x41804180u;
+  static constexpr int SHIFT = 3;  // ... 7 bits
 };
 MI355_DEVINL f32x4 mma_i4(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 MI355_DEVINL f32x4 mma_i4(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// 8 nibbles of a word as an operand: elements 0 4 1 5 2 6 3 7
+// 8 nibbles of a word, 16 + q each: elements 0 4 1 5 2 6 3 7
 template <typename T>
-MI355_DEVINL typename Nib<T>::vec nibbles(uint32_t w, f16x2 zz) {
+MI355_DEVINL typename Nib<T>::vec nibbles(uint32_t w) {
+  constexpr int SH = Nib<T>::SHIFT;
   u32x4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t two = ((w >> (4 * i)) & 0x000f000fu) | Nib<T>::MAGIC;
-    if constexpr (__is_same(T, _Float16)) two = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, two) - zz);
-    r[i] = two;
-  }
+  for (int i = 0; i < 4; ++i)
+    r[i] = ((4 * i < SH ? w << (SH - 4 * i) : w >> (4 * i - SH)) & (0x000f000fu << SH)) | Nib<T>::SIXTEEN;
   return __builtin_bit_cast(typename Nib<T>::vec, r);
 }
 // 8 elements in the order 0 4 1 5 2 6 3 7
@@ -62,140 +62,211 @@ MI355_DEVINL u32x4 nibble_order(u32x4 v) {
                __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
 }
 
-// MT tiles of 16 rows of x
-template <typename T, int GROUP, int MT, int NW, typename TO>
+// N consecutive values from any address of their type (one or two wide loads where they line up)
+template <int N, typename V>
+MI355_DEVINL void load_run(const V* src, V (&dst)[N]) {
+  struct Run { V v[N]; } __attribute__((packed, aligned(1)));
+  const Run run = *reinterpret_cast<const Run*>(src);
+#pragma unroll
+  for (int i = 0; i < N; ++i) dst[i] = run.v[i];
+}
+
+// MT tiles of 16 rows of x, R tiles of 16 features. Steps of 128 k in batches of 4, whose weights are
+// loaded a batch ahead; a feature's scales and zero points of a batch are neighbours and loaded together.
+template <typename T, int GROUP, int MT, int R, int NW, typename TO>
 __global__ __launch_bounds__(64 * NW) void linear_i4_kernel(I4Args p) {
   using vec = typename Nib<T>::vec;
-  constexpr int GP = 128 / GROUP;  // groups of a 128-k step
-  constexpr int U = 4;             // steps whose loads are in flight
+  constexpr int GP = 128 / GROUP;           // groups of a step
+  constexpr int U = 4;                      // steps of a batch
+  constexpr int XU = MT == 1 ? 2 : 1;       // steps whose x is in flight
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, feature = n0 + l16 < p.N ? n0 + l16 : p.N - 1;
-  const int m0 = blockIdx.y * (16 * MT);
-  const int groups = p.K / GROUP;
-  const uint8_t* wrow = p.w + static_cast<int64_t>(feature) * (p.K / 2);
-  const T* srow = static_cast<const T*>(p.scale) + static_cast<int64_t>(feature) * groups;
-  const uint8_t* zrow = p.zero != nullptr ? p.zero + static_cast<int64_t>(feature) * groups : nullptr;
-  const int steps = (p.K + 127) / 128, per = (steps + NW - 1) / NW;
+  const int n0 = blockIdx.x * (16 * R), m0 = blockIdx.y * (16 * MT);
+  const int groups = p.K / GROUP, steps = (p.K + 127) / 128;
+  const int per = ((steps + NW - 1) / NW + U - 1) / U * U;
   const int s_begin = wave * per, s_end = s_begin + per < steps ? s_begin + per : steps;
-
-  struct Step {
-    u32x4 w;
-    float s[GP];
-    float z[GP];
-  };
-  auto fetch = [&](int s, Step& d) MI355_LAMBDA_INLINE {
-    const int k = s * 128 + 32 * g;
-    d.w = s < s_end && k < p.K ? *reinterpret_cast<const u32x4*>(wrow + k / 2) : u32x4{0u, 0u, 0u, 0u};
+  const uint8_t* wrow[R];
+  const T* srow[R];
+  const uint8_t* zrow[R];
 #pragma unroll
-    for (int i = 0; i < GP; ++i) {
-      const int at = s * GP + i;
-      const bool in = s < s_end && at < groups;
-      d.s[i] = in ? to_f32(srow[at]) : 0.f;
-      d.z[i] = in && zrow != nullptr ? static_cast<float>(zrow[at]) : 8.f;
-    }
-  };
-  f32x4 total[MT];
+  for (int r = 0; r < R; ++r) {
+    // features past the last: any real one's, not stored
+    const int64_t f = n0 + 16 * r + l16 < p.N ? n0 + 16 * r + l16 : p.N - 1;
+    wrow[r] = p.w + f * (p.K / 2);
+    srow[r] = static_cast<const T*>(p.scale) + f * groups;
+    zrow[r] = p.zero + f * groups;  // (read only where there are any)
+  }
+  const T* xrow[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) total[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = m0 + 16 * t + l16 < p.M ? m0 + 16 * t + l16 : p.M - 1;
+    xrow[t] = static_cast<const T*>(p.x) + m * p.ldx;
+  }
+  f32x4 total[R][MT];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) total[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   vec ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
 
-  auto compute = [&](int s, const Step& d) MI355_LAMBDA_INLINE {
-    u32x4 w = d.w;
-    if constexpr (GROUP != 128) {
-      // words of the lanes g' become word g' of the lanes: a 4 x 4 transposition over (lane / 16, word)
-      auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-      auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-      auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-      auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-      w = u32x4{c[0], c[1], e[0], e[1]};
+  struct Batch {
+    u32x4 w[U][R];
+    T s[R][U * GP];
+    uint8_t z[R][U * GP];
+  };
+  // (steps past the wave's range load its last one again; k past K, the row's last ones)
+  auto fetch = [&](int s0, Batch& d) MI355_LAMBDA_INLINE {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u < s_end ? s0 + u : s_end - 1;
+      int k = s * 128 + 32 * g;
+      if constexpr (GROUP != 128) k = k < p.K ? k : p.K - 32;
+#pragma unroll
+      for (int r = 0; r < R; ++r) d.w[u][r] = *reinterpret_cast<const u32x4*>(wrow[r] + k / 2);
     }
-    f32x4 acc[MT], sum[MT];
+    const int at = s0 * GP;
+    if (at + U * GP <= groups) {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int i = m * GP / 4;  // the MFMA's group in the step
-      if (m * GP % 4 == 0) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < R; ++r) {
+        load_run(srow[r] + at, d.s[r]);
+        if (p.zero != nullptr) load_run(zrow[r] + at, d.z[r]);
       }
-      const _Float16 z1 = static_cast<_Float16>(1024.f + d.z[i]);
-      const vec wv = nibbles<T>(w[m], f16x2{z1, z1});
-      const int k = s * 128 + (GROUP == 128 ? 32 * g + 8 * m : 32 * m + 8 * g);
+    } else {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        u32x4 xv = {0u, 0u, 0u, 0u};
-        const int row = m0 + 16 * t + l16;
-        if (row < p.M && k < p.K) xv = *reinterpret_cast<const u32x4*>(static_cast<const T*>(p.x) + row * p.ldx + k);
-        const vec xo = __builtin_bit_cast(vec, nibble_order(xv));
-        acc[t] = mma_i4(xo, wv, acc[t]);
-        if constexpr (__is_same(T, __bf16)) sum[t] = mma_i4(xo, ones, sum[t]);
-      }
-      if ((m + 1) * GP % 4 == 0) {
+      for (int i = 0; i < U * GP; ++i)
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int r = 0; r < R; ++r) {
+          const int gi = at + i < groups ? at + i : groups - 1;
+          d.s[r][i] = srow[r][gi];
+          if (p.zero != nullptr) d.z[r][i] = zrow[r][gi];
+        }
+    }
+    if (p.zero == nullptr) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = acc[t][e];
-            if constexpr (__is_same(T, __bf16)) v = __builtin_fmaf(sum[t][e], -128.f - d.z[i], v);
-            total[t][e] = __builtin_fmaf(v, d.s[i], total[t][e]);
-          }
-      }
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < U * GP; ++i) d.z[r][i] = 8;
     }
   };
-  Step cur[U], nxt[U];
+  Batch cur;
+  if (s_begin < s_end) fetch(s_begin, cur);
+  for (int s0 = s_begin; s0 < s_end; s0 += U) {
+    u32x4 x[XU][4][MT];
+    auto fetch_x = [&](int s1) MI355_LAMBDA_INLINE {
 #pragma unroll
-  for (int u = 0; u < U; ++u) fetch(s_begin + u, cur[u]);
-  for (int s = s_begin; s < s_end; s += U) {
+      for (int u = 0; u < XU; ++u) {
+        const int s = s1 + u < s_end ? s1 + u : s_end - 1;
 #pragma unroll
-    for (int u = 0; u < U; ++u) fetch(s + U + u, nxt[u]);
+        for (int m = 0; m < 4; ++m) {
+          int k = s * 128 + (GROUP == 128 ? 32 * g + 8 * m : 32 * m + 8 * g);
+          if constexpr (GROUP != 128) k = k < p.K ? k : p.K - 8;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + u < s_end) compute(s + u, cur[u]);
+          for (int t = 0; t < MT; ++t) x[u][m][t] = *reinterpret_cast<const u32x4*>(xrow[t] + k);
+        }
+      }
+    };
+    fetch_x(s0);
+    Batch nxt;
+    if (s0 + U < s_end) fetch(s0 + U, nxt);
 #pragma unroll
-    for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= s_end) break;
+      if (u > 0 && u % XU == 0) fetch_x(s0 + u);
+      u32x4 wu[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        wu[r] = cur.w[u][r];
+        if constexpr (GROUP != 128) {
+          // word m of lanes j becomes word j of lanes m: a 4 x 4 transposition over (lane / 16, word)
+          auto a = __builtin_amdgcn_permlane32_swap(wu[r][0], wu[r][2], false, false);
+          auto b = __builtin_amdgcn_permlane32_swap(wu[r][1], wu[r][3], false, false);
+          auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+          auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+          wu[r] = u32x4{c[0], c[1], e[0], e[1]};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < GP; ++i) {
+        if (GROUP != 128 && (s0 + u) * GP + i >= groups) break;  // past K
+        f32x4 acc[R][MT], sum[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int m = i * 4 / GP; m < (i + 1) * 4 / GP; ++m) {
+          vec xo[MT];
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            xo[t] = __builtin_bit_cast(vec, nibble_order(x[u % XU][m][t]));
+            sum[t] = mma_i4(xo[t], ones, sum[t]);
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const vec wv = nibbles<T>(wu[r][m]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[r][t] = mma_i4(xo[t], wv, acc[r][t]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float z = -16.f - static_cast<float>(cur.z[r][u * GP + i]), sf = to_f32(cur.s[r][u * GP + i]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              total[r][t][e] = __builtin_fmaf(__builtin_fmaf(sum[t][e], z, acc[r][t][e]), sf, total[r][t][e]);
+        }
+      }
+    }
+    cur = nxt;
   }
 
-  __shared__ f32x4 part[NW][MT][64];
-  if constexpr (NW > 1) {
+  __shared__ f32x4 part[NW][R * MT][64];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = total[t];
-    __syncthreads();
-  }
-  // wave t' adds up tiles t', t' + NW ..
+  for (int i = 0; i < R * MT; ++i) part[wave][i][lane] = total[i / MT][i % MT];
+  __syncthreads();
+  // wave w adds up tiles w, w + NW ..
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    if (t % NW != wave) continue;
-    f32x4 v = total[t];
-    if constexpr (NW > 1) {
-      v = part[0][t][lane];
+  for (int i = 0; i < R * MT; ++i) {
+    if (i % NW != wave) continue;
+    const int r = i / MT, t = i % MT, n = n0 + 16 * r + l16;
+    f32x4 v = part[0][i][lane];
 #pragma unroll
-      for (int w = 1; w < NW; ++w)
+    for (int y = 1; y < NW; ++y)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += part[w][t][lane][e];
-    }
-    if (n0 + l16 < p.N) {
-      const float b = p.bias != nullptr ? p.bias[n0 + l16] : 0.f;
+      for (int e = 0; e < 4; ++e) v[e] += part[y][i][lane][e];
+    if (n < p.N) {
+      const float b = p.bias != nullptr ? p.bias[n] : 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = m0 + 16 * t + 4 * g + e;
-        if (row < p.M) static_cast<TO*>(p.y)[row * p.ldy + n0 + l16] = from_f32<TO>(v[e] + b);
+        if (row < p.M) static_cast<TO*>(p.y)[row * p.ldy + n] = from_f32<TO>(v[e] + b);
       }
     }
   }
 }
 
+template <typename T, int GROUP, int MT, int R, int NW, typename TO>
+int launch_one(const I4Args& a, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((a.N + 16 * R - 1) / (16 * R)), static_cast<unsigned>((a.M + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((linear_i4_kernel<T, GROUP, MT, R, NW, TO>), grid, dim3(64 * NW), 0, s, a);
+  return static_cast<int>(hipGetLastError());
+}
 template <typename T, int GROUP, int MT, typename TO>
 int launch_nw(const I4Args& a, hipStream_t s) {
-  const int64_t tiles = (a.N + 15) / 16, my = (a.M + 16 * MT - 1) / (16 * MT), steps = (a.K + 127) / 128;
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(my));
-  // waves that share a work-group's sum: as many as leave each 4 steps, until the CUs are full
-  if (steps > 16 && tiles * my < 1024)
-    hipLaunchKernelGGL((linear_i4_kernel<T, GROUP, MT, 8, TO>), grid, dim3(512), 0, s, a);
-  else
-    hipLaunchKernelGGL((linear_i4_kernel<T, GROUP, MT, 4, TO>), grid, dim3(256), 0, s, a);
-  return static_cast<int>(hipGetLastError());
+  const int64_t tiles = (a.N + 15) / 16, steps = (a.K + 127) / 128;
+  if constexpr (MT == 1 && GROUP != 32) {
+    // Two tiles a wave halve the loads of x: where its 16 rows are mostly real and two tiles a wave
+    // leave every CU work-groups
+    if (a.M > 4 && tiles >= 768) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
+  }
+  if constexpr (MT == 1) return steps > 16 ? launch_one<T, GROUP, MT, 1, 8, TO>(a, s) : launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
+  else return launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
 }
 template <typename T, int GROUP, typename TO>
 int launch_mt(const I4Args& a, hipStream_t s) {
