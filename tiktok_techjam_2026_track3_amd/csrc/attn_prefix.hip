@@ -22,6 +22,9 @@ struct Split {
   int64_t prefix_chunk, own_chunk, prefix_splits, own_splits;
 };
 
+// most splits of the prefix or of a cache, and of both together for one wave to join
+constexpr int MAX_SPLITS = 1280, WAVE_SPLITS = 16;
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 Split split_of(const Shape& s) {
@@ -33,8 +36,8 @@ Split split_of(const Shape& s) {
     const int64_t splits = std::max<int64_t>(1, want / std::max<int64_t>(1, groups));
     return std::max(least, ceil_div(ceil_div(keys, splits), 64) * 64);
   };
-  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows <= 32 ? 1280 : 512, 128);
-  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, 1280, 128);
+  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows <= 32 ? MAX_SPLITS : 512, 128);
+  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, MAX_SPLITS, 128);
   d.prefix_splits = ceil_div(s.prefix, d.prefix_chunk);
   d.own_splits = ceil_div(s.room, d.own_chunk);
   return d;
@@ -62,12 +65,18 @@ struct CombineArgs {
   const int32_t* lens;
 };
 
-// A wave per row: lane x holds elements 4 x .. of hd <= 256.
-template <typename T>
+// W waves a row, W divides 4 rows' worth of them: first each lane takes splits of its own (maximum, then
+// weights 2^(mu_s - M), left in LDS), then lanes of 4 elements each add up the weighted outputs, as many
+// splits at a time as the waves have lanes for, and what they hold is added up through LDS.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void combine_splits(CombineArgs p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= p.rows) return;
+  constexpr int RPG = 4 / W, NT = 64 * W;  // rows of a work-group, threads of a row
+  __shared__ float weight[RPG][W == 1 ? WAVE_SPLITS : 2 * MAX_SPLITS];
+  __shared__ float red[RPG][2][W];
+  __shared__ f32x4 sums[RPG][NT];
+  const int slot = threadIdx.x / NT, tid = threadIdx.x % NT, lane = threadIdx.x & 63, wave = tid >> 6;
+  const int64_t given_row = static_cast<int64_t>(blockIdx.x) * RPG + slot;
+  const int64_t row = given_row < p.rows ? given_row : p.rows - 1;  // (computed twice, stored once)
   const int head = static_cast<int>(row % p.H);
   const int64_t bt = row / p.H;
   const int b = static_cast<int>(bt / p.n_q), t = static_cast<int>(bt % p.n_q);
@@ -75,28 +84,66 @@ __global__ __launch_bounds__(256) void combine_splits(CombineArgs p) {
   const int len = given < 0 ? 0 : (given < p.room ? given : p.room);
   const int seen = len - p.n_q + t + 1;  // own keys of this token
   const int splits = p.prefix_splits + (seen > 0 ? (seen + p.own_chunk - 1) / p.own_chunk : 0);
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float m = NEG_INF, l = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float ms = p.ml[2 * (s * p.rows + row)], ls = p.ml[2 * (s * p.rows + row) + 1];
-    if (ms == NEG_INF) continue;  // no finite score there
-    const float m2 = vmax(m, ms);
-    const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2), w = fast_exp2(ms - m2);
-    l = __builtin_fmaf(l, a, ls * w);
-    if (4 * lane < p.hd) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + (s * p.rows + row) * p.hd + 4 * lane);
+  float m = NEG_INF;
+  for (int s = tid; s < splits; s += NT) m = vmax(m, p.ml[2 * (s * p.rows + row)]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(acc[e], a, x[e] * w);
-    }
-    m = m2;
+  for (int off = 32; off >= 1; off >>= 1) m = vmax(m, __shfl_xor(m, off));
+  if constexpr (W > 1) {
+    if (lane == 0) red[slot][0][wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = vmax(m, red[slot][0][i]);
   }
-  if (4 * lane >= p.hd) return;
+  float l = 0.f;
+  for (int s = tid; s < splits; s += NT) {
+    const float ms = p.ml[2 * (s * p.rows + row)], ls = p.ml[2 * (s * p.rows + row) + 1];
+    const float w = fast_exp2(ms - m);
+    weight[slot][s] = ms == NEG_INF ? NEG_INF : w;  // -inf: nothing there counts
+    l = ms == NEG_INF ? l : __builtin_fmaf(ls, w, l);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off);
+  if constexpr (W > 1) {
+    if (lane == 0) red[slot][1][wave] = l;
+  }
+  __syncthreads();
+  if constexpr (W > 1) {
+    l = red[slot][1][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) l += red[slot][1][i];
+  }
+  const int per = p.hd / 4, at_once = NT / per, mine = tid / per, x = tid % per;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (mine < at_once) {
+    const float* src = p.part + row * p.hd + 4 * x;
+    const int64_t pitch = p.rows * p.hd;
+    for (int s0 = mine; s0 < splits; s0 += 4 * at_once) {
+      f32x4 v[4];
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * at_once;
+        w[i] = s < splits ? weight[slot][s] : NEG_INF;
+        v[i] = *reinterpret_cast<const f32x4*>(src + (s < splits ? s : s0) * pitch);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = w[i] == NEG_INF ? acc[e] : __builtin_fmaf(v[i][e], w[i], acc[e]);
+    }
+  }
+  sums[slot][tid] = acc;
+  __syncthreads();
+  if (mine != 0 || given_row >= p.rows) return;
+  for (int i = 1; i < at_once; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += sums[slot][i * per + x][e];
   const bool none = p.prefix == 0 && seen <= 0;  // no key: zeros (no finite score: 0 / 0)
+  typedef T t4 __attribute__((ext_vector_type(4)));
   t4 w;
 #pragma unroll
   for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(none ? 0.f : acc[e] / l);
-  *reinterpret_cast<t4*>(static_cast<T*>(p.o) + b * p.ob + t * p.ot + head * p.oh + 4 * lane) = w;
+  *reinterpret_cast<t4*>(static_cast<T*>(p.o) + b * p.ob + t * p.ot + head * p.oh + 4 * x) = w;
 }
 
 template <typename T, int HD, int MODE>
@@ -151,7 +198,10 @@ int launch(const rows::Args& a, const rows::Args& own, const CombineArgs& c, con
     case 256: e = launch_hd<T, 256>(a, own, s, d, st); break;
   }
   if (e) return e;
-  hipLaunchKernelGGL((combine_splits<T>), dim3(static_cast<unsigned>(ceil_div(c.rows, 4))), dim3(256), 0, st, c);
+  if (d.prefix_splits + d.own_splits <= WAVE_SPLITS)
+    hipLaunchKernelGGL((combine_splits<T, 1>), dim3(static_cast<unsigned>(ceil_div(c.rows, 4))), dim3(256), 0, st, c);
+  else
+    hipLaunchKernelGGL((combine_splits<T, 4>), dim3(static_cast<unsigned>(c.rows)), dim3(256), 0, st, c);
   return static_cast<int>(hipGetLastError());
 }
 
