@@ -6,8 +6,8 @@ device. Nothing here synchronises the host, so the calls are hipGraph-capturable
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -548,50 +548,61 @@ def linear_i8(a: torch.Tensor, w: torch.Tensor, s_a: torch.Tensor, s_w: torch.Te
 # head dims of attention_packed and attention_shared_prefix
 GROUPED_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 192, 256)
 
-
-def _on_device(dev: torch.device):
-    """Makes ``dev`` current for a launch, where it is not."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
-
-
-def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
-                                 "or with detached tensors")
+# The operators below are called for single tokens, where a call's time is the host's. What their checks
+# look at (shapes, strides, types) is checked once per combination: the checks are cached functions of
+# those numbers alone, which also return the arguments made from them. Pointers, devices and gradients are
+# looked at in every call.
+_SIXTEEN_BIT = (torch.float16, torch.bfloat16)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _rows_view(name: str, t: torch.Tensor, dims: int, dtype: torch.dtype, align: int) -> None:
-    """Checks a [..., token, head, head_dim] view: 16-bit, unit last stride, strides of whole vectors."""
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, q is {dtype}")
-    if t.numel() == 0:
-        return
-    if t.stride(-1) != 1:
+class _Arrays(tuple):
+    """int64 arrays of strides for the library."""
+    def __new__(cls, *strides):
+        return super().__new__(cls, [_lib.i64_array(st) for st in strides])
+
+
+def _launch(device: int, fn, *args) -> int:
+    """Calls a library entry point with ``device``'s current stream as the last argument and that
+    device current."""
+    if _current_device() == device:
+        return fn(*args, _raw_stream(device))
+    with torch.cuda.device(device):
+        return fn(*args, _raw_stream(device))
+
+
+def _no_backward(*tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
+                             "or with detached tensors")
+
+
+def _rows_strides(name: str, shape, stride, align: int, kv_axis: Optional[int] = None) -> Tuple[int, ...]:
+    """Strides of a [..., token, head, head_dim] view but the last, checked: unit head_dim stride, whole
+    vectors between rows, and for K / V (kv_axis: the token axis) tokens that do not overlap. Axes of
+    one element get a stride that does not matter."""
+    if 0 in shape:
+        return tuple(shape[-1] if i == kv_axis else 0 for i in range(len(shape) - 1))
+    if stride[-1] != 1:
         raise ValueError(f"head_dim must be the unit-stride dimension of {name}")
-    if any(n > 1 and s % align for n, s in zip(t.shape[:-1], t.stride()[:-1])) or t.data_ptr() % (2 * align):
-        raise ValueError(f"{name} needs strides that are multiples of {align} elements and a "
-                         f"{2 * align}-byte aligned start")
+    out = []
+    for i, (n, st) in enumerate(zip(shape[:-1], stride[:-1])):
+        if n == 1:
+            st = shape[-1] if i == kv_axis else 0
+        elif st % align:
+            raise ValueError(f"{name} needs strides that are multiples of {align} elements, got {tuple(stride)}")
+        elif i == kv_axis and not shape[-1] <= st <= 1 << 24:
+            raise ValueError(f"the tokens of {name} overlap or are too far apart (stride {st})")
+        out.append(st)
+    return tuple(out)
 
 
-def _kv_strides(name: str, t: torch.Tensor, axis: int) -> Tuple[int, ...]:
-    """Strides but the last; a token stride that no second token uses is the row itself."""
-    st = list(t.stride()[:-1])
-    if t.shape[axis] <= 1:
-        st[axis] = t.shape[-1]
-    elif t.numel() and not t.shape[-1] <= st[axis] <= 1 << 24:
-        raise ValueError(f"the tokens of {name} overlap or are too far apart (stride {st[axis]})")
-    return _whole(t, st)
-
-
-def _whole(t: torch.Tensor, strides) -> Tuple[int, ...]:
-    """Strides for the library: those of axes of one element do not matter and become 0."""
-    return tuple(0 if n == 1 and s % 8 else s for n, s in zip(t.shape[:-1], strides))
+def _check_aligned(**pointers: int) -> None:
+    for name, ptr in pointers.items():
+        if ptr % (8 if name == "out" else 16):
+            raise ValueError(f"{name} must start at a multiple of {8 if name == 'out' else 16} bytes")
 
 
 def _scale(scale: Optional[float], head_dim: int) -> float:
@@ -601,15 +612,17 @@ def _scale(scale: Optional[float], head_dim: int) -> float:
     return scale
 
 
-def _overlaps(out: torch.Tensor, *others: torch.Tensor) -> bool:
-    """Whether out's bytes may meet another tensor's (by their storages' ranges)."""
+def _check_apart(out: torch.Tensor, *inputs: Optional[torch.Tensor]) -> None:
+    """Refuses an ``out`` whose bytes (first to last) meet an input's."""
     def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
     if out.numel() == 0:
-        return False
-    a, b = span(out)
-    return any(t is not None and t.numel() and span(t)[0] < b and a < span(t)[1] for t in others)
+        return
+    lo, hi = span(out)
+    for t in inputs:
+        if t is not None and t.numel() and span(t)[0] < hi and lo < span(t)[1]:
+            raise ValueError("out shares memory with an input")
 
 
 @dataclass(frozen=True, eq=False)
@@ -668,6 +681,23 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
                       count.value, on_gpu)
 
 
+@functools.lru_cache(maxsize=512)
+def _packed_views(q_tokens, k_tokens, heads, kv_heads, D, dtypes, qs, qst, ks, kst, vs, vst, os, ost):
+    """(library type code, stride arrays) of attention_packed's tensors, checked."""
+    if dtypes[0] not in _SIXTEEN_BIT:
+        raise TypeError(f"q must be fp16 or bf16, got {dtypes[0]}")
+    if len(set(dtypes)) > 1:
+        raise TypeError(f"q, k, v and out must share one dtype, got {dtypes}")
+    for name, shape, tokens, h in (("q", qs, q_tokens, heads), ("k", ks, k_tokens, kv_heads), ("v", vs, k_tokens, kv_heads)):
+        if len(shape) != 3 or shape[0] < tokens or tuple(shape[1:]) != (h, D):
+            raise ValueError(f"the plan needs {name} [{tokens} or more, {h}, {D}], got {tuple(shape)}")
+    if os is not None and os != qs:
+        raise ValueError(f"out must have q's shape {tuple(qs)}")
+    arrays = _Arrays(_rows_strides("q", qs, qst, 8), _rows_strides("k", ks, kst, 8, 0), _rows_strides("v", vs, vst, 8, 0),
+                     (heads * D, D) if os is None else _rows_strides("out", os, ost, 4))
+    return _lib.dtype_code(dtypes[0]), arrays
+
+
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PackedPlan,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Softmax attention of packed sequences with grouped heads: ``q`` ``[q_tokens, heads, head_dim]``,
@@ -678,40 +708,69 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     token sees them all); otherwise every token sees all keys of its sequence. A token that sees no
     key gives zeros, and a key that a token does not see never reaches it, NaN and infinities in its
     K or V included. ``out`` (default: a new contiguous tensor) must not share memory with the inputs;
-    rows behind the plan's tokens (``q`` and ``out`` may have more) are left as they are. fp32
-    statistics, probabilities rounded to the input type. No backward pass."""
-    dev = _on_gpu(q, k, v, plan.tiles, out)
-    _no_grad(q, k, v)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
-    for name, t, tokens, heads in (("q", q, plan.q_tokens, plan.heads), ("k", k, plan.k_tokens, plan.kv_heads),
-                                   ("v", v, plan.k_tokens, plan.kv_heads)):
-        _rows_view(name, t, 3, q.dtype, 8)
-        if t.shape[0] < tokens or t.shape[1:] != (heads, plan.head_dim):
-            raise ValueError(f"the plan needs {name} [{tokens} or more, {heads}, {plan.head_dim}], got {tuple(t.shape)}")
+    rows behind the plan's tokens (``q`` and ``out`` may have more) are left as they are, zeros in a new
+    ``out``. fp32 statistics, probabilities rounded to the input type. No backward pass."""
+    dev = q.get_device()
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or plan.tiles.get_device() != dev or (
+            out is not None and out.get_device() != dev):
+        _on_gpu(q, k, v, plan.tiles, out)
+    if torch.is_grad_enabled():
+        _no_backward(q, k, v)
+    given = out is not None
+    code, (qst, kst, vst, ost) = _packed_views(
+        plan.q_tokens, plan.k_tokens, plan.heads, plan.kv_heads, plan.head_dim,
+        (q.dtype, k.dtype, v.dtype, out.dtype) if given else (q.dtype, k.dtype, v.dtype),
+        q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), out.shape if given else None,
+        out.stride() if given else None)
     scale = _scale(scale, plan.head_dim)
-    if out is None:
-        if q.shape[0] == plan.q_tokens:
-            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        else:  # rows behind the last token have no value
-            out = torch.zeros(q.shape, device=dev, dtype=q.dtype)
-    else:
-        _rows_view("out", out, 3, q.dtype, 4)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
-        if _overlaps(out, q, k, v):
-            raise ValueError("out shares memory with an input")
+    if given:
+        _check_apart(out, q, k, v)
+    else:  # (rows behind the last token have no value)
+        out = (torch.empty if q.shape[0] == plan.q_tokens else torch.zeros)(q.shape, device=q.device, dtype=q.dtype)
     if plan.n_tiles == 0:
         return out
-    i64 = _lib.i64_array
-    with _on_device(dev):
-        st = _lib.lib().mi355_attn_packed(
-            _lib.dtype_code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), plan.heads,
-            plan.kv_heads, plan.head_dim, i64(_whole(q, q.stride()[:2])), i64(_kv_strides("k", k, 0)),
-            i64(_kv_strides("v", v, 0)), i64(_whole(out, out.stride()[:2])), scale, int(plan.causal),
-            plan.tiles.data_ptr(), plan.n_tiles, plan.tile_rows, _stream(q))
-    _lib.check("mi355_attn_packed", st)
+    qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if (qp | kp | vp) & 15 or op & 7:
+        _check_aligned(q=qp, k=kp, v=vp, out=op)
+    st = _launch(dev, _lib.lib().mi355_attn_packed, code, qp, kp, vp, op, plan.heads, plan.kv_heads,
+                 plan.head_dim, qst, kst, vst, ost, scale, plan.causal, plan.tiles.data_ptr(), plan.n_tiles,
+                 plan.tile_rows)
+    if st:
+        _lib.check("mi355_attn_packed", st)
     return out
+
+
+@functools.lru_cache(maxsize=512)
+def _prefix_views(dtypes, qs, qst, kps, kpst, vps, vpst, kos, kost, vos, vost, lens_dtype, lens_shape, os, ost):
+    """(type code, sizes, stride arrays, workspace bytes) of attention_shared_prefix's tensors, checked."""
+    if dtypes[0] not in _SIXTEEN_BIT:
+        raise TypeError(f"q must be fp16 or bf16, got {dtypes[0]}")
+    if len(set(dtypes)) > 1:
+        raise TypeError(f"q, K, V and out must share one dtype, got {dtypes}")
+    if len(qs) != 4 or len(kps) != 3 or len(kos) != 4:
+        raise ValueError("q is [B, n, heads, head_dim], the prefix [P, kv_heads, head_dim], the caches "
+                         "[B, room, kv_heads, head_dim]")
+    B, n, H, D = qs
+    P, Hkv = kps[:2]
+    room = kos[1]
+    if D not in GROUPED_HEAD_DIMS:
+        raise ValueError(f"head_dim {D} is not one of {GROUPED_HEAD_DIMS}")
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} K/V heads evenly")
+    if tuple(kps) != (P, Hkv, D) or vps != kps or tuple(kos) != (B, room, Hkv, D) or vos != kos:
+        raise ValueError(f"shape mismatch q={tuple(qs)} prefix={tuple(kps)}, {tuple(vps)} own={tuple(kos)}, {tuple(vos)}")
+    if lens_dtype != torch.int32 or tuple(lens_shape) != (B,):
+        raise ValueError(f"own_lens must be an int32 tensor of shape ({B},)")
+    if os is not None and os != qs:
+        raise ValueError(f"out must have q's shape {tuple(qs)}")
+    arrays = _Arrays(_rows_strides("q", qs, qst, 8), _rows_strides("k_prefix", kps, kpst, 8, 0),
+                     _rows_strides("v_prefix", vps, vpst, 8, 0), _rows_strides("k_own", kos, kost, 8, 1),
+                     _rows_strides("v_own", vos, vost, 8, 1),
+                     (n * H * D, H * D, D) if os is None else _rows_strides("out", os, ost, 4))
+    need = _lib.lib().mi355_attn_shared_prefix_workspace_bytes(B, n, H, Hkv, D, P, room)
+    if need < 0:
+        _lib.check("mi355_attn_shared_prefix_workspace_bytes", need)
+    return _lib.dtype_code(dtypes[0]), (B, n, H, Hkv, D, P, room), arrays, need
 
 
 def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
@@ -728,52 +787,37 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     ``own_lens`` is read by the kernels, so a captured graph follows its values; it is clamped to
     [0, room], and what a cache holds behind it does not matter. Types, head dims and roundings as
     ``attention_packed``. ``out`` must not share memory with the inputs. No backward pass."""
-    dev = _on_gpu(q, k_prefix, v_prefix, k_own, v_own, own_lens, out)
-    _no_grad(q, k_prefix, v_prefix, k_own, v_own)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be fp16 or bf16, got {q.dtype}")
-    for name, t, dims in (("q", q, 4), ("k_prefix", k_prefix, 3), ("v_prefix", v_prefix, 3),
-                          ("k_own", k_own, 4), ("v_own", v_own, 4)):
-        _rows_view(name, t, dims, q.dtype, 8)
-    B, n, H, D = q.shape
-    P, Hkv = k_prefix.shape[:2]
-    room = k_own.shape[1]
-    if D not in GROUPED_HEAD_DIMS:
-        raise ValueError(f"head_dim {D} is not one of {GROUPED_HEAD_DIMS}")
-    if H == 0 or Hkv == 0 or H % Hkv:
-        raise ValueError(f"{H} query heads cannot share {Hkv} K/V heads evenly")
-    if (tuple(k_prefix.shape) != (P, Hkv, D) or v_prefix.shape != k_prefix.shape
-            or tuple(k_own.shape) != (B, room, Hkv, D) or v_own.shape != k_own.shape):
-        raise ValueError(f"shape mismatch q={tuple(q.shape)} prefix={tuple(k_prefix.shape)}, "
-                         f"{tuple(v_prefix.shape)} own={tuple(k_own.shape)}, {tuple(v_own.shape)}")
-    if own_lens.dtype != torch.int32 or tuple(own_lens.shape) != (B,) or not own_lens.is_contiguous():
-        raise ValueError(f"own_lens must be a contiguous int32 tensor of shape ({B},)")
-    scale = _scale(scale, D)
-    if out is None:
-        out = torch.empty((B, n, H, D), device=dev, dtype=q.dtype)
+    dev = q.get_device()
+    given = out is not None
+    if dev < 0 or k_prefix.get_device() != dev or v_prefix.get_device() != dev or k_own.get_device() != dev or (
+            v_own.get_device() != dev or own_lens.get_device() != dev or (given and out.get_device() != dev)):
+        _on_gpu(q, k_prefix, v_prefix, k_own, v_own, own_lens, out)
+    if torch.is_grad_enabled():
+        _no_backward(q, k_prefix, v_prefix, k_own, v_own)
+    dt = q.dtype
+    dtypes = (dt, k_prefix.dtype, v_prefix.dtype, k_own.dtype, v_own.dtype)
+    code, sizes, strides, need = _prefix_views(
+        dtypes + (out.dtype,) if given else dtypes, q.shape, q.stride(), k_prefix.shape, k_prefix.stride(),
+        v_prefix.shape, v_prefix.stride(), k_own.shape, k_own.stride(), v_own.shape, v_own.stride(),
+        own_lens.dtype, own_lens.shape, out.shape if given else None, out.stride() if given else None)
+    if not own_lens.is_contiguous():
+        raise ValueError("own_lens must be contiguous")
+    scale = _scale(scale, sizes[4])
+    if given:
+        _check_apart(out, q, k_prefix, v_prefix, k_own, v_own, own_lens)
     else:
-        _rows_view("out", out, 4, q.dtype, 4)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have q's shape {tuple(q.shape)}")
-        if _overlaps(out, q, k_prefix, v_prefix, k_own, v_own):
-            raise ValueError("out shares memory with an input")
+        out = torch.empty(q.shape, device=q.device, dtype=dt)
     if out.numel() == 0:
         return out
-    L = _lib.lib()
-    need = L.mi355_attn_shared_prefix_workspace_bytes(B, n, H, Hkv, D, P, room)
-    if need < 0:
-        _lib.check("mi355_attn_shared_prefix_workspace_bytes", need)
-    i64 = _lib.i64_array
-    with _on_device(dev):
-        ws = torch.empty((max(need, 16),), device=dev, dtype=torch.uint8)
-        st = L.mi355_attn_shared_prefix(
-            _lib.dtype_code(q.dtype), q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(),
-            k_own.data_ptr(), v_own.data_ptr(), own_lens.data_ptr(), out.data_ptr(), B, n, H, Hkv, D, P,
-            room, i64(_whole(q, q.stride()[:3])), i64(_kv_strides("k_prefix", k_prefix, 0)),
-            i64(_kv_strides("v_prefix", v_prefix, 0)), i64(_kv_strides("k_own", k_own, 1)),
-            i64(_kv_strides("v_own", v_own, 1)), i64(_whole(out, out.stride()[:3])), scale,
-            ws.data_ptr(), need, _stream(q))
-    _lib.check("mi355_attn_shared_prefix", st)
+    qp, op = q.data_ptr(), out.data_ptr()
+    kp, vp, ko, vo = k_prefix.data_ptr(), v_prefix.data_ptr(), k_own.data_ptr(), v_own.data_ptr()
+    if (qp | kp | vp | ko | vo) & 15 or op & 7:
+        _check_aligned(q=qp, k_prefix=kp, v_prefix=vp, k_own=ko, v_own=vo, out=op)
+    ws = torch.empty((max(need, 16),), device=q.device, dtype=torch.uint8)
+    st = _launch(dev, _lib.lib().mi355_attn_shared_prefix, code, qp, kp, vp, ko, vo, own_lens.data_ptr(), op,
+                 *sizes, *strides, scale, ws.data_ptr(), need)
+    if st:
+        _lib.check("mi355_attn_shared_prefix", st)
     return out
 
 
@@ -787,7 +831,7 @@ def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
     ``w ~ scale[n, k / group] (q[n, k] - zero[n, k / group])``, q two to a byte (even k in the low
     half) ``[N, K / 2]`` uint8, scale of w's type. Each group's range (0 included) goes to 0 .. 15, or with
     ``symmetric`` its largest magnitude to +-7 around 8 (zero is None). Run once per weight."""
-    if w.dim() != 2 or w.dtype not in (torch.float16, torch.bfloat16):
+    if w.dim() != 2 or w.dtype not in _SIXTEEN_BIT:
         raise ValueError("quant_groups_i4 expects a 2-D fp16 or bf16 weight")
     if group not in I4_GROUPS or w.shape[1] % group:
         raise ValueError(f"group must be one of {I4_GROUPS} and divide K = {w.shape[1]}")
@@ -806,6 +850,38 @@ def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
         return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scale, zero
 
 
+@functools.lru_cache(maxsize=512)
+def _i4_views(xd, xs, xst, wd, ws, sd, ss, zd, zs, bd, bs, odt, os, ost):
+    """(type codes, M, N, K, group, ldx, ldy) of linear_i4's tensors, checked."""
+    if xd not in _SIXTEEN_BIT:
+        raise TypeError(f"x must be fp16 or bf16, got {xd}")
+    if len(xs) != 2 or len(ws) != 2 or len(ss) != 2:
+        raise ValueError("linear_i4 expects 2-D x, w and scale")
+    (M, K), N = xs, ws[0]
+    if wd != torch.uint8 or ws[1] * 2 != K:
+        raise ValueError(f"w must be a uint8 tensor of shape (N, {K // 2}) for K = {K}, got {tuple(ws)}")
+    group = K // ss[1] if ss[1] else 0
+    if group not in I4_GROUPS or tuple(ss) != (N, K // group) or K % group:
+        raise ValueError(f"scale must be [N, K / group] with a group of {I4_GROUPS}, got {tuple(ss)}")
+    if sd != xd:
+        raise TypeError(f"scale is {sd}, x is {xd}")
+    if zs is not None and (zd != torch.uint8 or zs != ss):
+        raise ValueError("zero must be a uint8 tensor of scale's shape")
+    if bs is not None and (tuple(bs) != (N,) or bd != torch.float32):
+        raise ValueError(f"bias must be an fp32 tensor of shape ({N},)")
+    ldx = xst[0] if M > 1 else (K + 7) // 8 * 8
+    if M and (xst[1] != 1 or ldx < K or ldx % 8):
+        raise ValueError("x needs unit column stride and a row stride that is a multiple of 8 and holds a row")
+    if odt not in (xd, torch.float32):
+        raise TypeError(f"out_dtype must be {xd} or float32, got {odt}")
+    ldy = N
+    if os is not None:
+        if tuple(os) != (M, N) or (M and N > 1 and ost[1] != 1) or (M > 1 and ost[0] < N):
+            raise ValueError("out must be [M, N] of out_dtype with unit column stride")
+        ldy = ost[0] if M > 1 else N
+    return _lib.dtype_code(xd), _lib.dtype_code(odt), M, N, K, group, ldx, ldy
+
+
 def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
               zero: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -816,47 +892,37 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     q two to a byte, the even k in the low half; ``scale`` ``[N, K / group]`` is of x's type, group 32,
     64 or 128; ``zero`` uint8 of scale's shape (None: 8); ``bias`` fp32 ``[N]``. Made for M of a few
     rows (the weights are read again for every 64). fp32 sums, the output (x's type, or fp32 with
-    ``out_dtype``) rounded once. bf16: |x| below 2^119. ``out`` must not share memory with ``x``.
-    No backward pass."""
-    dev = _on_gpu(x, w, scale, zero, bias, out)
-    _no_grad(x, scale, bias)
-    if x.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"x must be fp16 or bf16, got {x.dtype}")
-    if x.dim() != 2 or w.dim() != 2 or scale.dim() != 2:
-        raise ValueError("linear_i4 expects 2-D x, w and scale")
-    M, K = x.shape
-    N = w.shape[0]
-    if w.dtype != torch.uint8 or w.shape[1] * 2 != K or not w.is_contiguous():
-        raise ValueError(f"w must be a contiguous uint8 tensor of shape (N, {K // 2}) for K = {K}")
-    group = K // scale.shape[1] if scale.shape[1] else 0
-    if group not in I4_GROUPS or scale.shape != (N, K // group) or K % group:
-        raise ValueError(f"scale must be [N, K / group] with a group of {I4_GROUPS}, got {tuple(scale.shape)}")
-    if scale.dtype != x.dtype or not scale.is_contiguous():
-        raise ValueError("scale must be contiguous and of x's dtype")
-    if zero is not None and (zero.dtype != torch.uint8 or zero.shape != scale.shape or not zero.is_contiguous()):
-        raise ValueError("zero must be a contiguous uint8 tensor of scale's shape")
-    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous fp32 tensor of shape ({N},)")
-    ldx = x.stride(0) if M > 1 else (K + 7) // 8 * 8
-    if M and (x.stride(1) != 1 or ldx < K or ldx % 8 or x.data_ptr() % 16 or w.data_ptr() % 16):
-        raise ValueError("x needs unit column stride, a row stride of a multiple of 8 that holds a row, "
-                         "and x and w 16-byte aligned starts")
+    ``out_dtype``) rounded once. Infinities in x give NaN. ``out`` must not share memory with the
+    inputs. No backward pass."""
+    dev = x.get_device()
+    if dev < 0 or w.get_device() != dev or scale.get_device() != dev or (zero is not None and zero.get_device() != dev) \
+            or (bias is not None and bias.get_device() != dev) or (out is not None and out.get_device() != dev):
+        _on_gpu(x, w, scale, zero, bias, out)
+    if torch.is_grad_enabled():
+        _no_backward(x, scale, bias)
     odt = out_dtype or (out.dtype if out is not None else x.dtype)
-    if odt not in (x.dtype, torch.float32):
-        raise TypeError(f"out_dtype must be {x.dtype} or float32")
-    if out is None:
-        out = torch.empty((M, N), device=dev, dtype=odt)
-    elif out.shape != (M, N) or out.dtype != odt or (out.numel() and out.stride(1) != 1) \
-            or (M > 1 and out.stride(0) < N):
+    if out is not None and out.dtype != odt:
         raise ValueError("out must be [M, N] of out_dtype with unit column stride")
-    elif _overlaps(out, x, w, scale, zero, bias):
-        raise ValueError("out shares memory with an input")
-    if out.numel() == 0:
+    code, ocode, M, N, K, group, ldx, ldy = _i4_views(
+        x.dtype, x.shape, x.stride(), w.dtype, w.shape, scale.dtype, scale.shape,
+        *((zero.dtype, zero.shape) if zero is not None else (None, None)),
+        *((bias.dtype, bias.shape) if bias is not None else (None, None)), odt,
+        *((out.shape, out.stride()) if out is not None else (None, None)))
+    for name, t in (("w", w), ("scale", scale), ("zero", zero), ("bias", bias)):
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if out is None:
+        out = torch.empty((M, N), device=x.device, dtype=odt)
+    else:
+        _check_apart(out, x, w, scale, zero, bias)
+    if M == 0 or N == 0:
         return out
-    with _on_device(dev):
-        st = _lib.lib().mi355_linear_i4(
-            _lib.dtype_code(x.dtype), _lib.dtype_code(odt), x.data_ptr(), ldx, w.data_ptr(), scale.data_ptr(),
-            zero.data_ptr() if zero is not None else 0, bias.data_ptr() if bias is not None else 0,
-            out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K, group, _stream(x))
-    _lib.check("mi355_linear_i4", st)
+    xp, wp = x.data_ptr(), w.data_ptr()
+    if (xp | wp) & 15:
+        _check_aligned(x=xp, w=wp)
+    st = _launch(dev, _lib.lib().mi355_linear_i4, code, ocode, xp, ldx, wp, scale.data_ptr(),
+                 0 if zero is None else zero.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                 out.data_ptr(), ldy, M, N, K, group)
+    if st:
+        _lib.check("mi355_linear_i4", st)
     return out
