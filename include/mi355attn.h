@@ -397,25 +397,28 @@ int mi355_block_head(int dtype, const void* X, int64_t ldx, const void* gamma, c
  * Scores and softmax statistics are fp32, probabilities are rounded to the input type before P·V,
  * outputs once. dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256.
  *
- * mi355_attn_packed_plan runs on the host: from the lengths it writes the tiles of rows (32-bit
- * words, 8 a tile, longest first) that mi355_attn_packed walks. With tiles == NULL it only gives
- * *n_tiles and *tile_rows; otherwise capacity (in tiles) must hold them. Copy the tiles to the
- * device and pass them with the same heads, kv_heads, head_dim, causal and tile_rows; they hold for
- * every call (layer) with these lengths. Sequences follow each other in Q / O (q_lens) and in
- * K / V (k_lens); tokens behind the last one are not touched. Lengths may be 0; tokens in all
- * below 2^30.
+ * mi355_attn_packed_plan runs on the host: from the lengths it writes the work that
+ * mi355_attn_packed walks (32-bit words, 8 an entry: tiles of rows, longest first, split into ranges of
+ * keys where there are too few for the GPU, and what has to be joined again) and its sizes, counts[4]
+ * = {tiles of tile_rows rows, tiles of 32 rows, joins, partial rows}. With plan == NULL it only gives
+ * counts and *tile_rows; otherwise capacity (in entries) must hold the first three. Copy the plan to
+ * the device and pass it with the same heads, kv_heads, head_dim, causal, counts (on the host) and
+ * tile_rows; it holds for every call (layer) with these lengths. workspace (16-byte aligned) holds
+ * counts[3] * kv_heads * (head_dim + 2) * 4 bytes, NULL when there is nothing to join; calls that share
+ * one must be stream-ordered. Sequences follow each other in Q / O (q_lens) and in K / V (k_lens);
+ * tokens behind the last one are not touched. Lengths may be 0; tokens in all below 2^30.
  * Strides are {token, head} in elements, the head_dim stride is 1: Q, K, V multiples of 8 with
  * 16-byte aligned bases, O of 4 with an 8-byte aligned base; token strides of K and V at least
  * head_dim. scale must be positive and finite.
  */
 int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_lens, int64_t n_seqs,
                            int64_t heads, int64_t kv_heads, int64_t head_dim, int causal,
-                           int32_t* tiles, int64_t capacity, int64_t* n_tiles, int32_t* tile_rows);
+                           int32_t* plan, int64_t capacity, int64_t* counts, int32_t* tile_rows);
 int mi355_attn_packed(int dtype, const void* Q, const void* K, const void* V, void* O,
                       int64_t heads, int64_t kv_heads, int64_t head_dim, const int64_t* q_strides,
                       const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
-                      float scale, int causal, const int32_t* tiles, int64_t n_tiles,
-                      int32_t tile_rows, void* stream);
+                      float scale, int causal, const int32_t* plan, const int64_t* counts,
+                      int32_t tile_rows, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Attention of B sequences' n_q newest tokens (1 when generating) against a prefix of prefix_len

@@ -15,39 +15,64 @@ BAD_SIZE, NULL, DTYPE, ALIGN, HEAD, UNSUP = -2, -1, -3, -4, -5, -6
 def plan(q_lens, k_lens, heads=4, kv_heads=2, head_dim=64, causal=1):
     n = len(q_lens)
     arr = C.c_int32 * max(1, n)
-    count, rows = C.c_int64(0), C.c_int32(0)
+    counts, rows = _lib.i64_array((0, 0, 0, 0)), C.c_int32(0)
     args = (arr(*q_lens), arr(*k_lens), n, heads, kv_heads, head_dim, causal)
-    st = _lib.lib().mi355_attn_packed_plan(*args, 0, 0, C.byref(count), C.byref(rows))
+    st = _lib.lib().mi355_attn_packed_plan(*args, 0, 0, counts, C.byref(rows))
     if st:
-        return st, None, 0
-    tiles = torch.empty(count.value, 8, dtype=torch.int32)
-    if count.value:
-        assert _lib.lib().mi355_attn_packed_plan(*args, tiles.data_ptr(), count.value - 1, C.byref(count),
+        return st, None, counts, 0
+    entries = torch.empty(sum(counts[:3]), 8, dtype=torch.int32)
+    if entries.numel():
+        assert _lib.lib().mi355_attn_packed_plan(*args, entries.data_ptr(), len(entries) - 1, counts,
                                                  C.byref(rows)) == BAD_SIZE  # too small a buffer
-        st = _lib.lib().mi355_attn_packed_plan(*args, tiles.data_ptr(), count.value, C.byref(count), C.byref(rows))
-    return st, tiles, rows.value
+        st = _lib.lib().mi355_attn_packed_plan(*args, entries.data_ptr(), len(entries), counts, C.byref(rows))
+    return st, entries.tolist(), list(counts), rows.value
 
 
 @pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads", [
     ([5], [5], 4, 2), ([0, 3, 0, 900, 1], [4, 3, 0, 900, 77], 12, 4), ([4096] * 3, [5000, 4096, 100], 32, 8), ([], [], 1, 1),
-    ([1] * 200, list(range(200)), 8, 8)])
+    ([1] * 200, list(range(200)), 8, 8), ([1, 1], [70000, 3], 8, 1), ([40, 8, 1], [9000, 20000, 1000], 8, 2),
+    ([33, 32], [5000, 5000], 1, 1), ([500], [10], 4, 4), ([100, 1], [100, 512], 4, 2), ([100, 1], [100, 513], 4, 2)])
 @pytest.mark.parametrize("causal", [0, 1])
-def test_plan_covers_every_row_once_longest_first(q_lens, k_lens, heads, kv_heads, causal):
-    st, tiles, rows = plan(q_lens, k_lens, heads, kv_heads, causal=causal)
-    assert st == 0
+def test_plan_covers_every_row_and_key_once(q_lens, k_lens, heads, kv_heads, causal):
+    """Each row's visible keys are covered by ranges without gap or overlap, a tile in one range writes its
+    rows itself, the ranges of a split one have partial rows of their own that a join names; lists are
+    longest first."""
+    st, entries, (wide, narrow, joins, slots), rows = plan(q_lens, k_lens, heads, kv_heads, causal=causal)
+    assert st == 0 and len(entries) == wide + narrow + joins
     g = heads // kv_heads
-    want, q0, k0 = set(), 0, 0
+    few = [m for n, m in zip(q_lens, k_lens) if 0 < n * g <= 32]
+    limit = 0 if wide and len(few) * kv_heads <= 256 and max(few, default=0) <= 512 else 32  # rows of narrow tiles
+    tiles = {}
+    for i, (q0, q_len, k0, k_len, row0, k_begin, k_stop, slot) in enumerate(entries[:wide + narrow]):
+        tiles.setdefault((q0, q_len, k0, k_len, row0), []).append((k_begin, k_stop, slot))
+        assert (q_len * g > limit) == (i < wide)
+    for part in (entries[:wide], entries[wide:wide + narrow]):
+        keys = [t[6] - t[5] for t in part]
+        assert keys == sorted(keys, reverse=True)
+    joined = {(j[0], j[3]): j for j in entries[wide + narrow:]}
+    assert len(joined) == joins
+    want, used, q0, k0 = set(), [], 0, 0
     for n, m in zip(q_lens, k_lens):
-        want |= {(q0, n, k0, m, r) for r in range(0, n * g, rows)}
+        step = rows if n * g > limit else 32
+        for r in range(0, n * g, step):
+            want.add((q0, n, k0, m, r))
+            real = min(step, n * g - r)
+            last = (r + real - 1) // g
+            keys = max(0, min(m, last + m - n + 1)) if causal else m
+            ranges = sorted(tiles[(q0, n, k0, m, r)])
+            assert ranges[0][0] == 0 and ranges[-1][1] == keys
+            assert all(a[1] == b[0] for a, b in zip(ranges, ranges[1:]))
+            if len(ranges) == 1:
+                assert ranges[0][2] == -1 and (q0, r) not in joined
+            else:
+                assert all(a[0] < a[1] for a in ranges)
+                j = joined[(q0, r)]
+                assert j == [q0, n, m, r, real, ranges[0][2], len(ranges), 0]
+                assert [a[2] for a in ranges] == [j[5] + real * i for i in range(len(ranges))]
+                used += [x for a in ranges for x in range(a[2], a[2] + real)]
         q0, k0 = q0 + n, k0 + m
-    got = [tuple(t[:5]) for t in tiles.tolist()]
-    assert len(got) == len(want) and set(got) == want
-
-    def keys(t):
-        last = (min(t[4] + rows, t[1] * g) - 1) // g
-        return max(0, min(t[3], last + t[3] - t[1] + 1)) if causal else t[3]
-    order = [keys(t) for t in got]
-    assert order == sorted(order, reverse=True)
+    assert set(tiles) == want
+    assert sorted(used) == list(range(slots))
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -60,19 +85,21 @@ def test_plan_refusals(kw, status):
 
 
 def test_plan_null_pointers():
-    count, rows = C.c_int64(0), C.c_int32(0)
+    counts, rows = _lib.i64_array((0, 0, 0, 0)), C.c_int32(0)
     f = _lib.lib().mi355_attn_packed_plan
-    assert f(None, None, 1, 4, 2, 64, 1, 0, 0, C.byref(count), C.byref(rows)) == NULL
+    assert f(None, None, 1, 4, 2, 64, 1, 0, 0, counts, C.byref(rows)) == NULL
     assert f(None, None, 0, 4, 2, 64, 1, 0, 0, None, C.byref(rows)) == NULL
 
 
 PACKED = dict(dtype=F16, Q=64, K=64, V=64, O=64, heads=4, kv_heads=2, head_dim=64, qs=(256, 64), ks=(128, 64),
-              vs=(128, 64), os=(256, 64), scale=0.125, causal=1, tiles=64, n_tiles=3, tile_rows=32)
+              vs=(128, 64), os=(256, 64), scale=0.125, causal=1, tiles=64, counts=(3, 2, 1, 100), tile_rows=64,
+              ws=64, ws_bytes=100 * 2 * 66 * 4)
 
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=F32), DTYPE), (dict(dtype=9), DTYPE), (dict(heads=3), BAD_SIZE), (dict(kv_heads=0), BAD_SIZE),
-    (dict(n_tiles=-1), BAD_SIZE), (dict(n_tiles=1 << 31), BAD_SIZE), (dict(head_dim=40), HEAD), (dict(tile_rows=48), UNSUP),
+    (dict(counts=(-1, 0, 0, 0)), BAD_SIZE), (dict(counts=(1 << 30, 0, 0, 0)), BAD_SIZE), (dict(counts=None), NULL),
+    (dict(ws=0), NULL), (dict(ws=72), ALIGN), (dict(ws_bytes=100 * 2 * 66 * 4 - 1), BAD_SIZE), (dict(head_dim=40), HEAD), (dict(tile_rows=48), UNSUP),
     (dict(scale=0.0), UNSUP), (dict(scale=-1.0), UNSUP), (dict(scale=float("inf")), UNSUP), (dict(scale=float("nan")), UNSUP),
     (dict(Q=0), NULL), (dict(O=0), NULL), (dict(tiles=0), NULL), (dict(Q=72), ALIGN), (dict(K=68), ALIGN), (dict(V=8), ALIGN),
     (dict(O=68), ALIGN), (dict(qs=(257, 64)), ALIGN), (dict(ks=(132, 64)), ALIGN), (dict(vs=(128, 4)), ALIGN),
@@ -82,7 +109,8 @@ def test_packed_entry_refusals(kw, status):
     i64 = _lib.i64_array
     assert _lib.lib().mi355_attn_packed(
         a["dtype"], a["Q"], a["K"], a["V"], a["O"], a["heads"], a["kv_heads"], a["head_dim"], i64(a["qs"]), i64(a["ks"]),
-        i64(a["vs"]), i64(a["os"]), a["scale"], a["causal"], a["tiles"], a["n_tiles"], a["tile_rows"], None) == status
+        i64(a["vs"]), i64(a["os"]), a["scale"], a["causal"], a["tiles"], i64(a["counts"]) if a["counts"] else None,
+        a["tile_rows"], a["ws"], a["ws_bytes"], None) == status
 
 
 PREFIX = dict(dtype=F16, ptrs=[64] * 7, B=2, n=1, heads=4, kv_heads=2, head_dim=64, P=100, room=50, qs=(256, 256, 64),
@@ -132,7 +160,7 @@ def test_i4_entry_refusals(kw, status):
 
 def test_wrappers_refuse_cpu_tensors():
     q, k = torch.zeros(4, 4, 64, dtype=torch.float16), torch.zeros(4, 2, 64, dtype=torch.float16)
-    p = ops.PackedPlan(4, 4, 4, 2, 64, True, 32, 0, torch.zeros(0, 8, dtype=torch.int32))
+    p = ops.PackedPlan(4, 4, 4, 2, 64, True, 64, _lib.i64_array((0, 0, 0, 0)), torch.zeros(0, 8, dtype=torch.int32), 0)
     with pytest.raises(ValueError, match="GPU"):
         ops.attention_packed(q, k, k, p)
     with pytest.raises(ValueError, match="GPU"):

@@ -85,7 +85,7 @@ def run_packed(gpu, dtype, q_lens, k_lens, H, Hkv, D, causal, seed=1, scale=None
     plan = ops.packed_plan(q_lens, k_lens, heads=H, kv_heads=Hkv, head_dim=D, causal=causal, device=gpu)
     out = ops.attention_packed(q.to(gpu), k.to(gpu), v.to(gpu), plan, scale=scale)
     ref, tol = packed64(q, k, v, q_lens, k_lens, causal, scale or D ** -0.5)
-    check(f"packed {dtype} D={D} H={H}/{Hkv} q={q_lens} k={k_lens} causal={causal} rows={plan.tile_rows}", out, ref, tol)
+    check(f"packed {dtype} D={D} H={H}/{Hkv} q={q_lens} k={k_lens} causal={causal} counts={list(plan.counts)}", out, ref, tol)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -116,7 +116,8 @@ def test_packed_lengths(gpu, dtype, q_lens, k_lens, causal):
 
 
 @pytest.mark.parametrize("dtype,D,H,Hkv", [(torch.bfloat16, 128, 16, 4), (torch.float16, 64, 24, 8), (torch.float16, 256, 16, 8),
-                                          (torch.bfloat16, 80, 16, 16)])
+                                          (torch.bfloat16, 80, 16, 16), (torch.float16, 16, 16, 8), (torch.bfloat16, 32, 16, 8),
+                                          (torch.float16, 48, 16, 8), (torch.float16, 96, 16, 8), (torch.bfloat16, 192, 16, 8)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_packed_large_tiles(gpu, dtype, D, H, Hkv, causal):
     """Enough rows for the large tiles, tiles that end inside a sequence's rows and keys."""
@@ -124,7 +125,7 @@ def test_packed_large_tiles(gpu, dtype, D, H, Hkv, causal):
     k_lens = [1025, 1003, 66, 511]
     ops = _ops()
     plan = ops.packed_plan(q_lens * 4, k_lens * 4, heads=H, kv_heads=Hkv, head_dim=D, causal=causal, device=gpu)
-    assert plan.tile_rows > 32
+    assert plan.tile_rows == 128
     q, k, v = (_rand((sum(n) * 4, h, D), dtype, 20 + i) for i, (n, h) in enumerate([(q_lens, H), (k_lens, Hkv), (k_lens, Hkv)]))
     out = ops.attention_packed(q.to(gpu), k.to(gpu), v.to(gpu), plan).cpu()
     # a head of each group of the first and the last sequences
@@ -136,6 +137,42 @@ def test_packed_large_tiles(gpu, dtype, D, H, Hkv, causal):
                 ref, tol = attention64(q[q0:q0 + n, h], k[k0:k0 + m, h * Hkv // H], v[k0:k0 + m, h * Hkv // H], last, D ** -0.5)
                 check(f"sequence {i} head {h}", out[q0:q0 + n, h], ref, tol)
         q0, k0 = q0 + n, k0 + m
+
+
+@pytest.mark.parametrize("D", [16, 64, 80, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_lens,k_lens", [
+    ([1], [20001]),                      # one token, many ranges
+    ([3, 1, 2], [5000, 1, 0]),           # few rows, split and whole, one without keys
+    ([70], [4001]),                      # wide tiles in ranges; the last rows' range reaches furthest
+    ([90, 2, 200], [3000, 2500, 150]),   # both lists; more tokens than keys
+])
+def test_packed_split_keys(gpu, dtype, D, q_lens, k_lens):
+    """Few rows against many keys: tiles in ranges of keys that are joined, also where causal rows end
+    before a range."""
+    ops = _ops()
+    assert ops.packed_plan(q_lens, k_lens, heads=4, kv_heads=2, head_dim=D, device=gpu).counts[2] > 0
+    run_packed(gpu, dtype, q_lens, k_lens, 4, 2, D, True, seed=17)
+    run_packed(gpu, dtype, q_lens, k_lens, 4, 2, D, False, seed=18)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_packed_split_what_a_row_does_not_see(gpu, bad):
+    """... and a later token's not-finite K and V, in a range that some rows of the tile see nothing of."""
+    ops = _ops()
+    n, m, H, D = 40, 4000, 4, 64
+    q, k, v = _rand((n, H, D), torch.float16, 71), _rand((m, 2, D), torch.float16, 72), _rand((m, 2, D), torch.float16, 73)
+    plan = ops.packed_plan([n], [m], heads=H, kv_heads=2, head_dim=D, device=gpu)
+    assert plan.counts[2] > 0
+    ref, tol = packed64(q, k, v, [n], [m], True, D ** -0.5)
+    k[m - 1, :, 0], v[m - 1] = bad, bad
+    out = ops.attention_packed(q.to(gpu), k.to(gpu), v.to(gpu), plan).cpu()
+    check("rows before it", out[:n - 1], ref[:n - 1], tol[:n - 1])
+    assert not bool(torch.isfinite(out[n - 1]).any())
+    k[:], v[m - 1] = 0, 0  # every score of the first rows' keys -inf: NaN
+    k[:, :, 0] = -math.inf
+    out = ops.attention_packed(torch.ones_like(q).to(gpu), k.to(gpu), v.to(gpu), plan).cpu()
+    assert bool(torch.isnan(out).all())
 
 
 @pytest.mark.parametrize("scale", [0.02, 1.0, 6.0])

@@ -112,7 +112,8 @@ _SIGNATURES = {
     "mi355_attn_packed": (
         C.c_int,
         [C.c_int, _P, _P, _P, _P, _I64, _I64, _I64, C.POINTER(_I64), C.POINTER(_I64),
-         C.POINTER(_I64), C.POINTER(_I64), C.c_float, C.c_int, _P, _I64, C.c_int32, _P],
+         C.POINTER(_I64), C.POINTER(_I64), C.c_float, C.c_int, _P, C.POINTER(_I64), C.c_int32, _P, _I64,
+         _P],
     ),
     "mi355_attn_shared_prefix_workspace_bytes": (_I64, [_I64] * 7),
     "mi355_attn_shared_prefix": (

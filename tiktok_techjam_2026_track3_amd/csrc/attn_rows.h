@@ -18,12 +18,13 @@ namespace rows {
 
 enum Mode { PACKED = 0, PREFIX = 1, OWN = 2 };
 
-// One tile of rows of one packed sequence (mi355_attn_packed_plan writes them).
+// Work on one tile of rows of one packed sequence (mi355_attn_packed_plan writes them).
 struct PackedTile {
-  int32_t q0, q_len;  // the sequence's first token in q and its tokens
-  int32_t k0, k_len;  // ... in k / v
-  int32_t row0;       // first row of the tile: token row0 / G, head row0 % G of the group
-  int32_t pad[3];
+  int32_t q0, q_len;        // the sequence's first token in q and its tokens
+  int32_t k0, k_len;        // ... in k / v
+  int32_t row0;             // first row of the tile: token row0 / G, head row0 % G of the group
+  int32_t k_begin, k_stop;  // the range of its keys, of which it takes what its rows see
+  int32_t slot;             // first row of its partial result; -1: the range is all there is
 };
 static_assert(sizeof(PackedTile) == 32, "plan entry");
 
@@ -39,6 +40,7 @@ struct Args {
   // PACKED
   const PackedTile* tiles;
   int32_t causal;
+  int64_t slots;          // partial rows of a K/V head: row (h slots + slot + i) of part / ml
   // PREFIX / OWN: rows of a sequence are its n_q tokens' heads
   int32_t B, n_q;
   int32_t keys;           // PREFIX: prefix keys; OWN: keys a cache has room for
@@ -46,8 +48,8 @@ struct Args {
   int32_t chunk;          // keys of a split
   int32_t splits, row_tiles;
   int32_t part0;          // first split's index in part / ml
-  float* part;            // [splits][B n_q H][HD], unnormalised
-  float* ml;              // [splits][B n_q H][2]: mu (-inf: no key seen), sum
+  float* part;            // partial rows [HD], unnormalised; PREFIX / OWN: [splits][B n_q H]
+  float* ml;              // their mu (-inf: no key seen) and sum
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -55,10 +57,6 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 MI355_DEVINL f32x4 mma32(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 MI355_DEVINL f32x4 mma32(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-MI355_DEVINL f32x4 mma16(f16x4 a, f16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
-MI355_DEVINL f32x4 mma16(bf16x4 a, bf16x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
-}
 // sum of a fragment's probabilities, as rounded
 MI355_DEVINL float prob_sum(f16x8 f, float acc) {
   const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
@@ -108,8 +106,11 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   static_assert(HD % 16 == 0 && BN % 32 == 0, "shape");
   constexpr int QW = 16 * QG, BM = NW * QW;
   constexpr int NCH = HD / 8, ROWB = HD * 2;
-  constexpr int KS = HD / 32;              // 32-element MFMA steps of S^T
-  constexpr bool HALF = HD % 32 != 0;      // and one of 16
+  // MFMA steps of S^T, 32 elements each; of HD 16, 48 and 80 the last one's upper half is zeros in both
+  // operands. (A 16x16x16 MFMA for it, accumulating onto the 16x16x32 right before it, lost two of its four
+  // results: the compiler leaves no wait states between the two.)
+  constexpr int KS = (HD + 31) / 32;
+  constexpr bool HALF = HD % 32 != 0;
   constexpr int DT = HD / 16, KT = BN / 16;
   static_assert(BN * NCH % 64 == 0, "whole blocks of loads");
   constexpr int BLK = BN * NCH / 64, LPW = (BLK + NW - 1) / NW, TILE = BN * NCH;
@@ -122,18 +123,20 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   // the work-group's rows [row0, nrows) of a sequence (or of the batch), its K/V head and keys
   int h, row0, nrows, k_begin, k_end, k_off, split = 0, b = 0;
   const T *Qb, *Kb, *Vb;
-  int64_t out_tok = 0;
+  int64_t out_tok = 0, slot = -1;
   if constexpr (MODE == PACKED) {
     h = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.Hkv));
     const PackedTile t = p.tiles[blockIdx.x / static_cast<unsigned>(p.Hkv)];
     row0 = t.row0;
     nrows = t.q_len * p.G;
-    k_begin = 0;
+    k_begin = t.k_begin;
     // key j is seen by token i when j < i + k_off (causal), j < k_len
     k_off = p.causal ? t.k_len - t.q_len + 1 : 0x40000000;
     const int last = (row0 + BM < nrows ? row0 + BM : nrows) - 1;
     const int lim = last / p.G + k_off;
-    k_end = lim < t.k_len ? (lim > 0 ? lim : 0) : t.k_len;
+    k_end = lim < t.k_stop ? lim : t.k_stop;
+    k_end = k_end > k_begin ? k_end : k_begin;
+    if (t.slot >= 0) slot = h * p.slots + t.slot;
     Qb = static_cast<const T*>(p.q) + t.q0 * p.qt;
     Kb = static_cast<const T*>(p.k) + t.k0 * p.kt + h * p.kh;
     Vb = static_cast<const T*>(p.v) + t.k0 * p.vt + h * p.vh;
@@ -188,10 +191,21 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
     return lim < n_keys ? lim : n_keys;
   };
 
+  // row r's partial result
+  const auto part_of = [&](int r) MI355_LAMBDA_INLINE {
+    if constexpr (MODE == PACKED) {
+      return slot + (r - row0);
+    } else {
+      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+      return (static_cast<int64_t>(p.part0 + split) * p.B * p.n_q + (MODE == OWN ? static_cast<int64_t>(b) * p.n_q : 0) + t) * p.H + hh;
+    }
+  };
+
   // Q^T fragments: lane (row l16 of group n, slice g) holds elements 32 s + 8 g ..
-  frag qf[QG][KS > 0 ? KS : 1];
-  frag4 qh[QG];
+  frag qf[QG][KS];
   int lim[QG];
+  const bool upper = HALF && g >= 2;
+  const auto lower_half = [&](u32x4 v) MI355_LAMBDA_INLINE { return upper ? u32x4{0u, 0u, 0u, 0u} : v; };
 #pragma unroll
   for (int n = 0; n < QG; ++n) {
     const int r = row_w + 16 * n + l16;
@@ -199,8 +213,11 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
     const T* src = Qb + q_of(real ? r : nrows - 1);
     lim[n] = lim_of(real ? r : nrows - 1);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = __builtin_bit_cast(frag, *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * g));
-    if constexpr (HALF) qh[n] = __builtin_bit_cast(frag4, *reinterpret_cast<const u32x2*>(src + 32 * KS + 4 * g));
+    for (int s = 0; s < KS; ++s) {
+      const bool half = HALF && s == KS - 1;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * (half ? g & 1 : g));
+      qf[n][s] = __builtin_bit_cast(frag, half ? lower_half(v) : v);
+    }
   }
   const int lim_first = MODE == PREFIX ? n_keys : __builtin_amdgcn_readfirstlane(lim[0]);
   const int lim_last = MODE == PREFIX ? n_keys : lim_of(row_w + QW - 1 < nrows ? row_w + QW - 1 : nrows - 1);
@@ -243,12 +260,11 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   for (int i = 0; i < VV; ++i)
     v_at[i] = (4 * g + ve) * ROWB + ((2 * i + (vq >> 1)) ^ swz<NCH>(4 * g + ve)) * 16 + (vq & 1) * 8;
   auto kfrag = [&](int st, int kt, int s) MI355_LAMBDA_INLINE {
+    if (HALF && s == KS - 1)  // (rows of 2, 6, 10 chunks: no swizzle)
+      return __builtin_bit_cast(frag, lower_half(*reinterpret_cast<const u32x4*>(
+          ldsb + st * TILE * 16 + (16 * kt + l16) * ROWB + s * 64 + (g & 1) * 16)));
     return __builtin_bit_cast(frag, *reinterpret_cast<const u32x4*>(
         ldsb + st * TILE * 16 + 16 * kt * ROWB + s / KV * (KV * 64) + k_at[s % KV]));
-  };
-  auto khalf = [&](int st, int kt) MI355_LAMBDA_INLINE {  // (rows of 2, 6, 10 chunks: no swizzle)
-    return __builtin_bit_cast(frag4, *reinterpret_cast<const u32x2*>(
-        ldsb + st * TILE * 16 + (16 * kt + l16) * ROWB + KS * 64 + g * 8));
   };
   auto vfrag = [&](int st, int t, int dt) MI355_LAMBDA_INLINE {
     const char* base = ldsb + (RING + st) * TILE * 16 + 32 * t * ROWB + dt / VV * (VV * 32) + v_at[dt % VV];
@@ -280,11 +296,6 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
         const frag kf = kfrag(st, kt, x);
 #pragma unroll
         for (int n = 0; n < QG; ++n) s[n][kt] = mma32(kf, qf[n][x], s[n][kt]);
-      }
-      if constexpr (HALF) {
-        const frag4 kf = khalf(st, kt);
-#pragma unroll
-        for (int n = 0; n < QG; ++n) s[n][kt] = mma16(kf, qh[n], s[n][kt]);
       }
     }
     if (k0 + BN > lim_first) {  // the tile crosses a row's last key
@@ -377,7 +388,7 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
     const float sum = row_sum(lsum[n]);
     bool bad = false;
     if (r < nrows) {
-      if constexpr (MODE == PACKED) {
+      if (MODE == PACKED && slot < 0) {
         const int t = r / p.G, hh = h * p.G + (r - t * p.G);
         T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
         // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
@@ -394,9 +405,7 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
           *reinterpret_cast<frag4*>(dst + 16 * dt + 4 * g) = w;
         }
       } else {
-        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
-        const int64_t at = static_cast<int64_t>(p.part0 + split) * p.B * p.n_q * p.H +
-                           (static_cast<int64_t>(MODE == OWN ? b * p.n_q : 0) + t) * p.H + hh;
+        const int64_t at = part_of(r);
         float* dst = p.part + at * HD;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -452,15 +461,14 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
             if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
           m = m2;
         }
-        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
-        if constexpr (MODE == PACKED) {
+        if (MODE == PACKED && slot < 0) {
+          const int t = r / p.G, hh = h * p.G + (r - t * p.G);
           T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
 #pragma unroll
           for (int i = 0; i < DL; ++i)
             if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
         } else {
-          const int64_t at = static_cast<int64_t>(p.part0 + split) * p.B * p.n_q * p.H +
-                             (static_cast<int64_t>(b) * p.n_q + t) * p.H + hh;
+          const int64_t at = part_of(r);
 #pragma unroll
           for (int i = 0; i < DL; ++i)
             if (lane + 64 * i < HD) p.part[at * HD + lane + 64 * i] = acc[i];

@@ -636,8 +636,9 @@ class PackedPlan:
     head_dim: int
     causal: bool
     tile_rows: int
-    n_tiles: int
+    counts: ctypes.Array  # tiles of tile_rows rows, of 32 rows, joins, partial rows
     tiles: torch.Tensor
+    workspace_bytes: int
 
 
 def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, heads: int,
@@ -663,22 +664,22 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
     n = len(q_lens)
     arr = ctypes.c_int32 * max(n, 1)
     ql, kl = arr(*q_lens), arr(*k_lens)
-    count, rows = ctypes.c_int64(0), ctypes.c_int32(0)
+    counts, rows = _lib.i64_array((0, 0, 0, 0)), ctypes.c_int32(0)
 
     def plan(tiles: int, capacity: int) -> None:
         st = _lib.lib().mi355_attn_packed_plan(ql, kl, n, heads, kv_heads, head_dim, int(causal), tiles,
-                                               capacity, ctypes.byref(count), ctypes.byref(rows))
+                                               capacity, counts, ctypes.byref(rows))
         _lib.check("mi355_attn_packed_plan", st)
 
     plan(0, 0)
-    tiles = torch.empty((count.value, 8), dtype=torch.int32)
-    if count.value:
-        plan(tiles.data_ptr(), count.value)
+    tiles = torch.empty((sum(counts[:3]), 8), dtype=torch.int32)
+    if tiles.numel():
+        plan(tiles.data_ptr(), tiles.shape[0])
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     on_gpu = tiles.to(device)  # (from pageable memory: there when this returns, for every stream)
     return PackedPlan(sum(q_lens), sum(k_lens), heads, kv_heads, head_dim, bool(causal), rows.value,
-                      count.value, on_gpu)
+                      counts, on_gpu, counts[3] * kv_heads * (head_dim + 2) * 4)
 
 
 @functools.lru_cache(maxsize=512)
@@ -727,14 +728,16 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
         _check_apart(out, q, k, v)
     else:  # (rows behind the last token have no value)
         out = (torch.empty if q.shape[0] == plan.q_tokens else torch.zeros)(q.shape, device=q.device, dtype=q.dtype)
-    if plan.n_tiles == 0:
+    if plan.tiles.shape[0] == 0:
         return out
     qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if (qp | kp | vp) & 15 or op & 7:
         _check_aligned(q=qp, k=kp, v=vp, out=op)
+    need = plan.workspace_bytes
+    ws = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
     st = _launch(dev, _lib.lib().mi355_attn_packed, code, qp, kp, vp, op, plan.heads, plan.kv_heads,
-                 plan.head_dim, qst, kst, vst, ost, scale, plan.causal, plan.tiles.data_ptr(), plan.n_tiles,
-                 plan.tile_rows)
+                 plan.head_dim, qst, kst, vst, ost, scale, plan.causal, plan.tiles.data_ptr(), plan.counts,
+                 plan.tile_rows, ws.data_ptr() if need else 0, need)
     if st:
         _lib.check("mi355_attn_packed", st)
     return out
