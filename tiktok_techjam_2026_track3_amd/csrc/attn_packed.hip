@@ -16,7 +16,7 @@ bool packed_head_dim(int64_t hd) {
 
 constexpr int64_t MAX_TOKENS = int64_t(1) << 30;
 
-// Rows of a tile. Sequences of up to 32 rows (a token or a few) take NARROW ones, a wave each; the others
+// Rows of a tile. Sequences of up to 32 rows (a token or a few) take NARROW ones, whose keys four waves share out; the others
 // WIDE ones of four waves, two groups of 16 rows each, where those give every CU two work-groups, else
 // of one group (HALF). Measured (TFLOP/s; 8192 tokens with 32/8 heads of 128, 24 prompts of 33-2011 with 32/4
 // heads of 128, 8 pieces of 200-512 tokens against up to 5500 keys, 16 heads of 64 (416 WIDE tiles)):
@@ -35,19 +35,25 @@ struct Join {
 };
 static_assert(sizeof(Join) == sizeof(rows::PackedTile), "plan entry");
 
+template <typename T, int HD, int QG, int BN, bool OWN_KEYS>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_rows_packed(rows::Args p) {
+  __shared__ u32x4 lds[rows::lds_chunks<HD, 4, BN, OWN_KEYS>()];
+  rows::attn_rows<T, HD, 4, QG, BN, OWN_KEYS, OWN_KEYS ? 2 : 1, rows::PACKED>(p, lds, blockIdx.x);
+}
+
 template <typename T, int HD>
 int launch_hd(const rows::Args& a, const Counts& n, int wide_rows, hipStream_t s) {
   if (n.wide > 0) {
     const dim3 grid(static_cast<unsigned>(n.wide * a.Hkv));
     if (wide_rows == WIDE)
-      hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 4, 2, 32, 2, HD <= 128 ? 2 : 1, 1, rows::PACKED>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((attn_rows_packed<T, HD, 2, 32, false>), grid, dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 4, 1, HD <= 64 ? 64 : 32, 2, HD <= 128 ? 2 : 1, 1, rows::PACKED>), grid, dim3(256), 0, s, a);
+      hipLaunchKernelGGL((attn_rows_packed<T, HD, 1, HD <= 64 ? 64 : 32, false>), grid, dim3(256), 0, s, a);
   }
   if (n.narrow > 0) {
     rows::Args b = a;
     b.tiles += n.wide;
-    hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 1, 2, 32, 2, 1, 2, rows::PACKED>), dim3(static_cast<unsigned>(n.narrow * a.Hkv)), dim3(64), 0, s, b);
+    hipLaunchKernelGGL((attn_rows_packed<T, HD, 2, 32, true>), dim3(static_cast<unsigned>(n.narrow * a.Hkv)), dim3(256), 0, s, b);
   }
   return static_cast<int>(hipGetLastError());
 }
@@ -182,9 +188,8 @@ extern "C" int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_le
   Counts n{};
   try {
     // Tiles, then ranges of their keys where the tiles alone leave CUs idle: as many as fill the work-groups
-    // that run at once (two of four waves a CU; five of one wave, which is what 32 KB of LDS leave at head
-    // dim 128), each of a like share of all keys, but not so short that writing and reading a range's
-    // partial rows outweighs reading its keys.
+    // that run at once (two a CU), each of a like share of all keys, but not so short that writing and
+    // reading a range's partial rows outweighs reading its keys.
     int64_t keys_of[2] = {0, 0}, tiles_of[2] = {0, 0};
     const auto visit = [&](auto&& each) {
       int64_t q0 = 0, k0 = 0;
@@ -213,7 +218,7 @@ extern "C" int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_le
     });
     int64_t chunk[2];
     for (int w = 0; w < 2; ++w) {
-      const int64_t at_once = w ? 1280 : 512, least = w ? 128 : 512;
+      const int64_t at_once = 512, least = w ? 256 : 512;
       const int64_t share = ceil_div(ceil_div(keys_of[w] * kv_heads, at_once), 64) * 64;
       chunk[w] = tiles_of[w] * kv_heads >= at_once ? MAX_TOKENS : std::max(least, share);
     }

@@ -23,7 +23,8 @@ struct Split {
 };
 
 // most splits of the prefix or of a cache, and of both together for one wave to join
-constexpr int MAX_SPLITS = 1280, WAVE_SPLITS = 16;
+constexpr int64_t MAX_SPLITS = 512;
+constexpr int WAVE_SPLITS = 16;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -31,13 +32,15 @@ Split split_of(const Shape& s) {
   Split d{};
   const int64_t G = s.H / s.Hkv, pr = s.B * s.n_q * G, orows = s.n_q * G;
   d.prefix_rows = pr <= 16 ? 16 : pr <= 32 ? 32 : pr <= 64 ? 64 : 128;
-  d.own_rows = orows <= 16 ? 16 : 32;
-  const auto chunk = [](int64_t keys, int64_t groups, int64_t want, int64_t least) {
-    const int64_t splits = std::max<int64_t>(1, want / std::max<int64_t>(1, groups));
-    return std::max(least, ceil_div(ceil_div(keys, splits), 64) * 64);
+  d.own_rows = orows <= 16 && d.prefix_rows != 32 ? 16 : 32;
+  // As many ranges as fill the work-groups that run at once (two a CU), half of them where the prefix is
+  // matrix work: each range writes partial rows, and the caches' ranges run beside it.
+  const auto chunk = [](int64_t keys, int64_t groups, int64_t want) {
+    const int64_t splits = std::min(MAX_SPLITS, std::max<int64_t>(1, want / std::max<int64_t>(1, groups)));
+    return std::max<int64_t>(256, ceil_div(ceil_div(keys, splits), 64) * 64);
   };
-  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows <= 32 ? MAX_SPLITS : 512, 128);
-  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, MAX_SPLITS, 128);
+  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows <= 64 ? 512 : 256);
+  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, 512);
   d.prefix_splits = ceil_div(s.prefix, d.prefix_chunk);
   d.own_splits = ceil_div(s.room, d.own_chunk);
   return d;
@@ -146,56 +149,54 @@ __global__ __launch_bounds__(256) void combine_splits(CombineArgs p) {
   *reinterpret_cast<t4*>(static_cast<T*>(p.o) + b * p.ob + t * p.ot + head * p.oh + 4 * x) = w;
 }
 
-template <typename T, int HD, int MODE>
-int launch_rows(const rows::Args& a, int tile_rows, int64_t blocks, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (tile_rows == 16)
-    hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 1, 1, 32, 2, 1, 2, MODE>), grid, dim3(64), 0, s, a);
-  else if (tile_rows == 32)
-    hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 1, 2, 32, 2, 1, 2, MODE>), grid, dim3(64), 0, s, a);
-  else if constexpr (MODE == rows::PREFIX) {
-    if (tile_rows == 64)
-      hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 4, 1, HD <= 128 ? 64 : 32, 2, 1, 2, MODE>), grid, dim3(256), 0, s, a);
-    else
-      hipLaunchKernelGGL((rows::attn_rows_kernel<T, HD, 4, 2, HD <= 128 ? 64 : 32, 2, HD <= 128 ? 2 : 1, 1, MODE>), grid, dim3(256), 0, s, a);
-  }
-  return static_cast<int>(hipGetLastError());
+// Both kinds of range in one launch, the prefix's (matrix work, where the batch is large) first, so that the
+// caches' (memory) run beside them. PR, OR: rows of a prefix and of a cache work-group.
+template <typename T, int HD, int PR, int OR>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_rows_prefix(rows::Args a, rows::Args own, unsigned n_prefix) {
+  constexpr bool SPLIT = PR <= 32;  // few rows: the waves share out the keys
+  constexpr int BN = SPLIT || HD > 128 ? 32 : 64, QG = SPLIT ? PR / 16 : PR / 64;
+  constexpr int CHUNKS = rows::lds_chunks<HD, 4, 32, true>() > rows::lds_chunks<HD, 4, BN, SPLIT>()
+                             ? rows::lds_chunks<HD, 4, 32, true>() : rows::lds_chunks<HD, 4, BN, SPLIT>();
+  __shared__ u32x4 lds[CHUNKS];
+  if (blockIdx.x < n_prefix)
+    rows::attn_rows<T, HD, 4, QG, BN, SPLIT, PR <= 64 ? 2 : 1, rows::PREFIX>(a, lds, blockIdx.x);
+  else
+    rows::attn_rows<T, HD, 4, OR / 16, 32, true, 2, rows::OWN>(own, lds, blockIdx.x - n_prefix);
+}
+
+template <typename T, int HD, int PR, int OR>
+void launch_one(const rows::Args& a, const rows::Args& own, int64_t n_prefix, int64_t n_own, hipStream_t st) {
+  hipLaunchKernelGGL((attn_rows_prefix<T, HD, PR, OR>), dim3(static_cast<unsigned>(n_prefix + n_own)), dim3(256), 0, st,
+                     a, own, static_cast<unsigned>(n_prefix));
 }
 
 template <typename T, int HD>
-int launch_hd(rows::Args a, const rows::Args& own, const Shape& s, const Split& d, hipStream_t st) {
-  const int64_t G = s.H / s.Hkv;
-  if (s.prefix > 0) {
-    a.chunk = static_cast<int32_t>(d.prefix_chunk);
-    a.splits = static_cast<int32_t>(d.prefix_splits);
-    a.row_tiles = static_cast<int32_t>(ceil_div(s.B * s.n_q * G, d.prefix_rows));
-    const int e = launch_rows<T, HD, rows::PREFIX>(a, d.prefix_rows, s.Hkv * d.prefix_splits * a.row_tiles, st);
-    if (e) return e;
-  }
-  if (s.room > 0) {
-    rows::Args w = own;
-    w.chunk = static_cast<int32_t>(d.own_chunk);
-    w.splits = static_cast<int32_t>(d.own_splits);
-    w.row_tiles = static_cast<int32_t>(ceil_div(s.n_q * G, d.own_rows));
-    w.part0 = static_cast<int32_t>(d.prefix_splits);
-    return launch_rows<T, HD, rows::OWN>(w, d.own_rows, s.Hkv * d.own_splits * w.row_tiles * s.B, st);
-  }
-  return MI355_OK;
+int launch_hd(const rows::Args& a, const rows::Args& own, const Split& d, hipStream_t st) {
+  const int64_t np = static_cast<int64_t>(a.Hkv) * a.splits * a.row_tiles;
+  const int64_t no = static_cast<int64_t>(a.Hkv) * own.splits * own.row_tiles * own.B;
+  if (d.prefix_rows <= 16) launch_one<T, HD, 16, 16>(a, own, np, no, st);
+  else if (d.prefix_rows == 32) launch_one<T, HD, 32, 32>(a, own, np, no, st);
+  else if (d.prefix_rows == 64 && d.own_rows == 16) launch_one<T, HD, 64, 16>(a, own, np, no, st);
+  else if (d.prefix_rows == 64) launch_one<T, HD, 64, 32>(a, own, np, no, st);
+  else if (d.own_rows == 16) launch_one<T, HD, 128, 16>(a, own, np, no, st);
+  else launch_one<T, HD, 128, 32>(a, own, np, no, st);
+  return static_cast<int>(hipGetLastError());
 }
 
 template <typename T>
 int launch(const rows::Args& a, const rows::Args& own, const CombineArgs& c, const Shape& s, const Split& d, hipStream_t st) {
   int e = MI355_E_HEAD_DIM;
-  switch (s.hd) {
-    case 16: e = launch_hd<T, 16>(a, own, s, d, st); break;
-    case 32: e = launch_hd<T, 32>(a, own, s, d, st); break;
-    case 48: e = launch_hd<T, 48>(a, own, s, d, st); break;
-    case 64: e = launch_hd<T, 64>(a, own, s, d, st); break;
-    case 80: e = launch_hd<T, 80>(a, own, s, d, st); break;
-    case 96: e = launch_hd<T, 96>(a, own, s, d, st); break;
-    case 128: e = launch_hd<T, 128>(a, own, s, d, st); break;
-    case 192: e = launch_hd<T, 192>(a, own, s, d, st); break;
-    case 256: e = launch_hd<T, 256>(a, own, s, d, st); break;
+  if (d.prefix_splits + d.own_splits == 0) e = MI355_OK;  // no key at all: the join writes zeros
+  else switch (s.hd) {
+    case 16: e = launch_hd<T, 16>(a, own, d, st); break;
+    case 32: e = launch_hd<T, 32>(a, own, d, st); break;
+    case 48: e = launch_hd<T, 48>(a, own, d, st); break;
+    case 64: e = launch_hd<T, 64>(a, own, d, st); break;
+    case 80: e = launch_hd<T, 80>(a, own, d, st); break;
+    case 96: e = launch_hd<T, 96>(a, own, d, st); break;
+    case 128: e = launch_hd<T, 128>(a, own, d, st); break;
+    case 192: e = launch_hd<T, 192>(a, own, d, st); break;
+    case 256: e = launch_hd<T, 256>(a, own, d, st); break;
   }
   if (e) return e;
   if (d.prefix_splits + d.own_splits <= WAVE_SPLITS)
@@ -249,7 +250,7 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
       !aligned16(workspace) || (reinterpret_cast<uintptr_t>(O) & 7u) || (reinterpret_cast<uintptr_t>(own_lens) & 3u))
     return MI355_E_ALIGNMENT;
   const int64_t G = heads / kv_heads;
-  if (kv_heads * d.prefix_splits * ceil_div(B * n_q * G, d.prefix_rows) > 0x7fffffffLL ||
+  if (kv_heads * d.prefix_splits * ceil_div(B * n_q * G, d.prefix_rows) +
       kv_heads * d.own_splits * ceil_div(n_q * G, d.own_rows) * B > 0x7fffffffLL)
     return MI355_E_BAD_SIZE;
   rows::Args a{};
@@ -273,6 +274,13 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
   own.vb = vo_strides[0]; own.vt = vo_strides[1]; own.vh = vo_strides[2];
   own.keys = static_cast<int32_t>(room);
   own.lens = own_lens;
+  a.chunk = static_cast<int32_t>(d.prefix_chunk);
+  a.splits = static_cast<int32_t>(d.prefix_splits);
+  a.row_tiles = static_cast<int32_t>(ceil_div(B * n_q * G, d.prefix_rows));
+  own.chunk = static_cast<int32_t>(d.own_chunk);
+  own.splits = static_cast<int32_t>(d.own_splits);
+  own.row_tiles = static_cast<int32_t>(ceil_div(n_q * G, d.own_rows));
+  own.part0 = a.splits;
   CombineArgs c{};
   c.part = a.part;
   c.ml = a.ml;

@@ -97,14 +97,25 @@ MI355_DEVINL int swz(int r) {
     return 0;
 }
 
-// NW waves of QG groups of 16 rows; EU: waves a SIMD shall hold; TERMS: the probabilities enter
-// P · V as that many terms of the input type.
-template <typename T, int HD, int NW, int QG, int BN, int RING, int EU, int TERMS, int MODE>
-__global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
+// 16-byte chunks of LDS that a body needs
+template <int HD, int NW, int BN, bool OWN_KEYS>
+constexpr int lds_chunks() { return 2 * BN * (HD / 8) * (OWN_KEYS ? NW : 2); }
+
+// The work of one work-group: NW waves of QG groups of 16 rows.
+//   OWN_KEYS = false: each wave has rows of its own, the waves share tiles of BN keys (double-buffered).
+//   OWN_KEYS = true, for at most 16 QG rows: the waves have the same rows and keys of their own, tile w,
+//     w + NW .. of the range (single-buffered: there a work-group waits for memory, and while one wave
+//     computes the others' loads are in flight), and are joined through LDS at the end.
+// TERMS: the probabilities enter P · V as that many terms of the input type.
+template <typename T, int HD, int NW, int QG, int BN, bool OWN_KEYS, int TERMS, int MODE>
+MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
+  constexpr int RING = OWN_KEYS ? 1 : 2;
   using frag = typename Mfma<T>::frag;
   typedef T frag4 __attribute__((ext_vector_type(4)));
   static_assert(HD % 16 == 0 && BN % 32 == 0, "shape");
-  constexpr int QW = 16 * QG, BM = NW * QW;
+  constexpr int QW = 16 * QG, BM = OWN_KEYS ? QW : NW * QW;
+  constexpr int LW = OWN_KEYS ? 1 : NW;  // waves that load a tile
+  static_assert(QW <= 32 || !OWN_KEYS, "rows of a word");
   constexpr int NCH = HD / 8, ROWB = HD * 2;
   // MFMA steps of S^T, 32 elements each; of HD 16, 48 and 80 the last one's upper half is zeros in both
   // operands. (A 16x16x16 MFMA for it, accumulating onto the 16x16x32 right before it, lost two of its four
@@ -113,8 +124,7 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   constexpr bool HALF = HD % 32 != 0;
   constexpr int DT = HD / 16, KT = BN / 16;
   static_assert(BN * NCH % 64 == 0, "whole blocks of loads");
-  constexpr int BLK = BN * NCH / 64, LPW = (BLK + NW - 1) / NW, TILE = BN * NCH;
-  __shared__ u32x4 lds[2 * RING * TILE];   // K ring, V ring
+  constexpr int BLK = BN * NCH / 64, LPW = (BLK + LW - 1) / LW, TILE = BN * NCH;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -125,8 +135,8 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   const T *Qb, *Kb, *Vb;
   int64_t out_tok = 0, slot = -1;
   if constexpr (MODE == PACKED) {
-    h = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.Hkv));
-    const PackedTile t = p.tiles[blockIdx.x / static_cast<unsigned>(p.Hkv)];
+    h = static_cast<int>(block % static_cast<unsigned>(p.Hkv));
+    const PackedTile t = p.tiles[block / static_cast<unsigned>(p.Hkv)];
     row0 = t.row0;
     nrows = t.q_len * p.G;
     k_begin = t.k_begin;
@@ -142,7 +152,7 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
     Vb = static_cast<const T*>(p.v) + t.k0 * p.vt + h * p.vh;
     out_tok = t.q0;
   } else {
-    unsigned x = blockIdx.x;
+    unsigned x = block;
     h = static_cast<int>(x % static_cast<unsigned>(p.Hkv));
     x /= static_cast<unsigned>(p.Hkv);
     split = static_cast<int>(x % static_cast<unsigned>(p.splits));
@@ -172,7 +182,9 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
   Vb = uniform_ptr(Vb + static_cast<int64_t>(k_begin) * p.vt);
   const int n_keys = k_end - k_begin;  // keys from here on are counted from k_begin
-  const int row_w = row0 + wave * QW;
+  const int row_w = OWN_KEYS ? row0 : row0 + wave * QW;
+  const int lwave = OWN_KEYS ? 0 : wave;
+  if constexpr (OWN_KEYS) lds += wave * 2 * TILE;
   const bool idle = row_w >= nrows;    // no row of this wave is real: it only loads
 
   // token (of the batch in PREFIX) of a row, and its offset in q
@@ -229,7 +241,7 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   uint32_t koff[LPW], voff[LPW];
 #pragma unroll
   for (int i = 0; i < LPW; ++i) {
-    const int at = (wave + i * NW) * 64 + lane, row = at / NCH, ch = (at % NCH) ^ swz<NCH>(row);
+    const int at = (lwave + i * LW) * 64 + lane, row = at / NCH, ch = (at % NCH) ^ swz<NCH>(row);
     koff[i] = static_cast<uint32_t>(row) * kstride + ch * 16;
     voff[i] = static_cast<uint32_t>(row) * vstride + ch * 16;
   }
@@ -241,8 +253,8 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
                                  rem > vcap ? 0xffffffffu : rem * vstride);
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
-      const int blk = wave + i * NW;
-      if (BLK % NW != 0 && blk >= BLK) break;
+      const int blk = lwave + i * LW;
+      if (BLK % LW != 0 && blk >= BLK) break;
       buffer_dma_lds16(kr, koff[i], 0, lds_addr_of(&lds[st * TILE + blk * 64]));
       buffer_dma_lds16(vr, voff[i], 0, lds_addr_of(&lds[(RING + st) * TILE + blk * 64]));
     }
@@ -362,121 +374,180 @@ __global__ __launch_bounds__(NW * 64, EU) void attn_rows_kernel(Args p) {
   };
 
   const int n_kt = (n_keys + BN - 1) / BN;
-  if (n_kt > 0) issue(0, 0);
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
-    if (j + 1 < n_kt) issue(j + 1, st ^ 1);
-    if (!idle && j * BN < lim_last) tile(j, st);
-    // this wave's loads of tile j + 1 have landed and its reads of tile j are done
+  if constexpr (OWN_KEYS) {
+    for (int j = wave; j < n_kt && j * BN < lim_last; j += NW) {
+      issue(j, 0);
+      __builtin_amdgcn_s_waitcnt(0);
+      tile(j, 0);
+      __builtin_amdgcn_s_waitcnt(0);  // the tile is read: the next may land on it
+    }
+  } else {
+    if (n_kt > 0) issue(0, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-  };
-  static_assert(RING == 2, "double buffering");
-  int j = 0;
-  for (; j + 2 <= n_kt; j += 2) {
-    step(j, 0);
-    step(j + 1, 1);
-  }
-  if (j < n_kt) step(j, 0);
-
-  // rows out: each lane holds runs of 4 of its row's elements
-  uint64_t nan_rows[QG];
-#pragma unroll
-  for (int n = 0; n < QG; ++n) {
-    const int r = row_w + 16 * n + l16;
-    const float sum = row_sum(lsum[n]);
-    bool bad = false;
-    if (r < nrows) {
-      if (MODE == PACKED && slot < 0) {
-        const int t = r / p.G, hh = h * p.G + (r - t * p.G);
-        T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
-        // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
-        const float inv = 1.0f / sum;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          frag4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = lim[n] > 0 ? o[n][dt][e] * inv : 0.f;
-            bad |= x != x;
-            w[e] = from_f32<T>(x);
-          }
-          *reinterpret_cast<frag4*>(dst + 16 * dt + 4 * g) = w;
-        }
-      } else {
-        const int64_t at = part_of(r);
-        float* dst = p.part + at * HD;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bad |= o[n][dt][e] != o[n][dt][e];
-          *reinterpret_cast<f32x4*>(dst + 16 * dt + 4 * g) = o[n][dt];
-        }
-        if (g == 0) {
-          // (a sum that is not 0 without a maximum is NaN's)
-          p.ml[2 * at] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
-          p.ml[2 * at + 1] = sum;
-        }
-      }
+    auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
+      if (j + 1 < n_kt) issue(j + 1, st ^ 1);
+      if (!idle && j * BN < lim_last) tile(j, st);
+      // this wave's loads of tile j + 1 have landed and its reads of tile j are done
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    int j = 0;
+    for (; j + 2 <= n_kt; j += 2) {
+      step(j, 0);
+      step(j + 1, 1);
     }
-    const uint64_t m = __builtin_amdgcn_ballot_w64(bad);
-    nan_rows[n] = (m | (m >> 16) | (m >> 32) | (m >> 48)) & 0xffffu;
+    if (j < n_kt) step(j, 0);
   }
 
   // A key behind a row's last one has probability 0, but its v row is in the tile: 0 · inf and
-  // 0 · NaN leave NaN in rows that do not see it. Rows with NaN whose tile held such keys are
-  // computed again, one key at a time over the keys they see (a row that sees a NaN gets it again).
-  if constexpr (MODE != PREFIX) {
+  // 0 · NaN leave NaN in rows that do not see it. Rows with NaN whose range held such keys are
+  // computed again, by a wave, one key at a time over the keys they see (a row that sees a NaN gets it again).
+  const auto again = [&](int r) MI355_LAMBDA_INLINE {
+    const int keys = lim_of(r);
+    if (MODE == PREFIX || keys <= 0 || keys >= n_keys) return;
+    constexpr int DL = (HD + 63) / 64;
+    const T* src = Qb + q_of(r);
+    float q[DL], acc[DL], m = NEG_INF, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < DL; ++i) {
+      q[i] = lane + 64 * i < HD ? to_f32(src[lane + 64 * i]) : 0.f;
+      acc[i] = 0.f;
+    }
+    for (int key = 0; key < keys; ++key) {
+      const T* kr = Kb + static_cast<int64_t>(key) * p.kt;
+      const T* vr = Vb + static_cast<int64_t>(key) * p.vt;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
+      for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+      s *= p.c;
+      const float m2 = vmax(m, s);
+      const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
+      const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
+      l = __builtin_fmaf(l, a, e);
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
+      m = m2;
+    }
+    if (MODE == PACKED && slot < 0) {
+      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+      T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
+    } else {
+      const int64_t at = part_of(r);
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (lane + 64 * i < HD) p.part[at * HD + lane + 64 * i] = acc[i];
+      if (lane == 0) {
+        p.ml[2 * at] = m;
+        p.ml[2 * at + 1] = l;
+      }
+    }
+  };
+  // 4 elements of row r from element d on; returns whether one is NaN
+  const auto put = [&](int r, int d, f32x4 v, float sum, bool sees) MI355_LAMBDA_INLINE {
+    bool bad = false;
+    if (MODE == PACKED && slot < 0) {
+      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+      // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
+      const float inv = 1.0f / sum;
+      frag4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = sees ? v[e] * inv : 0.f;
+        bad |= x != x;
+        w[e] = from_f32<T>(x);
+      }
+      *reinterpret_cast<frag4*>(static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh + d) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= v[e] != v[e];
+      *reinterpret_cast<f32x4*>(p.part + part_of(r) * HD + d) = v;
+    }
+    return bad;
+  };
+  const auto put_ml = [&](int r, float m, float sum) MI355_LAMBDA_INLINE {
+    if (MODE == PACKED && slot < 0) return;
+    const int64_t at = part_of(r);
+    p.ml[2 * at] = m;
+    p.ml[2 * at + 1] = sum;
+  };
+
+  if constexpr (OWN_KEYS) {
+    // The waves' rows meet in LDS: each wave's outputs where its tiles were, its maxima and sums beside.
+    __shared__ float ml[NW][QW][2];
+    __shared__ uint32_t nan_rows;
+    static_assert(QW * HD * 4 <= 2 * TILE * 16, "a wave's outputs fit its tiles");
+    f32x4* const mine = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
     for (int n = 0; n < QG; ++n) {
-      if (nan_rows[n] == 0) continue;
+      const float sum = row_sum(lsum[n]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) mine[(16 * n + l16) * (HD / 4) + 4 * dt + g] = o[n][dt];
+      if (g == 0) {
+        // (a sum that is not 0 without a maximum is NaN's)
+        ml[wave][16 * n + l16][0] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
+        ml[wave][16 * n + l16][1] = sum;
+      }
+    }
+    if (tid == 0) nan_rows = 0;
+    __syncthreads();
+    const f32x4* const all = reinterpret_cast<const f32x4*>(lds - wave * 2 * TILE);
+    const int real = nrows - row0 < QW ? nrows - row0 : QW;
+    for (int at = tid; at < real * (HD / 4); at += NW * 64) {
+      const int x = at / (HD / 4), d = at % (HD / 4);
+      float m = NEG_INF, sum = 0.f;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = vmax(m, ml[w][x][0]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = ml[w][x][0];
+        if (mw == NEG_INF) continue;  // no finite score there
+        const float f = fast_exp2(mw - m);
+        sum = __builtin_fmaf(ml[w][x][1], f, sum);
+        const f32x4 ow = all[w * 2 * TILE + x * (HD / 4) + d];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], f, v[e]);
+      }
+      if (put(row0 + x, 4 * d, v, sum, lim_of(row0 + x) > 0)) atomicOr(&nan_rows, 1u << x);
+      if (d == 0) put_ml(row0 + x, m, sum);
+    }
+    if constexpr (MODE != PREFIX) {
       __builtin_amdgcn_s_waitcnt(0);  // the stores above are done
-      constexpr int DL = (HD + 63) / 64;
-      for (int x = 0; x < 16; ++x) {
-        const int r = row_w + 16 * n + x, keys = lim_of(r < nrows ? r : nrows - 1);
-        if (!((nan_rows[n] >> x) & 1) || r >= nrows || keys <= 0 || keys >= n_keys) continue;
-        const T* src = Qb + q_of(r);
-        float q[DL], acc[DL], m = NEG_INF, l = 0.f;
+      __syncthreads();
+      const uint32_t bad = nan_rows;
+      for (int x = wave; x < real; x += NW)
+        if ((bad >> x) & 1) again(row0 + x);
+    }
+  } else {
+    // each lane holds runs of 4 of its row's elements
+    uint64_t nan_rows[QG];
 #pragma unroll
-        for (int i = 0; i < DL; ++i) {
-          q[i] = lane + 64 * i < HD ? to_f32(src[lane + 64 * i]) : 0.f;
-          acc[i] = 0.f;
-        }
-        for (int key = 0; key < keys; ++key) {
-          const T* kr = Kb + static_cast<int64_t>(key) * p.kt;
-          const T* vr = Vb + static_cast<int64_t>(key) * p.vt;
-          float s = 0.f;
+    for (int n = 0; n < QG; ++n) {
+      const int r = row_w + 16 * n + l16;
+      const float sum = row_sum(lsum[n]);
+      bool bad = false;
+      if (r < nrows) {
 #pragma unroll
-          for (int i = 0; i < DL; ++i)
-            if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
-          for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
-          s *= p.c;
-          const float m2 = vmax(m, s);
-          const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
-          const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
-          l = __builtin_fmaf(l, a, e);
+        for (int dt = 0; dt < DT; ++dt) bad |= put(r, 16 * dt + 4 * g, o[n][dt], sum, lim[n] > 0);
+        if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n], sum);
+      }
+      const uint64_t m = __builtin_amdgcn_ballot_w64(bad);
+      nan_rows[n] = (m | (m >> 16) | (m >> 32) | (m >> 48)) & 0xffffu;
+    }
+    if constexpr (MODE != PREFIX) {
 #pragma unroll
-          for (int i = 0; i < DL; ++i)
-            if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
-          m = m2;
-        }
-        if (MODE == PACKED && slot < 0) {
-          const int t = r / p.G, hh = h * p.G + (r - t * p.G);
-          T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
-#pragma unroll
-          for (int i = 0; i < DL; ++i)
-            if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
-        } else {
-          const int64_t at = part_of(r);
-#pragma unroll
-          for (int i = 0; i < DL; ++i)
-            if (lane + 64 * i < HD) p.part[at * HD + lane + 64 * i] = acc[i];
-          if (lane == 0) {
-            p.ml[2 * at] = m;
-            p.ml[2 * at + 1] = l;
-          }
-        }
+      for (int n = 0; n < QG; ++n) {
+        if (nan_rows[n] == 0) continue;
+        __builtin_amdgcn_s_waitcnt(0);  // the stores above are done
+        for (int x = 0; x < 16; ++x)
+          if ((nan_rows[n] >> x) & 1) again(row_w + 16 * n + x);
       }
     }
   }
