@@ -104,8 +104,7 @@ constexpr int lds_chunks() { return 2 * BN * (HD / 8) * (OWN_KEYS ? NW : 2); }
 // The work of one work-group: NW waves of QG groups of 16 rows.
 //   OWN_KEYS = false: each wave has rows of its own, the waves share tiles of BN keys (double-buffered).
 //   OWN_KEYS = true, for at most 16 QG rows: the waves have the same rows and keys of their own, tile w,
-//     w + NW .. of the range (single-buffered: there a work-group waits for memory, and while one wave
-//     computes the others' loads are in flight), and are joined through LDS at the end.
+//     w + NW .. of the range, in one buffer each for K and V, and are joined through LDS at the end.
 // TERMS: the probabilities enter P · V as that many terms of the input type.
 template <typename T, int HD, int NW, int QG, int BN, bool OWN_KEYS, int TERMS, int MODE>
 MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
@@ -245,17 +244,25 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     koff[i] = static_cast<uint32_t>(row) * kstride + ch * 16;
     voff[i] = static_cast<uint32_t>(row) * vstride + ch * 16;
   }
-  auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
+  auto issue_k = [&](int j, int st) MI355_LAMBDA_INLINE {
     const uint32_t key = static_cast<uint32_t>(j) * BN, rem = static_cast<uint32_t>(n_keys) - key;
     const u32x4 kr = buffer_rsrc(reinterpret_cast<const char*>(Kb) + static_cast<uint64_t>(key) * kstride,
                                  rem > kcap ? 0xffffffffu : rem * kstride);
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int blk = lwave + i * LW;
+      if (BLK % LW != 0 && blk >= BLK) break;
+      buffer_dma_lds16(kr, koff[i], 0, lds_addr_of(&lds[st * TILE + blk * 64]));
+    }
+  };
+  auto issue_v = [&](int j, int st) MI355_LAMBDA_INLINE {
+    const uint32_t key = static_cast<uint32_t>(j) * BN, rem = static_cast<uint32_t>(n_keys) - key;
     const u32x4 vr = buffer_rsrc(reinterpret_cast<const char*>(Vb) + static_cast<uint64_t>(key) * vstride,
                                  rem > vcap ? 0xffffffffu : rem * vstride);
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
       const int blk = lwave + i * LW;
       if (BLK % LW != 0 && blk >= BLK) break;
-      buffer_dma_lds16(kr, koff[i], 0, lds_addr_of(&lds[st * TILE + blk * 64]));
       buffer_dma_lds16(vr, voff[i], 0, lds_addr_of(&lds[(RING + st) * TILE + blk * 64]));
     }
   };
@@ -296,7 +303,8 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     lsum[n] = 0.f;
   }
 
-  auto tile = [&](const int j, const int st) MI355_LAMBDA_INLINE {
+  // scores_done: the tile's K has been read; need_v: its V is about to be
+  auto tile = [&](const int j, const int st, auto&& scores_done, auto&& need_v) MI355_LAMBDA_INLINE {
     const int k0 = j * BN;
     f32x4 s[QG][KT];
 #pragma unroll
@@ -310,6 +318,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
         for (int n = 0; n < QG; ++n) s[n][kt] = mma32(kf, qf[n][x], s[n][kt]);
       }
     }
+    scores_done();
     if (k0 + BN > lim_first) {  // the tile crosses a row's last key
 #pragma unroll
       for (int n = 0; n < QG; ++n) {
@@ -361,6 +370,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
           lsum[n] = prob_sum(pf[0][n][t], lsum[n]);
         }
       }
+    need_v();
 #pragma unroll
     for (int t = 0; t < KT / 2; ++t)
 #pragma unroll
@@ -375,19 +385,43 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 
   const int n_kt = (n_keys + BN - 1) / BN;
   if constexpr (OWN_KEYS) {
-    for (int j = wave; j < n_kt && j * BN < lim_last; j += NW) {
-      issue(j, 0);
-      __builtin_amdgcn_s_waitcnt(0);
-      tile(j, 0);
-      __builtin_amdgcn_s_waitcnt(0);  // the tile is read: the next may land on it
+    // K of the next tile is requested as soon as this one's has been read, V likewise, so that one of
+    // them is always in flight: of the 2 LPW newest loads the older LPW have to be there.
+    static_assert(LPW < 64, "vmcnt");
+    constexpr int OLDER = (LPW & 15) | (LPW >> 4) << 14 | 7 << 4 | 15 << 8;  // vmcnt(LPW)
+    constexpr int READ = 15 | 3 << 14 | 7 << 4;                              // lgkmcnt(0)
+    const int n_mine = n_kt < (lim_last + BN - 1) / BN ? n_kt : (lim_last + BN - 1) / BN;
+    if (wave < n_mine) {
+      issue_k(wave, 0);
+      issue_v(wave, 0);
+    }
+    for (int j = wave; j < n_mine; j += NW) {
+      const bool more = j + NW < n_mine;
+      __builtin_amdgcn_s_waitcnt(OLDER);
+      tile(j, 0,
+           [&]() MI355_LAMBDA_INLINE {
+             __builtin_amdgcn_s_waitcnt(READ);
+             if (more) issue_k(j + NW, 0);
+           },
+           [&]() MI355_LAMBDA_INLINE {
+             if (more) __builtin_amdgcn_s_waitcnt(OLDER);
+             else __builtin_amdgcn_s_waitcnt(0);
+           });
+      __builtin_amdgcn_s_waitcnt(READ);
+      if (more) issue_v(j + NW, 0);
     }
   } else {
+    const auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
+      issue_k(j, st);
+      issue_v(j, st);
+    };
+    const auto nothing = []() MI355_LAMBDA_INLINE {};
     if (n_kt > 0) issue(0, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
       if (j + 1 < n_kt) issue(j + 1, st ^ 1);
-      if (!idle && j * BN < lim_last) tile(j, st);
+      if (!idle && j * BN < lim_last) tile(j, st, nothing, nothing);
       // this wave's loads of tile j + 1 have landed and its reads of tile j are done
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
