@@ -18,6 +18,9 @@
 
 namespace {
 
+// most features of a wave of linear_i4_few
+constexpr int MAX_FEW = 32;
+
 struct I4Args {
   const void* x;
   const uint8_t* w;
@@ -251,6 +254,168 @@ __global__ __launch_bounds__(64 * NW) void linear_i4_kernel(I4Args p) {
   }
 }
 
+// Up to 4 rows of x on the vector ALUs. The MFMA kernel above loads x for 16 rows however few are real; here
+// a wave holds its k of every row in registers (32 neighbouring k a lane, CH chunks of 2048) and walks
+// features, whose weights, scales and zero points it reads as whole lines: 16, 2 and 1 bytes a lane. KW waves
+// share a feature's k. 4 features at a time: q x in packed dot products, the zero point as above, and one
+// exchange that adds up 64 lanes for 4 features together (2.5 instructions a sum instead of 7).
+template <typename T>
+MI355_DEVINL float dot2(uint32_t a, uint32_t b, float c);
+template <>
+MI355_DEVINL float dot2<_Float16>(uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+}
+template <>
+MI355_DEVINL float dot2<__bf16>(uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+}
+template <int CTRL>
+MI355_DEVINL float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+// Sums over the wave of 4 values a lane: lanes 16 i .. get the sum of value 0, 2, 1, 3 for i = 0 .. 3.
+MI355_DEVINL float wave_sum4(float v0, float v1, float v2, float v3) {
+  const auto u = [](float x) MI355_LAMBDA_INLINE { return __float_as_uint(x); };
+  const auto f = [](uint32_t x) MI355_LAMBDA_INLINE { return __uint_as_float(x); };
+  const auto a = __builtin_amdgcn_permlane32_swap(u(v0), u(v1), false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(u(v2), u(v3), false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(u(f(a[0]) + f(a[1])), u(f(b[0]) + f(b[1])), false, false);
+  return dpp_add<0x121>(dpp_add<0x122>(dpp_add<0x124>(dpp_add<0x128>(f(c[0]) + f(c[1])))));  // row_ror 8 4 2 1
+}
+
+template <typename T, int GROUP, int M, int CH, int KW, typename TO>
+__global__ __launch_bounds__(KW == 8 ? 512 : 256) void linear_i4_few(I4Args p, int per_wave) {
+  constexpr int SH = Nib<T>::SHIFT, F = 4, NW = KW == 8 ? 8 : 4;
+  __shared__ float part[NW][MAX_FEW][M];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = wave % KW, wg_features = per_wave * (NW / KW);
+  const int n_wave = blockIdx.x * wg_features + wave / KW * per_wave;  // first feature of this wave
+  const int groups = p.K / GROUP;
+  const uint8_t* wp[CH];
+  int at[CH];
+  bool in[CH];
+  uint32_t x[CH][M][16];
+  float sx[CH][M];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int k0 = (kw * CH + c) * 2048 + lane * 32;
+    in[c] = k0 < p.K;
+    const int k = in[c] ? k0 : 0;  // (lanes past K: x = 0)
+    wp[c] = p.w + k / 2;
+    at[c] = k / GROUP;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const T* row = static_cast<const T*>(p.x) + static_cast<int64_t>(m < p.M ? m : 0) * p.ldx + k;
+      sx[c][m] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x4 v = *reinterpret_cast<const u32x4*>(row + 8 * i);
+        if (!in[c]) v = u32x4{0u, 0u, 0u, 0u};
+        v = nibble_order(v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[c][m][4 * i + e] = v[e];
+      }
+    }
+  }
+  const T one1 = static_cast<T>(1.0f);
+  const uint32_t one = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, one1)) * 0x10001u;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sx[c][m] = dot2<T>(x[c][m][i], one, sx[c][m]);
+
+  struct Four {
+    u32x4 w[F][CH];
+    T s[F][CH];
+    uint8_t z[F][CH];
+  };
+  auto fetch = [&](int n, Four& d) MI355_LAMBDA_INLINE {
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int64_t f = n + i < p.N ? n + i : p.N - 1;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        d.w[i][c] = *reinterpret_cast<const u32x4*>(wp[c] + f * (p.K / 2));
+        d.s[i][c] = static_cast<const T*>(p.scale)[f * groups + at[c]];
+        d.z[i][c] = p.zero != nullptr ? p.zero[f * groups + at[c]] : uint8_t(8);
+      }
+    }
+  };
+  Four cur;
+  fetch(n_wave, cur);
+  for (int n = 0; n < per_wave; n += F) {
+    Four nxt;
+    if (n + F < per_wave) fetch(n_wave + n + F, nxt);
+    float v[F][M];
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) v[i][m] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        float d[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) d[m] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = cur.w[i][c][j];
+            const uint32_t q = ((4 * e < SH ? w << (SH - 4 * e) : w >> (4 * e - SH)) & (0x000f000fu << SH)) | Nib<T>::SIXTEEN;
+#pragma unroll
+            for (int m = 0; m < M; ++m) d[m] = dot2<T>(q, x[c][m][4 * j + e], d[m]);
+          }
+        const float z = -16.f - static_cast<float>(cur.z[i][c]), s = to_f32(cur.s[i][c]);
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[i][m] = __builtin_fmaf(__builtin_fmaf(sx[c][m], z, d[m]), s, v[i][m]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const float sum = wave_sum4(v[0][m], v[1][m], v[2][m], v[3][m]);
+      const int g = lane >> 4, i = g == 1 ? 2 : g == 2 ? 1 : g;
+      if ((lane & 15) == 0) part[wave][n + i][m] = sum;
+    }
+    cur = nxt;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < wg_features * M; i += 64 * NW) {
+    const int f = i % wg_features, m = i / wg_features, n = blockIdx.x * wg_features + f;
+    if (n >= p.N || m >= p.M) continue;
+    float v = p.bias != nullptr ? p.bias[n] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) sum += part[f / per_wave * KW + w][f % per_wave][m];
+    static_cast<TO*>(p.y)[m * p.ldy + n] = from_f32<TO>(sum + v);
+  }
+}
+
+template <typename T, int GROUP, int M, int CH, int KW, typename TO>
+int launch_few(const I4Args& a, hipStream_t s) {
+  // enough waves for the CUs (12 each), several groups of 4 features a wave beyond that
+  const int64_t waves = static_cast<int64_t>(a.N) * KW / 3072;
+  const int per_wave = static_cast<int>(waves < 8 ? 4 : waves >= MAX_FEW ? MAX_FEW : waves / 4 * 4);
+  constexpr int NW = KW == 8 ? 8 : 4;
+  const int64_t wg = per_wave * (NW / KW);
+  hipLaunchKernelGGL((linear_i4_few<T, GROUP, M, CH, KW, TO>), dim3(static_cast<unsigned>((a.N + wg - 1) / wg)), dim3(64 * NW), 0, s, a, per_wave);
+  return static_cast<int>(hipGetLastError());
+}
+template <typename T, int GROUP, int M, typename TO>
+int launch_few_k(const I4Args& a, hipStream_t s) {
+  if (a.K <= 2048) return launch_few<T, GROUP, M, 1, 1, TO>(a, s);
+  if constexpr (M == 1) {
+    if (a.K <= 4096) return launch_few<T, GROUP, M, 2, 1, TO>(a, s);
+    if (a.K <= 8192) return launch_few<T, GROUP, M, 2, 2, TO>(a, s);
+    return launch_few<T, GROUP, M, 2, 4, TO>(a, s);
+  } else {
+    if (a.K <= 4096) return launch_few<T, GROUP, M, 1, 2, TO>(a, s);
+    if (a.K <= 8192) return launch_few<T, GROUP, M, 1, 4, TO>(a, s);
+    return launch_few<T, GROUP, M, 1, 8, TO>(a, s);
+  }
+}
+
 template <typename T, int GROUP, int MT, int R, int NW, typename TO>
 int launch_one(const I4Args& a, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((a.N + 16 * R - 1) / (16 * R)), static_cast<unsigned>((a.M + 16 * MT - 1) / (16 * MT)));
@@ -270,6 +435,17 @@ int launch_nw(const I4Args& a, hipStream_t s) {
 }
 template <typename T, int GROUP, typename TO>
 int launch_mt(const I4Args& a, hipStream_t s) {
+  // One or two rows: linear_i4_few (1 x 12288 x 4096 7.9 us against 11.5, 1 x 4096 x 16384, group 64, 10.1
+  // against 17.3; with two rows 9.2 against 11.7 and 13.2 against 17.6). Three and four, where it multiplies
+  // four, only with groups of 32, whose many scales cost the MFMA kernel more (4 x 11008 x 4096 12.9
+  // against 17.2; group 128: 4 x 65536 x 2048 31.0 against 26.5). Below 512 k most of a wave would idle.
+  if (a.K >= 512 && a.K <= 16384) {
+    if (a.M == 1) return launch_few_k<T, GROUP, 1, TO>(a, s);
+    if (a.M == 2) return launch_few_k<T, GROUP, 2, TO>(a, s);
+    if constexpr (GROUP == 32) {
+      if (a.M <= 4) return launch_few_k<T, GROUP, 4, TO>(a, s);
+    }
+  }
   if (a.M <= 16) return launch_nw<T, GROUP, 1, TO>(a, s);
   if (a.M <= 32) return launch_nw<T, GROUP, 2, TO>(a, s);
   return launch_nw<T, GROUP, 4, TO>(a, s);
