@@ -113,7 +113,7 @@ def test_packed_entry_refusals(kw, status):
         a["tile_rows"], a["ws"], a["ws_bytes"], None) == status
 
 
-PREFIX = dict(dtype=F16, ptrs=[64] * 7, B=2, n=1, heads=4, kv_heads=2, head_dim=64, P=100, room=50, qs=(256, 256, 64),
+PREFIX = dict(dtype=F16, ptrs=[64] * 7, B=2, n=1, heads=4, kv_heads=2, head_dim=64, P=1000, room=50, qs=(256, 256, 64),
               kps=(128, 64), vps=(128, 64), kos=(6400, 128, 64), vos=(6400, 128, 64), os=(256, 256, 64), scale=0.125, ws=64,
               ws_bytes=1 << 30)
 
@@ -139,7 +139,9 @@ def test_prefix_entry_refusals(kw, status):
 def test_prefix_workspace_size():
     f = _lib.lib().mi355_attn_shared_prefix_workspace_bytes
     assert f(2, 1, 4, 2, 64, 0, 0) == 0
-    assert f(2, 1, 4, 2, 64, 100, 50) == 2 * 2 * 4 * (64 + 2) * 4  # one range of keys each
+    assert f(2, 1, 4, 2, 64, 974, 50) == 0  # a work-group goes through all keys of its rows
+    assert f(2, 1, 4, 2, 64, 975, 50) == (4 + 1) * 2 * 4 * (64 + 2) * 4  # ranges of 256 keys
+    assert f(2, 17, 4, 2, 64, 100, 50) == 2 * 2 * 17 * 4 * (64 + 2) * 4  # more than 32 rows
     assert f(2, 1, 4, 3, 64, 100, 50) == BAD_SIZE and f(2, 1, 4, 2, 65, 100, 50) == HEAD
     assert f(64, 1, 32, 8, 128, 1 << 20, 4096) > 0
 

@@ -320,19 +320,22 @@ def run_prefix(gpu, dtype, B, n, H, Hkv, D, P, room, lens, seed=1, behind=None):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 128, 192, 256])
-def test_prefix_head_dims(gpu, dtype, D):
-    run_prefix(gpu, dtype, 3, 1, 4, 2, D, 333, 130, [130, 1, 64], behind=math.nan)
+@pytest.mark.parametrize("P", [333, 1333])
+def test_prefix_head_dims(gpu, dtype, D, P):
+    """Prefix and cache by one work-group (up to 1024 keys), and in ranges that are joined."""
+    run_prefix(gpu, dtype, 3, 1, 4, 2, D, P, 130, [130, 1, 64], behind=math.nan)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("B,n,H,Hkv", [(1, 1, 1, 1), (2, 1, 32, 2), (9, 1, 8, 2), (20, 1, 8, 2), (40, 1, 8, 2), (5, 3, 12, 2),
                                        (2, 40, 4, 4)])
-def test_prefix_row_tiles(gpu, D, B, n, H, Hkv):
+@pytest.mark.parametrize("P", [500, 1500])
+def test_prefix_row_tiles(gpu, D, B, n, H, Hkv, P):
     """Batches and groups that fill 16, 32, 64 and several 128 rows of the prefix, and own rows of one
     tile and of several."""
     g = torch.Generator().manual_seed(B * n)
     lens = [int(x) for x in torch.randint(n, 101, (B,), generator=g)]
-    run_prefix(gpu, torch.bfloat16, B, n, H, Hkv, D, 500, 100, lens, seed=B, behind=math.inf)
+    run_prefix(gpu, torch.bfloat16, B, n, H, Hkv, D, P, 100, lens, seed=B, behind=math.inf)
 
 
 @pytest.mark.parametrize("P,room,lens", [
@@ -341,6 +344,8 @@ def test_prefix_row_tiles(gpu, D, B, n, H, Hkv):
     (0, 0, [0, 0, 0]),
     (1, 1, [1, 0, 1]),
     (129, 65, [-3, 70, 65]),   # lengths outside [0, room] are clamped
+    (1290, 65, [-3, 70, 65]),
+    (0, 3000, [2999, 0, 1]),
     (64, 4000, [3999, 5, 2049]),  # several splits of a cache, most of them empty
     (5000, 16, [16, 3, 0]),
 ])
@@ -349,10 +354,11 @@ def test_prefix_lengths(gpu, P, room, lens, n):
     run_prefix(gpu, torch.float16, 3, n, 8, 2, 64, P, room, lens, seed=7, behind=math.nan)
 
 
-def test_prefix_strides_and_out(gpu):
+@pytest.mark.parametrize("P", [200, 1200])
+def test_prefix_strides_and_out(gpu, P):
     """Caches as views of one buffer for K and V, a strided query and output."""
     ops = _ops()
-    B, n, H, Hkv, D, P, room = 4, 2, 8, 4, 64, 200, 96
+    B, n, H, Hkv, D, room = 4, 2, 8, 4, 64, 96
     cache = _rand((B, room, 2, Hkv, D), torch.bfloat16, 11).to(gpu)
     pre = _rand((2, Hkv, P, D), torch.bfloat16, 12).to(gpu)  # head-major
     kp, vp = (pre[i].transpose(0, 1) for i in range(2))
@@ -367,10 +373,11 @@ def test_prefix_strides_and_out(gpu):
 
 
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
-def test_prefix_later_tokens(gpu, bad):
+@pytest.mark.parametrize("P", [0, 100, 1100])
+def test_prefix_later_tokens(gpu, bad, P):
     """A not-finite V of the last new token does not reach the new tokens before it."""
     ops = _ops()
-    B, n, H, D, P, room = 2, 3, 4, 64, 100, 50
+    B, n, H, D, room = 2, 3, 4, 64, 50
     q, kp, vp, ko, vo = (_rand(s, torch.float16, 21 + i) for i, s in enumerate(
         [(B, n, H, D), (P, 2, D), (P, 2, D), (B, room, 2, D), (B, room, 2, D)]))
     lens = [50, 17]
@@ -384,10 +391,11 @@ def test_prefix_later_tokens(gpu, bad):
 
 
 @pytest.mark.parametrize("at", ["prefix", "own"])
-def test_prefix_infinite_scores(gpu, at):
+@pytest.mark.parametrize("P", [70, 1070])
+def test_prefix_infinite_scores(gpu, at, P):
     """A range of keys with no finite score counts nothing; a row with none at all is NaN."""
     ops = _ops()
-    B, H, D, P, room = 2, 2, 32, 70, 40
+    B, H, D, room = 2, 2, 32, 40
     q = torch.ones(B, 1, H, D).half()
     kp, vp, ko, vo = (_rand(s, torch.float16, 31 + i) for i, s in enumerate([(P, 2, D), (P, 2, D), (B, room, 2, D), (B, room, 2, D)]))
     lens = [40, 0]
@@ -407,10 +415,11 @@ def test_prefix_infinite_scores(gpu, at):
             check(f"{at} {b} {h}", out[b, :, h], ref, tol)
 
 
-def test_prefix_graph_follows_lengths(gpu):
+@pytest.mark.parametrize("P", [300, 3000])
+def test_prefix_graph_follows_lengths(gpu, P):
     """A captured step replayed while the caches grow, beside a second graph and eager calls."""
     ops = _ops()
-    B, H, D, P, room = 5, 8, 64, 300, 200
+    B, H, D, room = 5, 8, 64, 200
 
     def inputs(seed):
         return [_rand(s, torch.float16, seed + i).to(gpu) for i, s in enumerate(
@@ -482,7 +491,12 @@ def test_i4_groups(gpu, dtype, group, zeros):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K,group", [(1, 1, 32, 32), (1, 16, 128, 128), (2, 17, 96, 32), (15, 33, 4096, 128),
                                          (16, 300, 2048, 64), (17, 64, 1024, 128), (33, 40, 544, 32), (64, 96, 8192, 64),
-                                         (65, 50, 256, 128), (200, 31, 192, 64), (1, 17000, 256, 128), (5, 1000, 11008, 128)])
+                                         (65, 50, 256, 128), (200, 31, 192, 64), (1, 17000, 256, 128), (5, 1000, 11008, 128),
+                                         # one to four rows in registers: each of its numbers of chunks and waves
+                                         (1, 7, 512, 128), (1, 300, 2048, 64), (1, 101, 4096, 32), (1, 30, 8192, 128), (1, 18, 16384, 32),
+                                         (2, 33, 2016, 32), (2, 50, 2176, 128), (2, 20, 6144, 64), (2, 9, 16384, 64), (3, 21, 1024, 32),
+                                         (4, 77, 4064, 32), (3, 50, 8064, 64), (4, 19, 16320, 64), (1, 9001, 544, 32), (4, 70000, 512, 128),
+                                         (1, 20, 16512, 128)])
 def test_i4_sizes(gpu, dtype, M, N, K, group):
     """One row to several tiles of rows, few and many work-groups (both wave counts)."""
     run_i4(gpu, dtype, M, N, K, group, seed=M)
@@ -507,10 +521,11 @@ def test_i4_every_value(gpu):
             assert torch.equal(out.double(), ref.t()), (dtype, group)
 
 
-def test_i4_strides_and_out(gpu):
+@pytest.mark.parametrize("M,K", [(5, 256), (3, 1024)])
+def test_i4_strides_and_out(gpu, M, K):
     """Row-strided x and out; what lies between and behind the rows stays."""
     ops = _ops()
-    M, N, K = 5, 70, 256
+    N = 70
     x = _rand((M, K + 40), torch.float16, 1).to(gpu)[:, 8:8 + K]
     w, scale, zero = (t.to(gpu) for t in weights(N, K, 64, "4 bits", torch.float16, 2))
     buf = torch.full((M + 1, N + 3), 5.0, device=gpu, dtype=torch.float16)
@@ -520,11 +535,31 @@ def test_i4_strides_and_out(gpu):
     assert bool((buf[M:] == 5.0).all()) and bool((buf[:, N:] == 5.0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_i4_small_values(gpu, dtype):
+    """x of fp16's subnormal range and scales near the least: nothing is flushed to zero."""
+    ops = _ops()
+    for M in (1, 2, 4, 9):
+        x = (_rand((M, 640), torch.float32, M) * 2.0 ** -18).to(dtype)
+        w, scale, zero = weights(40, 640, 64, "4 bits", dtype, 12)
+        scale = (scale.float() * 2.0 ** -10).to(dtype)
+        out = ops.linear_i4(x.to(gpu), w.to(gpu), scale.to(gpu), zero.to(gpu), out_dtype=torch.float32).cpu().double()
+        ref, tol = linear64(x, w, scale, zero, None, 64, torch.float32)
+        tol = tol - 2.0 ** -24 + 2.0 ** -149
+        assert bool(((out - ref).abs() <= tol).all()), M
+
+
 def test_i4_rows_stand_alone(gpu):
     """A not-finite row of x stays in its row; a row's bits do not depend on the others of its tile."""
     ops = _ops()
     w, scale, zero = (t.to(gpu) for t in weights(64, 512, 128, "4 bits", torch.bfloat16, 4))
     x = _rand((16, 512), torch.bfloat16, 5).to(gpu)
+    for M in (2, 4):  # the kernel of few rows
+        x2 = x[:M].clone()
+        x2[1, 7] = math.nan
+        got, clean = ops.linear_i4(x2, w, scale, zero), ops.linear_i4(x[:M].contiguous(), w, scale, zero)
+        keep = [i for i in range(M) if i != 1]
+        assert torch.equal(got[keep], clean[keep]) and bool(torch.isnan(got[1]).all())
     clean = ops.linear_i4(x, w, scale, zero)
     x2 = x.clone()
     x2[3, 7], x2[9, 100] = math.nan, math.inf
@@ -532,7 +567,7 @@ def test_i4_rows_stand_alone(gpu):
     keep = [i for i in range(16) if i not in (3, 9)]
     assert torch.equal(got[keep], clean[keep])
     assert bool(torch.isnan(got[3]).all()) and not bool(torch.isfinite(got[9]).any())
-    assert torch.equal(ops.linear_i4(x[4:5], w, scale, zero), clean[4:5])
+    assert torch.equal(ops.linear_i4(x[4:10], w, scale, zero), clean[4:10])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -20,6 +20,7 @@ struct Shape {
 struct Split {
   int prefix_rows, own_rows;
   int64_t prefix_chunk, own_chunk, prefix_splits, own_splits;
+  bool whole;  // neither is split, nothing to join
 };
 
 // most splits of the prefix or of a cache, and of both together for one wave to join
@@ -33,6 +34,13 @@ Split split_of(const Shape& s) {
   const int64_t G = s.H / s.Hkv, pr = s.B * s.n_q * G, orows = s.n_q * G;
   d.prefix_rows = pr <= 16 ? 16 : pr <= 32 ? 32 : pr <= 64 ? 64 : 128;
   d.own_rows = orows <= 16 && d.prefix_rows != 32 ? 16 : 32;
+  // Few keys for few work-groups: the joining launch (4 us and its place in the stream) costs more than reading the
+  // prefix for every sequence (4 sequences, 8/2 heads of 64, behind 300 + 128 keys: 6.3 against 9.6 us).
+  d.whole = orows <= 32 && s.prefix + s.room <= 1024 && s.B * s.Hkv <= 512;
+  if (d.whole) {
+    d.own_rows = orows <= 16 ? 16 : 32;
+    return d;
+  }
   // As many ranges as fill the work-groups that run at once (two a CU), half of them where the prefix is
   // matrix work: each range writes partial rows, and the caches' ranges run beside it.
   const auto chunk = [](int64_t keys, int64_t groups, int64_t want) {
@@ -170,8 +178,26 @@ void launch_one(const rows::Args& a, const rows::Args& own, int64_t n_prefix, in
                      a, own, static_cast<unsigned>(n_prefix));
 }
 
+// A work-group per sequence and K/V head goes through the prefix and the sequence's cache itself.
+template <typename T, int HD, int OR>
+__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_rows_whole(rows::Args p) {
+  __shared__ u32x4 lds[rows::lds_chunks<HD, 4, 32, true>()];
+  rows::attn_rows<T, HD, 4, OR / 16, 32, true, 2, rows::WHOLE>(p, lds, blockIdx.x);
+}
+
+template <typename T, int HD>
+int launch_whole(const rows::Args& own, const Split& d, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(own.B * own.Hkv));
+  if (d.own_rows == 16)
+    hipLaunchKernelGGL((attn_rows_whole<T, HD, 16>), grid, dim3(256), 0, st, own);
+  else
+    hipLaunchKernelGGL((attn_rows_whole<T, HD, 32>), grid, dim3(256), 0, st, own);
+  return static_cast<int>(hipGetLastError());
+}
+
 template <typename T, int HD>
 int launch_hd(const rows::Args& a, const rows::Args& own, const Split& d, hipStream_t st) {
+  if (d.whole) return launch_whole<T, HD>(own, d, st);
   const int64_t np = static_cast<int64_t>(a.Hkv) * a.splits * a.row_tiles;
   const int64_t no = static_cast<int64_t>(a.Hkv) * own.splits * own.row_tiles * own.B;
   if (d.prefix_rows <= 16) launch_one<T, HD, 16, 16>(a, own, np, no, st);
@@ -186,8 +212,7 @@ int launch_hd(const rows::Args& a, const rows::Args& own, const Split& d, hipStr
 template <typename T>
 int launch(const rows::Args& a, const rows::Args& own, const CombineArgs& c, const Shape& s, const Split& d, hipStream_t st) {
   int e = MI355_E_HEAD_DIM;
-  if (d.prefix_splits + d.own_splits == 0) e = MI355_OK;  // no key at all: the join writes zeros
-  else switch (s.hd) {
+  switch (s.hd) {
     case 16: e = launch_hd<T, 16>(a, own, d, st); break;
     case 32: e = launch_hd<T, 32>(a, own, d, st); break;
     case 48: e = launch_hd<T, 48>(a, own, d, st); break;
@@ -198,7 +223,7 @@ int launch(const rows::Args& a, const rows::Args& own, const CombineArgs& c, con
     case 192: e = launch_hd<T, 192>(a, own, d, st); break;
     case 256: e = launch_hd<T, 256>(a, own, d, st); break;
   }
-  if (e) return e;
+  if (e || d.whole) return e;
   if (d.prefix_splits + d.own_splits <= WAVE_SPLITS)
     hipLaunchKernelGGL((combine_splits<T, 1>), dim3(static_cast<unsigned>(ceil_div(c.rows, 4))), dim3(256), 0, st, c);
   else
@@ -233,9 +258,10 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
   if (!(scale > 0.f) || scale > 1e30f) return MI355_E_UNSUPPORTED;
   if (s.rows() == 0) return MI355_OK;
   if (!Q || !O || !own_lens || !q_strides || !kp_strides || !vp_strides || !ko_strides || !vo_strides ||
-      !o_strides || !workspace || (prefix_len > 0 && (!K_prefix || !V_prefix)) || (room > 0 && (!K_own || !V_own)))
+      !o_strides || (prefix_len > 0 && (!K_prefix || !V_prefix)) || (room > 0 && (!K_own || !V_own)))
     return MI355_E_NULL_POINTER;
   const Split d = split_of(s);
+  if (!d.whole && !workspace) return MI355_E_NULL_POINTER;
   if (workspace_bytes < (d.prefix_splits + d.own_splits) * s.rows() * (head_dim + 2) * 4) return MI355_E_BAD_SIZE;
   // token strides of K and V: rows that do not overlap, whose tiles' offsets fit 32 bits
   for (const int64_t t : {prefix_len > 0 ? kp_strides[0] : head_dim, prefix_len > 0 ? vp_strides[0] : head_dim,
@@ -274,6 +300,12 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
   own.vb = vo_strides[0]; own.vt = vo_strides[1]; own.vh = vo_strides[2];
   own.keys = static_cast<int32_t>(room);
   own.lens = own_lens;
+  own.pk = K_prefix; own.pv = V_prefix;
+  own.pkt = kp_strides[0]; own.pkh = kp_strides[1];
+  own.pvt = vp_strides[0]; own.pvh = vp_strides[1];
+  own.pkeys = a.keys;
+  own.o = O;
+  own.ob = o_strides[0]; own.ot = o_strides[1]; own.oh = o_strides[2];
   a.chunk = static_cast<int32_t>(d.prefix_chunk);
   a.splits = static_cast<int32_t>(d.prefix_splits);
   a.row_tiles = static_cast<int32_t>(ceil_div(B * n_q * G, d.prefix_rows));

@@ -16,7 +16,9 @@
 
 namespace rows {
 
-enum Mode { PACKED = 0, PREFIX = 1, OWN = 2 };
+// What a work-group's rows attend to: a range of a packed sequence's keys; of the prefix, for rows of the
+// whole batch; of one sequence's own cache; prefix and cache one after the other (WHOLE: nothing to join).
+enum Mode { PACKED = 0, PREFIX = 1, OWN = 2, WHOLE = 3 };
 
 // Work on one tile of rows of one packed sequence (mi355_attn_packed_plan writes them).
 struct PackedTile {
@@ -41,10 +43,13 @@ struct Args {
   const PackedTile* tiles;
   int32_t causal;
   int64_t slots;          // partial rows of a K/V head: row (h slots + slot + i) of part / ml
-  // PREFIX / OWN: rows of a sequence are its n_q tokens' heads
+  // PREFIX / OWN / WHOLE: rows of a sequence are its n_q tokens' heads
   int32_t B, n_q;
-  int32_t keys;           // PREFIX: prefix keys; OWN: keys a cache has room for
-  const int32_t* lens;    // OWN: keys in each cache (clamped to [0, keys])
+  int32_t keys;           // PREFIX: prefix keys; OWN, WHOLE: keys a cache has room for
+  const int32_t* lens;    // OWN, WHOLE: keys in each cache (clamped to [0, keys])
+  const void *pk, *pv;    // WHOLE: the prefix, its token and head strides and keys (k, v: the caches)
+  int64_t pkt, pkh, pvt, pvh;
+  int32_t pkeys;
   int32_t chunk;          // keys of a split
   int32_t splits, row_tiles;
   int32_t part0;          // first split's index in part / ml
@@ -150,6 +155,17 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     Kb = static_cast<const T*>(p.k) + t.k0 * p.kt + h * p.kh;
     Vb = static_cast<const T*>(p.v) + t.k0 * p.vt + h * p.vh;
     out_tok = t.q0;
+  } else if constexpr (MODE == WHOLE) {
+    h = static_cast<int>(block % static_cast<unsigned>(p.Hkv));
+    b = static_cast<int>(block / static_cast<unsigned>(p.Hkv));
+    row0 = k_begin = 0;
+    nrows = p.n_q * p.G;
+    const int given = p.lens[b];
+    k_end = given < 0 ? 0 : (given < p.keys ? given : p.keys);
+    k_off = k_end - p.n_q + 1;
+    Qb = static_cast<const T*>(p.q) + b * p.qb;
+    Kb = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
+    Vb = static_cast<const T*>(p.v) + b * p.vb + h * p.vh;
   } else {
     unsigned x = block;
     h = static_cast<int>(x % static_cast<unsigned>(p.Hkv));
@@ -180,7 +196,8 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   }
   Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
   Vb = uniform_ptr(Vb + static_cast<int64_t>(k_begin) * p.vt);
-  const int n_keys = k_end - k_begin;  // keys from here on are counted from k_begin
+  int n_keys = k_end - k_begin;  // keys from here on are counted from k_begin
+  int64_t kt = p.kt, vt = p.vt;
   const int row_w = OWN_KEYS ? row0 : row0 + wave * QW;
   const int lwave = OWN_KEYS ? 0 : wave;
   if constexpr (OWN_KEYS) lds += wave * 2 * TILE;
@@ -197,12 +214,18 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     }
   };
   // keys [0, lim) of the work-group's range are seen by row r
+  int lim_off = k_off - k_begin;
   const auto lim_of = [&](int r) MI355_LAMBDA_INLINE {
-    const int lim = r / p.G + k_off - k_begin;
+    const int lim = r / p.G + lim_off;
     return lim < n_keys ? lim : n_keys;
   };
 
-  // row r's partial result
+  // row r's output, or its partial result
+  const bool direct = MODE == WHOLE || (MODE == PACKED && slot < 0);
+  const auto out_of = [&](int r) MI355_LAMBDA_INLINE {
+    const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+    return static_cast<T*>(p.o) + (MODE == WHOLE ? b * p.ob : out_tok * p.ot) + t * p.ot + hh * p.oh;
+  };
   const auto part_of = [&](int r) MI355_LAMBDA_INLINE {
     if constexpr (MODE == PACKED) {
       return slot + (r - row0);
@@ -214,7 +237,6 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 
   // Q^T fragments: lane (row l16 of group n, slice g) holds elements 32 s + 8 g ..
   frag qf[QG][KS];
-  int lim[QG];
   const bool upper = HALF && g >= 2;
   const auto lower_half = [&](u32x4 v) MI355_LAMBDA_INLINE { return upper ? u32x4{0u, 0u, 0u, 0u} : v; };
 #pragma unroll
@@ -222,7 +244,6 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     const int r = row_w + 16 * n + l16;
     const bool real = r < nrows;
     const T* src = Qb + q_of(real ? r : nrows - 1);
-    lim[n] = lim_of(real ? r : nrows - 1);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const bool half = HALF && s == KS - 1;
@@ -230,20 +251,42 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       qf[n][s] = __builtin_bit_cast(frag, half ? lower_half(v) : v);
     }
   }
-  const int lim_first = MODE == PREFIX ? n_keys : __builtin_amdgcn_readfirstlane(lim[0]);
-  const int lim_last = MODE == PREFIX ? n_keys : lim_of(row_w + QW - 1 < nrows ? row_w + QW - 1 : nrows - 1);
-
-  // loads: lane i of block blk lands at chunk 64 blk + i of the tile, so it fetches the logical
-  // chunk that the swizzle places there; rows past the last key read as zeros
-  const uint32_t kstride = static_cast<uint32_t>(p.kt) * sizeof(T), vstride = static_cast<uint32_t>(p.vt) * sizeof(T);
-  const uint32_t kcap = 0xffffffffu / kstride, vcap = 0xffffffffu / vstride;
-  uint32_t koff[LPW], voff[LPW];
+  // What the sweep over the keys goes by. Loads: lane i of block blk lands at chunk 64 blk + i of the tile,
+  // so it fetches the logical chunk that the swizzle places there; rows past the last key read as zeros.
+  int lim[QG], lim_first, lim_last;
+  uint32_t kstride, vstride, kcap, vcap, koff[LPW], voff[LPW];
+  const auto bind = [&]() MI355_LAMBDA_INLINE {
 #pragma unroll
-  for (int i = 0; i < LPW; ++i) {
-    const int at = (lwave + i * LW) * 64 + lane, row = at / NCH, ch = (at % NCH) ^ swz<NCH>(row);
-    koff[i] = static_cast<uint32_t>(row) * kstride + ch * 16;
-    voff[i] = static_cast<uint32_t>(row) * vstride + ch * 16;
-  }
+    for (int n = 0; n < QG; ++n) lim[n] = lim_of(row_w + 16 * n + l16 < nrows ? row_w + 16 * n + l16 : nrows - 1);
+    lim_first = MODE == PREFIX ? n_keys : __builtin_amdgcn_readfirstlane(lim[0]);
+    lim_last = MODE == PREFIX ? n_keys : lim_of(row_w + QW - 1 < nrows ? row_w + QW - 1 : nrows - 1);
+    kstride = static_cast<uint32_t>(kt) * sizeof(T);
+    vstride = static_cast<uint32_t>(vt) * sizeof(T);
+    kcap = 0xffffffffu / kstride;
+    vcap = 0xffffffffu / vstride;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int at = (lwave + i * LW) * 64 + lane, row = at / NCH, ch = (at % NCH) ^ swz<NCH>(row);
+      koff[i] = static_cast<uint32_t>(row) * kstride + ch * 16;
+      voff[i] = static_cast<uint32_t>(row) * vstride + ch * 16;
+    }
+  };
+  // WHOLE: the prefix in the place of the cache, and back
+  const T *const own_k = Kb, *const own_v = Vb;
+  const int own_keys = n_keys;
+  const auto bind_part = [&](int part) MI355_LAMBDA_INLINE {
+    if constexpr (MODE == WHOLE) {
+      const T* pk = uniform_ptr(static_cast<const T*>(p.pk) + h * p.pkh);
+      const T* pv = uniform_ptr(static_cast<const T*>(p.pv) + h * p.pvh);
+      Kb = part == 0 ? pk : own_k;
+      Vb = part == 0 ? pv : own_v;
+      n_keys = part == 0 ? p.pkeys : own_keys;
+      kt = part == 0 ? p.pkt : p.kt;
+      vt = part == 0 ? p.pvt : p.vt;
+      lim_off = part == 0 ? 0x40000000 : k_off;
+    }
+    bind();
+  };
   auto issue_k = [&](int j, int st) MI355_LAMBDA_INLINE {
     const uint32_t key = static_cast<uint32_t>(j) * BN, rem = static_cast<uint32_t>(n_keys) - key;
     const u32x4 kr = buffer_rsrc(reinterpret_cast<const char*>(Kb) + static_cast<uint64_t>(key) * kstride,
@@ -383,34 +426,39 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       }
   };
 
-  const int n_kt = (n_keys + BN - 1) / BN;
   if constexpr (OWN_KEYS) {
     // K of the next tile is requested as soon as this one's has been read, V likewise, so that one of
     // them is always in flight: of the 2 LPW newest loads the older LPW have to be there.
     static_assert(LPW < 64, "vmcnt");
     constexpr int OLDER = (LPW & 15) | (LPW >> 4) << 14 | 7 << 4 | 15 << 8;  // vmcnt(LPW)
     constexpr int READ = 15 | 3 << 14 | 7 << 4;                              // lgkmcnt(0)
-    const int n_mine = n_kt < (lim_last + BN - 1) / BN ? n_kt : (lim_last + BN - 1) / BN;
-    if (wave < n_mine) {
-      issue_k(wave, 0);
-      issue_v(wave, 0);
-    }
-    for (int j = wave; j < n_mine; j += NW) {
-      const bool more = j + NW < n_mine;
-      __builtin_amdgcn_s_waitcnt(OLDER);
-      tile(j, 0,
-           [&]() MI355_LAMBDA_INLINE {
-             __builtin_amdgcn_s_waitcnt(READ);
-             if (more) issue_k(j + NW, 0);
-           },
-           [&]() MI355_LAMBDA_INLINE {
-             if (more) __builtin_amdgcn_s_waitcnt(OLDER);
-             else __builtin_amdgcn_s_waitcnt(0);
-           });
-      __builtin_amdgcn_s_waitcnt(READ);
-      if (more) issue_v(j + NW, 0);
+    for (int part = MODE == WHOLE ? 0 : 1; part < 2; ++part) {
+      bind_part(part);
+      const int n_kt = (n_keys + BN - 1) / BN;
+      const int n_mine = n_kt < (lim_last + BN - 1) / BN ? n_kt : (lim_last + BN - 1) / BN;
+      if (wave < n_mine) {
+        issue_k(wave, 0);
+        issue_v(wave, 0);
+      }
+      for (int j = wave; j < n_mine; j += NW) {
+        const bool more = j + NW < n_mine;
+        __builtin_amdgcn_s_waitcnt(OLDER);
+        tile(j, 0,
+             [&]() MI355_LAMBDA_INLINE {
+               __builtin_amdgcn_s_waitcnt(READ);
+               if (more) issue_k(j + NW, 0);
+             },
+             [&]() MI355_LAMBDA_INLINE {
+               if (more) __builtin_amdgcn_s_waitcnt(OLDER);
+               else __builtin_amdgcn_s_waitcnt(0);
+             });
+        __builtin_amdgcn_s_waitcnt(READ);
+        if (more) issue_v(j + NW, 0);
+      }
     }
   } else {
+    bind();
+    const int n_kt = (n_keys + BN - 1) / BN;
     const auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
       issue_k(j, st);
       issue_v(j, st);
@@ -439,7 +487,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   // computed again, by a wave, one key at a time over the keys they see (a row that sees a NaN gets it again).
   const auto again = [&](int r) MI355_LAMBDA_INLINE {
     const int keys = lim_of(r);
-    if (MODE == PREFIX || keys <= 0 || keys >= n_keys) return;
+    if (MODE == PREFIX || keys >= n_keys || (MODE != WHOLE && keys <= 0)) return;
     constexpr int DL = (HD + 63) / 64;
     const T* src = Qb + q_of(r);
     float q[DL], acc[DL], m = NEG_INF, l = 0.f;
@@ -448,27 +496,30 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       q[i] = lane + 64 * i < HD ? to_f32(src[lane + 64 * i]) : 0.f;
       acc[i] = 0.f;
     }
-    for (int key = 0; key < keys; ++key) {
-      const T* kr = Kb + static_cast<int64_t>(key) * p.kt;
-      const T* vr = Vb + static_cast<int64_t>(key) * p.vt;
-      float s = 0.f;
+    for (int part = MODE == WHOLE ? 0 : 1; part < 2; ++part) {
+      if constexpr (MODE == WHOLE) bind_part(part);
+      const int count = part == 0 ? n_keys : keys;
+      for (int key = 0; key < count; ++key) {
+        const T* kr = Kb + key * kt;
+        const T* vr = Vb + key * vt;
+        float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < DL; ++i)
-        if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
-      for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
-      s *= p.c;
-      const float m2 = vmax(m, s);
-      const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
-      const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
-      l = __builtin_fmaf(l, a, e);
+        for (int i = 0; i < DL; ++i)
+          if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
+        for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+        s *= p.c;
+        const float m2 = vmax(m, s);
+        const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
+        const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
+        l = __builtin_fmaf(l, a, e);
 #pragma unroll
-      for (int i = 0; i < DL; ++i)
-        if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
-      m = m2;
+        for (int i = 0; i < DL; ++i)
+          if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
+        m = m2;
+      }
     }
-    if (MODE == PACKED && slot < 0) {
-      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
-      T* dst = static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh;
+    if (direct) {
+      T* dst = out_of(r);
 #pragma unroll
       for (int i = 0; i < DL; ++i)
         if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
@@ -486,8 +537,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   // 4 elements of row r from element d on; returns whether one is NaN
   const auto put = [&](int r, int d, f32x4 v, float sum, bool sees) MI355_LAMBDA_INLINE {
     bool bad = false;
-    if (MODE == PACKED && slot < 0) {
-      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+    if (direct) {
       // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
       const float inv = 1.0f / sum;
       frag4 w;
@@ -497,7 +547,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
         bad |= x != x;
         w[e] = from_f32<T>(x);
       }
-      *reinterpret_cast<frag4*>(static_cast<T*>(p.o) + (out_tok + t) * p.ot + hh * p.oh + d) = w;
+      *reinterpret_cast<frag4*>(out_of(r) + d) = w;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) bad |= v[e] != v[e];
@@ -506,7 +556,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     return bad;
   };
   const auto put_ml = [&](int r, float m, float sum) MI355_LAMBDA_INLINE {
-    if (MODE == PACKED && slot < 0) return;
+    if (direct) return;
     const int64_t at = part_of(r);
     p.ml[2 * at] = m;
     p.ml[2 * at + 1] = sum;
@@ -549,7 +599,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], f, v[e]);
       }
-      if (put(row0 + x, 4 * d, v, sum, lim_of(row0 + x) > 0)) atomicOr(&nan_rows, 1u << x);
+      if (put(row0 + x, 4 * d, v, sum, lim_of(row0 + x) > 0 || (MODE == WHOLE && p.pkeys > 0))) atomicOr(&nan_rows, 1u << x);
       if (d == 0) put_ml(row0 + x, m, sum);
     }
     if constexpr (MODE != PREFIX) {

@@ -394,8 +394,9 @@ __global__ __launch_bounds__(KW == 8 ? 512 : 256) void linear_i4_few(I4Args p, i
 
 template <typename T, int GROUP, int M, int CH, int KW, typename TO>
 int launch_few(const I4Args& a, hipStream_t s) {
-  // enough waves for the CUs (12 each), several groups of 4 features a wave beyond that
-  const int64_t waves = static_cast<int64_t>(a.N) * KW / 3072;
+  // enough waves for the CUs (8 each), several groups of 4 features a wave beyond that: each wave loads x
+  // (1024 to 4096 waves: 2 x 4096 x 16384 18.6, 13.4, 11.9, 13.3, 13.2 us, 1 x 65536 x 2048 19.7, 18.4, 15.8, 17.8, 16.2)
+  const int64_t waves = static_cast<int64_t>(a.N) * KW / 2048;
   const int per_wave = static_cast<int>(waves < 8 ? 4 : waves >= MAX_FEW ? MAX_FEW : waves / 4 * 4);
   constexpr int NW = KW == 8 ? 8 : 4;
   const int64_t wg = per_wave * (NW / KW);
@@ -435,16 +436,13 @@ int launch_nw(const I4Args& a, hipStream_t s) {
 }
 template <typename T, int GROUP, typename TO>
 int launch_mt(const I4Args& a, hipStream_t s) {
-  // One or two rows: linear_i4_few (1 x 12288 x 4096 7.9 us against 11.5, 1 x 4096 x 16384, group 64, 10.1
-  // against 17.3; with two rows 9.2 against 11.7 and 13.2 against 17.6). Three and four, where it multiplies
-  // four, only with groups of 32, whose many scales cost the MFMA kernel more (4 x 11008 x 4096 12.9
-  // against 17.2; group 128: 4 x 65536 x 2048 31.0 against 26.5). Below 512 k most of a wave would idle.
+  // Up to four rows: linear_i4_few (against the MFMA kernel, us: 1 x 12288 x 4096 7.7 / 11.5, 2 x 9.4 / 11.7,
+  // 4 x 12.9 / 13.0; 1 x 4096 x 16384, group 64, 10.2 / 17.3, 2 x 11.9 / 17.6, 4 x 15.6 / 18.7;
+  // 4 x 11008 x 4096, group 32, 12.3 / 17.2; eight rows 18.4 / 14.4). Below 512 k most of a wave would idle.
   if (a.K >= 512 && a.K <= 16384) {
     if (a.M == 1) return launch_few_k<T, GROUP, 1, TO>(a, s);
     if (a.M == 2) return launch_few_k<T, GROUP, 2, TO>(a, s);
-    if constexpr (GROUP == 32) {
-      if (a.M <= 4) return launch_few_k<T, GROUP, 4, TO>(a, s);
-    }
+    if (a.M <= 4) return launch_few_k<T, GROUP, 4, TO>(a, s);
   }
   if (a.M <= 16) return launch_nw<T, GROUP, 1, TO>(a, s);
   if (a.M <= 32) return launch_nw<T, GROUP, 2, TO>(a, s);

@@ -816,9 +816,9 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     kp, vp, ko, vo = k_prefix.data_ptr(), v_prefix.data_ptr(), k_own.data_ptr(), v_own.data_ptr()
     if (qp | kp | vp | ko | vo) & 15 or op & 7:
         _check_aligned(q=qp, k_prefix=kp, v_prefix=vp, k_own=ko, v_own=vo, out=op)
-    ws = torch.empty((max(need, 16),), device=q.device, dtype=torch.uint8)
+    ws = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
     st = _launch(dev, _lib.lib().mi355_attn_shared_prefix, code, qp, kp, vp, ko, vo, own_lens.data_ptr(), op,
-                 *sizes, *strides, scale, ws.data_ptr(), need)
+                 *sizes, *strides, scale, ws.data_ptr() if need else 0, need)
     if st:
         _lib.check("mi355_attn_shared_prefix", st)
     return out
