@@ -612,17 +612,23 @@ def _scale(scale: Optional[float], head_dim: int) -> float:
     return scale
 
 
+@functools.lru_cache(maxsize=2048)
+def _bytes(shape, stride, dtype) -> int:
+    """From a view's first to behind its last byte."""
+    if 0 in shape:
+        return 0
+    return (1 + sum((n - 1) * st for n, st in zip(shape, stride))) * dtype.itemsize
+
+
 def _check_apart(out: torch.Tensor, *inputs: Optional[torch.Tensor]) -> None:
     """Refuses an ``out`` whose bytes (first to last) meet an input's."""
-    def span(t):
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    if out.numel() == 0:
-        return
-    lo, hi = span(out)
+    lo = out.data_ptr()
+    hi = lo + _bytes(out.shape, out.stride(), out.dtype)
     for t in inputs:
-        if t is not None and t.numel() and span(t)[0] < hi and lo < span(t)[1]:
-            raise ValueError("out shares memory with an input")
+        if t is not None:
+            start = t.data_ptr()
+            if start < hi and lo < start + _bytes(t.shape, t.stride(), t.dtype):
+                raise ValueError("out shares memory with an input")
 
 
 @dataclass(frozen=True, eq=False)
@@ -715,7 +721,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     if dev < 0 or k.get_device() != dev or v.get_device() != dev or plan.tiles.get_device() != dev or (
             out is not None and out.get_device() != dev):
         _on_gpu(q, k, v, plan.tiles, out)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         _no_backward(q, k, v)
     given = out is not None
     code, (qst, kst, vst, ost) = _packed_views(
@@ -727,7 +733,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     if given:
         _check_apart(out, q, k, v)
     else:  # (rows behind the last token have no value)
-        out = (torch.empty if q.shape[0] == plan.q_tokens else torch.zeros)(q.shape, device=q.device, dtype=q.dtype)
+        out = q.new_empty(q.shape) if q.shape[0] == plan.q_tokens else q.new_zeros(q.shape)
     if plan.tiles.shape[0] == 0:
         return out
     qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
@@ -809,7 +815,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
     if given:
         _check_apart(out, q, k_prefix, v_prefix, k_own, v_own, own_lens)
     else:
-        out = torch.empty(q.shape, device=q.device, dtype=dt)
+        out = q.new_empty(q.shape)
     if out.numel() == 0:
         return out
     qp, op = q.data_ptr(), out.data_ptr()
@@ -901,7 +907,7 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     if dev < 0 or w.get_device() != dev or scale.get_device() != dev or (zero is not None and zero.get_device() != dev) \
             or (bias is not None and bias.get_device() != dev) or (out is not None and out.get_device() != dev):
         _on_gpu(x, w, scale, zero, bias, out)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)):
         _no_backward(x, scale, bias)
     odt = out_dtype or (out.dtype if out is not None else x.dtype)
     if out is not None and out.dtype != odt:
@@ -911,11 +917,11 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
         *((zero.dtype, zero.shape) if zero is not None else (None, None)),
         *((bias.dtype, bias.shape) if bias is not None else (None, None)), odt,
         *((out.shape, out.stride()) if out is not None else (None, None)))
-    for name, t in (("w", w), ("scale", scale), ("zero", zero), ("bias", bias)):
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+    if not (w.is_contiguous() and scale.is_contiguous() and (zero is None or zero.is_contiguous())
+            and (bias is None or bias.is_contiguous())):
+        raise ValueError("w, scale, zero and bias must be contiguous")
     if out is None:
-        out = torch.empty((M, N), device=x.device, dtype=odt)
+        out = x.new_empty((M, N)) if odt is x.dtype else x.new_empty((M, N), dtype=odt)
     else:
         _check_apart(out, x, w, scale, zero, bias)
     if M == 0 or N == 0:
