@@ -16,13 +16,19 @@ bool packed_head_dim(int64_t hd) {
 
 constexpr int64_t MAX_TOKENS = int64_t(1) << 30;
 
-// Rows of a tile. Sequences of up to 32 rows (a token or a few) take NARROW ones, whose keys four waves share out; the others
-// WIDE ones of four waves, two groups of 16 rows each, where those give every CU two work-groups, else
-// of one group (HALF). Measured (TFLOP/s; 8192 tokens with 32/8 heads of 128, 24 prompts of 33-2011 with 32/4
-// heads of 128, 8 pieces of 200-512 tokens against up to 5500 keys, 16 heads of 64 (416 WIDE tiles)):
-// WIDE with 32-key tiles 1156, 918, 432; with 64-key tiles 1148, 842, 510; HALF 990, 805, 544 and 908, 686, 613;
-// a wave of 32 rows 286, 232, 320; eight waves of 32 rows 1098-1174, 776, 341-408.
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Rows of a tile. Sequences of up to 32 rows (a token or a few) take NARROW ones, whose keys four waves
+// share out; the others WIDE ones of four waves of two groups of 16 rows, or HALF ones of one group where WIDE
+// ones leave CUs without work: fewer than two a CU, above head dim 64 counting the ranges that their keys are
+// split into. Measured (us, WIDE / HALF; 32/8 heads of 128 but where noted): 8192 tokens 478 / 555; 24 prompts of
+// 33-2011 (32/4) 135 / 152; 512 tokens against 8192 keys 80 / 100; 2048 against 16384 (8/2) 151 / 176; 4 x 100
+// against 3000 42 / 41; 3 x 700 (16/4) 30 / 19; 1000 32 / 28; heads of 64: 8 pieces of 200-512 against up to 5500
+// keys (16/16) 77 / 59, 300 against 6000 (16/16) 24 / 22. WIDE tiles take 32 keys at a time (64 keys: 8192 tokens
+// 479, the 24 prompts 146), HALF ones 64 up to head dim 64 (32 keys: the pieces 67).
 constexpr int WIDE = 128, HALF = 64, NARROW = 32;
+// Least keys of a range of a WIDE or HALF tile: its partial rows are 4 bytes an element, twice.
+constexpr int64_t WIDE_KEYS = 512;
 
 // What a plan starts with: its sizes; tiles of 128 or 64 rows, then of 32, then the joins.
 struct Counts {
@@ -144,8 +150,6 @@ int launch(const rows::Args& a, int64_t hd, const Counts& n, int wide_rows, hipS
   return static_cast<int>(hipGetLastError());
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 bool fits(const Counts& n, int64_t kv_heads) {
   const int64_t most = 0x7fffffffLL;
   return n.wide >= 0 && n.narrow >= 0 && n.joins >= 0 && n.slots >= 0 && n.wide <= most / kv_heads &&
@@ -163,20 +167,22 @@ extern "C" int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_le
   if (!packed_head_dim(head_dim)) return MI355_E_HEAD_DIM;
   if (!counts || !tile_rows || (n_seqs > 0 && (!q_lens || !k_lens))) return MI355_E_NULL_POINTER;
   const int64_t G = heads / kv_heads;
-  int64_t tq = 0, tk = 0, wide = 0, few = 0, few_keys = 0;
+  int64_t tq = 0, tk = 0, wide = 0, wide_ranges = 0, few = 0, few_keys = 0;
   for (int64_t i = 0; i < n_seqs; ++i) {
     if (q_lens[i] < 0 || k_lens[i] < 0) return MI355_E_BAD_SIZE;
     tq += q_lens[i];
     tk += k_lens[i];
     if (tq >= MAX_TOKENS || tk >= MAX_TOKENS || q_lens[i] * G >= MAX_TOKENS) return MI355_E_BAD_SIZE;
     if (q_lens[i] * G > NARROW) {
-      wide += ceil_div(q_lens[i] * G, WIDE);
+      const int64_t tiles = ceil_div(q_lens[i] * G, WIDE);
+      wide += tiles;
+      wide_ranges += tiles * std::max<int64_t>(1, k_lens[i] / WIDE_KEYS);
     } else if (q_lens[i] > 0) {
       ++few;
       few_keys = std::max<int64_t>(few_keys, k_lens[i]);
     }
   }
-  const int wide_rows = wide * kv_heads >= 512 ? WIDE : HALF;
+  const int wide_rows = (head_dim > 64 ? wide_ranges : wide) * kv_heads >= 512 ? WIDE : HALF;
   // A few short sequences of few rows beside others take the others' tiles, which saves a launch.
   const int64_t narrow = wide > 0 && few * kv_heads <= 256 && few_keys <= 512 ? 0 : NARROW;
   struct Ref {
@@ -218,7 +224,7 @@ extern "C" int mi355_attn_packed_plan(const int32_t* q_lens, const int32_t* k_le
     });
     int64_t chunk[2];
     for (int w = 0; w < 2; ++w) {
-      const int64_t at_once = 512, least = w ? 256 : 512;
+      const int64_t at_once = 512, least = w ? 256 : WIDE_KEYS;
       const int64_t share = ceil_div(ceil_div(keys_of[w] * kv_heads, at_once), 64) * 64;
       chunk[w] = tiles_of[w] * kv_heads >= at_once ? MAX_TOKENS : std::max(least, share);
     }
