@@ -25,7 +25,7 @@ struct Split {
 
 // most splits of the prefix or of a cache, and of both together for one wave to join
 constexpr int64_t MAX_SPLITS = 512;
-constexpr int WAVE_SPLITS = 16;
+constexpr int WAVE_SPLITS = 32;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -42,13 +42,20 @@ Split split_of(const Shape& s) {
     return d;
   }
   // As many ranges as fill the work-groups that run at once (two a CU), half of them where the prefix is
-  // matrix work: each range writes partial rows, and the caches' ranges run beside it.
-  const auto chunk = [](int64_t keys, int64_t groups, int64_t want) {
+  // matrix work. There each range writes 128 partial rows a head, so ranges are longer still where the caches
+  // run beside them for long enough, at 40 keys of a range for each us of half-full caches at 5 TB/s (64
+  // sequences, 32/8 heads of 128, behind 8192 keys, caches of up to 1024: 52 us with at least 1024 keys, 56 with
+  // 256; 128 sequences behind 2048, up to 512: 43 and 49; but 27 and 33 with caches of 16; 24 x 4 tokens, 16/16
+  // heads of 64, behind 2047, up to 777: 22 and 17).
+  const auto chunk = [](int64_t keys, int64_t groups, int64_t want, int64_t least) {
     const int64_t splits = std::min(MAX_SPLITS, std::max<int64_t>(1, want / std::max<int64_t>(1, groups)));
-    return std::max<int64_t>(256, ceil_div(ceil_div(keys, splits), 64) * 64);
+    return std::max<int64_t>(least, ceil_div(ceil_div(keys, splits), 64) * 64);
   };
-  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows <= 64 ? 512 : 256);
-  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, 512);
+  const bool matrix = d.prefix_rows == 128;
+  const int64_t beside = s.B * s.room * s.Hkv * s.hd * 4 / 250000;
+  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, matrix ? 256 : 512,
+                         matrix ? std::min<int64_t>(1024, std::max<int64_t>(256, beside / 64 * 64)) : 256);
+  d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, 512, 256);
   d.prefix_splits = ceil_div(s.prefix, d.prefix_chunk);
   d.own_splits = ceil_div(s.room, d.own_chunk);
   return d;
