@@ -41,8 +41,9 @@ Split split_of(const Shape& s) {
     d.own_rows = orows <= 16 ? 16 : 32;
     return d;
   }
-  // As many ranges as fill the work-groups that run at once (two a CU), half of them where the prefix is
-  // matrix work. There each range writes 128 partial rows a head, so ranges are longer still where the caches
+  // As many ranges as fill the work-groups that run at once (two a CU), half of them where the prefix has 64 rows
+  // and more: there the waves share tiles (16 sequences, 32/8 heads of 128, behind 65521 keys: 88 us with one a
+  // CU, 91 with two, 98 with four). With 128 rows (matrix work) each range writes 128 partial rows a head, so ranges are longer still where the caches
   // run beside them for long enough, at 40 keys of a range for each us of half-full caches at 5 TB/s (64
   // sequences, 32/8 heads of 128, behind 8192 keys, caches of up to 1024: 52 us with at least 1024 keys, 56 with
   // 256; 128 sequences behind 2048, up to 512: 43 and 49; but 27 and 33 with caches of 16; 24 x 4 tokens, 16/16
@@ -53,7 +54,7 @@ Split split_of(const Shape& s) {
   };
   const bool matrix = d.prefix_rows == 128;
   const int64_t beside = s.B * s.room * s.Hkv * s.hd * 4 / 250000;
-  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, matrix ? 256 : 512,
+  d.prefix_chunk = chunk(s.prefix, ceil_div(pr, d.prefix_rows) * s.Hkv, d.prefix_rows >= 64 ? 256 : 512,
                          matrix ? std::min<int64_t>(1024, std::max<int64_t>(256, beside / 64 * 64)) : 256);
   d.own_chunk = chunk(s.room, s.B * ceil_div(orows, d.own_rows) * s.Hkv, 512, 256);
   d.prefix_splits = ceil_div(s.prefix, d.prefix_chunk);
