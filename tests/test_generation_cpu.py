@@ -78,7 +78,7 @@ def test_plan_covers_every_row_and_key_once(q_lens, k_lens, heads, kv_heads, cau
 @pytest.mark.parametrize("kw,status", [
     (dict(heads=3), BAD_SIZE), (dict(heads=0), BAD_SIZE), (dict(kv_heads=0), BAD_SIZE), (dict(head_dim=8), HEAD),
     (dict(head_dim=0), HEAD), (dict(q_lens=[-1]), BAD_SIZE), (dict(k_lens=[-1]), BAD_SIZE),
-    (dict(q_lens=[1 << 29], heads=8, kv_heads=1), BAD_SIZE), (dict(q_lens=[1 << 29, 1 << 29], k_lens=[1, 1]), BAD_SIZE)])
+    (dict(q_lens=[1 << 29], heads=8, kv_heads=1), BAD_SIZE), (dict(q_lens=[1 << 25], k_lens=[1], heads=4096, kv_heads=4096), BAD_SIZE), (dict(q_lens=[1 << 29, 1 << 29], k_lens=[1, 1]), BAD_SIZE)])
 def test_plan_refusals(kw, status):
     kw = {"q_lens": [4], "k_lens": [4], **kw}
     assert plan(**kw)[0] == status
@@ -119,7 +119,7 @@ PREFIX = dict(dtype=F16, ptrs=[64] * 7, B=2, n=1, heads=4, kv_heads=2, head_dim=
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(dtype=F32), DTYPE), (dict(heads=5), BAD_SIZE), (dict(B=-1), BAD_SIZE), (dict(n=-1), BAD_SIZE), (dict(P=-1), BAD_SIZE),
+    (dict(dtype=F32), DTYPE), (dict(heads=5), BAD_SIZE), (dict(B=-1), BAD_SIZE), (dict(B=60000, n=100), BAD_SIZE), (dict(n=-1), BAD_SIZE), (dict(P=-1), BAD_SIZE),
     (dict(room=1 << 30), BAD_SIZE), (dict(head_dim=24), HEAD), (dict(scale=0.0), UNSUP), (dict(scale=float("nan")), UNSUP),
     (dict(ws=0), NULL), (dict(ws_bytes=16), BAD_SIZE), (dict(ws=72), ALIGN), (dict(kps=(56, 64)), BAD_SIZE),
     (dict(vos=(6400, 64, 64), kv_heads=2, head_dim=128), BAD_SIZE), (dict(qs=(256, 256, 63)), ALIGN),
@@ -151,7 +151,7 @@ I4 = dict(dtype=F16, odt=F16, X=64, ldx=256, W=64, s=64, Y=64, ldy=100, M=3, N=1
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=F32), DTYPE), (dict(odt=BF16), DTYPE), (dict(odt=7), DTYPE), (dict(group=16), UNSUP), (dict(group=0), UNSUP),
-    (dict(K=224), BAD_SIZE), (dict(M=-1), BAD_SIZE), (dict(N=-1), BAD_SIZE), (dict(ldx=248), BAD_SIZE), (dict(ldy=99), BAD_SIZE),
+    (dict(K=224), BAD_SIZE), (dict(M=-1), BAD_SIZE), (dict(N=(1 << 26) + 1), BAD_SIZE), (dict(K=1 << 27, group=128), BAD_SIZE), (dict(N=-1), BAD_SIZE), (dict(ldx=248), BAD_SIZE), (dict(ldy=99), BAD_SIZE),
     (dict(ldx=260), ALIGN), (dict(X=72), ALIGN), (dict(W=68), ALIGN), (dict(X=0), NULL), (dict(W=0), NULL), (dict(s=0), NULL),
     (dict(Y=0), NULL)])
 def test_i4_entry_refusals(kw, status):
@@ -198,3 +198,22 @@ def test_quant_groups_i4_values():
     assert bool((((values - z.repeat_interleave(32, 1)) * s.float().repeat_interleave(32, 1))[1] + 7).abs().max() < 0.01)
     q, s, z = ops.quant_groups_i4(w, 32, symmetric=True)
     assert z is None and bool((q[1] == 0x11).all()) and bool((s[1] == 1).all())
+
+
+@pytest.mark.parametrize("shape,stride,kw", [
+    ((4, 2, 64), (128, 64, 2), {}), ((4, 2, 64), (130, 64, 1), {}), ((4, 2, 64), (128, 68, 1), {}),
+    ((4, 2, 64), (56, 64, 1), dict(kv_axis=0)), ((4, 2, 64), (0, 64, 1), dict(kv_axis=0)), ((4, 2, 64), (1 << 25, 64, 1), dict(kv_axis=0)),
+    ((4, 2, 64), (0, 64, 1), dict(written=True)), ((4, 2, 64), (128, 0, 1), dict(written=True)), ((4, 2, 64), (64, 128, 1), dict(written=True)),
+    ((4, 2, 64), (128, 32, 1), dict(written=True))])
+def test_view_refusals(shape, stride, kw):
+    with pytest.raises(ValueError):
+        ops._rows_strides("t", shape, stride, 8, **kw)
+
+
+@pytest.mark.parametrize("shape,stride,kw,want", [
+    ((4, 2, 64), (128, 64, 1), {}, (128, 64)), ((4, 2, 64), (64, 256, 1), dict(written=True), (64, 256)),
+    ((1, 2, 64), (3, 64, 1), dict(kv_axis=0), (64, 64)), ((4, 1, 64), (64, 5, 1), {}, (64, 0)),
+    ((4, 2, 64), (64, 0, 1), dict(kv_axis=0), (64, 0)), ((0, 2, 64), (128, 64, 1), dict(kv_axis=0), (64, 0))])
+def test_view_strides(shape, stride, kw, want):
+    """Axes of one element have any stride; heads may share one K / V head; orders other than the usual."""
+    assert ops._rows_strides("t", shape, stride, 8, **kw) == want

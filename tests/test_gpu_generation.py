@@ -604,6 +604,97 @@ def test_i4_graph_replay(gpu):
         assert torch.equal(out, ops.linear_i4(x, w, scale, zero))
 
 
+# ------------------------------------------------------------------------------ refusals, far offsets
+def test_refusals_on_the_gpu(gpu):
+    """What the kernels are not made for raises before anything is launched."""
+    ops = _ops()
+    q, k = torch.zeros(8, 4, 64, device=gpu).half(), torch.zeros(8, 2, 64, device=gpu).half()
+    plan = ops.packed_plan([5, 3], heads=4, kv_heads=2, head_dim=64, device=gpu)
+    cache, lens = torch.zeros(8, 10, 2, 64, device=gpu).half(), torch.zeros(8, dtype=torch.int32, device=gpu)
+    q4 = q.unsqueeze(1)
+    x, w = torch.zeros(3, 128, device=gpu).half(), torch.zeros(10, 64, dtype=torch.uint8, device=gpu)
+    s, z, b = torch.ones(10, 2, device=gpu).half(), torch.zeros(10, 2, dtype=torch.uint8, device=gpu), torch.zeros(10, device=gpu)
+    packed, prefix, i4 = ops.attention_packed, ops.attention_shared_prefix, ops.linear_i4
+    odd = torch.zeros(8 * 2 * 64 + 1, device=gpu).half()[1:].view(8, 2, 64)
+    grad = q.clone().requires_grad_()
+    own = [k, k, cache, cache, lens]
+    for error, call in [
+        (TypeError, lambda: packed(q.float(), k.float(), k.float(), plan)), (TypeError, lambda: packed(q, k.bfloat16(), k, plan)),
+        (ValueError, lambda: packed(q[:7], k, k, plan)), (ValueError, lambda: packed(q, k[:, :1], k, plan)),
+        (ValueError, lambda: packed(q, k, k[:7], plan)), (ValueError, lambda: packed(q[..., :32], k, k, plan)),
+        (ValueError, lambda: packed(q, odd, k, plan)), (ValueError, lambda: packed(q, k[:1].expand(8, 2, 64), k, plan)),
+        (ValueError, lambda: packed(q, k, k, plan, scale=0.0)), (ValueError, lambda: packed(q, k, k, plan, scale=math.inf)),
+        (ValueError, lambda: packed(q, k, k, plan, scale=math.nan)), (ValueError, lambda: packed(q, k, k, plan, out=q)),
+        (ValueError, lambda: packed(q, k, k, plan, out=q.new_zeros(8, 4, 32))), (TypeError, lambda: packed(q, k, k, plan, out=q.float())),
+        (ValueError, lambda: packed(q, k, k, plan, out=q.new_zeros(1, 4, 64).expand(8, 4, 64))),
+        (ValueError, lambda: packed(grad, k, k, plan)), (ValueError, lambda: packed(q.cpu(), k, k, plan)),
+        (ValueError, lambda: packed(q, k.cpu(), k, plan)),
+        (TypeError, lambda: prefix(q4.float(), *own)), (TypeError, lambda: prefix(q4, k.bfloat16(), *own[1:])),
+        (ValueError, lambda: prefix(q, *own)), (ValueError, lambda: prefix(q4[:7], *own)), (ValueError, lambda: prefix(q4[:, :, :3], *own)),
+        (ValueError, lambda: prefix(q4, k[:7], *own[1:])), (ValueError, lambda: prefix(q4, k, k, cache[:, :9], cache, lens)),
+        (ValueError, lambda: prefix(q4, *own[:4], lens.long())), (ValueError, lambda: prefix(q4, *own[:4], lens[:7])),
+        (ValueError, lambda: prefix(q4, *own[:4], torch.zeros(16, dtype=torch.int32, device=gpu)[::2])),
+        (ValueError, lambda: prefix(q4, *own, out=q4)), (ValueError, lambda: prefix(q4, *own[:4], lens.cpu())),
+        (ValueError, lambda: prefix(grad.unsqueeze(1), *own)), (ValueError, lambda: prefix(q4, *own, scale=-1.0)),
+        (ValueError, lambda: prefix(q4[..., :40], k[..., :40], k[..., :40], cache[..., :40], cache[..., :40], lens)),
+        (TypeError, lambda: i4(x.float(), w, s, z, b)), (TypeError, lambda: i4(x, w, s.bfloat16(), z, b)),
+        (TypeError, lambda: i4(x, w, s, z, b, out_dtype=torch.bfloat16)), (ValueError, lambda: i4(x, w[:9], s, z, b)),
+        (ValueError, lambda: i4(x[:, :96], w, s, z, b)), (ValueError, lambda: i4(x, w, s[:, :1], z, b)),
+        (ValueError, lambda: i4(x, w.char(), s, z, b)), (ValueError, lambda: i4(x, w, s, z.int(), b)), (ValueError, lambda: i4(x, w, s, z, b.half())),
+        (ValueError, lambda: i4(x, w, torch.ones(2, 10, device=gpu).half().t(), z, b)), (ValueError, lambda: i4(x.t().contiguous().t(), w, s, z, b)),
+        (ValueError, lambda: i4(torch.zeros(3, 129, device=gpu).half()[:, 1:], w, s, z, b)), (ValueError, lambda: i4(x[0], w, s, z, b)),
+        (ValueError, lambda: i4(x, w, s, z, b, out=x[:, :10])), (ValueError, lambda: i4(x, w, s, z, b, out=x.new_zeros(10, 3).t())),
+        (ValueError, lambda: i4(x.clone().requires_grad_(), w, s, z, b)), (ValueError, lambda: i4(x, w.cpu(), s, z, b)),
+    ]:
+        with pytest.raises(error):
+            call()
+    with torch.no_grad():
+        packed(grad, k, k, plan)
+    i4(x, w, s, z, b)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A sequence of a cache, tokens of a prefix and features of a weight that start past 2^32 elements or bytes."""
+    ops = _ops()
+    H, Hkv, D, P, room = 4, 2, 64, 290, 50
+    far, apart = 1 << 32, 1 << 24
+    big = torch.empty(far + room * Hkv * D, device=gpu, dtype=torch.float16)
+    ko = big.as_strided((2, room, Hkv, D), (far, Hkv * D, D, 1))
+    wide = torch.empty(P * apart, device=gpu, dtype=torch.float16)
+    kp = wide.as_strided((P, Hkv, D), (apart, D, 1))
+    vo, vp = _rand((2, room, Hkv, D), torch.float16, 2).to(gpu), _rand((P, Hkv, D), torch.float16, 3).to(gpu)
+    ko.copy_(_rand((2, room, Hkv, D), torch.float16, 4))
+    kp.copy_(_rand((P, Hkv, D), torch.float16, 5))
+    q = _rand((2, 1, H, D), torch.float16, 6).to(gpu)
+    lens = [50, 33]
+    ref, tol = prefix64(q.cpu(), kp.cpu(), vp.cpu(), ko.cpu(), vo.cpu(), lens, D ** -0.5)
+    lt = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    check("far caches and tokens", ops.attention_shared_prefix(q, kp, vp, ko, vo, lt), ref, tol)
+    plan = ops.packed_plan([2], [P], heads=H, kv_heads=Hkv, head_dim=D, device=gpu)
+    qq = q[:, 0].contiguous()
+    ref, tol = packed64(qq.cpu(), kp.cpu(), vp.cpu(), [2], [P], True, D ** -0.5)
+    check("far tokens", ops.attention_packed(qq, kp, vp, plan), ref, tol)
+    del big, wide, ko, kp
+    N, K = (1 << 17) + 40, 65536  # 4 GiB of weights and more
+    w = torch.empty(N, K // 2, dtype=torch.uint8, device=gpu)
+    tail, scale, zero = weights(40, K, 128, "4 bits", torch.float16, 7)
+    w[-40:] = tail.to(gpu)
+    s = torch.ones(N, K // 128, device=gpu, dtype=torch.float16)
+    z = torch.zeros(N, K // 128, device=gpu, dtype=torch.uint8)
+    s[-40:], z[-40:] = scale.to(gpu), zero.to(gpu)
+    x = _rand((2, K), torch.float16, 8, 0.05)
+    ref, tol = linear64(x, tail, scale, zero, None, 128, torch.float16)
+    check("far features", ops.linear_i4(x.to(gpu), w, s, z)[:, -40:], ref, tol)
+    K = 16384  # ... and of the kernel of few rows
+    w = w.view(-1)[:((1 << 19) + 40) * (K // 2)].view(-1, K // 2)
+    tail, scale, zero = weights(40, K, 128, "4 bits", torch.float16, 9)
+    w[-40:] = tail.to(gpu)
+    s, z = (t.view(-1)[:w.shape[0] * 128].view(-1, 128) for t in (s, z))
+    s[-40:], z[-40:] = scale.to(gpu), zero.to(gpu)
+    ref, tol = linear64(x[:, :K].contiguous(), tail, scale, zero, None, 128, torch.float16)
+    check("far features", ops.linear_i4(x[:, :K].contiguous().to(gpu), w, s, z)[:, -40:], ref, tol)
+
+
 # ------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_generation_steps(gpu, dtype):

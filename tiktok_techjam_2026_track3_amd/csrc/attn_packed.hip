@@ -151,9 +151,9 @@ int launch(const rows::Args& a, int64_t hd, const Counts& n, int wide_rows, hipS
 }
 
 bool fits(const Counts& n, int64_t kv_heads) {
-  const int64_t most = 0x7fffffffLL;
+  const int64_t most = 0xffffffffLL / 256;  // a launch has at most 2^32 - 1 threads
   return n.wide >= 0 && n.narrow >= 0 && n.joins >= 0 && n.slots >= 0 && n.wide <= most / kv_heads &&
-         n.narrow <= most / kv_heads && n.joins <= most / kv_heads && n.slots <= most;
+         n.narrow <= most / kv_heads && n.joins <= most / kv_heads && n.slots <= 0x7fffffffLL;
 }
 
 }  // namespace

@@ -25,6 +25,8 @@ struct Split {
 
 // most splits of the prefix or of a cache, and of both together for one wave to join
 constexpr int64_t MAX_SPLITS = 512;
+// most work-groups (and rows, each joined by one) of a launch, which has at most 2^32 - 1 threads
+constexpr int64_t MAX_BLOCKS = 0xffffffffLL / 256;
 constexpr int WAVE_SPLITS = 32;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -65,7 +67,7 @@ Split split_of(const Shape& s) {
 int check(const Shape& s) {
   if (s.B < 0 || s.n_q < 0 || s.H <= 0 || s.Hkv <= 0 || s.H % s.Hkv != 0 || s.H > 65535 || s.prefix < 0 ||
       s.room < 0 || s.prefix >= (int64_t(1) << 30) || s.room >= (int64_t(1) << 30) || s.B > 65535 ||
-      s.n_q > 65535 || s.B * s.n_q * s.H >= (int64_t(1) << 30))
+      s.n_q > 65535 || s.B * s.n_q * s.H > MAX_BLOCKS)
     return MI355_E_BAD_SIZE;
   switch (s.hd) {
     case 16: case 32: case 48: case 64: case 80: case 96: case 128: case 192: case 256: break;
@@ -285,7 +287,7 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
     return MI355_E_ALIGNMENT;
   const int64_t G = heads / kv_heads;
   if (kv_heads * d.prefix_splits * ceil_div(B * n_q * G, d.prefix_rows) +
-      kv_heads * d.own_splits * ceil_div(n_q * G, d.own_rows) * B > 0x7fffffffLL)
+      kv_heads * d.own_splits * ceil_div(n_q * G, d.own_rows) * B > MAX_BLOCKS)
     return MI355_E_BAD_SIZE;
   rows::Args a{};
   a.q = Q;

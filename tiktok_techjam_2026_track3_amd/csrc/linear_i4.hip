@@ -367,7 +367,7 @@ __global__ __launch_bounds__(KW == 8 ? 512 : 256) void linear_i4_few(I4Args p, i
 #pragma unroll
             for (int m = 0; m < M; ++m) d[m] = dot2<T>(q, x[c][m][4 * j + e], d[m]);
           }
-        const float z = -16.f - static_cast<float>(cur.z[i][c]), s = to_f32(cur.s[i][c]);
+        const float z = -16.f - static_cast<float>(cur.z[i][c]), s = in[c] ? to_f32(cur.s[i][c]) : 0.f;
 #pragma unroll
         for (int m = 0; m < M; ++m) v[i][m] = __builtin_fmaf(__builtin_fmaf(sx[c][m], z, d[m]), s, v[i][m]);
       }
@@ -460,7 +460,7 @@ int launch_group(const I4Args& a, int64_t group, hipStream_t s) {
 extern "C" int mi355_linear_i4(int dtype, int out_dtype, const void* X, int64_t ldx, const uint8_t* Wq,
                                const void* scale, const uint8_t* zero, const float* bias, void* Y,
                                int64_t ldy, int64_t M, int64_t N, int64_t K, int64_t group, void* stream) {
-  if (M < 0 || N < 0 || K < 0 || M > (int64_t(1) << 20) || N > (int64_t(1) << 30) || K > (int64_t(1) << 30))
+  if (M < 0 || N < 0 || K < 0 || M > (int64_t(1) << 20) || N > (int64_t(1) << 26) || K > (int64_t(1) << 26))
     return MI355_E_BAD_SIZE;
   if (dtype != MI355_F16 && dtype != MI355_BF16) return MI355_E_BAD_DTYPE;
   if (out_dtype != dtype && out_dtype != MI355_F32) return MI355_E_BAD_DTYPE;

@@ -579,10 +579,11 @@ def _no_backward(*tensors: Optional[torch.Tensor]) -> None:
                              "or with detached tensors")
 
 
-def _rows_strides(name: str, shape, stride, align: int, kv_axis: Optional[int] = None) -> Tuple[int, ...]:
+def _rows_strides(name: str, shape, stride, align: int, kv_axis: Optional[int] = None,
+                  written: bool = False) -> Tuple[int, ...]:
     """Strides of a [..., token, head, head_dim] view but the last, checked: unit head_dim stride, whole
-    vectors between rows, and for K / V (kv_axis: the token axis) tokens that do not overlap. Axes of
-    one element get a stride that does not matter."""
+    vectors between rows, for K / V (kv_axis: the token axis) tokens that do not overlap, and for what is
+    written no rows that do. Axes of one element get a stride that does not matter."""
     if 0 in shape:
         return tuple(shape[-1] if i == kv_axis else 0 for i in range(len(shape) - 1))
     if stride[-1] != 1:
@@ -596,6 +597,12 @@ def _rows_strides(name: str, shape, stride, align: int, kv_axis: Optional[int] =
         elif i == kv_axis and not shape[-1] <= st <= 1 << 24:
             raise ValueError(f"the tokens of {name} overlap or are too far apart (stride {st})")
         out.append(st)
+    if written:  # no two elements in one place
+        extent = shape[-1]
+        for st, n in sorted((st, n) for n, st in zip(shape[:-1], stride[:-1]) if n > 1):
+            if st < extent:
+                raise ValueError(f"rows of {name} overlap (strides {tuple(stride)})")
+            extent = st * n
     return tuple(out)
 
 
@@ -701,7 +708,7 @@ def _packed_views(q_tokens, k_tokens, heads, kv_heads, D, dtypes, qs, qst, ks, k
     if os is not None and os != qs:
         raise ValueError(f"out must have q's shape {tuple(qs)}")
     arrays = _Arrays(_rows_strides("q", qs, qst, 8), _rows_strides("k", ks, kst, 8, 0), _rows_strides("v", vs, vst, 8, 0),
-                     (heads * D, D) if os is None else _rows_strides("out", os, ost, 4))
+                     (heads * D, D) if os is None else _rows_strides("out", os, ost, 4, written=True))
     return _lib.dtype_code(dtypes[0]), arrays
 
 
@@ -775,7 +782,7 @@ def _prefix_views(dtypes, qs, qst, kps, kpst, vps, vpst, kos, kost, vos, vost, l
     arrays = _Arrays(_rows_strides("q", qs, qst, 8), _rows_strides("k_prefix", kps, kpst, 8, 0),
                      _rows_strides("v_prefix", vps, vpst, 8, 0), _rows_strides("k_own", kos, kost, 8, 1),
                      _rows_strides("v_own", vos, vost, 8, 1),
-                     (n * H * D, H * D, D) if os is None else _rows_strides("out", os, ost, 4))
+                     (n * H * D, H * D, D) if os is None else _rows_strides("out", os, ost, 4, written=True))
     need = _lib.lib().mi355_attn_shared_prefix_workspace_bytes(B, n, H, Hkv, D, P, room)
     if need < 0:
         _lib.check("mi355_attn_shared_prefix_workspace_bytes", need)
