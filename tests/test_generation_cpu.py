@@ -217,3 +217,24 @@ def test_view_refusals(shape, stride, kw):
 def test_view_strides(shape, stride, kw, want):
     """Axes of one element have any stride; heads may share one K / V head; orders other than the usual."""
     assert ops._rows_strides("t", shape, stride, 8, **kw) == want
+
+
+def _dma_asm(*between):
+    return "\n".join(["attn_rows_x:", "  v_readfirstlane_b32 s6, v1", *between, "  s_mov_b32 m0, s20", "  s_nop 0",
+                      "  buffer_load_dwordx4 v2, s[4:7], s9 offen lds", "  s_endpgm", ".Lfunc_end0:"])
+
+
+@pytest.mark.parametrize("between,bad", [
+    ([], True), (["  s_add_i32 s8, s8, 1"] * 2, True), (["  s_add_i32 s8, s8, 1"] * 3, False), (["  s_nop 2"], False),
+    (["  s_mov_b32 s6, s30"], False),                       # written again by the scalar ALU
+    (["  s_cmp_eq_u32 s6, s30"], True),                     # only read
+    (["  s_branch .L1", ".L0:", "  s_nop 7", ".L1:"], True)])  # over a branch
+def test_build_finds_scalars_read_too_soon(between, bad):
+    """The build's check of LDS-DMA loads whose resource the vector ALU has just written."""
+    from tiktok_techjam_2026_track3_amd import _lib  # noqa: F401  (the package's build attribute is a function)
+    import importlib
+    B = importlib.import_module("tiktok_techjam_2026_track3_amd.build")
+    assert bool(B.dma_hazards(_dma_asm(*between))) == bad
+    if bad:
+        with pytest.raises(RuntimeError):
+            B.check_dma_hazards("x.hip", _dma_asm(*between))

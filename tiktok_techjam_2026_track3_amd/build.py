@@ -125,23 +125,23 @@ def _hazards(seq: list) -> list:
     return bad
 
 
-def mfma_hazards(asm: str) -> list:
-    """(kernel, first instruction, second instruction) of every pair closer than the distances above
-    in a unit's device assembly: along the text, and over every branch to its target."""
+def _walk(asm: str, kernels: re.Pattern, check, reach: int) -> list:
+    """(kernel, first instruction, second instruction) of the pairs that ``check`` finds in a unit's device
+    assembly: along the text, and over every branch to its target (``reach`` instructions on each side)."""
     out, kernel, code, labels = [], "", [], {}
 
     def flush():
-        if not ASM_MFMA_KERNELS.search(kernel):
-            return  # (builtin MFMAs: the compiler's own wait states)
-        bad, start, reach = [], 0, 2 * MFMA_TO_OTHER
+        if not kernels.search(kernel):
+            return  # (builtins: the compiler's own wait states)
+        bad, start = [], 0
         for i, text in enumerate(code + ["s_endpgm"]):
             op, _, target = text.partition(" ")
             if op == "s_branch" or op.startswith("s_cbranch"):
                 to = labels.get(target.strip())
                 if to is not None:
-                    bad += _hazards(code[max(start, i - reach):i + 1] + code[to:to + reach])
+                    bad += check(code[max(start, i - reach):i + 1] + code[to:to + reach])
             if op in ("s_branch", "s_endpgm", "s_setpc_b64"):  # nothing falls through
-                bad += _hazards(code[start:i])
+                bad += check(code[start:i])
                 start = i + 1
         out.extend((kernel, a, b) for a, b in dict.fromkeys(bad))
 
@@ -162,6 +162,52 @@ def mfma_hazards(asm: str) -> list:
     return out
 
 
+def mfma_hazards(asm: str) -> list:
+    """(kernel, first instruction, second instruction) of every pair closer than the distances above
+    in a unit's device assembly."""
+    return _walk(asm, ASM_MFMA_KERNELS, _hazards, 2 * MFMA_TO_OTHER)
+
+
+# The LDS-DMA loads of inline assembly read their buffer resource and offset from scalar registers. Written by
+# the vector ALU (v_readfirstlane, v_readlane, a compare's mask), those have to be this many wait states older.
+ASM_DMA_SOURCES = re.compile(r"attn_(packed|prefix)$")
+ASM_DMA_KERNELS = re.compile(r"attn_rows_")
+VALU_TO_VMEM_SGPR = 5
+_SREG = re.compile(r"\bs(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def _sregs(text: str) -> set:
+    out = set()
+    for m in _SREG.finditer(text):
+        lo, hi = (m[1], m[1]) if m[1] else (m[2], m[3])
+        out.update(range(int(lo), int(hi) + 1))
+    return out
+
+
+def _dma_hazards(seq: list) -> list:
+    bad, at, wrote = [], 0, {}  # wrote: SGPR -> (wait state after the vector instruction that wrote it, text)
+    for text in seq:
+        op, _, args = text.partition(" ")
+        if op == "s_nop":
+            at += int(args, 0) + 1
+            continue
+        dst, _, src = args.partition(",")
+        if op.startswith("buffer_load") and args.endswith(" lds"):
+            bad += [(wrote[r][1], text) for r in sorted(_sregs(src)) if r in wrote and at - wrote[r][0] < VALU_TO_VMEM_SGPR]
+        at += 1
+        for r in _sregs(dst):
+            if op.startswith("v_"):
+                wrote[r] = (at, text)
+            elif op.startswith("s_") and not op.startswith(("s_cmp", "s_bitcmp")):
+                wrote.pop(r, None)
+    return bad
+
+
+def dma_hazards(asm: str) -> list:
+    """(kernel, vector instruction, load) of every LDS-DMA load that reads a scalar register too soon."""
+    return _walk(asm, ASM_DMA_KERNELS, _dma_hazards, 2 * VALU_TO_VMEM_SGPR)
+
+
 def check_mfma_hazards(src_name: str, asm: str) -> None:
     bad = mfma_hazards(asm)
     if bad:
@@ -169,9 +215,17 @@ def check_mfma_hazards(src_name: str, asm: str) -> None:
                            "states, first:\n  " + "\n  ".join(f"{k}: {a}  ->  {b}" for k, a, b in bad[:5]))
 
 
+def check_dma_hazards(src_name: str, asm: str) -> None:
+    bad = dma_hazards(asm)
+    if bad:
+        raise RuntimeError(f"{src_name}: {len(bad)} LDS-DMA loads read a scalar register too soon, first:\n  "
+                           + "\n  ".join(f"{k}: {a}  ->  {b}" for k, a, b in bad[:5]))
+
+
 def _compile(src: Path) -> Path:
     obj = BUILD_DIR / (src.stem + ".o")
-    check = ASM_MFMA_SOURCES.match(src.stem)
+    mfma, dma = ASM_MFMA_SOURCES.match(src.stem), ASM_DMA_SOURCES.match(src.stem)
+    check = mfma or dma
     cmd = [hipcc(), *HIPCC_FLAGS, "-Rpass-analysis=kernel-resource-usage",
            *(["-save-temps=obj"] if check else []), "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -181,7 +235,11 @@ def _compile(src: Path) -> Path:
     if check:
         temps = [p for p in BUILD_DIR.glob(f"{src.stem}*") if p != obj]
         asm = [p for p in temps if p.suffix == ".s" and "amdgcn" in p.name]
-        check_mfma_hazards(src.name, "\n".join(p.read_text() for p in asm))
+        text = "\n".join(p.read_text() for p in asm)
+        if mfma:
+            check_mfma_hazards(src.name, text)
+        if dma:
+            check_dma_hazards(src.name, text)
         if not any("v_mfma" in p.read_text() for p in asm):
             raise RuntimeError(f"{src.name}: no device assembly to check")
         for p in temps:

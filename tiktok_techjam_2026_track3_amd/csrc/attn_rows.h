@@ -196,7 +196,11 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   }
   Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
   Vb = uniform_ptr(Vb + static_cast<int64_t>(k_begin) * p.vt);
-  int n_keys = k_end - k_begin;  // keys from here on are counted from k_begin
+  // Keys from here on are counted from k_begin. In scalar registers from here on as well: lengths come from
+  // memory, and a load's range must not be a scalar that the vector ALU has just written (inline assembly gets
+  // no wait states; the build checks).
+  int n_keys = __builtin_amdgcn_readfirstlane(k_end - k_begin);
+  k_off = __builtin_amdgcn_readfirstlane(k_off);
   int64_t kt = p.kt, vt = p.vt;
   const int row_w = OWN_KEYS ? row0 : row0 + wave * QW;
   const int lwave = OWN_KEYS ? 0 : wave;
