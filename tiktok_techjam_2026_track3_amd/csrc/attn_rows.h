@@ -85,6 +85,14 @@ MI355_DEVINL float row_sum(float v) {
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// buffer_dma_lds16 (common.h) for a resource that the vector ALU may have written just before, as it does with a
+// range that depends on a length from memory: five wait states before the load reads it.
+MI355_DEVINL void buffer_dma_lds16_after_valu(u32x4 rsrc, uint32_t voffset, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc),
+               "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+               : "memory", "m0");
+}
+
 // XOR of a row's 16-byte chunks (NCH per row) by its low 4 bits. 16 lanes are served together: of a
 // K fragment read (16 rows, 4 neighbouring chunks) rows 0-3 and 12-15 at one chunk with rows 4-11 at
 // the next, of a V transpose read 4 rows at 2 neighbouring chunks. Row pitches of 2, 6 and 10 chunks
@@ -196,10 +204,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   }
   Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
   Vb = uniform_ptr(Vb + static_cast<int64_t>(k_begin) * p.vt);
-  // Keys from here on are counted from k_begin. In scalar registers from here on as well: lengths come from
-  // memory, and a load's range must not be a scalar that the vector ALU has just written (inline assembly gets
-  // no wait states; the build checks).
-  int n_keys = __builtin_amdgcn_readfirstlane(k_end - k_begin);
+  int n_keys = __builtin_amdgcn_readfirstlane(k_end - k_begin);  // keys from here on are counted from k_begin
   k_off = __builtin_amdgcn_readfirstlane(k_off);
   int64_t kt = p.kt, vt = p.vt;
   const int row_w = OWN_KEYS ? row0 : row0 + wave * QW;
@@ -299,7 +304,9 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     for (int i = 0; i < LPW; ++i) {
       const int blk = lwave + i * LW;
       if (BLK % LW != 0 && blk >= BLK) break;
-      buffer_dma_lds16(kr, koff[i], 0, lds_addr_of(&lds[st * TILE + blk * 64]));
+      const uint32_t to = lds_addr_of(&lds[st * TILE + blk * 64]);
+      if (OWN_KEYS && i == 0) buffer_dma_lds16_after_valu(kr, koff[i], to);
+      else buffer_dma_lds16(kr, koff[i], 0, to);
     }
   };
   auto issue_v = [&](int j, int st) MI355_LAMBDA_INLINE {
@@ -310,7 +317,9 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     for (int i = 0; i < LPW; ++i) {
       const int blk = lwave + i * LW;
       if (BLK % LW != 0 && blk >= BLK) break;
-      buffer_dma_lds16(vr, voff[i], 0, lds_addr_of(&lds[(RING + st) * TILE + blk * 64]));
+      const uint32_t to = lds_addr_of(&lds[(RING + st) * TILE + blk * 64]);
+      if (OWN_KEYS && i == 0) buffer_dma_lds16_after_valu(vr, voff[i], to);
+      else buffer_dma_lds16(vr, voff[i], 0, to);
     }
   };
 
