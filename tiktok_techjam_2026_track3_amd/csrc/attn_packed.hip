@@ -309,6 +309,8 @@ extern "C" int mi355_attn_packed(int dtype, const void* Q, const void* K, const 
   a.G = static_cast<int32_t>(heads / kv_heads);
   a.H = static_cast<int32_t>(heads);
   a.Hkv = static_cast<int32_t>(kv_heads);
+  a.by_G = rows::make_div(a.G);
+  a.by_Hkv = rows::make_div(a.Hkv);
   a.tiles = reinterpret_cast<const rows::PackedTile*>(plan);
   a.causal = causal != 0;
   a.slots = n.slots;

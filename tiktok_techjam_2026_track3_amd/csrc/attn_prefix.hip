@@ -298,6 +298,9 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
   a.Hkv = static_cast<int32_t>(kv_heads);
   a.B = static_cast<int32_t>(B);
   a.n_q = static_cast<int32_t>(n_q);
+  a.by_G = rows::make_div(a.G);
+  a.by_Hkv = rows::make_div(a.Hkv);
+  a.by_n_q = rows::make_div(n_q);
   a.part = static_cast<float*>(workspace);
   a.ml = a.part + (d.prefix_splits + d.own_splits) * s.rows() * head_dim;
   rows::Args own = a;
@@ -323,6 +326,10 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
   own.splits = static_cast<int32_t>(d.own_splits);
   own.row_tiles = static_cast<int32_t>(ceil_div(n_q * G, d.own_rows));
   own.part0 = a.splits;
+  for (rows::Args* x : {&a, &own}) {
+    x->by_splits = rows::make_div(x->splits);
+    x->by_row_tiles = rows::make_div(x->row_tiles);
+  }
   CombineArgs c{};
   c.part = a.part;
   c.ml = a.ml;

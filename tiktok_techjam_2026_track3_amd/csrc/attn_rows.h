@@ -30,6 +30,22 @@ struct PackedTile {
 };
 static_assert(sizeof(PackedTile) == 32, "plan entry");
 
+// Division of n < 2^31 by a fixed d >= 1: with 2^(l - 1) < d <= 2^l and mul = ceil(2^(31 + l) / d), which
+// exceeds the quotient by less than d / d, floor(n / d) = floor(n mul / 2^(31 + l)), since n (mul d - 2^(31 + l)) <
+// 2^31 d <= 2^(31 + l). Two instructions for the compiler's twenty-five.
+struct Div {
+  uint32_t mul, shift;  // d = 1: mul 0
+};
+inline Div make_div(int64_t d) {
+  if (d <= 1) return Div{0u, 0u};
+  uint32_t l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return Div{static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1};
+}
+MI355_DEVINL int quotient(int n, Div d) {
+  return d.mul == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.mul) >> d.shift);
+}
+
 struct Args {
   const void *q, *k, *v;
   void* o;                // PACKED: output
@@ -39,6 +55,7 @@ struct Args {
   int64_t ob, ot, oh;
   float c;                // scale * log2(e)
   int32_t G, H, Hkv;      // query heads of a K/V head, query heads, K/V heads
+  Div by_G, by_Hkv;
   // PACKED
   const PackedTile* tiles;
   int32_t causal;
@@ -52,6 +69,7 @@ struct Args {
   int32_t pkeys;
   int32_t chunk;          // keys of a split
   int32_t splits, row_tiles;
+  Div by_n_q, by_splits, by_row_tiles;
   int32_t part0;          // first split's index in part / ml
   float* part;            // partial rows [HD], unnormalised; PREFIX / OWN: [splits][B n_q H]
   float* ml;              // their mu (-inf: no key seen) and sum
@@ -147,15 +165,16 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   const T *Qb, *Kb, *Vb;
   int64_t out_tok = 0, slot = -1;
   if constexpr (MODE == PACKED) {
-    h = static_cast<int>(block % static_cast<unsigned>(p.Hkv));
-    const PackedTile t = p.tiles[block / static_cast<unsigned>(p.Hkv)];
+    const int entry = quotient(static_cast<int>(block), p.by_Hkv);
+    h = static_cast<int>(block) - entry * p.Hkv;
+    const PackedTile t = p.tiles[entry];
     row0 = t.row0;
     nrows = t.q_len * p.G;
     k_begin = t.k_begin;
     // key j is seen by token i when j < i + k_off (causal), j < k_len
     k_off = p.causal ? t.k_len - t.q_len + 1 : 0x40000000;
     const int last = (row0 + BM < nrows ? row0 + BM : nrows) - 1;
-    const int lim = last / p.G + k_off;
+    const int lim = quotient(last, p.by_G) + k_off;
     k_end = lim < t.k_stop ? lim : t.k_stop;
     k_end = k_end > k_begin ? k_end : k_begin;
     if (t.slot >= 0) slot = h * p.slots + t.slot;
@@ -164,8 +183,8 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     Vb = static_cast<const T*>(p.v) + t.k0 * p.vt + h * p.vh;
     out_tok = t.q0;
   } else if constexpr (MODE == WHOLE) {
-    h = static_cast<int>(block % static_cast<unsigned>(p.Hkv));
-    b = static_cast<int>(block / static_cast<unsigned>(p.Hkv));
+    b = quotient(static_cast<int>(block), p.by_Hkv);
+    h = static_cast<int>(block) - b * p.Hkv;
     row0 = k_begin = 0;
     nrows = p.n_q * p.G;
     const int given = p.lens[b];
@@ -175,13 +194,11 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     Kb = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
     Vb = static_cast<const T*>(p.v) + b * p.vb + h * p.vh;
   } else {
-    unsigned x = block;
-    h = static_cast<int>(x % static_cast<unsigned>(p.Hkv));
-    x /= static_cast<unsigned>(p.Hkv);
-    split = static_cast<int>(x % static_cast<unsigned>(p.splits));
-    x /= static_cast<unsigned>(p.splits);
-    row0 = static_cast<int>(x % static_cast<unsigned>(p.row_tiles)) * BM;
-    b = static_cast<int>(x / static_cast<unsigned>(p.row_tiles));
+    const int x = quotient(static_cast<int>(block), p.by_Hkv), y = quotient(x, p.by_splits);
+    h = static_cast<int>(block) - x * p.Hkv;
+    split = x - y * p.splits;
+    b = quotient(y, p.by_row_tiles);
+    row0 = (y - b * p.row_tiles) * BM;
     k_begin = split * p.chunk;
     Qb = static_cast<const T*>(p.q);
     Kb = static_cast<const T*>(p.k) + h * p.kh;
@@ -214,9 +231,9 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 
   // token (of the batch in PREFIX) of a row, and its offset in q
   const auto q_of = [&](int r) MI355_LAMBDA_INLINE {
-    const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+    const int t = quotient(r, p.by_G), hh = h * p.G + (r - t * p.G);
     if constexpr (MODE == PREFIX) {
-      const int bb = t / p.n_q;
+      const int bb = quotient(t, p.by_n_q);
       return bb * p.qb + (t - bb * p.n_q) * p.qt + hh * p.qh;
     } else {
       return t * p.qt + hh * p.qh;
@@ -225,21 +242,21 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   // keys [0, lim) of the work-group's range are seen by row r
   int lim_off = k_off - k_begin;
   const auto lim_of = [&](int r) MI355_LAMBDA_INLINE {
-    const int lim = r / p.G + lim_off;
+    const int lim = quotient(r, p.by_G) + lim_off;
     return lim < n_keys ? lim : n_keys;
   };
 
   // row r's output, or its partial result
   const bool direct = MODE == WHOLE || (MODE == PACKED && slot < 0);
   const auto out_of = [&](int r) MI355_LAMBDA_INLINE {
-    const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+    const int t = quotient(r, p.by_G), hh = h * p.G + (r - t * p.G);
     return static_cast<T*>(p.o) + (MODE == WHOLE ? b * p.ob : out_tok * p.ot) + t * p.ot + hh * p.oh;
   };
   const auto part_of = [&](int r) MI355_LAMBDA_INLINE {
     if constexpr (MODE == PACKED) {
       return slot + (r - row0);
     } else {
-      const int t = r / p.G, hh = h * p.G + (r - t * p.G);
+      const int t = quotient(r, p.by_G), hh = h * p.G + (r - t * p.G);
       return (static_cast<int64_t>(p.part0 + split) * p.B * p.n_q + (MODE == OWN ? static_cast<int64_t>(b) * p.n_q : 0) + t) * p.H + hh;
     }
   };
@@ -397,12 +414,14 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
         mx = row_maximum(mx) * p.c;
         const bool grow = mx > gate[n];
         const float m2 = grow ? mx : mu[n];
-        const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(mu[n] - m2);
-        lsum[n] *= alpha;
+        if (__builtin_amdgcn_ballot_w64(gate[n] != NEG_INF) != 0) {  // (sums and outputs are 0 before the first maximum)
+          const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(mu[n] - m2);
+          lsum[n] *= alpha;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+          for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][t][i] *= alpha;
+            for (int i = 0; i < 4; ++i) o[n][t][i] *= alpha;
+        }
         mu[n] = m2;
         gate[n] = grow ? mx + 8.f : gate[n];
       }
@@ -547,26 +566,21 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       }
     }
   };
-  // 4 elements of row r from element d on; returns whether one is NaN
-  const auto put = [&](int r, int d, f32x4 v, float sum, bool sees) MI355_LAMBDA_INLINE {
-    bool bad = false;
+  // 4 elements of a row whose output (or partial result) starts at dst (part); NaN stays in nan
+  const auto put = [&](T* dst, float* part, int d, f32x4 v, float inv, bool sees, float& nan) MI355_LAMBDA_INLINE {
     if (direct) {
       // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
-      const float inv = 1.0f / sum;
       frag4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = sees ? v[e] * inv : 0.f;
-        bad |= x != x;
-        w[e] = from_f32<T>(x);
+        v[e] = sees ? v[e] * inv : 0.f;
+        w[e] = from_f32<T>(v[e]);
       }
-      *reinterpret_cast<frag4*>(out_of(r) + d) = w;
+      *reinterpret_cast<frag4*>(dst + d) = w;
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= v[e] != v[e];
-      *reinterpret_cast<f32x4*>(p.part + part_of(r) * HD + d) = v;
+      *reinterpret_cast<f32x4*>(part + d) = v;
     }
-    return bad;
+    if constexpr (MODE != PREFIX) nan = vmax(nan, vmax(vmax(v[0], v[1]), vmax(v[2], v[3])));
   };
   const auto put_ml = [&](int r, float m, float sum) MI355_LAMBDA_INLINE {
     if (direct) return;
@@ -612,7 +626,11 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], f, v[e]);
       }
-      if (put(row0 + x, 4 * d, v, sum, lim_of(row0 + x) > 0 || (MODE == WHOLE && p.pkeys > 0))) atomicOr(&nan_rows, 1u << x);
+      float nan = 0.f;
+      T* const dst = direct ? out_of(row0 + x) : nullptr;
+      float* const part = direct ? nullptr : p.part + part_of(row0 + x) * HD;
+      put(dst, part, 4 * d, v, 1.0f / sum, lim_of(row0 + x) > 0 || (MODE == WHOLE && p.pkeys > 0), nan);
+      if (nan != nan) atomicOr(&nan_rows, 1u << x);
       if (d == 0) put_ml(row0 + x, m, sum);
     }
     if constexpr (MODE != PREFIX) {
@@ -629,13 +647,21 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
     for (int n = 0; n < QG; ++n) {
       const int r = row_w + 16 * n + l16;
       const float sum = row_sum(lsum[n]);
-      bool bad = false;
+      float nan = 0.f;
       if (r < nrows) {
+        T* const dst = direct ? out_of(r) : nullptr;
+        float* const part = direct ? nullptr : p.part + part_of(r) * HD;
+        const float inv = 1.0f / sum;
+        if (direct) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) bad |= put(r, 16 * dt + 4 * g, o[n][dt], sum, lim[n] > 0);
+          for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
+        } else {
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
+        }
         if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n], sum);
       }
-      const uint64_t m = __builtin_amdgcn_ballot_w64(bad);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(nan != nan);
       nan_rows[n] = (m | (m >> 16) | (m >> 32) | (m >> 48)) & 0xffffu;
     }
     if constexpr (MODE != PREFIX) {
