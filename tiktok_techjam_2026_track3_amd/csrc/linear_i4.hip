@@ -14,6 +14,8 @@
 //   A lane's 16 bytes are 32 neighbouring k. For GROUP 128 the four lanes of a feature hold the
 //   whole group and each word is one MFMA's operand as it is; for 32 and 64 the words change
 //   places between the four lanes (4 lane swaps) so that one MFMA's 32 k are neighbours.
+// 16 x 16384 x 4096 (bf16, group 128) 16.1 us, 2.2 TB/s: without the loads of x, which every work-group takes from
+// L2, it took 11; 7 x 4096 x 16384 (group 64) 18 us. 1 x 12288 x 4096 (linear_i4_few) 8 us, 3.2 TB/s.
 #include "common.h"
 
 namespace {
@@ -427,12 +429,16 @@ template <typename T, int GROUP, int MT, typename TO>
 int launch_nw(const I4Args& a, hipStream_t s) {
   const int64_t tiles = (a.N + 15) / 16, steps = (a.K + 127) / 128;
   if constexpr (MT == 1 && GROUP != 32) {
-    // Two tiles a wave halve the loads of x: where its 16 rows are mostly real and two tiles a wave
-    // leave every CU work-groups
+    // Two tiles a wave halve the loads of x: where two tiles a wave leave every CU work-groups (16 x 16384 x 4096
+    // 16.7 us with two, 22.9 with one; 8 x 12288 x 4096 14.0 and 13.7; 7 x 4096 x 16384 38 and 19)
     if (a.M > 4 && tiles >= 768) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
   }
-  if constexpr (MT == 1) return steps > 16 ? launch_one<T, GROUP, MT, 1, 8, TO>(a, s) : launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
-  else return launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
+  if (MT == 1) return steps > 16 ? launch_one<T, GROUP, MT, 1, 8, TO>(a, s) : launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
+  // (32 x 8192 x 8192 27.8, 64 x 12288 x 4096 45.0 us with two tiles a wave, 36.2 and 51.1 with one)
+  if constexpr (GROUP != 32) {
+    if (tiles >= 512) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
+  }
+  return launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
 }
 template <typename T, int GROUP, typename TO>
 int launch_mt(const I4Args& a, hipStream_t s) {
