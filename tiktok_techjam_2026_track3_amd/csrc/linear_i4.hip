@@ -427,18 +427,21 @@ int launch_one(const I4Args& a, hipStream_t s) {
 }
 template <typename T, int GROUP, int MT, typename TO>
 int launch_nw(const I4Args& a, hipStream_t s) {
-  const int64_t tiles = (a.N + 15) / 16, steps = (a.K + 127) / 128;
+  [[maybe_unused]] const int64_t tiles = (a.N + 15) / 16, steps = (a.K + 127) / 128;
   if constexpr (MT == 1 && GROUP != 32) {
     // Two tiles a wave halve the loads of x: where two tiles a wave leave every CU work-groups (16 x 16384 x 4096
     // 16.7 us with two, 22.9 with one; 8 x 12288 x 4096 14.0 and 13.7; 7 x 4096 x 16384 38 and 19)
     if (a.M > 4 && tiles >= 768) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
   }
-  if (MT == 1) return steps > 16 ? launch_one<T, GROUP, MT, 1, 8, TO>(a, s) : launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
-  // (32 x 8192 x 8192 27.8, 64 x 12288 x 4096 45.0 us with two tiles a wave, 36.2 and 51.1 with one)
-  if constexpr (GROUP != 32) {
-    if (tiles >= 512) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
+  if constexpr (MT == 1) {
+    return steps > 16 ? launch_one<T, GROUP, MT, 1, 8, TO>(a, s) : launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
+  } else {
+    if constexpr (GROUP != 32) {
+      // (32 x 8192 x 8192 27.8, 64 x 12288 x 4096 45.0 us with two tiles a wave, 36.2 and 51.1 with one)
+      if (tiles >= 512) return launch_one<T, GROUP, MT, 2, 4, TO>(a, s);
+    }
+    return launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
   }
-  return launch_one<T, GROUP, MT, 1, 4, TO>(a, s);
 }
 template <typename T, int GROUP, typename TO>
 int launch_mt(const I4Args& a, hipStream_t s) {
