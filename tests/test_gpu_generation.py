@@ -354,6 +354,17 @@ def test_prefix_lengths(gpu, P, room, lens, n):
     run_prefix(gpu, torch.float16, 3, n, 8, 2, 64, P, room, lens, seed=7, behind=math.nan)
 
 
+@pytest.mark.parametrize("B,n", [(2, 40), (600, 1)])
+def test_prefix_without_any_keys(gpu, B, n):
+    """Neither prefix nor caches, where rows or work-groups are too many for one launch of whole rows."""
+    ops = _ops()
+    q = _rand((B, n, 4, 64), torch.bfloat16, 1).to(gpu)
+    none, caches = q.new_empty(0, 2, 64), q.new_empty(B, 0, 2, 64)
+    out = torch.full_like(q, math.nan)
+    ops.attention_shared_prefix(q, none, none, caches, caches, torch.zeros(B, dtype=torch.int32, device=gpu), out=out)
+    assert not out.any()
+
+
 @pytest.mark.parametrize("P", [200, 1200])
 def test_prefix_strides_and_out(gpu, P):
     """Caches as views of one buffer for K and V, a strided query and output."""

@@ -213,6 +213,7 @@ int launch_hd(const rows::Args& a, const rows::Args& own, const Split& d, hipStr
   if (d.whole) return launch_whole<T, HD>(own, d, st);
   const int64_t np = static_cast<int64_t>(a.Hkv) * a.splits * a.row_tiles;
   const int64_t no = static_cast<int64_t>(a.Hkv) * own.splits * own.row_tiles * own.B;
+  if (np + no == 0) return MI355_OK;  // no prefix and no caches: only the zeros
   if (d.prefix_rows <= 16) launch_one<T, HD, 16, 16>(a, own, np, no, st);
   else if (d.prefix_rows == 32) launch_one<T, HD, 32, 32>(a, own, np, no, st);
   else if (d.prefix_rows == 64 && d.own_rows == 16) launch_one<T, HD, 64, 16>(a, own, np, no, st);
@@ -274,8 +275,9 @@ extern "C" int mi355_attn_shared_prefix(int dtype, const void* Q, const void* K_
       !o_strides || (prefix_len > 0 && (!K_prefix || !V_prefix)) || (room > 0 && (!K_own || !V_own)))
     return MI355_E_NULL_POINTER;
   const Split d = split_of(s);
-  if (!d.whole && !workspace) return MI355_E_NULL_POINTER;
-  if (workspace_bytes < (d.prefix_splits + d.own_splits) * s.rows() * (head_dim + 2) * 4) return MI355_E_BAD_SIZE;
+  const int64_t need = (d.prefix_splits + d.own_splits) * s.rows() * (head_dim + 2) * 4;
+  if (need > 0 && !workspace) return MI355_E_NULL_POINTER;
+  if (workspace_bytes < need) return MI355_E_BAD_SIZE;
   // token strides of K and V: rows that do not overlap, whose tiles' offsets fit 32 bits
   for (const int64_t t : {prefix_len > 0 ? kp_strides[0] : head_dim, prefix_len > 0 ? vp_strides[0] : head_dim,
                           room > 0 ? ko_strides[1] : head_dim, room > 0 ? vo_strides[1] : head_dim})
