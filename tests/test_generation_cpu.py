@@ -238,3 +238,8 @@ def test_build_finds_scalars_read_too_soon(between, bad):
     if bad:
         with pytest.raises(RuntimeError):
             B.check_dma_hazards("x.hip", _dma_asm(*between))
+
+
+def test_packed_plan_takes_whole_lengths():
+    with pytest.raises(TypeError):
+        ops.packed_plan([2.5], heads=4, head_dim=64)

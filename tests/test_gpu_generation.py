@@ -638,6 +638,9 @@ def test_refusals_on_the_gpu(gpu):
         (ValueError, lambda: packed(q, k, k, plan, scale=math.nan)), (ValueError, lambda: packed(q, k, k, plan, out=q)),
         (ValueError, lambda: packed(q, k, k, plan, out=q.new_zeros(8, 4, 32))), (TypeError, lambda: packed(q, k, k, plan, out=q.float())),
         (ValueError, lambda: packed(q, k, k, plan, out=q.new_zeros(1, 4, 64).expand(8, 4, 64))),
+        (ValueError, lambda: packed(q, k, k, plan, out=torch.empty_like(q).requires_grad_())),
+        (ValueError, lambda: prefix(q4, *own, out=torch.empty_like(q4).requires_grad_())),
+        (ValueError, lambda: i4(x, w, s, z, b, out=x.new_empty(3, 10).requires_grad_())),
         (ValueError, lambda: packed(grad, k, k, plan)), (ValueError, lambda: packed(q.cpu(), k, k, plan)),
         (ValueError, lambda: packed(q, k.cpu(), k, plan)),
         (TypeError, lambda: prefix(q4.float(), *own)), (TypeError, lambda: prefix(q4, k.bfloat16(), *own[1:])),

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -661,8 +662,8 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
     each (default: the same lengths). Lengths are host integers (0 included). Made once per batch,
     outside a graph capture: it copies the tiles to ``device``."""
     kv_heads = heads if kv_heads is None else kv_heads
-    q_lens = [int(n) for n in q_lens]
-    k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+    q_lens = [operator.index(n) for n in q_lens]
+    k_lens = q_lens if k_lens is None else [operator.index(n) for n in k_lens]
     if len(q_lens) != len(k_lens):
         raise ValueError(f"{len(q_lens)} query lengths and {len(k_lens)} key lengths")
     if any(not 0 <= n < 1 << 30 for n in q_lens + k_lens):
@@ -728,9 +729,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     if dev < 0 or k.get_device() != dev or v.get_device() != dev or plan.tiles.get_device() != dev or (
             out is not None and out.get_device() != dev):
         _on_gpu(q, k, v, plan.tiles, out)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        _no_backward(q, k, v)
     given = out is not None
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad)):
+        _no_backward(q, k, v, out)
     code, (qst, kst, vst, ost) = _packed_views(
         plan.q_tokens, plan.k_tokens, plan.heads, plan.kv_heads, plan.head_dim,
         (q.dtype, k.dtype, v.dtype, out.dtype) if given else (q.dtype, k.dtype, v.dtype),
@@ -809,7 +810,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
             v_own.get_device() != dev or own_lens.get_device() != dev or (given and out.get_device() != dev)):
         _on_gpu(q, k_prefix, v_prefix, k_own, v_own, own_lens, out)
     if torch.is_grad_enabled():
-        _no_backward(q, k_prefix, v_prefix, k_own, v_own)
+        _no_backward(q, k_prefix, v_prefix, k_own, v_own, out)
     dt = q.dtype
     dtypes = (dt, k_prefix.dtype, v_prefix.dtype, k_own.dtype, v_own.dtype)
     code, sizes, strides, need = _prefix_views(
@@ -914,8 +915,9 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     if dev < 0 or w.get_device() != dev or scale.get_device() != dev or (zero is not None and zero.get_device() != dev) \
             or (bias is not None and bias.get_device() != dev) or (out is not None and out.get_device() != dev):
         _on_gpu(x, w, scale, zero, bias, out)
-    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)):
-        _no_backward(x, scale, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (out is not None and out.requires_grad)):
+        _no_backward(x, scale, bias, out)
     odt = out_dtype or (out.dtype if out is not None else x.dtype)
     if out is not None and out.dtype != odt:
         raise ValueError("out must be [M, N] of out_dtype with unit column stride")
