@@ -514,6 +514,34 @@ def test_i4_sizes(gpu, dtype, M, N, K, group):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K,group", [
+    # x in registers: each number of steps, ranges of k that overlap and one that does not, one tile a work-group and several
+    (16, 37, 128, 128), (8, 6000, 128, 128), (5, 4200, 160, 32), (2, 33, 1024, 64), (9, 8300, 1088, 64), (16, 50, 2080, 32), (3, 4097, 4128, 32),
+    (2, 19, 4096, 128), (7, 20, 4224, 128), (12, 100, 6144, 32), (16, 40, 6208, 64), (4, 33, 8192, 128), (11, 4500, 992, 32),
+    # not: two tiles a wave, batches that overlap, less than a batch
+    (16, 33, 6176, 32), (16, 12300, 8320, 128), (6, 30, 64, 32), (20, 40, 480, 32), (17, 9000, 576, 64), (40, 8200, 640, 128),
+    (16, 9, 16448, 64), (25, 70, 704, 64)])
+def test_i4_held_rows(gpu, dtype, M, N, K, group):
+    run_i4(gpu, dtype, M, N, K, group, zeros=None if N % 2 else True, bias=N % 3 != 0, seed=K)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_i4_held_rows_every_value(gpu, dtype, group):
+    """One-hot rows, 16 at a time, read back exactly, where the ranges of k of the waves overlap."""
+    ops = _ops()
+    N, K = 20, 1152
+    w, _, zero = weights(N, K, group, "4 bits", dtype, group)
+    scale = 2.0 ** torch.randint(-3, 4, (N, K // group), generator=torch.Generator().manual_seed(1)).to(dtype)
+    eye = torch.eye(K, dtype=dtype, device=gpu)
+    args = [t.to(gpu) for t in (w, scale, zero)]
+    out = torch.cat([ops.linear_i4(eye[i:i + 16], *args) for i in range(0, K, 16)]).cpu()
+    q = torch.stack((w & 15, w >> 4), -1).reshape(N, K).double()
+    ref = (q - zero.double().repeat_interleave(group, 1)) * scale.double().repeat_interleave(group, 1)
+    assert torch.equal(out.double(), ref.t())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_i4_fp32_output_and_no_bias(gpu, dtype):
     run_i4(gpu, dtype, 9, 130, 1024, 64, None, bias=False, out_dtype=torch.float32, seed=3)
 
