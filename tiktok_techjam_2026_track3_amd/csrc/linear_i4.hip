@@ -16,7 +16,8 @@
 //   whole group and each word is one MFMA's operand as it is; for 32 and 64 the words change
 //   places between the four lanes (4 lane swaps) so that one MFMA's 32 k are neighbours.
 // 16 x 16384 x 4096 (bf16, group 128) 12.5 us, 2.9 TB/s (linear_i4_held; 17.4 with x from L2 for every two tiles),
-// 7 x 4096 x 16384 (group 64) 17.3 us, 1 x 12288 x 4096 (linear_i4_few) 7.9 us, 3.3 TB/s.
+// 7 x 4096 x 16384 (group 64; linear_i4_kernel, bound by what a CU can have in flight of the 360 kB of x and weights
+// that it takes in: one work-group alone takes as long) 17.3 us, 1 x 12288 x 4096 (linear_i4_few) 7.9 us, 3.3 TB/s.
 #include "common.h"
 
 namespace {
@@ -66,6 +67,15 @@ MI355_DEVINL typename Nib<T>::vec nibbles(uint32_t w) {
 MI355_DEVINL u32x4 nibble_order(u32x4 v) {
   return u32x4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
+}
+
+// A 4 x 4 transposition over (lane / 16, word): word m of lanes j becomes word j of lanes m.
+MI355_DEVINL u32x4 transposed(u32x4 w) {
+  const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  return u32x4{c[0], c[1], e[0], e[1]};
 }
 
 // BYTES bytes from any address, into words (one or two wide loads; nothing waits for them here)
@@ -188,17 +198,7 @@ __global__ __launch_bounds__(64 * NW) void linear_i4_kernel(I4Args p) {
       if (u > 0 && u % XU == 0) fetch_x(x, k0, u);
       u32x4 wu[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        wu[r] = cur.w[u][r];
-        if constexpr (GROUP != 128) {
-          // word m of lanes j becomes word j of lanes m: a 4 x 4 transposition over (lane / 16, word)
-          auto a = __builtin_amdgcn_permlane32_swap(wu[r][0], wu[r][2], false, false);
-          auto b = __builtin_amdgcn_permlane32_swap(wu[r][1], wu[r][3], false, false);
-          auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-          auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-          wu[r] = u32x4{c[0], c[1], e[0], e[1]};
-        }
-      }
+      for (int r = 0; r < R; ++r) wu[r] = GROUP == 128 ? cur.w[u][r] : transposed(cur.w[u][r]);
 #pragma unroll
       for (int i = 0; i < GP; ++i) {
         f32x4 acc[R][MT], sum[MT];
@@ -320,8 +320,7 @@ __global__ __launch_bounds__(512) void linear_i4_held(I4Args p, int per) {
     for (int u = 0; u < S; ++u)
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        const int k = begin + u * 128 + (GROUP == 128 ? 32 * g + 8 * m : 32 * m + 8 * g);
-        x[u][m] = __builtin_bit_cast(vec, *reinterpret_cast<const u32x4*>(row + k));
+        x[u][m] = __builtin_bit_cast(vec, *reinterpret_cast<const u32x4*>(row + begin + u * 128 + 32 * m + 8 * g));
       }
   }
   vec ones;
@@ -329,11 +328,21 @@ __global__ __launch_bounds__(512) void linear_i4_held(I4Args p, int per) {
   for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
   f32x4 sx[HOLD ? S * GP : 1];
 #pragma unroll
-  for (int u = 0; u < S; ++u)
+  for (int u = 0; u < S; ++u) {
+    u32x4 v[4];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      x[u][m] = __builtin_bit_cast(vec, nibble_order(__builtin_bit_cast(u32x4, x[u][m])));
+    for (int m = 0; m < 4; ++m) v[m] = nibble_order(__builtin_bit_cast(u32x4, x[u][m]));
+    if constexpr (GROUP == 128) {  // x, once, instead of the weights (loaded in that order it took 0.4 us longer)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32x4 c = transposed(u32x4{v[0][e], v[1][e], v[2][e], v[3][e]});
+#pragma unroll
+        for (int m = 0; m < 4; ++m) v[m][e] = c[m];
+      }
     }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) x[u][m] = __builtin_bit_cast(vec, v[m]);
+  }
   auto sum_of = [&](int u, int i) MI355_LAMBDA_INLINE {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -351,14 +360,7 @@ __global__ __launch_bounds__(512) void linear_i4_held(I4Args p, int per) {
     f32x4 total = {b0, b0, b0, b0};
 #pragma unroll
     for (int u = 0; u < S; ++u) {
-      u32x4 w = d.w[u];
-      if constexpr (GROUP != 128) {
-        auto c0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-        auto c1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        auto c2 = __builtin_amdgcn_permlane16_swap(c0[0], c1[0], false, false);
-        auto c3 = __builtin_amdgcn_permlane16_swap(c0[1], c1[1], false, false);
-        w = u32x4{c2[0], c2[1], c3[0], c3[1]};
-      }
+      const u32x4 w = GROUP == 128 ? d.w[u] : transposed(d.w[u]);
 #pragma unroll
       for (int i = 0; i < GP; ++i) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -575,8 +577,8 @@ template <typename T, int GROUP, int MT, typename TO>
 int launch_tiles(const I4Args& a, hipStream_t s) {
   if (a.K < 512) return launch_one<T, GROUP, MT, 1, 4, true, TO>(a, s);
   if constexpr (MT == 1) {  // (K > HELD_K)
-    // Two tiles a wave halve the loads of x, where that leaves every CU work-groups (16 x 12288 x 11008 39.7 us
-    // with two, 42.2 with one, 16 x 16384 x 12288, group 64, 47 and 63)
+    // Two tiles a wave halve the loads of x, where that leaves every CU work-groups (16 x 12288 x 11008 40 us
+    // with two, 42 with one, 16 x 16384 x 12288, group 64, 47 and 63)
     if ((a.N + 15) / 16 >= 768) return launch_one<T, GROUP, MT, 2, 4, false, TO>(a, s);
     return launch_one<T, GROUP, MT, 1, 8, false, TO>(a, s);
   } else {
