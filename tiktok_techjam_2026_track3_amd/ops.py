@@ -642,7 +642,9 @@ def _check_apart(out: torch.Tensor, *inputs: Optional[torch.Tensor]) -> None:
 @dataclass(frozen=True, eq=False)
 class PackedPlan:
     """How ``attention_packed`` walks one batch of packed sequences (``packed_plan``). It holds for
-    every call with these lengths (all layers of a model), on any stream of its device."""
+    every call with these lengths (all layers of a model), on any stream of its device. It may be dropped
+    while such calls are under way, but a captured graph reads ``tiles`` in every replay: like the graph's
+    inputs, its plan has to be kept as long as the graph."""
     q_tokens: int
     k_tokens: int
     heads: int
@@ -653,6 +655,14 @@ class PackedPlan:
     counts: ctypes.Array  # tiles of tile_rows rows, of 32 rows, joins, partial rows
     tiles: torch.Tensor
     workspace_bytes: int
+    stream: int = 0  # (raw) that tiles were allocated on
+
+    def used_on(self, device: int) -> None:
+        """Tells the allocator of a call on ``device``'s current stream where that is not the tiles' own: the
+        block is not handed out again before what the stream holds by then is done. Not while capturing:
+        the call's replays come at times that nobody knows here."""
+        if _raw_stream(device) != self.stream and not torch.cuda.is_current_stream_capturing():
+            self.tiles.record_stream(torch.cuda.current_stream(device))
 
 
 def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, heads: int,
@@ -660,7 +670,8 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
                 device="cuda") -> PackedPlan:
     """Plans ``attention_packed`` over sequences of ``q_lens`` new tokens against ``k_lens`` keys
     each (default: the same lengths). Lengths are host integers (0 included). Made once per batch,
-    outside a graph capture: it copies the tiles to ``device``."""
+    outside a graph capture: it lays the tiles out on the host and copies them to ``device``, which waits for
+    the copy. A captured graph's plan has to be kept as long as the graph."""
     kv_heads = heads if kv_heads is None else kv_heads
     q_lens = [operator.index(n) for n in q_lens]
     k_lens = q_lens if k_lens is None else [operator.index(n) for n in k_lens]
@@ -693,7 +704,7 @@ def packed_plan(q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *
         device = torch.device("cuda", torch.cuda.current_device())
     on_gpu = tiles.to(device)  # (from pageable memory: there when this returns, for every stream)
     return PackedPlan(sum(q_lens), sum(k_lens), heads, kv_heads, head_dim, bool(causal), rows.value,
-                      counts, on_gpu, counts[3] * kv_heads * (head_dim + 2) * 4)
+                      counts, on_gpu, counts[3] * kv_heads * (head_dim + 2) * 4, _raw_stream(device.index))
 
 
 @functools.lru_cache(maxsize=512)
@@ -747,6 +758,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if (qp | kp | vp) & 15 or op & 7:
         _check_aligned(q=qp, k=kp, v=vp, out=op)
+    plan.used_on(dev)
     need = plan.workspace_bytes
     ws = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
     st = _launch(dev, _lib.lib().mi355_attn_packed, code, qp, kp, vp, op, plan.heads, plan.kv_heads,
