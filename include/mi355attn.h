@@ -393,7 +393,8 @@ int mi355_block_head(int dtype, const void* X, int64_t ldx, const void* gamma, c
  * j over the keys of token i's own sequence; causal != 0: only j <= i + (k_len - q_len), positions
  * counted within the sequence (the last query sees the last key). A token that sees no key gives
  * zeros. Keys a token does not see do not reach its output, whatever their K and V hold (infinities
- * and NaN too); a row whose every visible score is -inf is NaN, as softmax's.
+ * and NaN too); an infinity in V that it does see gives infinities (NaN where its probability rounds to 0);
+ * a row whose every visible score is -inf is NaN, as softmax's.
  * Scores and softmax statistics are fp32, probabilities are rounded to the input type before P·V,
  * outputs once. dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256.
  *

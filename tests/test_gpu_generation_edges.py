@@ -1,5 +1,15 @@
 """The token-generation operators where their documentation allows what the first tests do not do: plans
-dropped while another stream still has to read them."""
+dropped while another stream still has to read them; infinities and NaN in V.
+
+Error bounds (u = half a step of a type): a probability taken as one term enters the numerator and the sum with one
+rounding, 2 u (P |V|), fp16 ones off by 2^-25 at least; as two, the first cut off (below 2 u p is left) and the second
+rounded (u of that), 2 u^2 (P |V|) in the numerator alone, and fp16's second term, at least its least number, is off
+by up to 2^-24, where the row's largest probability is 1 or more. The exponent c s - mu carries
+(D + 3) 2^-24 c sum_d |q_d k_jd| and the exponential 2^-22, both twice; a sum of n terms at most n 2^-24, twice;
+the output u |ref|.
+"""
+import math
+
 import pytest
 import torch
 
@@ -14,6 +24,42 @@ def _ops():
 def _rand(shape, dtype, seed, scale=1.0):
     g = torch.Generator().manual_seed(seed)
     return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def attention64(q, k, v, last, scale, terms):
+    """Rows q [n, D] over keys k, v [m, D]: row i sees keys j < last[i]. Returns (ref, error bound). A V that is
+    no number gives what the formula gives: inf and -inf where a row sees only one of them, NaN else."""
+    dtype = q.dtype
+    q, k, v = q.double(), k.double(), v.double()
+    m, D = k.shape
+    seen = torch.arange(m)[None, :] < last[:, None]
+    s = torch.where(seen, q @ k.t() * scale, -math.inf)
+    p = torch.nan_to_num(torch.softmax(s, 1))  # (rows that see nothing)
+    clean = torch.where(torch.isfinite(v), v, 0.0)
+    ref = p @ clean
+    score = (D + 3) * 2.0 ** -24 * scale * 1.4427 * torch.where(seen, q.abs() @ k.abs().t(), 0.0).amax(1)
+    rel = 2 * UNIT[dtype] ** terms + 2 * (2.0 ** -22 + score) + m * 2.0 ** -23
+    small = m * 2.0 ** -24 * clean.abs().max() if dtype == torch.float16 else 0.0
+    tol = rel[:, None] * (p @ clean.abs()) + small + UNIT[dtype] * ref.abs() + 2.0 ** -24
+    for sign in (math.inf, -math.inf, math.nan):
+        where = torch.isnan(v) if sign != sign else v == sign
+        hit = seen.double() @ where.double() > 0
+        ref = torch.where(hit, torch.where(torch.isfinite(ref), torch.tensor(sign, dtype=ref.dtype), ref + sign), ref)
+    return ref, tol
+
+
+def check(name, out, ref, tol):
+    out = out.detach().cpu().double()
+    finite = torch.isfinite(ref)
+    err = torch.where(finite, (out - torch.where(finite, ref, 0.0)).abs(), 0.0)
+    worst = float((err / tol).max())
+    print(f"{name}: worst err/bound {worst:.3f}", flush=True)
+    assert torch.equal(torch.where(finite, 0.0, out).nan_to_num(7.0, 8.0, 9.0), torch.where(finite, 0.0, ref).nan_to_num(7.0, 8.0, 9.0)), name
+    assert worst <= 1.0, name
 
 
 # ------------------------------------------------------------------------------ a plan's table
@@ -41,3 +87,34 @@ def test_plan_dropped_while_another_stream_has_to_read_it(gpu):
         t.zero_()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------ infinities and NaN in V
+def _spoil(v, at):
+    """One element of V inf, one -inf, one NaN and one inf and -inf, at keys from ``at`` on."""
+    for i, bad in enumerate((math.inf, -math.inf, math.nan, math.inf)):
+        v[at + i, :, 3 * i] = bad
+    v[at + 5, :, 9] = -math.inf
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,P", [(2, 4, 100), (2, 4, 1100), (3, 16, 1100), (9, 16, 1100), (40, 8, 1100)])
+def test_prefix_infinite_v_that_all_rows_see(gpu, dtype, B, H, P):
+    """An infinity in V gives infinities of its sign, whether probabilities enter P · V as one term or two (of which
+    the second must not be 0 or negative where the first is not), in the prefix and in a cache."""
+    ops = _ops()
+    Hkv, D, room = 2, 64, 40
+    q, kp, vp, ko, vo = (_rand(s, dtype, 5 + i, 0.5 if i in (1, 3) else 1.0) for i, s in enumerate(
+        [(B, 1, H, D), (P, Hkv, D), (P, Hkv, D), (B, room, Hkv, D), (B, room, Hkv, D)]))
+    _spoil(vp, 60)
+    _spoil(vo[1, :, :, 20:], 7)
+    lens = [40 - b % 3 for b in range(B)]
+    out = ops.attention_shared_prefix(*(t.to(gpu) for t in (q, kp, vp, ko, vo)),
+                                      torch.tensor(lens, dtype=torch.int32, device=gpu)).cpu()
+    terms = 1 if B * H // Hkv > 64 else 2  # (of the prefix's part)
+    for b in (0, 1):
+        for h in (0, H - 1):
+            y = h * Hkv // H
+            ref, tol = attention64(q[b, :, h], torch.cat((kp[:, y], ko[b, :lens[b], y])), torch.cat((vp[:, y], vo[b, :lens[b], y])),
+                                   torch.tensor([P + lens[b]]), D ** -0.5, terms)
+            check(f"{dtype} sequence {b} head {h}", out[b, :, h], ref, tol)

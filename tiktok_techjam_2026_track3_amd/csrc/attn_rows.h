@@ -96,6 +96,28 @@ MI355_DEVINL float prob_sum(bf16x8 f, float acc) {
   for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{f[2 * r], f[2 * r + 1]}, one, acc, false);
   return acc;
 }
+// A fragment of probabilities as two terms: what is left of each after its lower bits are cut off, and those. The
+// second is positive where the first is (at least the type's least number; in all off by at most 2^-21 of the
+// probability or 2^-24 in fp16, 2^-15 of it in bf16), so that both have an infinite v's product with its sign.
+MI355_DEVINL void two_terms(const float (&e)[8], f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int r = 0; r < 8; r += 2) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(e[r], e[r + 1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      hi[r + i] = h[i];
+      lo[r + i] = static_cast<_Float16>(__builtin_amdgcn_fmed3f(e[r + i] - static_cast<float>(h[i]), 0x1p-24f, e[r + i]));
+    }
+  }
+}
+MI355_DEVINL void two_terms(const float (&e)[8], bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float h = __uint_as_float(__float_as_uint(e[r]) & 0xffff0000u);
+    hi[r] = static_cast<__bf16>(h);
+    lo[r] = static_cast<__bf16>(__builtin_amdgcn_fmed3f(e[r] - h, 0x1p-126f, e[r]));
+  }
+}
 // reductions over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a row
 MI355_DEVINL float row_maximum(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -438,11 +460,10 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           e[r] = fast_exp2(__builtin_fmaf(s[n][2 * t + r / 4][r % 4], p.c, -mu[n]));
-          pf[0][n][t][r] = from_f32<T>(e[r]);
+          if constexpr (TERMS == 1) pf[0][n][t][r] = from_f32<T>(e[r]);
         }
         if constexpr (TERMS == 2) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) pf[1][n][t][r] = from_f32<T>(e[r] - to_f32(pf[0][n][t][r]));
+          two_terms(e, pf[0][n][t], pf[1][n][t]);
           lsum[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         } else {
           lsum[n] = prob_sum(pf[0][n][t], lsum[n]);
