@@ -1,5 +1,5 @@
 """The token-generation operators where their documentation allows what the first tests do not do: plans
-dropped while another stream still has to read them; infinities and NaN in V.
+dropped while another stream still has to read them; infinities and NaN in V, for every kind of tile.
 
 Error bounds (u = half a step of a type): a probability taken as one term enters the numerator and the sum with one
 rounding, 2 u (P |V|), fp16 ones off by 2^-25 at least; as two, the first cut off (below 2 u p is left) and the second
@@ -118,3 +118,89 @@ def test_prefix_infinite_v_that_all_rows_see(gpu, dtype, B, H, P):
             ref, tol = attention64(q[b, :, h], torch.cat((kp[:, y], ko[b, :lens[b], y])), torch.cat((vp[:, y], vo[b, :lens[b], y])),
                                    torch.tensor([P + lens[b]]), D ** -0.5, terms)
             check(f"{dtype} sequence {b} head {h}", out[b, :, h], ref, tol)
+
+
+KINDS = {  # q_lens, k_lens, heads, K/V heads, tiles of 128 rows
+    "wide": ([150] * 20, [150] * 20, 16, 16, True),       # 128 rows, one and two tiles of keys behind a row's last
+    "half": ([150, 40], [150, 47], 4, 2, False),          # 64 rows
+    "narrow": ([7, 16], [130, 77], 4, 2, False),          # up to 32 rows, keys of their own
+    "ranges": ([40, 5], [4000, 3000], 4, 2, False),       # joined
+}
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.bfloat16, 128), (torch.float16, 256), (torch.bfloat16, 80),
+                                     (torch.bfloat16, 16), (torch.float16, 96), (torch.float16, 32), (torch.bfloat16, 192), (torch.float16, 48)])
+def test_packed_not_finite_v(gpu, kind, dtype, D):
+    """Elements of V that are no numbers reach the rows that see them, as the formula has it, and no others, early in a
+    sequence (nearly all rows see them), in the middle and at its end."""
+    ops = _ops()
+    q_lens, k_lens, H, Hkv, wide = KINDS[kind]
+    q, k, v = _rand((sum(q_lens), H, D), dtype, 1), _rand((sum(k_lens), Hkv, D), dtype, 2, 0.5), _rand((sum(k_lens), Hkv, D), dtype, 3)
+    starts = [sum(k_lens[:i]) for i in range(len(k_lens))]
+    for i, (k0, m) in enumerate(zip(starts, k_lens)):
+        _spoil(v, k0 + (2, m // 2, m - 6, m - 30)[i % 4])
+    plan = ops.packed_plan(q_lens, k_lens, heads=H, kv_heads=Hkv, head_dim=D, device=gpu)
+    assert (plan.counts[0] > 0 and plan.tile_rows == 128) == wide and (plan.counts[2] > 0) == (kind == "ranges")
+    out = ops.attention_packed(q.to(gpu), k.to(gpu), v.to(gpu), plan).cpu()
+    narrow = plan.counts[0] == 0
+    q0 = 0
+    for i, (n, m, k0) in enumerate(zip(q_lens, k_lens, starts)):
+        if i < 5:
+            for h in (0, H - 1):
+                ref, tol = attention64(q[q0:q0 + n, h], k[k0:k0 + m, h * Hkv // H], v[k0:k0 + m, h * Hkv // H],
+                                       torch.arange(n) + m - n + 1, D ** -0.5, 2 if narrow or (n * H // Hkv <= 32 and m > 512) else 1)
+                check(f"{kind} {dtype} {D} sequence {i} head {h}", out[q0:q0 + n, h], ref, tol)
+        q0 += n
+
+
+@pytest.mark.parametrize("n,H,P", [(3, 4, 100), (3, 4, 1100), (9, 16, 40), (9, 16, 1100), (24, 4, 1100)])
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.bfloat16, 128), (torch.float16, 80), (torch.bfloat16, 256)])
+def test_prefix_not_finite_v(gpu, n, H, P, dtype, D):
+    """... and of a cache's V, those of the newest tokens and of earlier ones, and of the prefix."""
+    ops = _ops()
+    B, Hkv, room = 3, 2, 90
+    q, kp, vp, ko, vo = (_rand(s, dtype, 5 + i, 0.5 if i in (1, 3) else 1.0) for i, s in enumerate(
+        [(B, n, H, D), (P, Hkv, D), (P, Hkv, D), (B, room, Hkv, D), (B, room, Hkv, D)]))
+    lens = [90, 70, 33]
+    _spoil(vo[0], 90 - 6)
+    _spoil(vo[1], 3)
+    vo[2, 33:] = math.nan
+    vp[P // 2, 1, 7] = math.inf
+    out = ops.attention_shared_prefix(*(t.to(gpu) for t in (q, kp, vp, ko, vo)),
+                                      torch.tensor(lens, dtype=torch.int32, device=gpu)).cpu()
+    terms = 1 if B * n * H // Hkv > 64 else 2  # (of the prefix's part)
+    for b, m in enumerate(lens):
+        for h in range(0, H, H - 1):
+            y = h * Hkv // H
+            ref, tol = attention64(q[b, :, h], torch.cat((kp[:, y], ko[b, :m, y])), torch.cat((vp[:, y], vo[b, :m, y])),
+                                   torch.arange(n) + P + m - n + 1, D ** -0.5, terms)
+            check(f"{b} {h}", out[b, :, h], ref, tol)
+
+
+def test_packed_not_finite_v_costs_little(gpu):
+    """A call whose rows nearly all see a NaN, or just do not see it, takes a clean one's time, not hundreds of
+    times as long: a sequence that went wrong does not hold up its batch."""
+    ops = _ops()
+    T = 1536
+    q, k, v = (_rand((T, h, 64), torch.float16, h).to(gpu) for h in (16, 4, 4))
+    plan = ops.packed_plan([T], heads=16, kv_heads=4, head_dim=64, device=gpu)
+
+    def least(n=8):
+        times = []
+        for _ in range(n):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.attention_packed(q, k, v, plan)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    least()
+    clean = least()
+    for at in (0, T // 2, T - 1):
+        v2, v = v, v.clone()
+        v[at] = math.nan
+        assert least() < 6 * clean
+        v = v2

@@ -41,8 +41,17 @@ struct Join {
 };
 static_assert(sizeof(Join) == sizeof(rows::PackedTile), "plan entry");
 
+// Work-groups a CU that the registers have to leave room for: what the first sweep takes by itself, which the ones
+// over V that is not finite must not exceed.
+template <int HD, int QG, bool OWN_KEYS>
+constexpr int waves() {
+  if (HD > 128) return 1;
+  if (OWN_KEYS) return HD > 96 ? 2 : HD > 64 ? 3 : 4;
+  return QG == 1 ? (HD > 96 ? 4 : 5) : HD > 64 ? 3 : 4;
+}
+
 template <typename T, int HD, int QG, int BN, bool OWN_KEYS>
-__global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_rows_packed(rows::Args p) {
+__global__ __launch_bounds__(256, (waves<HD, QG, OWN_KEYS>())) void attn_rows_packed(rows::Args p) {
   __shared__ u32x4 lds[rows::lds_chunks<HD, 4, BN, OWN_KEYS>()];
   rows::attn_rows<T, HD, 4, QG, BN, OWN_KEYS, OWN_KEYS ? 2 : 1, rows::PACKED>(p, lds, blockIdx.x);
 }

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void attn_rows_prefix(rows:
   if (blockIdx.x < n_prefix)
     rows::attn_rows<T, HD, 4, QG, BN, SPLIT, PR <= 64 ? 2 : 1, rows::PREFIX>(a, lds, blockIdx.x);
   else
-    rows::attn_rows<T, HD, 4, OR / 16, 32, true, 2, rows::OWN>(own, lds, blockIdx.x - n_prefix);
+    rows::attn_rows<T, HD, 4, OR / 16, 32, true, 2, rows::OWN, sizeof(rows::Args)>(own, lds, blockIdx.x - n_prefix);
 }
 
 template <typename T, int HD, int PR, int OR>

@@ -15,6 +15,8 @@
 // at 1.9 GHz), by the bytes of K and V where they are few (32 single tokens against 4000 keys each: 100 us, 5.2 TB/s).
 #pragma once
 
+#include <type_traits>
+
 #include "attn.h"
 
 namespace rows {
@@ -157,20 +159,35 @@ MI355_DEVINL int swz(int r) {
 template <int HD, int NW, int BN, bool OWN_KEYS>
 constexpr int lds_chunks() { return 2 * BN * (HD / 8) * (OWN_KEYS ? NW : 2); }
 
+// What waves with the same rows leave for each other: maximum and sum of each row, and of all whether one has a NaN.
+template <int NW, int QW>
+struct Joined {
+  float ml[NW][QW][2];
+  uint32_t flags[NW];
+};
+
+enum Pass { GIVEN = 0, CLEAN = 1, UP = 2, DOWN = 3 };
+
 // The work of one work-group: NW waves of QG groups of 16 rows.
 //   OWN_KEYS = false: each wave has rows of its own, the waves share tiles of BN keys (double-buffered).
 //   OWN_KEYS = true, for at most 16 QG rows: the waves have the same rows and keys of their own, tile w,
 //     w + NW .. of the range, in one buffer each for K and V, and are joined through LDS at the end.
 // TERMS: the probabilities enter P · V as that many terms of the input type.
-template <typename T, int HD, int NW, int QG, int BN, bool OWN_KEYS, int TERMS, int MODE>
-MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
+// A key that a row does not see has probability 0, but its v row is in the tile: 0 · inf and 0 · NaN leave NaN in rows
+// that do not see it. Where that may have happened (a NaN beside keys that not all rows see: true is returned) the
+// work-group goes through its keys again (AGAIN: three passes, but if V has no such element at those keys), with
+//   CLEAN: infinities and NaN of V as 0, for the outputs; then, with K = 0 (every key that a row sees counts 1), for
+//   the outputs that such elements reach: UP: V = 1 for inf and NaN, 0 else, and inf is added where anything is left,
+//   DOWN: V = 1 for -inf and NaN, and -inf is added.
+// (2048 tokens, 32/8 heads of 128, bf16, all of which see a NaN: 71 us instead of 65.)
+template <typename T, int HD, int NW, int QG, int BN, bool OWN_KEYS, int TERMS, int MODE, bool AGAIN>
+MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* join, const unsigned block, const int pass) {
   constexpr int RING = OWN_KEYS ? 1 : 2;
   using frag = typename Mfma<T>::frag;
   typedef T frag4 __attribute__((ext_vector_type(4)));
   static_assert(HD % 16 == 0 && BN % 32 == 0, "shape");
   constexpr int QW = 16 * QG, BM = OWN_KEYS ? QW : NW * QW;
   constexpr int LW = OWN_KEYS ? 1 : NW;  // waves that load a tile
-  static_assert(QW <= 32 || !OWN_KEYS, "rows of a word");
   constexpr int NCH = HD / 8, ROWB = HD * 2;
   // MFMA steps of S^T, 32 elements each; of HD 16, 48 and 80 the last one's upper half is zeros in both
   // operands. (A 16x16x16 MFMA for it, accumulating onto the 16x16x32 right before it, lost two of its four
@@ -181,7 +198,9 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
   static_assert(BN * NCH % 64 == 0, "whole blocks of loads");
   constexpr int BLK = BN * NCH / 64, LPW = (BLK + LW - 1) / LW, TILE = BN * NCH;
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  int tid = threadIdx.x;
+  if constexpr (AGAIN) asm volatile("" : "+v"(tid));
+  const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, l16 = lane & 15;
 
@@ -241,7 +260,7 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       nrows = p.B * p.n_q * p.G;
       k_off = 0x40000000;
     }
-    if (k_begin >= len) return;  // (the combining kernel does not read this split)
+    if (k_begin >= len) return false;  // (the combining kernel does not read this split)
     k_end = k_begin + p.chunk < len ? k_begin + p.chunk : len;
   }
   Kb = uniform_ptr(Kb + static_cast<int64_t>(k_begin) * p.kt);
@@ -392,14 +411,30 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
 
   f32x4 o[QG][DT];
   float mu[QG], gate[QG], lsum[QG];  // running max (log2 domain), the score that moves it, row sum
+
+  constexpr bool F16 = std::is_same_v<T, _Float16>;
+  constexpr uint32_t LOWEST = 0x00010001u << (F16 ? 10 : 7), EXP = 0x80008000u - LOWEST, ONES = F16 ? 0x3c003c00u : 0x3f803f80u;
+  const auto all_ones = [](uint32_t sign) MI355_LAMBDA_INLINE { return (sign >> 15 & 0x00010001u) * 0xffffu; };
+  // halves of all ones where an exponent has all bits set: adding the lowest carries into the sign's place
+  const auto not_finite = [&](uint32_t w) MI355_LAMBDA_INLINE { return all_ones((w & EXP) + LOWEST); };
+  // this wave's part of a tile as `pass` has it, K and V
+  const auto pass_k = [&](int st) MI355_LAMBDA_INLINE {
+#pragma nounroll
+    for (int blk = lwave; blk < BLK && pass > CLEAN; blk += LW) lds[st * TILE + 64 * blk + lane] = u32x4{0u, 0u, 0u, 0u};
+  };
+  const auto pass_v = [&](int st) MI355_LAMBDA_INLINE {
+#pragma nounroll
+    for (int blk = lwave; blk < BLK; blk += LW) {
+      u32x4 w = lds[(RING + st) * TILE + 64 * blk + lane];
 #pragma unroll
-  for (int n = 0; n < QG; ++n) {
-#pragma unroll
-    for (int t = 0; t < DT; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    mu[n] = 0.f;
-    gate[n] = NEG_INF;
-    lsum[n] = 0.f;
-  }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t bad = not_finite(w[e]), nan = all_ones((w[e] & (LOWEST - 0x00010001u)) + 0x7fff7fffu);
+        const uint32_t one = bad & (nan | (pass == UP ? ~all_ones(w[e]) : all_ones(w[e])));
+        w[e] = pass == CLEAN ? w[e] & ~bad : one & ONES;
+      }
+      lds[(RING + st) * TILE + 64 * blk + lane] = w;
+    }
+  };
 
   // scores_done: the tile's K has been read; need_v: its V is about to be
   auto tile = [&](const int j, const int st, auto&& scores_done, auto&& need_v) MI355_LAMBDA_INLINE {
@@ -482,116 +517,93 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
       }
   };
 
-  if constexpr (OWN_KEYS) {
-    // K of the next tile is requested as soon as this one's has been read, V likewise, so that one of
-    // them is always in flight: of the 2 LPW newest loads the older LPW have to be there.
-    static_assert(LPW < 64, "vmcnt");
-    constexpr int OLDER = (LPW & 15) | (LPW >> 4) << 14 | 7 << 4 | 15 << 8;  // vmcnt(LPW)
-    constexpr int READ = 15 | 3 << 14 | 7 << 4;                              // lgkmcnt(0)
-    for (int part = MODE == WHOLE ? 0 : 1; part < 2; ++part) {
-      bind_part(part);
-      const int n_kt = (n_keys + BN - 1) / BN;
-      const int n_mine = n_kt < (lim_last + BN - 1) / BN ? n_kt : (lim_last + BN - 1) / BN;
-      if (wave < n_mine) {
-        issue_k(wave, 0);
-        issue_v(wave, 0);
-      }
-      for (int j = wave; j < n_mine; j += NW) {
-        const bool more = j + NW < n_mine;
-        __builtin_amdgcn_s_waitcnt(OLDER);
-        tile(j, 0,
-             [&]() MI355_LAMBDA_INLINE {
-               __builtin_amdgcn_s_waitcnt(READ);
-               if (more) issue_k(j + NW, 0);
-             },
-             [&]() MI355_LAMBDA_INLINE {
-               if (more) __builtin_amdgcn_s_waitcnt(OLDER);
-               else __builtin_amdgcn_s_waitcnt(0);
-             });
-        __builtin_amdgcn_s_waitcnt(READ);
-        if (more) issue_v(j + NW, 0);
-      }
+  const auto sweep = [&]() MI355_LAMBDA_INLINE {
+#pragma unroll
+    for (int n = 0; n < QG; ++n) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mu[n] = 0.f;
+      gate[n] = NEG_INF;
+      lsum[n] = 0.f;
     }
-  } else {
-    bind();
-    const int n_kt = (n_keys + BN - 1) / BN;
-    const auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
-      issue_k(j, st);
-      issue_v(j, st);
-    };
-    const auto nothing = []() MI355_LAMBDA_INLINE {};
-    if (n_kt > 0) issue(0, 0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
-      if (j + 1 < n_kt) issue(j + 1, st ^ 1);
-      if (!idle && j * BN < lim_last) tile(j, st, nothing, nothing);
-      // this wave's loads of tile j + 1 have landed and its reads of tile j are done
+    if constexpr (OWN_KEYS) {
+      // K of the next tile is requested as soon as this one's has been read, V likewise, so that one of
+      // them is always in flight: of the 2 LPW newest loads the older LPW have to be there.
+      static_assert(LPW < 64, "vmcnt");
+      constexpr int OLDER = (LPW & 15) | (LPW >> 4) << 14 | 7 << 4 | 15 << 8;  // vmcnt(LPW)
+      constexpr int READ = 15 | 3 << 14 | 7 << 4;                              // lgkmcnt(0)
+      for (int part = MODE == WHOLE ? 0 : 1; part < 2; ++part) {
+        bind_part(part);
+        const int n_kt = (n_keys + BN - 1) / BN;
+        const int n_mine = n_kt < (lim_last + BN - 1) / BN ? n_kt : (lim_last + BN - 1) / BN;
+        if (wave < n_mine) {
+          issue_k(wave, 0);
+          issue_v(wave, 0);
+        }
+        for (int j = wave; j < n_mine; j += NW) {
+          const bool more = j + NW < n_mine;
+          __builtin_amdgcn_s_waitcnt(OLDER);
+          if constexpr (AGAIN) pass_k(0);
+          tile(j, 0,
+               [&]() MI355_LAMBDA_INLINE {
+                 __builtin_amdgcn_s_waitcnt(READ);
+                 if (more) issue_k(j + NW, 0);
+               },
+               [&]() MI355_LAMBDA_INLINE {
+                 if (more) __builtin_amdgcn_s_waitcnt(OLDER);
+                 else __builtin_amdgcn_s_waitcnt(0);
+                 if constexpr (AGAIN) pass_v(0);
+               });
+          __builtin_amdgcn_s_waitcnt(READ);
+          if (more) issue_v(j + NW, 0);
+        }
+      }
+    } else {
+      bind();
+      const int n_kt = (n_keys + BN - 1) / BN;
+      const auto issue = [&](int j, int st) MI355_LAMBDA_INLINE {
+        issue_k(j, st);
+        issue_v(j, st);
+      };
+      const auto nothing = []() MI355_LAMBDA_INLINE {};
+      if (n_kt > 0) issue(0, 0);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-    };
-    int j = 0;
-    for (; j + 2 <= n_kt; j += 2) {
-      step(j, 0);
-      step(j + 1, 1);
-    }
-    if (j < n_kt) step(j, 0);
-  }
-
-  // A key behind a row's last one has probability 0, but its v row is in the tile: 0 · inf and
-  // 0 · NaN leave NaN in rows that do not see it. Rows with NaN whose range held such keys are
-  // computed again, by a wave, one key at a time over the keys they see (a row that sees a NaN gets it again).
-  const auto again = [&](int r) MI355_LAMBDA_INLINE {
-    const int keys = lim_of(r);
-    if (MODE == PREFIX || keys >= n_keys || (MODE != WHOLE && keys <= 0)) return;
-    constexpr int DL = (HD + 63) / 64;
-    const T* src = Qb + q_of(r);
-    float q[DL], acc[DL], m = NEG_INF, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < DL; ++i) {
-      q[i] = lane + 64 * i < HD ? to_f32(src[lane + 64 * i]) : 0.f;
-      acc[i] = 0.f;
-    }
-    for (int part = MODE == WHOLE ? 0 : 1; part < 2; ++part) {
-      if constexpr (MODE == WHOLE) bind_part(part);
-      const int count = part == 0 ? n_keys : keys;
-      for (int key = 0; key < count; ++key) {
-        const T* kr = Kb + key * kt;
-        const T* vr = Vb + key * vt;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < DL; ++i)
-          if (lane + 64 * i < HD) s = __builtin_fmaf(q[i], to_f32(kr[lane + 64 * i]), s);
-        for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
-        s *= p.c;
-        const float m2 = vmax(m, s);
-        const float a = m == NEG_INF ? 0.f : fast_exp2(m - m2);
-        const float e = s == NEG_INF ? 0.f : fast_exp2(s - m2);
-        l = __builtin_fmaf(l, a, e);
-#pragma unroll
-        for (int i = 0; i < DL; ++i)
-          if (lane + 64 * i < HD) acc[i] = __builtin_fmaf(acc[i], a, e * to_f32(vr[lane + 64 * i]));
-        m = m2;
+      auto step = [&](const int j, const int st) MI355_LAMBDA_INLINE {
+        if (j + 1 < n_kt) issue(j + 1, st ^ 1);
+        if constexpr (AGAIN) {
+          pass_k(st);
+          pass_v(st);
+          __syncthreads();
+        }
+        if (!idle && j * BN < lim_last) tile(j, st, nothing, nothing);
+        // this wave's loads of tile j + 1 have landed and its reads of tile j are done
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+      };
+      int j = 0;
+      for (; j + 2 <= n_kt; j += 2) {
+        step(j, 0);
+        step(j + 1, 1);
       }
-    }
-    if (direct) {
-      T* dst = out_of(r);
-#pragma unroll
-      for (int i = 0; i < DL; ++i)
-        if (lane + 64 * i < HD) dst[lane + 64 * i] = from_f32<T>(acc[i] / l);
-    } else {
-      const int64_t at = part_of(r);
-#pragma unroll
-      for (int i = 0; i < DL; ++i)
-        if (lane + 64 * i < HD) p.part[at * HD + lane + 64 * i] = acc[i];
-      if (lane == 0) {
-        p.ml[2 * at] = m;
-        p.ml[2 * at + 1] = l;
-      }
+      if (j < n_kt) step(j, 0);
     }
   };
-  // 4 elements of a row whose output (or partial result) starts at dst (part); NaN stays in nan
-  const auto put = [&](T* dst, float* part, int d, f32x4 v, float inv, bool sees, float& nan) MI355_LAMBDA_INLINE {
+
+  // 4 elements of a row whose output (or partial result) starts at dst (part); whether one is NaN
+  const auto put = [&](T* dst, float* part, int d, f32x4 v, float inv, bool sees, bool& nan) MI355_LAMBDA_INLINE {
+    frag4* const out = reinterpret_cast<frag4*>(dst + d);
+    f32x4* const some = reinterpret_cast<f32x4*>(part + d);
+    if (AGAIN && pass > CLEAN) {
+      const float add = pass == UP ? -NEG_INF : NEG_INF;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (v[e] == 0.f || (direct && !sees)) continue;
+        if (direct) (*out)[e] = from_f32<T>(to_f32((*out)[e]) + add);
+        else (*some)[e] += add;
+      }
+      return;
+    }
     if (direct) {
       // no key seen: zeros; keys seen, all with a score of -inf: 0 / 0, as softmax's
       frag4 w;
@@ -600,102 +612,133 @@ MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
         v[e] = sees ? v[e] * inv : 0.f;
         w[e] = from_f32<T>(v[e]);
       }
-      *reinterpret_cast<frag4*>(dst + d) = w;
+      *out = w;
     } else {
-      *reinterpret_cast<f32x4*>(part + d) = v;
+      *some = v;
     }
-    if constexpr (MODE != PREFIX) nan = vmax(nan, vmax(vmax(v[0], v[1]), vmax(v[2], v[3])));
+    if constexpr (MODE != PREFIX && !AGAIN) {
+      const float m = vmax(vmax(v[0], v[1]), vmax(v[2], v[3]));
+      nan |= m != m;
+    }
   };
   const auto put_ml = [&](int r, float m, float sum) MI355_LAMBDA_INLINE {
-    if (direct) return;
+    if (direct || AGAIN) return;
     const int64_t at = part_of(r);
     p.ml[2 * at] = m;
     p.ml[2 * at + 1] = sum;
   };
-
-  if constexpr (OWN_KEYS) {
-    // The waves' rows meet in LDS: each wave's outputs where its tiles were, its maxima and sums beside.
-    __shared__ float ml[NW][QW][2];
-    __shared__ uint32_t nan_rows;
-    static_assert(QW * HD * 4 <= 2 * TILE * 16, "a wave's outputs fit its tiles");
-    f32x4* const mine = reinterpret_cast<f32x4*>(lds);
-#pragma unroll
-    for (int n = 0; n < QG; ++n) {
-      const float sum = row_sum(lsum[n]);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) mine[(16 * n + l16) * (HD / 4) + 4 * dt + g] = o[n][dt];
-      if (g == 0) {
-        // (a sum that is not 0 without a maximum is NaN's)
-        ml[wave][16 * n + l16][0] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
-        ml[wave][16 * n + l16][1] = sum;
-      }
-    }
-    if (tid == 0) nan_rows = 0;
-    __syncthreads();
-    const f32x4* const all = reinterpret_cast<const f32x4*>(lds - wave * 2 * TILE);
-    const int real = nrows - row0 < QW ? nrows - row0 : QW;
-    for (int at = tid; at < real * (HD / 4); at += NW * 64) {
-      const int x = at / (HD / 4), d = at % (HD / 4);
-      float m = NEG_INF, sum = 0.f;
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < NW; ++w) m = vmax(m, ml[w][x][0]);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float mw = ml[w][x][0];
-        if (mw == NEG_INF) continue;  // no finite score there
-        const float f = fast_exp2(mw - m);
-        sum = __builtin_fmaf(ml[w][x][1], f, sum);
-        const f32x4 ow = all[w * 2 * TILE + x * (HD / 4) + d];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], f, v[e]);
-      }
-      float nan = 0.f;
-      T* const dst = direct ? out_of(row0 + x) : nullptr;
-      float* const part = direct ? nullptr : p.part + part_of(row0 + x) * HD;
-      put(dst, part, 4 * d, v, 1.0f / sum, lim_of(row0 + x) > 0 || (MODE == WHOLE && p.pkeys > 0), nan);
-      if (nan != nan) atomicOr(&nan_rows, 1u << x);
-      if (d == 0) put_ml(row0 + x, m, sum);
-    }
-    if constexpr (MODE != PREFIX) {
-      __builtin_amdgcn_s_waitcnt(0);  // the stores above are done
-      __syncthreads();
-      const uint32_t bad = nan_rows;
-      for (int x = wave; x < real; x += NW)
-        if ((bad >> x) & 1) again(row0 + x);
-    }
-  } else {
-    // each lane holds runs of 4 of its row's elements
-    uint64_t nan_rows[QG];
-#pragma unroll
-    for (int n = 0; n < QG; ++n) {
-      const int r = row_w + 16 * n + l16;
-      const float sum = row_sum(lsum[n]);
-      float nan = 0.f;
-      if (r < nrows) {
-        T* const dst = direct ? out_of(r) : nullptr;
-        float* const part = direct ? nullptr : p.part + part_of(r) * HD;
-        const float inv = 1.0f / sum;
-        if (direct) {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
-        } else {
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
-        }
-        if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n], sum);
-      }
-      const uint64_t m = __builtin_amdgcn_ballot_w64(nan != nan);
-      nan_rows[n] = (m | (m >> 16) | (m >> 32) | (m >> 48)) & 0xffffu;
-    }
-    if constexpr (MODE != PREFIX) {
+  // writes what the sweep has left; whether there is a NaN among what this thread wrote
+  const auto results = [&]() MI355_LAMBDA_INLINE {
+    bool nan = false;
+    if constexpr (OWN_KEYS) {
+      // The waves' rows meet in LDS: each wave's outputs where its tiles were, its maxima and sums beside.
+      static_assert(QW * HD * 4 <= 2 * TILE * 16, "a wave's outputs fit its tiles");
+      f32x4* const mine = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
       for (int n = 0; n < QG; ++n) {
-        if (nan_rows[n] == 0) continue;
-        __builtin_amdgcn_s_waitcnt(0);  // the stores above are done
-        for (int x = 0; x < 16; ++x)
-          if ((nan_rows[n] >> x) & 1) again(row_w + 16 * n + x);
+        const float sum = row_sum(lsum[n]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) mine[(16 * n + l16) * (HD / 4) + 4 * dt + g] = o[n][dt];
+        if (g == 0) {
+          // (a sum that is not 0 without a maximum is NaN's)
+          join->ml[wave][16 * n + l16][0] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
+          join->ml[wave][16 * n + l16][1] = sum;
+        }
       }
+      __syncthreads();
+      const f32x4* const all = reinterpret_cast<const f32x4*>(lds - wave * 2 * TILE);
+      const int real = nrows - row0 < QW ? nrows - row0 : QW;
+      for (int at = tid; at < real * (HD / 4); at += NW * 64) {
+        const int x = at / (HD / 4), d = at % (HD / 4);
+        float m = NEG_INF, sum = 0.f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = vmax(m, join->ml[w][x][0]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float mw = join->ml[w][x][0];
+          if (mw == NEG_INF) continue;  // no finite score there
+          const float f = fast_exp2(mw - m);
+          sum = __builtin_fmaf(join->ml[w][x][1], f, sum);
+          const f32x4 ow = all[w * 2 * TILE + x * (HD / 4) + d];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(ow[e], f, v[e]);
+        }
+        T* const dst = direct ? out_of(row0 + x) : nullptr;
+        float* const part = direct ? nullptr : p.part + part_of(row0 + x) * HD;
+        put(dst, part, 4 * d, v, 1.0f / sum, lim_of(row0 + x) > 0 || (MODE == WHOLE && p.pkeys > 0), nan);
+        if (d == 0) put_ml(row0 + x, m, sum);
+      }
+    } else {
+      // each lane holds runs of 4 of its row's elements
+#pragma unroll
+      for (int n = 0; n < QG; ++n) {
+        const int r = row_w + 16 * n + l16;
+        const float sum = row_sum(lsum[n]);
+        if (r < nrows) {
+          T* const dst = direct ? out_of(r) : nullptr;
+          float* const part = direct ? nullptr : p.part + part_of(r) * HD;
+          const float inv = 1.0f / sum;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
+          if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n], sum);
+        }
+      }
+    }
+    return nan;
+  };
+  // Whether any thread of the work-group says so; nothing but LDS is waited for, the outputs above are still on their
+  // way. (Where the waves share tiles, those have all been read.)
+  const auto any_wave = [&](bool mine) MI355_LAMBDA_INLINE {
+    uint32_t* const flags = OWN_KEYS ? join->flags : reinterpret_cast<uint32_t*>(lds);
+    const bool any = __builtin_amdgcn_ballot_w64(mine) != 0;
+    if (lane == 0) flags[wave] = any;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all |= flags[w];
+    return __builtin_amdgcn_readfirstlane(all) != 0;
+  };
+  // keys that every row sees; from there on (of the work-group's keys) those that only some do
+  const int first = lim_of(row0) > 0 ? lim_of(row0) : 0;
+  if (AGAIN && pass == CLEAN) {
+    bool leak = false;
+    for (int at = tid; at < (n_keys - first) * NCH; at += NW * 64) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(Vb + (first + at / NCH) * vt + at % NCH * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) leak |= not_finite(w[e]) != 0;
+    }
+    if (!any_wave(leak)) return false;
+    __syncthreads();  // the flags have been read
+  }
+  sweep();
+  const bool nan = results();
+  if constexpr (AGAIN) return pass < DOWN;
+  return MODE != PREFIX && first < n_keys && any_wave(nan);
+}
+
+// ... from its kernel's arguments, ARGS bytes of which come before p
+template <typename T, int HD, int NW, int QG, int BN, bool OWN_KEYS, int TERMS, int MODE, int ARGS = 0>
+MI355_DEVINL void attn_rows(const Args& p, u32x4* lds, const unsigned block) {
+  __shared__ Joined<NW, 16 * QG> own_join;
+  Joined<NW, 16 * QG>* const join = OWN_KEYS ? &own_join : nullptr;
+  bool more = sweep_rows<T, HD, NW, QG, BN, OWN_KEYS, TERMS, MODE, false>(p, lds, join, block, GIVEN);
+  if constexpr (MODE != PREFIX) {
+#pragma nounroll
+    for (int pass = CLEAN; more; ++pass) {
+      __syncthreads();  // what the waves have in LDS has been read
+      // The arguments once more from memory: the compiler would keep all that the sweeps share in registers throughout.
+      auto args = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr());
+      unsigned same = block;
+      asm volatile("" : "+s"(args), "+s"(same));
+      struct Words { uint64_t v[sizeof(Args) / 8]; } words;
+      static_assert(sizeof(words) == sizeof(Args), "8-byte words");
+#pragma unroll
+      for (size_t i = 0; i < sizeof(Args) / 8; ++i)
+        words.v[i] = reinterpret_cast<const __attribute__((address_space(4))) uint64_t*>(args + ARGS)[i];
+      more = sweep_rows<T, HD, NW, QG, BN, OWN_KEYS, TERMS, MODE, true>(__builtin_bit_cast(Args, words), lds, join, same, pass);
     }
   }
 }
