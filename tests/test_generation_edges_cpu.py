@@ -1,5 +1,5 @@
 """What the token-generation operators do at the edges of their documentation, as far as it shows without a
-GPU: how long a plan's table lives."""
+GPU: how long a plan's table lives, 4-bit weights of every magnitude."""
 import importlib
 from types import SimpleNamespace
 
@@ -22,3 +22,52 @@ def test_plan_tells_the_allocator_of_other_streams(monkeypatch, current, capturi
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: ("stream", device, current))
     plan.used_on(3)
     assert seen == ([("stream", 3, current)] if told else [])
+
+
+# ------------------------------------------------------------------------------ 4-bit weights
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def dequantised(q, scale, zero, group):
+    n, k = q.shape[0], 2 * q.shape[1]
+    v = torch.stack((q & 15, q >> 4), -1).reshape(n, k).double()
+    z = zero.double().repeat_interleave(group, 1) if zero is not None else 8.0
+    return (v - z) * scale.double().repeat_interleave(group, 1)
+
+
+@pytest.mark.parametrize("dtype,exps", [(torch.float16, range(0, 25)), (torch.bfloat16, (0, 60, 110, 120, 124, 126, 128, 130, 133))])
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+def test_quant_groups_i4_of_every_magnitude(dtype, exps, symmetric, group):
+    """The error relative to the group's own range, down to weights of a few of the type's least numbers. A step
+    is range / 15 (largest / 7), its scale off by u of it, or, below the least normal number, up to a least number
+    more; a value is off by half a step, the zero point by another half, and by the scale's error over 15 (7) steps
+    where it was rounded down."""
+    least = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    for e in exps:
+        w = (torch.randn(24, 256, generator=torch.Generator().manual_seed(e)) * 2.0 ** -e).to(dtype)
+        w[3, :group] = 0
+        q, scale, zero = ops.quant_groups_i4(w, group, symmetric)
+        assert scale.dtype == dtype and bool((scale > 0).all())
+        x = w.double().reshape(24, -1, group)
+        span = x.abs().amax(2) / 7 if symmetric else (x.amax(2).clamp_min(0) - x.amin(2).clamp_max(0)) / 15
+        bound = (span + least) * (0.5 + (0 if symmetric else 0.5) + 16 * UNIT[dtype])
+        err = (dequantised(q, scale, zero, group).reshape(x.shape) - x).abs().amax(2)
+        assert bool((err <= bound).all()), (e, float((err / bound).max()))
+
+
+def test_quant_groups_i4_least_numbers_come_back():
+    """Weights that are up to 15 of fp16's least numbers are kept exactly."""
+    step = 2.0 ** -24
+    w = (torch.randint(0, 16, (8, 64), generator=torch.Generator().manual_seed(1)).double() * step).to(torch.float16)
+    w[:, 0], w[:, 32] = 0, 15 * step
+    w[:, 1], w[:, 33] = 15 * step, 0
+    got = dequantised(*ops.quant_groups_i4(w, 32), 32)
+    assert torch.equal(got, w.double())
+
+
+def test_quant_groups_i4_without_rows_or_columns():
+    q, scale, zero = ops.quant_groups_i4(torch.zeros(0, 64).half(), 32)
+    assert q.shape == (0, 32) and scale.shape == zero.shape == (0, 2)
+    with pytest.raises(ValueError):
+        ops.quant_groups_i4(torch.zeros(4, 0).half(), 32)

@@ -1,5 +1,6 @@
 """The token-generation operators where their documentation allows what the first tests do not do: plans
-dropped while another stream still has to read them; infinities and NaN in V, for every kind of tile.
+dropped while another stream still has to read them; infinities and NaN in V, for every kind of tile;
+4-bit weights of every magnitude.
 
 Error bounds (u = half a step of a type): a probability taken as one term enters the numerator and the sum with one
 rounding, 2 u (P |V|), fp16 ones off by 2^-25 at least; as two, the first cut off (below 2 u p is left) and the second
@@ -204,3 +205,22 @@ def test_packed_not_finite_v_costs_little(gpu):
         v[at] = math.nan
         assert least() < 6 * clean
         v = v2
+
+
+# ------------------------------------------------------------------------------ 4-bit weights
+@pytest.mark.parametrize("dtype,exps", [(torch.float16, (0, 10, 14, 17, 20, 24)), (torch.bfloat16, (0, 110, 124, 128, 133))])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_i4_weights_of_every_magnitude(gpu, dtype, exps, symmetric):
+    """Weights down to a few of the type's least numbers, quantised on the GPU and read back by one-hot rows of the
+    projection: within a step (half of one and half a zero point; u of 15 steps and a least number for the scale)."""
+    ops = _ops()
+    least = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    for e in exps:
+        w = _rand((24, 256), torch.float32, e, 2.0 ** -e).to(dtype)
+        q, scale, zero = ops.quant_groups_i4(w.to(gpu), 64, symmetric)
+        out = ops.linear_i4(torch.eye(256, dtype=dtype, device=gpu), q, scale, zero, out_dtype=torch.float32)
+        x = w.double().reshape(24, -1, 64)
+        span = x.abs().amax(2) / 7 if symmetric else (x.amax(2).clamp_min(0) - x.amin(2).clamp_max(0)) / 15
+        bound = (span + least) * (0.5 + (0 if symmetric else 0.5) + 16 * UNIT[dtype])
+        err = (out.t().cpu().double().reshape(x.shape) - x).abs().amax(2)
+        assert bool((err <= bound).all()), (e, float((err / bound).max()))

@@ -854,6 +854,16 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 I4_GROUPS = (32, 64, 128)
 
 
+def _group_scale(step: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Scales for ``step``, rounded to ``dtype``: to the nearest, but upwards below its least normal number, where
+    a step rounded down would leave a group's ends out of reach by whole steps, and at least its least number
+    (groups of zeros)."""
+    info = torch.finfo(dtype)
+    least = info.tiny * info.eps
+    up = ((step.double() / least).ceil().clamp_min(1) * least).float()
+    return torch.where(step < info.tiny, up, step).to(dtype)
+
+
 def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
                     ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """4-bit weights for ``linear_i4`` from ``w`` ``[N, K]`` (fp16 or bf16): ``(q, scale, zero)`` with
@@ -862,17 +872,16 @@ def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
     ``symmetric`` its largest magnitude to +-7 around 8 (zero is None). Run once per weight."""
     if w.dim() != 2 or w.dtype not in _SIXTEEN_BIT:
         raise ValueError("quant_groups_i4 expects a 2-D fp16 or bf16 weight")
-    if group not in I4_GROUPS or w.shape[1] % group:
+    if group not in I4_GROUPS or w.shape[1] % group or w.shape[1] == 0:
         raise ValueError(f"group must be one of {I4_GROUPS} and divide K = {w.shape[1]}")
     with torch.no_grad():
-        x = w.detach().float().reshape(w.shape[0], -1, group)
-        tiny = torch.finfo(w.dtype).tiny  # an all-zero group's scale
+        x = w.detach().float().reshape(w.shape[0], w.shape[1] // group, group)
         if symmetric:
-            scale = (x.abs().amax(2) / 7).clamp_min(tiny).to(w.dtype)
+            scale = _group_scale(x.abs().amax(2) / 7, w.dtype)
             zero, z = None, 8.0
         else:
             lo, hi = x.amin(2).clamp_max(0), x.amax(2).clamp_min(0)
-            scale = ((hi - lo) / 15).clamp_min(tiny).to(w.dtype)
+            scale = _group_scale((hi - lo) / 15, w.dtype)
             z = (-lo / scale.float()).round().clamp(0, 15)
             zero, z = z.to(torch.uint8), z[..., None]
         q = ((x / scale.float()[..., None]).round() + z).clamp(0, 15).to(torch.uint8).reshape(w.shape)
