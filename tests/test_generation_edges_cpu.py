@@ -1,12 +1,14 @@
 """What the token-generation operators do at the edges of their documentation, as far as it shows without a
-GPU: how long a plan's table lives, 4-bit weights of every magnitude."""
-import importlib
+GPU: how long a plan's table lives, 4-bit weights of every magnitude,
+what profiles and the build look for."""
+import re
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from tiktok_techjam_2026_track3_amd import _lib, ops
+from tiktok_techjam_2026_track3_amd import _lib, ops, profiling
 
 
 # ------------------------------------------------------------------------------ a plan's table
@@ -71,3 +73,13 @@ def test_quant_groups_i4_without_rows_or_columns():
     assert q.shape == (0, 32) and scale.shape == zero.shape == (0, 2)
     with pytest.raises(ValueError):
         ops.quant_groups_i4(torch.zeros(4, 0).half(), 32)
+
+
+# ------------------------------------------------------------------------------ profiles and the build's checks
+def test_profiles_name_every_kernel():
+    """The profiler's summaries know every kernel of the library's sources by its own name."""
+    csrc = Path(ops.__file__).parent / "csrc"
+    names = [n for f in sorted(csrc.iterdir()) for n in re.findall(r"__global__[^;{]*?\bvoid\s+(\w+)\s*\(", f.read_text())]
+    assert len(names) > 15 and "linear_i4_held" in names
+    for n in names:
+        assert profiling.short_name(f"_ZN12_GLOBAL__N_1{len(n)}{n}IDF16_Li64EEEvNS_4ArgsE") == f"{n}<f16,64>"
