@@ -1,6 +1,7 @@
 """What the token-generation operators do at the edges of their documentation, as far as it shows without a
 GPU: how long a plan's table lives, 4-bit weights of every magnitude,
 what profiles and the build look for."""
+import importlib
 import re
 from pathlib import Path
 from types import SimpleNamespace
@@ -83,3 +84,18 @@ def test_profiles_name_every_kernel():
     assert len(names) > 15 and "linear_i4_held" in names
     for n in names:
         assert profiling.short_name(f"_ZN12_GLOBAL__N_1{len(n)}{n}IDF16_Li64EEEvNS_4ArgsE") == f"{n}<f16,64>"
+
+
+@pytest.mark.parametrize("vector,bad", [
+    ("v_mad_u64_u32 v[2:3], s[6:7], v4, v5, v[6:7]", True), ("v_mad_i64_i32 v[2:3], s[4:5], v4, v5, 0", True),
+    ("v_add_co_u32_e64 v2, s[6:7], v3, v4", True), ("v_addc_co_u32_e64 v2, s[6:7], v3, v4, s[8:9]", True),
+    ("v_subbrev_co_u32_e64 v2, s[6:7], v3, v4, vcc", True), ("v_div_scale_f32 v2, s[6:7], v3, v4, v5", True),
+    ("v_addc_co_u32_e64 v2, vcc, v3, v4, s[6:7]", False),    # carry in only
+    ("v_cndmask_b32_e64 v2, v3, v4, s[6:7]", False), ("v_add_u32_e64 v2, s6, v3", False)])
+def test_build_sees_carries_as_writes(vector, bad):
+    """A carry or scale mask that the vector ALU leaves in scalar registers is a write like any other to the check of
+    LDS-DMA loads."""
+    build = importlib.import_module("tiktok_techjam_2026_track3_amd.build")
+    asm = "\n".join(["attn_rows_x:", "  " + vector, "  s_mov_b32 m0, s20", "  s_nop 0",
+                     "  buffer_load_dwordx4 v2, s[4:7], s9 offen lds", "  s_endpgm", ".Lfunc_end0:"])
+    assert bool(build.dma_hazards(asm)) == bad

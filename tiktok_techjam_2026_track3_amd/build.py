@@ -169,11 +169,12 @@ def mfma_hazards(asm: str) -> list:
 
 
 # The LDS-DMA loads of inline assembly read their buffer resource and offset from scalar registers. Written by
-# the vector ALU (v_readfirstlane, v_readlane, a compare's mask), those have to be this many wait states older.
+# the vector ALU (v_readfirstlane, v_readlane, a compare's mask, a carry), those have to be this many wait states older.
 ASM_DMA_SOURCES = re.compile(r"attn_(packed|prefix)$")
 ASM_DMA_KERNELS = re.compile(r"attn_rows_")
 VALU_TO_VMEM_SGPR = 5
 _SREG = re.compile(r"\bs(?:(\d+)\b|\[(\d+):(\d+)\])")
+_CARRY_OUT = re.compile(r"v_\w+_co_|v_mad_[ui]64_|v_div_scale_")  # a scalar result as second operand
 
 
 def _sregs(text: str) -> set:
@@ -195,6 +196,8 @@ def _dma_hazards(seq: list) -> list:
         if op.startswith("buffer_load") and args.endswith(" lds"):
             bad += [(wrote[r][1], text) for r in sorted(_sregs(src)) if r in wrote and at - wrote[r][0] < VALU_TO_VMEM_SGPR]
         at += 1
+        if _CARRY_OUT.match(op):
+            dst += src.partition(",")[0]
         for r in _sregs(dst):
             if op.startswith("v_"):
                 wrote[r] = (at, text)
