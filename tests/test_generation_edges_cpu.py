@@ -8,6 +8,7 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tiktok_techjam_2026_track3_amd import _lib, ops, profiling
 
@@ -99,3 +100,14 @@ def test_build_sees_carries_as_writes(vector, bad):
     asm = "\n".join(["attn_rows_x:", "  " + vector, "  s_mov_b32 m0, s20", "  s_nop 0",
                      "  buffer_load_dwordx4 v2, s[4:7], s9 offen lds", "  s_endpgm", ".Lfunc_end0:"])
     assert bool(build.dma_hazards(asm)) == bad
+
+
+# ------------------------------------------------------------------------------ derivatives
+def test_forward_mode_tangents_are_found():
+    """A dual tensor is refused, under no_grad too, which leaves forward mode on; plain ones in a level are not."""
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            ops._no_tangent(None, x, dual)
+        ops._no_tangent(x, None, forward_ad.unpack_dual(dual).primal)

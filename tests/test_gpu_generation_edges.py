@@ -1,6 +1,6 @@
 """The token-generation operators where their documentation allows what the first tests do not do: plans
 dropped while another stream still has to read them; infinities and NaN in V, for every kind of tile;
-4-bit weights of every magnitude.
+4-bit weights of every magnitude; tensors with tangents.
 
 Error bounds (u = half a step of a type): a probability taken as one term enters the numerator and the sum with one
 rounding, 2 u (P |V|), fp16 ones off by 2^-25 at least; as two, the first cut off (below 2 u p is left) and the second
@@ -13,6 +13,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -224,3 +225,25 @@ def test_i4_weights_of_every_magnitude(gpu, dtype, exps, symmetric):
         bound = (span + least) * (0.5 + (0 if symmetric else 0.5) + 16 * UNIT[dtype])
         err = (out.t().cpu().double().reshape(x.shape) - x).abs().amax(2)
         assert bool((err <= bound).all()), (e, float((err / bound).max()))
+
+
+# ------------------------------------------------------------------------------ derivatives
+def test_forward_mode_tangents_are_refused(gpu):
+    """Each operator refuses each tensor that carries a tangent, and runs beside one that it is not given."""
+    ops = _ops()
+    q, k = torch.zeros(8, 4, 64, device=gpu).half(), torch.zeros(8, 2, 64, device=gpu).half()
+    plan = ops.packed_plan([5, 3], heads=4, kv_heads=2, head_dim=64, device=gpu)
+    cache, lens = torch.zeros(8, 10, 2, 64, device=gpu).half(), torch.zeros(8, dtype=torch.int32, device=gpu)
+    x, w = torch.zeros(3, 128, device=gpu).half(), torch.zeros(10, 64, dtype=torch.uint8, device=gpu)
+    scale, bias = torch.ones(10, 2, device=gpu).half(), torch.zeros(10, device=gpu)
+    calls = [(lambda q, k, v: ops.attention_packed(q, k, v, plan), [q, k, k]),
+             (lambda *a: ops.attention_shared_prefix(*a, lens), [q.unsqueeze(1), k, k, cache, cache]),
+             (lambda x, s, b: ops.linear_i4(x, w, s, None, b), [x, scale, bias])]
+    with forward_ad.dual_level():
+        for call, args in calls:
+            for i, t in enumerate(args):
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                for context in (torch.enable_grad, torch.no_grad):
+                    with context(), pytest.raises(ValueError, match="forward-mode"):
+                        call(*args[:i], dual, *args[i + 1:])
+            call(*args)

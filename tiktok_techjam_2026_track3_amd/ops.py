@@ -13,6 +13,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -580,6 +581,13 @@ def _no_backward(*tensors: Optional[torch.Tensor]) -> None:
                              "or with detached tensors")
 
 
+def _no_tangent(*tensors: Optional[torch.Tensor]) -> None:
+    """(called inside a forward-mode level, which no_grad does not turn off)"""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("this operator has no forward-mode derivative: call it with unpacked tensors")
+
+
 def _rows_strides(name: str, shape, stride, align: int, kv_axis: Optional[int] = None,
                   written: bool = False) -> Tuple[int, ...]:
     """Strides of a [..., token, head, head_dim] view but the last, checked: unit head_dim stride, whole
@@ -735,7 +743,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     key gives zeros, and a key that a token does not see never reaches it, NaN and infinities in its
     K or V included. ``out`` (default: a new contiguous tensor) must not share memory with the inputs;
     rows behind the plan's tokens (``q`` and ``out`` may have more) are left as they are, zeros in a new
-    ``out``. fp32 statistics, probabilities rounded to the input type. No backward pass."""
+    ``out``. fp32 statistics, probabilities rounded to the input type. No derivatives."""
     dev = q.get_device()
     if dev < 0 or k.get_device() != dev or v.get_device() != dev or plan.tiles.get_device() != dev or (
             out is not None and out.get_device() != dev):
@@ -743,6 +751,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pa
     given = out is not None
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (given and out.requires_grad)):
         _no_backward(q, k, v, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(q, k, v, out)
     code, (qst, kst, vst, ost) = _packed_views(
         plan.q_tokens, plan.k_tokens, plan.heads, plan.kv_heads, plan.head_dim,
         (q.dtype, k.dtype, v.dtype, out.dtype) if given else (q.dtype, k.dtype, v.dtype),
@@ -815,7 +825,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
 
     ``own_lens`` is read by the kernels, so a captured graph follows its values; it is clamped to
     [0, room], and what a cache holds behind it does not matter. Types, head dims and roundings as
-    ``attention_packed``. ``out`` must not share memory with the inputs. No backward pass."""
+    ``attention_packed``. ``out`` must not share memory with the inputs. No derivatives."""
     dev = q.get_device()
     given = out is not None
     if dev < 0 or k_prefix.get_device() != dev or v_prefix.get_device() != dev or k_own.get_device() != dev or (
@@ -823,6 +833,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         _on_gpu(q, k_prefix, v_prefix, k_own, v_own, own_lens, out)
     if torch.is_grad_enabled():
         _no_backward(q, k_prefix, v_prefix, k_own, v_own, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(q, k_prefix, v_prefix, k_own, v_own, out)
     dt = q.dtype
     dtypes = (dt, k_prefix.dtype, v_prefix.dtype, k_own.dtype, v_own.dtype)
     code, sizes, strides, need = _prefix_views(
@@ -931,7 +943,7 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     64 or 128; ``zero`` uint8 of scale's shape (None: 8); ``bias`` fp32 ``[N]``. Made for M of a few
     rows (the weights are read again for every 64). fp32 sums, the output (x's type, or fp32 with
     ``out_dtype``) rounded once. Infinities in x give NaN. ``out`` must not share memory with the
-    inputs. No backward pass."""
+    inputs. No derivatives."""
     dev = x.get_device()
     if dev < 0 or w.get_device() != dev or scale.get_device() != dev or (zero is not None and zero.get_device() != dev) \
             or (bias is not None and bias.get_device() != dev) or (out is not None and out.get_device() != dev):
@@ -939,6 +951,8 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
     if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)
                                     or (out is not None and out.requires_grad)):
         _no_backward(x, scale, bias, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(x, scale, bias, out)
     odt = out_dtype or (out.dtype if out is not None else x.dtype)
     if out is not None and out.dtype != odt:
         raise ValueError("out must be [M, N] of out_dtype with unit column stride")
