@@ -1,8 +1,8 @@
 // Attention over rows = (token, query head of a K/V head's group): what packed prompts
 // (attn_packed.hip) and a batch's new tokens behind a shared prefix (attn_prefix.hip) have in common.
 //
-// For one K/V head and a range of keys, each row i keeps the running maximum mu and sum of its
-// softmax and the output O = sum_j 2^(c s_ij - mu) v_j, c = scale * log2 e:
+// For one K/V head and a range of keys, each row i keeps the running maximum top of its scores, the sum of its softmax and
+// the output O = sum_j 2^(c s_ij - mu) v_j, c = scale * log2 e, mu = c top:
 //   S^T = K · Q^T and O^T += V^T · P^T on 16x16x32 MFMAs, keys in BN-key tiles through a ring of LDS
 //   tiles filled by LDS-DMA, V^T fragments by transpose reads of the key-major tile. A lane holds
 //   one row (lane % 16) and 4 keys of every 16, so the scores of a 32-key unit are its P^T operand
@@ -165,6 +165,10 @@ struct Joined {
   float ml[NW][QW][2];
   uint32_t flags[NW];
 };
+
+// Scores whose product with c is so large that its rounding, 2^-24 of it, shifts a probability by a factor of 2 and
+// more; fp16 probabilities would overflow from 2^28 on.
+constexpr float FAR = 0x1p24f;
 
 enum Pass { GIVEN = 0, CLEAN = 1, UP = 2, DOWN = 3 };
 
@@ -410,7 +414,8 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
   };
 
   f32x4 o[QG][DT];
-  float mu[QG], gate[QG], lsum[QG];  // running max (log2 domain), the score that moves it, row sum
+  float top[QG], gate[QG], lsum[QG];  // running max, the score (log2 domain) that moves it, row sum
+  uint32_t far = 0;                   // bit n: group n has a maximum of 2^FAR or more
 
   constexpr bool F16 = std::is_same_v<T, _Float16>;
   constexpr uint32_t LOWEST = 0x00010001u << (F16 ? 10 : 7), EXP = 0x80008000u - LOWEST, ONES = F16 ? 0x3c003c00u : 0x3f803f80u;
@@ -471,19 +476,35 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = vmax(mx, s[n][kt][i]);
       if (__builtin_amdgcn_ballot_w64(mx * p.c > gate[n]) != 0) {
-        mx = row_maximum(mx) * p.c;
-        const bool grow = mx > gate[n];
-        const float m2 = grow ? mx : mu[n];
+        mx = row_maximum(mx);
+        const bool grow = mx * p.c > gate[n];
+        const float t2 = grow ? mx : top[n];
+        const bool was_far = (far >> n) & 1;
+        if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(t2 * p.c) >= FAR) != 0) far |= 1u << n;
         if (__builtin_amdgcn_ballot_w64(gate[n] != NEG_INF) != 0) {  // (sums and outputs are 0 before the first maximum)
-          const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(mu[n] - m2);
+          const float by = was_far ? (top[n] - t2) * p.c : (far >> n) & 1 ? __builtin_fmaf(-t2, p.c, top[n] * p.c) : top[n] * p.c - t2 * p.c;
+          const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(by);
           lsum[n] *= alpha;
 #pragma unroll
           for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[n][t][i] *= alpha;
         }
-        mu[n] = m2;
-        gate[n] = grow ? mx + 8.f : gate[n];
+        top[n] = t2;
+        gate[n] = grow ? mx * p.c + 8.f : gate[n];
+      }
+    }
+    // (a far maximum times c is off by more than a score's share of the sum may be: taken off before)
+    float mu[QG];
+#pragma unroll
+    for (int n = 0; n < QG; ++n) {
+      mu[n] = top[n] * p.c;
+      if ((far >> n) & 1) {
+        mu[n] = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][kt][i] -= top[n];
       }
     }
     frag pf[TERMS][QG][KT / 2];
@@ -522,10 +543,11 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
     for (int n = 0; n < QG; ++n) {
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      mu[n] = 0.f;
+      top[n] = 0.f;
       gate[n] = NEG_INF;
       lsum[n] = 0.f;
     }
+    far = 0;
     if constexpr (OWN_KEYS) {
       // K of the next tile is requested as soon as this one's has been read, V likewise, so that one of
       // them is always in flight: of the 2 LPW newest loads the older LPW have to be there.
@@ -641,7 +663,7 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
         for (int dt = 0; dt < DT; ++dt) mine[(16 * n + l16) * (HD / 4) + 4 * dt + g] = o[n][dt];
         if (g == 0) {
           // (a sum that is not 0 without a maximum is NaN's)
-          join->ml[wave][16 * n + l16][0] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n];
+          join->ml[wave][16 * n + l16][0] = gate[n] == NEG_INF && sum == 0.f ? NEG_INF : top[n] * p.c;
           join->ml[wave][16 * n + l16][1] = sum;
         }
       }
@@ -681,7 +703,7 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
           const float inv = 1.0f / sum;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) put(dst, part, 16 * dt + 4 * g, o[n][dt], inv, lim[n] > 0, nan);
-          if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : mu[n], sum);
+          if (g == 0) put_ml(r, gate[n] == NEG_INF && sum == 0.f ? NEG_INF : top[n] * p.c, sum);
         }
       }
     }
