@@ -94,3 +94,23 @@ def test_prefix_scores_of_every_size(gpu, dtype, sign, B, n, H, Hkv, P, room):
             ref, tol = far64(q[b, :, h], torch.cat((kp[:, y], ko[b, :lens[b], y])), torch.cat((vp[:, y], vo[b, :lens[b], y])),
                              torch.arange(n) + P + lens[b] - n + 1, terms, dtype)
             check(f"sequence {b} head {h}", out[b, :, h], ref, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,P", [(4, 300), (4, 1500), (40, 1500)])
+@pytest.mark.parametrize("huge", [2.0 ** 14, math.inf])
+def test_rows_beside_large_scores_keep_their_bits(gpu, dtype, B, P, huge):
+    """A sequence whose scores are huge or infinite is a row beside others of the batch: theirs stay as they are."""
+    ops = _ops()
+    H, Hkv, D, room = 4, 2, 64, 100
+    g = torch.Generator().manual_seed(B + P)
+    q, kp, vp, ko, vo = (torch.randn(*s, generator=g).to(dtype).to(gpu) for s in (
+        (B, 1, H, D), (P, Hkv, D), (P, Hkv, D), (B, room, Hkv, D), (B, room, Hkv, D)))
+    lens = torch.full((B,), room, dtype=torch.int32, device=gpu)
+    clean = ops.attention_shared_prefix(q, kp * 100, vp, ko * 100, vo, lens, scale=1.0)
+    q2 = q.clone()
+    q2[1] *= huge
+    out = ops.attention_shared_prefix(q2, kp * 100, vp, ko * 100, vo, lens, scale=1.0)
+    keep = [b for b in range(B) if b != 1]
+    assert torch.equal(out[keep], clean[keep])
+    assert bool(torch.isfinite(out[1]).all()) == (huge < math.inf)

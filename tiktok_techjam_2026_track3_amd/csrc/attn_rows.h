@@ -415,7 +415,7 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
 
   f32x4 o[QG][DT];
   float top[QG], gate[QG], lsum[QG];  // running max, the score (log2 domain) that moves it, row sum
-  uint32_t far = 0;                   // bit n: group n has a maximum of 2^FAR or more
+  uint32_t far = 0;                   // bit n: a row of group n has had a maximum of FAR or more
 
   constexpr bool F16 = std::is_same_v<T, _Float16>;
   constexpr uint32_t LOWEST = 0x00010001u << (F16 ? 10 : 7), EXP = 0x80008000u - LOWEST, ONES = F16 ? 0x3c003c00u : 0x3f803f80u;
@@ -479,10 +479,13 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
         mx = row_maximum(mx);
         const bool grow = mx * p.c > gate[n];
         const float t2 = grow ? mx : top[n];
-        const bool was_far = (far >> n) & 1;
-        if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(t2 * p.c) >= FAR) != 0) far |= 1u << n;
+        const float m1 = top[n] * p.c, m2 = t2 * p.c;
+        const bool far1 = __builtin_fabsf(m1) >= FAR, far2 = __builtin_fabsf(m2) >= FAR;
+        if (__builtin_amdgcn_ballot_w64(far2) != 0) far |= 1u << n;
         if (__builtin_amdgcn_ballot_w64(gate[n] != NEG_INF) != 0) {  // (sums and outputs are 0 before the first maximum)
-          const float by = was_far ? (top[n] - t2) * p.c : (far >> n) & 1 ? __builtin_fmaf(-t2, p.c, top[n] * p.c) : top[n] * p.c - t2 * p.c;
+          float by = m1 - m2;
+          if ((far >> n) & 1)
+            by = far1 ? (far2 ? (top[n] - t2) * p.c : __builtin_fmaf(top[n], p.c, -m2)) : far2 ? __builtin_fmaf(-t2, p.c, m1) : by;
           const float alpha = gate[n] == NEG_INF ? 1.f : fast_exp2(by);
           lsum[n] *= alpha;
 #pragma unroll
@@ -494,17 +497,18 @@ MI355_DEVINL bool sweep_rows(const Args& p, u32x4* lds, Joined<NW, 16 * QG>* joi
         gate[n] = grow ? mx * p.c + 8.f : gate[n];
       }
     }
-    // (a far maximum times c is off by more than a score's share of the sum may be: taken off before)
     float mu[QG];
 #pragma unroll
     for (int n = 0; n < QG; ++n) {
       mu[n] = top[n] * p.c;
-      if ((far >> n) & 1) {
-        mu[n] = 0.f;
+      if ((far >> n) & 1) {  // rows whose maximum is: it is taken off before the product
+        const bool is = __builtin_fabsf(mu[n]) >= FAR;
+        const float off = is ? top[n] : 0.f;
+        mu[n] = is ? 0.f : mu[n];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][kt][i] -= top[n];
+          for (int i = 0; i < 4; ++i) s[n][kt][i] -= off;
       }
     }
     frag pf[TERMS][QG][KT / 2];
