@@ -395,8 +395,8 @@ int mi355_block_head(int dtype, const void* X, int64_t ldx, const void* gamma, c
  * zeros. Keys a token does not see do not reach its output, whatever their K and V hold (infinities
  * and NaN too); an infinity in V that it does see gives infinities (NaN where its probability rounds to 0);
  * a row whose every visible score is -inf is NaN, as softmax's.
- * Scores and softmax statistics are fp32, probabilities are rounded to the input type before P·V,
- * outputs once. dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256.
+ * Scores and softmax statistics are fp32, probabilities are rounded to the input type before P·V
+ * (to two terms of it where a tile has up to 32 rows, or 64 of a shared prefix), outputs once. dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256.
  *
  * mi355_attn_packed_plan runs on the host: from the lengths it writes the work that
  * mi355_attn_packed walks (32-bit words, 8 an entry: tiles of rows, longest first, split into ranges of
@@ -426,7 +426,8 @@ int mi355_attn_packed(int dtype, const void* Q, const void* K, const void* V, vo
  * tokens that all of them share and their own caches (room for `room` tokens each, own_lens[b] of
  * them filled, the n_q newest among them, last): the softmax of mi355_attn_packed over
  * prefix ++ own[: own_lens[b]]; token i of the n_q sees own keys j <= own_lens[b] - n_q + i.
- * The prefix is read once for the whole batch. own_lens is read on the device (a captured graph
+ * The prefix is read once for the whole batch, a cache once for every 32 rows (n_q * heads / kv_heads): n_q is
+ * meant to be a few. own_lens is read on the device (a captured graph
  * follows its values) and clamped to [0, room]; what a cache holds behind it does not matter. A token
  * that sees no key gives zeros. Types, head dims and roundings as mi355_attn_packed, partial results
  * in fp32.

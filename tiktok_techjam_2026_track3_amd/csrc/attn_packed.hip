@@ -21,11 +21,12 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Rows of a tile. Sequences of up to 32 rows (a token or a few) take NARROW ones, whose keys four waves
 // share out; the others WIDE ones of four waves of two groups of 16 rows, or HALF ones of one group where WIDE
 // ones leave CUs without work: fewer than two a CU, above head dim 64 counting the ranges that their keys are
-// split into. Measured (us, WIDE / HALF; 32/8 heads of 128 but where noted): 8192 tokens 478 / 555; 24 prompts of
-// 33-2011 (32/4) 135 / 152; 512 tokens against 8192 keys 80 / 100; 2048 against 16384 (8/2) 151 / 176; 4 x 100
-// against 3000 42 / 41; 3 x 700 (16/4) 30 / 19; 1000 32 / 28; heads of 64: 8 pieces of 200-512 against up to 5500
-// keys (16/16) 77 / 59, 300 against 6000 (16/16) 24 / 22. WIDE tiles take 32 keys at a time (64 keys: 8192 tokens
-// 479, the 24 prompts 146), HALF ones 64 up to head dim 64 (32 keys: the pieces 67).
+// split into. Measured (us, WIDE / HALF; bf16, 32/8 heads of 128 but where noted; from card to card up to 4% either way):
+// 8192 tokens 479 / 553; 24 prompts of 33-2011 (32/4) 157 / 169; 512 tokens against 8192 keys 81 / 103; 2048 against
+// 16384 (8/2) 150 / 176; 4 x 100 against 3000 44 / 43; 3 x 700 (16/4) 30 / 22; 1000 34 / 30; heads of 64, 16/16: 8
+// pieces of 200-512 against up to 5500 keys (fp16) 85 / 70, 300 against 6000 27 / 24. WIDE tiles take 32 keys at a time
+// (64, two work-groups a CU then: 8192 tokens 531 beside 498, the 24 prompts 172 beside 154), HALF ones 64 up to head
+// dim 64 (32: the pieces 104 beside 70).
 constexpr int WIDE = 128, HALF = 64, NARROW = 32;
 // Least keys of a range of a WIDE or HALF tile: its partial rows are 4 bytes an element, twice.
 constexpr int64_t WIDE_KEYS = 512;

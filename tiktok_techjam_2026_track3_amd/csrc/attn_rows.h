@@ -11,8 +11,9 @@
 //   The maximum moves only when a score exceeds it by more than 8 (log2 units), and only then do
 //   the four lanes of a row exchange anything; sums are exchanged once at the end.
 // Bound by the matrix cores and the exponentials' vector instructions where rows are many (one prompt of 8192
-// tokens, 32/8 heads of 128, bf16: 479 us, 1.15 PFLOP/s, matrix cores busy 52% and vector ALU 32% of the cycles
-// at 1.9 GHz), by the bytes of K and V where they are few (32 single tokens against 4000 keys each: 100 us, 5.2 TB/s).
+// tokens, 32/8 heads of 128, bf16: 479 to 498 us on different cards, 1.10 to 1.15 PFLOP/s, matrix cores busy 52% and
+// vector ALU 32% of the cycles at 1.9 GHz), by the bytes of K and V where they are few (32 single tokens against 4000 keys
+// each: 96 us and 5 of joining, 5.2 TB/s).
 #pragma once
 
 #include <type_traits>
@@ -176,7 +177,11 @@ enum Pass { GIVEN = 0, CLEAN = 1, UP = 2, DOWN = 3 };
 //   OWN_KEYS = false: each wave has rows of its own, the waves share tiles of BN keys (double-buffered).
 //   OWN_KEYS = true, for at most 16 QG rows: the waves have the same rows and keys of their own, tile w,
 //     w + NW .. of the range, in one buffer each for K and V, and are joined through LDS at the end.
-// TERMS: the probabilities enter P · V as that many terms of the input type.
+// TERMS: the probabilities enter P · V as that many terms of the input type. One where tiles have rows enough to be matrix
+// work (packed tiles of 64 and 128 rows, prefix tiles of 128), as in the framework's other attention kernels: against 64
+// bits the outputs are then off by 1.1 to 1.4 times their own rounding (8 pieces of prompts, fp16: 2.9e-4 of the norm
+// beside 2.1e-4). Two terms would cost the pieces half of their speed and 64 x 4 tokens behind 8192 keys 60 -> 71 us. Two
+// where K and V are waited for (up to 32 rows, prefix tiles up to 64): it costs nothing there, and the error is the rounding's.
 // A key that a row does not see has probability 0, but its v row is in the tile: 0 · inf and 0 · NaN leave NaN in rows
 // that do not see it. Where that may have happened (a NaN beside keys that not all rows see: true is returned) the
 // work-group goes through its keys again (AGAIN: three passes, but if V has no such element at those keys), with

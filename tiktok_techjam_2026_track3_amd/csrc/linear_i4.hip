@@ -583,7 +583,8 @@ int launch_tiles(const I4Args& a, hipStream_t s) {
     return launch_one<T, GROUP, MT, 1, 8, false, TO>(a, s);
   } else {
     if constexpr (GROUP != 32) {
-      // (32 x 8192 x 8192 28.8, 64 x 12288 x 4096 42 us with two tiles a wave, 36.2 and 51.1 with one)
+      // (32 x 8192 x 8192 28.8, 64 x 12288 x 4096 42 us with two tiles a wave, 36.2 and 51.1 with one; 64 rows and
+      // two tiles at group 128 take all 512 registers and 4 more in scratch, at one wave a SIMD)
       if ((a.N + 15) / 16 >= 512) return launch_one<T, GROUP, MT, 2, 4, false, TO>(a, s);
     }
     return launch_one<T, GROUP, MT, 1, 4, false, TO>(a, s);
