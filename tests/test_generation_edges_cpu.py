@@ -22,10 +22,32 @@ def test_plan_tells_the_allocator_of_other_streams(monkeypatch, current, capturi
     tiles = SimpleNamespace(record_stream=seen.append)
     plan = ops.PackedPlan(4, 4, 4, 2, 64, True, 64, _lib.i64_array((0, 0, 0, 0)), tiles, 0, stream=11)
     monkeypatch.setattr(ops, "_raw_stream", lambda device: current)
+    monkeypatch.setattr(ops, "_current_device", lambda: 3)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: ("stream", device, current))
     plan.used_on(3)
     assert seen == ([("stream", 3, current)] if told else [])
+
+
+@pytest.mark.parametrize("current,capturing", [(3, {3}), (0, {3}), (0, {0}), (3, set())])
+def test_capture_is_asked_of_the_plans_device(monkeypatch, current, capturing):
+    """... which need not be the current one."""
+    at = [current]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            at.append(self.index)
+
+        def __exit__(self, *_):
+            at.pop()
+
+    monkeypatch.setattr(ops, "_current_device", lambda: at[-1])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: at[-1] in capturing)
+    assert ops._capturing(3) == (3 in capturing) and at == [current]
 
 
 # ------------------------------------------------------------------------------ 4-bit weights

@@ -574,6 +574,14 @@ def _launch(device: int, fn, *args) -> int:
         return fn(*args, _raw_stream(device))
 
 
+def _capturing(device: int) -> bool:
+    """Whether ``device``'s current stream is being captured."""
+    if _current_device() == device:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _no_backward(*tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.requires_grad:
@@ -669,7 +677,7 @@ class PackedPlan:
         """Tells the allocator of a call on ``device``'s current stream where that is not the tiles' own: the
         block is not handed out again before what the stream holds by then is done. Not while capturing:
         the call's replays come at times that nobody knows here."""
-        if _raw_stream(device) != self.stream and not torch.cuda.is_current_stream_capturing():
+        if _raw_stream(device) != self.stream and not _capturing(device):
             self.tiles.record_stream(torch.cuda.current_stream(device))
 
 
