@@ -92,6 +92,23 @@ def test_quant_groups_i4_least_numbers_come_back():
     assert torch.equal(got, w.double())
 
 
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_quant_groups_i4_refuses_what_is_not_finite(bad, symmetric):
+    for dtype in UNIT:
+        w = torch.ones(4, 64, dtype=dtype)
+        w[2, 40] = bad
+        with pytest.raises(ValueError, match="finite"):
+            ops.quant_groups_i4(w, 32, symmetric)
+    w = torch.full((4, 64), 3e38, dtype=torch.bfloat16)
+    w[:, ::2] = -3e38
+    if symmetric:  # +-7 steps reach it
+        assert bool(torch.isfinite(ops.quant_groups_i4(w, 32, True)[1]).all())
+    else:
+        with pytest.raises(ValueError, match="finite"):
+            ops.quant_groups_i4(w, 32)
+
+
 def test_quant_groups_i4_without_rows_or_columns():
     q, scale, zero = ops.quant_groups_i4(torch.zeros(0, 64).half(), 32)
     assert q.shape == (0, 32) and scale.shape == zero.shape == (0, 2)

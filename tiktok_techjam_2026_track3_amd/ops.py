@@ -893,7 +893,8 @@ def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
     """4-bit weights for ``linear_i4`` from ``w`` ``[N, K]`` (fp16 or bf16): ``(q, scale, zero)`` with
     ``w ~ scale[n, k / group] (q[n, k] - zero[n, k / group])``, q two to a byte (even k in the low
     half) ``[N, K / 2]`` uint8, scale of w's type. Each group's range (0 included) goes to 0 .. 15, or with
-    ``symmetric`` its largest magnitude to +-7 around 8 (zero is None). Run once per weight."""
+    ``symmetric`` its largest magnitude to +-7 around 8 (zero is None). Run once per weight: it waits for the GPU to see that
+    all of it is finite."""
     if w.dim() != 2 or w.dtype not in _SIXTEEN_BIT:
         raise ValueError("quant_groups_i4 expects a 2-D fp16 or bf16 weight")
     if group not in I4_GROUPS or w.shape[1] % group or w.shape[1] == 0:
@@ -902,10 +903,14 @@ def quant_groups_i4(w: torch.Tensor, group: int = 128, symmetric: bool = False
         x = w.detach().float().reshape(w.shape[0], w.shape[1] // group, group)
         if symmetric:
             scale = _group_scale(x.abs().amax(2) / 7, w.dtype)
-            zero, z = None, 8.0
         else:
             lo, hi = x.amin(2).clamp_max(0), x.amax(2).clamp_min(0)
             scale = _group_scale((hi - lo) / 15, w.dtype)
+        if not bool(torch.isfinite(scale).all()):
+            raise ValueError("quant_groups_i4 needs finite weights, of which a group's range is finite in fp32")
+        if symmetric:
+            zero, z = None, 8.0
+        else:
             z = (-lo / scale.float()).round().clamp(0, 15)
             zero, z = z.to(torch.uint8), z[..., None]
         q = ((x / scale.float()[..., None]).round() + z).clamp(0, 15).to(torch.uint8).reshape(w.shape)
