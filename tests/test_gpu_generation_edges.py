@@ -180,6 +180,42 @@ def test_prefix_not_finite_v(gpu, n, H, P, dtype, D):
             check(f"{b} {h}", out[b, :, h], ref, tol)
 
 
+def test_not_finite_v_in_replayed_graphs(gpu):
+    """Elements that turn up between replays, and go again: every replay gives what an eager call gives."""
+    ops = _ops()
+    q_lens, k_lens, H, Hkv, D = [70, 5, 40], [700, 300, 3000], 4, 2, 64
+    plan = ops.packed_plan(q_lens, k_lens, heads=H, kv_heads=Hkv, head_dim=D, device=gpu)
+    assert plan.counts[2] > 0
+    packed = [_rand((sum(n), h, D), torch.float16, 30 + h).to(gpu) for n, h in ((q_lens, H), (k_lens, Hkv), (k_lens, Hkv))]
+    prefix = [_rand(s, torch.float16, 40 + i).to(gpu) for i, s in enumerate(
+        [(3, 4, H, D), (1100, Hkv, D), (1100, Hkv, D), (3, 60, Hkv, D), (3, 60, Hkv, D)])]
+    lens = torch.tensor([60, 33, 4], dtype=torch.int32, device=gpu)
+    calls = [lambda: ops.attention_packed(*packed, plan), lambda: ops.attention_shared_prefix(*prefix, lens)]
+    outs, graphs = [], []
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call())
+        graphs.append(graph)
+    for at, bad in ((None, 0.0), (695, math.nan), (100, math.inf), (3999, -math.inf), (None, 0.0)):
+        v, vo = packed[2].clone(), prefix[4].clone()
+        if at is not None:
+            packed[2][at, :, 5] = bad
+            prefix[4][0, 58, :, 7] = bad
+            prefix[4][2, 1] = bad
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, call in zip(outs, calls):
+            want = call()
+            assert torch.equal(out.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+            assert bool(torch.isfinite(want).all()) == (at is None)
+        packed[2].copy_(v)
+        prefix[4].copy_(vo)
+
+
 def test_packed_not_finite_v_costs_little(gpu):
     """A call whose rows nearly all see a NaN, or just do not see it, takes a clean one's time, not hundreds of
     times as long: a sequence that went wrong does not hold up its batch."""
