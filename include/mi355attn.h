@@ -463,6 +463,76 @@ int mi355_linear_i4(int dtype, int out_dtype, const void* X, int64_t ldx, const 
                     const void* scale, const uint8_t* zero, const float* bias, void* Y, int64_t ldy,
                     int64_t M, int64_t N, int64_t K, int64_t group, void* stream);
 
+/*
+ * Rotation of pairs of a head's elements by position and frequency (rotary positions):
+ *   y1 = a (x1 cos t - x2 sin t),  y2 = a (x2 cos t + x1 sin t),  t = position * f_j,  a = amplitude,
+ * over the first rot_dim elements of a head: pair j is (x_j, x_{j + rot_dim / 2}), or with interleaved
+ * != 0 (x_2j, x_2j+1); the elements behind them are copied. inverse != 0 turns the other way (with
+ * the same amplitude: the transposed map, which is the gradient's).
+ * frequencies [rot_dim / 2] (device) are fractions of a full turn for each position, times 2^64
+ * (modulo 2^64): angles are exact to 2^-31 of a turn at any position. fp32 arithmetic, rounded once.
+ * X and Y are [n0, n1, heads, head_dim] views given by element strides {batch, token, head}, the
+ * head_dim stride 1; positions [n0, n1] int32 (int64 with positions_64 != 0), strides {batch, token}, any sign.
+ * Y may be X with the same strides, and must not overlap it otherwise. dtype F32, F16 or BF16;
+ * head_dim even, up to 512, rot_dim even; n0 n1 up to 2^31. Any alignment of whole elements (16-byte runs are faster).
+ */
+int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int positions_64,
+                 const uint64_t* frequencies, float amplitude, int64_t n0, int64_t n1, int64_t heads,
+                 int64_t head_dim, int64_t rot_dim, const int64_t* position_strides,
+                 const int64_t* x_strides, const int64_t* y_strides, int interleaved, int inverse,
+                 void* stream);
+
+/*
+ * A K/V cache in pages, 8 bits an element:
+ *   cache_k, cache_v [pages, kv_heads, page, head_dim] e4m3 (no infinities), contiguous, 16-byte aligned;
+ *   k_scale, v_scale [pages, kv_heads, page / 16] fp32 powers of two; an element is its byte's value times the
+ *   scale of its block of 16 tokens and head. page: a power of two from 16 to 1024.
+ * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32, row stride
+ * table_stride). lens [B] counts a sequence's tokens in the cache, its n new ones included, which are the
+ * last. New tokens are packed: sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not
+ * decreasing) of Q, K, V and the outputs, `most` at most (those behind it are ignored); offsets NULL:
+ * rows b * most .. of `most` each. table, lens and offsets are read on the device, so a captured graph
+ * follows their values, and checked there: no value makes an access leave the tensors.
+ *
+ * mi355_paged_append writes the new tokens' K and V. K is rotated by its position p (mi355_rotary's formula
+ * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q; with zero_tail != 0
+ * rows behind the last sequence's become zeros, otherwise they are left). Rotated values are not rounded before
+ * they are quantised: with m the largest finite magnitude of a block's new elements, the scale becomes
+ * max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens); elements are
+ * rounded to nearest even, infinities and NaN become NaN; when the scale grows, the block's older elements are
+ * rounded to it anew. Tokens whose page is none of [0, pages), or behind the table, are not written. A page that
+ * several tokens of the batch are to be written to must be one sequence's.
+ *
+ * mi355_attn_paged: softmax attention of the new tokens: the token at position p sees keys 0 .. p of its
+ * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32, probabilities enter P·V
+ * as two bf16 terms (off by 2^-16 of each at most), outputs are rounded once. A token that sees no key gives zeros; one that sees a
+ * key whose page is missing gives NaN. What pages hold behind lens does not matter, nor do NaN that a
+ * token does not see. bf16: |q| below 2^110, |v| below 2^100. workspace (16-byte aligned) holds
+ * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be
+ * stream-ordered. Rows behind the last sequence's as above.
+ *
+ * Both: dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256; strides {token, head} in
+ * elements, multiples of 8 with 16-byte aligned bases (O: of 4, 8-byte); rot_dim a multiple of 8; width * page below 2^30;
+ * pages, tokens, most and B below 2^30, B most heads below 2^23.
+ */
+int mi355_paged_append(int dtype, const void* K, const void* V, const void* Q, void* Q_out,
+                       uint8_t* cache_k, uint8_t* cache_v, float* k_scale, float* v_scale,
+                       const int32_t* table, int64_t table_stride, const int32_t* lens,
+                       const int32_t* offsets, int64_t B, int64_t most, int64_t tokens, int64_t heads,
+                       int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page, int64_t width,
+                       const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                       const int64_t* out_strides, const uint64_t* frequencies, int64_t rot_dim,
+                       int interleaved, float amplitude, int zero_tail, void* stream);
+int64_t mi355_attn_paged_workspace_bytes(int64_t B, int64_t most, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t page, int64_t width);
+int mi355_attn_paged(int dtype, const void* Q, const uint8_t* cache_k, const uint8_t* cache_v,
+                     const float* k_scale, const float* v_scale, const int32_t* table,
+                     int64_t table_stride, const int32_t* lens, const int32_t* offsets, void* O,
+                     int64_t B, int64_t most, int64_t tokens, int64_t heads, int64_t kv_heads,
+                     int64_t head_dim, int64_t pages, int64_t page, int64_t width,
+                     const int64_t* q_strides, const int64_t* o_strides, float scale, int zero_tail,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

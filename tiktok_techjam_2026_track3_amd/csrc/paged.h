@@ -1,0 +1,71 @@
+// A K/V cache in pages, held in e4m3 with one scale for each block of 16 tokens and head, and the batch of sequences
+// that lives in it: what paged_append.hip writes and attn_paged.hip reads.
+//
+//   K, V     [pages][kv_heads][page][head_dim] bytes   token p of a sequence: row p % page of page table[b][p / page]
+//   scales   [pages][kv_heads][page / 16] fp32, powers of two   value = scale * e4m3
+//
+// Pages are head-major, so that a head's 16 tokens are one run of 16 head_dim bytes. Power-of-two scales cost e4m3
+// nothing (its steps are relative) and make what happens when a later token raises its block's scale exact: bytes move
+// to smaller exponents, and only those that fall below e4m3's least normal value are rounded again.
+#pragma once
+
+#include "common.h"
+
+namespace paged {
+
+constexpr int BLOCK = 16;  // tokens that share a scale: the rows of one 16x16x32 MFMA operand
+
+struct Cache {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int32_t pages, kv_heads, head_dim;
+  int32_t page_shift;  // page = 2^page_shift tokens
+};
+
+// Sequences of a batch and their newest tokens. Everything that is read on the device is checked there: no value of
+// it makes an access leave its tensor.
+struct Batch {
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;     // tokens in the cache, the new ones among them, last
+  const int32_t* offsets;  // [B + 1] first new token of each sequence; NULL: sequence b's are b * most ..
+  int32_t B, width, most, tokens;
+};
+
+struct Sequence {
+  int32_t first, n;  // its new tokens are first .. first + n
+  int32_t len;       // tokens with them
+};
+
+MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
+  Sequence s;
+  s.len = p.lens[b];
+  if (p.offsets == nullptr) {
+    s.first = b * p.most;
+    s.n = p.most;
+  } else {
+    const int lo = p.offsets[b], hi = p.offsets[b + 1];
+    s.first = lo < 0 ? 0 : (lo < p.tokens ? lo : p.tokens);
+    const int end = hi < s.first ? s.first : (hi < p.tokens ? hi : p.tokens);
+    s.n = end - s.first < p.most ? end - s.first : p.most;
+  }
+  return s;
+}
+
+// What both entry points refuse.
+inline int check(int dtype, int64_t B, int64_t most, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                 int64_t pages, int64_t page, int64_t width) {
+  if (dtype != MI355_F16 && dtype != MI355_BF16) return MI355_E_BAD_DTYPE;
+  switch (head_dim) {
+    case 16: case 32: case 48: case 64: case 80: case 96: case 128: case 192: case 256: break;
+    default: return MI355_E_HEAD_DIM;
+  }
+  constexpr int64_t MOST = int64_t(1) << 30;
+  for (const int64_t n : {B, most, tokens, pages, width})
+    if (n < 0 || n >= MOST) return MI355_E_BAD_SIZE;
+  if (B > (1 << 20) || heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads) return MI355_E_BAD_SIZE;
+  if (page < BLOCK || page > 1024 || (page & (page - 1)) || width * page >= MOST) return MI355_E_BAD_SIZE;
+  return MI355_OK;
+}
+
+}  // namespace paged

@@ -1,0 +1,283 @@
+// New tokens' K and V into the pages of an e4m3 cache, K rotated by its position on the way, and the queries of the same
+// tokens rotated in the same launch.
+//
+// A work-group has a block of 16 positions of one sequence. It computes the angles of the block's new tokens once,
+// into LDS; then a wave takes a K/V head's rows at a time: rotate, largest magnitude of all, scale, convert, store;
+// the queries are rotated by all threads. For a block with older tokens the scale can only grow; when it does, the
+// wave converts their bytes to the new one. Nothing else writes that block and head, so there are no atomics.
+//   scale = the least power of two with max|x| <= 448 scale (448: e4m3's largest), at least 2^-118;
+//   byte = e4m3(x / scale), nearest, ties to even; infinities and NaN are held as NaN and do not count for the scale.
+// Bound by bytes in long prompts (16 bits in, 8 out, the queries in and out), by the chain of its loads (lengths, page,
+// old scale) for single tokens.
+#include "paged.h"
+#include "rotary.h"
+
+namespace {
+
+using paged::BLOCK;
+
+struct AppendArgs {
+  paged::Cache cache;
+  paged::Batch batch;
+  const void *k, *v, *q;
+  void* qo;
+  int64_t kt, kh, vt, vh, qt, qh, ot, oh;  // token and head strides in elements
+  const uint64_t* freqs;                   // NULL: no rotation
+  float amplitude;
+  int32_t rot, interleaved, heads, blocks, slices, zero_tail;
+};
+
+MI355_DEVINL float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  return v;
+}
+
+// four floats as e4m3 bytes
+MI355_DEVINL uint32_t to_e4m3(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
+}
+
+// Rotates 8 elements of a token's head: four pairs (a_i, b_i), a the first four and b the last four of x, or
+// neighbours where interleaved.
+template <bool INTERLEAVED>
+MI355_DEVINL void rotate8(float (&x)[8], const float2* cs) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float& a = x[INTERLEAVED ? 2 * i : i];
+    float& b = x[INTERLEAVED ? 2 * i + 1 : 4 + i];
+    const float a0 = a, b0 = b;
+    a = __builtin_fmaf(a0, cs[i].x, -b0 * cs[i].y);
+    b = __builtin_fmaf(b0, cs[i].x, a0 * cs[i].y);
+  }
+}
+
+// The two runs of 4 elements that unit c of a head's row has: for pairs across half the rotated part, they are apart.
+template <bool INTERLEAVED>
+MI355_DEVINL void runs_of(int c, int rot, int& first, int& second) {
+  if (!INTERLEAVED && c < rot / 8) {
+    first = 4 * c;
+    second = 4 * c + rot / 2;
+  } else {
+    first = 8 * c;
+    second = first + 4;
+  }
+}
+
+template <typename T>
+MI355_DEVINL void load8(const T* row, int first, int second, float (&x)[8]) {
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  const V4 a = *reinterpret_cast<const V4*>(row + first), b = *reinterpret_cast<const V4*>(row + second);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = to_f32(static_cast<T>(a[i]));
+    x[4 + i] = to_f32(static_cast<T>(b[i]));
+  }
+}
+
+// UNITS: units of 8 elements that a lane has at most, head_dim / 32 of a whole block.
+template <typename T, int UNITS, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
+  extern __shared__ float2 angles[];  // [16][rot / 2] of the new tokens
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int slice = blockIdx.x % p.slices, at = blockIdx.x / p.slices;
+  const int b = at / p.blocks, nth = at % p.blocks;
+  const paged::Sequence s = paged::sequence_of(p.batch, b);
+  if (p.zero_tail && at == p.batch.B * p.blocks - 1 && slice == p.slices - 1) {  // rows that no sequence has
+    for (int64_t t = s.first + s.n; t < p.batch.tokens; ++t)
+      for (int i = tid; i < p.heads * p.cache.head_dim; i += 256)
+        static_cast<T*>(p.qo)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
+  }
+  const int64_t begin = static_cast<int64_t>(s.len) - s.n;  // position of the first new token
+  const int64_t block = (begin >> 4) + nth;                 // (floor: positions can be negative)
+  const int64_t base = block * BLOCK;
+  const int t0 = begin > base ? static_cast<int>(begin - base) : 0;
+  const int64_t left = s.len - base;
+  const int t1 = left < BLOCK ? static_cast<int>(left) : BLOCK;  // new tokens t0 .. t1 of the block
+  if (t1 <= t0) return;
+  const int hd = p.cache.head_dim, hu = hd / 8, half = p.rot / 2, nt = t1 - t0;
+  const int64_t token0 = s.first + (base - begin);  // token of the block's position 0 (t0 and later ones exist)
+
+  if (p.freqs != nullptr) {
+    for (int i = tid; i < nt * half; i += 256) {
+      const int t = i / half, j = i - t * half;
+      float si, co;
+      sincos_of_turn(base + t0 + t, p.freqs[j], si, co);
+      angles[t * half + j] = make_float2(co * p.amplitude, si * p.amplitude);
+    }
+    __syncthreads();
+  }
+
+  // the page that holds the block
+  int page = -1;
+  if (block >= 0 && (base >> p.cache.page_shift) < p.batch.width) page = p.batch.table[b * p.batch.table_stride + (base >> p.cache.page_shift)];
+  if (page >= 0 && page < p.cache.pages) {
+    const int in_page = static_cast<int>(base & ((1 << p.cache.page_shift) - 1));
+    for (int item = wave + 4 * slice; item < 2 * p.cache.kv_heads; item += 4 * p.slices) {
+      const bool is_v = item >= p.cache.kv_heads;
+      const int h = is_v ? item - p.cache.kv_heads : item;
+      const T* src = is_v ? static_cast<const T*>(p.v) + h * p.vh : static_cast<const T*>(p.k) + h * p.kh;
+      const int64_t ts = is_v ? p.vt : p.kt;
+      const int64_t head = static_cast<int64_t>(page) * p.cache.kv_heads + h;
+      uint8_t* dst = (is_v ? p.cache.v : p.cache.k) + ((head << p.cache.page_shift) + in_page) * hd;
+      float* scale = (is_v ? p.cache.vs : p.cache.ks) + ((head << p.cache.page_shift) + in_page) / BLOCK;
+      const float old = t0 > 0 ? *scale : 0.0f;
+      const bool turn = !is_v && p.freqs != nullptr;
+      const int rot = turn ? p.rot : 0;
+      float x[UNITS][8], top = 0.0f;
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
+        int first, second;
+        runs_of<INTERLEAVED>(c, rot, first, second);
+        if (t < nt) {
+          load8(src + (token0 + t0 + t) * ts, first, second, x[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[u][e] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
+        if (t < nt && c < rot / 8) rotate8<INTERLEAVED>(x[u], angles + t * half + 4 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float m = __builtin_fabsf(x[u][e]);
+          top = m < __builtin_huge_valf() && m > top ? m : top;
+        }
+      }
+      top = fmaxf(wave_max(top), 0x1p-110f);
+      // 448 = 1.75 * 2^8: the exponent of `top` less 8, and one more where its mantissa is over 1.75
+      const uint32_t bits = __float_as_uint(top);
+      const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased
+      float s_new = __uint_as_float(static_cast<uint32_t>(e) << 23);
+      const bool grows = t0 > 0 && s_new > old;
+      s_new = s_new > old ? s_new : old;
+      const float inv = 1.0f / s_new;
+      if (grows) {
+        const float ratio = old * inv;
+        for (int i = lane; i < t0 * hu; i += 64) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(dst) + 2 * i;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[r], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[r], true);
+            w[r] = to_e4m3(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
+        int first, second;
+        runs_of<INTERLEAVED>(c, rot, first, second);
+        if (t < nt) {
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {  // (an infinity to NaN: inf - inf)
+            const float w = x[u][k] * inv;
+            y[k] = __builtin_fabsf(w) < __builtin_huge_valf() ? w : w - w;
+          }
+          uint8_t* row = dst + (t0 + t) * hd;
+          *reinterpret_cast<uint32_t*>(row + first) = to_e4m3(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint32_t*>(row + second) = to_e4m3(y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (lane == 0) *scale = s_new;
+    }
+  }
+
+  if (p.q != nullptr) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    const int units = nt * p.heads * hu;
+    for (int i = tid + 256 * slice; i < units; i += 256 * p.slices) {
+      const int th = i / hu, c = i - th * hu, t = th / p.heads, h = th - t * p.heads;
+      int first, second;
+      runs_of<INTERLEAVED>(c, p.rot, first, second);
+      float x[8];
+      load8(static_cast<const T*>(p.q) + (token0 + t0 + t) * p.qt + h * p.qh, first, second, x);
+      if (c < p.rot / 8) rotate8<INTERLEAVED>(x, angles + t * half + 4 * c);
+      T* row = static_cast<T*>(p.qo) + (token0 + t0 + t) * p.ot + h * p.oh;
+      *reinterpret_cast<V4*>(row + first) = V4{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
+      *reinterpret_cast<V4*>(row + second) = V4{from_f32<T>(x[4]), from_f32<T>(x[5]), from_f32<T>(x[6]), from_f32<T>(x[7])};
+    }
+  }
+}
+
+template <typename T, int UNITS>
+int launch(const AppendArgs& p, hipStream_t s) {
+  const uint32_t grid = static_cast<uint32_t>(p.batch.B) * p.blocks * p.slices;
+  const size_t lds = p.freqs ? size_t(BLOCK) * (p.rot / 2) * sizeof(float2) : 0;
+  if (p.interleaved)
+    paged_append_kernel<T, UNITS, true><<<grid, 256, lds, s>>>(p);
+  else
+    paged_append_kernel<T, UNITS, false><<<grid, 256, lds, s>>>(p);
+  return static_cast<int>(hipGetLastError());
+}
+
+template <typename T>
+int launch_dim(const AppendArgs& p, hipStream_t s) {
+  if (p.cache.head_dim <= 64) return launch<T, 2>(p, s);
+  if (p.cache.head_dim <= 128) return launch<T, 4>(p, s);
+  return launch<T, 8>(p, s);
+}
+
+}  // namespace
+
+extern "C" int mi355_paged_append(int dtype, const void* K, const void* V, const void* Q, void* Q_out, uint8_t* cache_k,
+                                  uint8_t* cache_v, float* k_scale, float* v_scale, const int32_t* table,
+                                  int64_t table_stride, const int32_t* lens, const int32_t* offsets, int64_t B, int64_t most,
+                                  int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                  int64_t page, int64_t width, const int64_t* k_strides, const int64_t* v_strides,
+                                  const int64_t* q_strides, const int64_t* out_strides, const uint64_t* frequencies,
+                                  int64_t rot_dim, int interleaved, float amplitude, int zero_tail, void* stream) {
+  AppendArgs p{};
+  if (const int st = paged::check(dtype, B, most, tokens, heads, kv_heads, head_dim, pages, page, width)) return st;
+  if (B * most == 0 || tokens == 0) return MI355_OK;
+  if (!K || !V || !lens || !k_strides || !v_strides || (pages > 0 && (!cache_k || !cache_v || !k_scale || !v_scale)) ||
+      (width > 0 && !table))
+    return MI355_E_NULL_POINTER;
+  if (Q && (!Q_out || !q_strides || !out_strides || !frequencies)) return MI355_E_NULL_POINTER;
+  if (!offsets && B * most > tokens) return MI355_E_BAD_SIZE;
+  if (frequencies && (rot_dim < 8 || rot_dim > head_dim || rot_dim % 8)) return MI355_E_HEAD_DIM;
+  const auto even = [](const void* base, const int64_t* st) {
+    return aligned16(base) && st[0] % 8 == 0 && st[1] % 8 == 0;
+  };
+  if (!even(K, k_strides) || !even(V, v_strides) || (Q && (!even(Q, q_strides) || !even(Q_out, out_strides))) ||
+      !aligned16(cache_k) || !aligned16(cache_v))
+    return MI355_E_ALIGNMENT;
+  p.cache = paged::Cache{cache_k, cache_v, k_scale, v_scale, static_cast<int32_t>(pages), static_cast<int32_t>(kv_heads),
+                         static_cast<int32_t>(head_dim), __builtin_ctzll(static_cast<uint64_t>(page))};
+  p.batch = paged::Batch{table, table_stride, lens, offsets, static_cast<int32_t>(B), static_cast<int32_t>(width),
+                         static_cast<int32_t>(most), static_cast<int32_t>(tokens)};
+  p.k = K;
+  p.v = V;
+  p.q = Q;
+  p.qo = Q_out;
+  p.kt = k_strides[0];
+  p.kh = k_strides[1];
+  p.vt = v_strides[0];
+  p.vh = v_strides[1];
+  if (Q) {
+    p.qt = q_strides[0];
+    p.qh = q_strides[1];
+    p.ot = out_strides[0];
+    p.oh = out_strides[1];
+  }
+  p.freqs = frequencies;
+  p.amplitude = amplitude;
+  p.rot = frequencies ? static_cast<int32_t>(rot_dim) : 0;
+  p.interleaved = interleaved;
+  p.heads = static_cast<int32_t>(heads);
+  p.zero_tail = Q && zero_tail;
+  p.blocks = static_cast<int32_t>((most + 2 * BLOCK - 2) / BLOCK);
+  // work-groups that share a block's heads: enough to have two a CU, no more than heads can use
+  const int64_t groups = B * p.blocks;
+  int64_t slices = (512 + groups - 1) / groups;
+  const int64_t useful = (2 * kv_heads + 3) / 4;
+  p.slices = static_cast<int32_t>(slices < useful ? slices : useful);
+  if (groups * p.slices >= (int64_t(1) << 23)) return MI355_E_BAD_SIZE;  // 2^31 threads
+  const auto s = static_cast<hipStream_t>(stream);
+  return dtype == MI355_F16 ? launch_dim<_Float16>(p, s) : launch_dim<__bf16>(p, s);
+}

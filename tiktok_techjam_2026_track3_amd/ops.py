@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import operator
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
@@ -995,4 +996,368 @@ def linear_i4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor,
                  out.data_ptr(), ldy, M, N, K, group)
     if st:
         _lib.check("mi355_linear_i4", st)
+    return out
+
+
+@dataclass(frozen=True, eq=False)
+class RotaryPlan:
+    """Frequencies of rotary positions (``rotary_plan``): ``turns`` holds each pair's fraction of a full turn for
+    a position, times 2^64 (int64 bits of the unsigned number), on the GPU."""
+    turns: torch.Tensor
+    dim: int
+    interleaved: bool
+    amplitude: float
+
+
+def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: Optional[str] = None,
+                factor: float = 1.0, original: Optional[int] = None, slow: float = 1.0, fast: float = 32.0,
+                freqs: Optional[Sequence[float]] = None, amplitude: float = 1.0, device="cuda") -> RotaryPlan:
+    """Frequencies for rotating the first ``dim`` elements of a head, f_j = base^(-2 j / dim) radians a position
+    for pair j of ``dim / 2``: elements (j, j + dim / 2), or with ``interleaved`` (2 j, 2 j + 1). Longer contexts:
+
+    - ``scaling="linear"``: f_j / factor (positions are squeezed together);
+    - ``"base"``: base * factor^(dim / (dim - 2)), which leaves the fastest pair as it is and slows the last by factor;
+    - ``"parts"``: by the turns r = original * f_j / 2 pi that a pair makes in the original context: those of
+      ``fast`` and more stay, those of ``slow`` and fewer become f_j / factor, and in between
+      f_j (g + (1 - g) / factor), g = (r - slow) / (fast - slow).
+
+    ``freqs`` gives the radians themselves instead. ``amplitude`` multiplies the rotated elements. Host arithmetic in
+    64 bits; made once, outside a graph capture."""
+    dim = operator.index(dim)
+    if dim < 2 or dim % 2 or dim > 512:
+        raise ValueError(f"dim must be even and between 2 and 512, got {dim}")
+    base, factor, amplitude = float(base), float(factor), float(amplitude)
+    if not 0.0 < base < math.inf or not 0.0 < factor < math.inf or not math.isfinite(amplitude):
+        raise ValueError("base and factor must be positive and finite, amplitude finite")
+    if freqs is not None:
+        if scaling is not None:
+            raise ValueError("freqs are given: nothing to scale")
+        f = [float(x) for x in freqs]
+        if len(f) != dim // 2 or not all(math.isfinite(x) for x in f):
+            raise ValueError(f"freqs must be {dim // 2} finite numbers")
+    else:
+        if scaling == "base":
+            if dim == 2:
+                raise ValueError("scaling 'base' needs more than one pair")
+            grown = math.log(base) + math.log(factor) * dim / (dim - 2)
+            if abs(grown) > 700.0:
+                raise ValueError("factor is out of range for scaling 'base'")
+            base = math.exp(grown)
+        f = [base ** (-2.0 * j / dim) for j in range(dim // 2)]
+        if scaling == "linear":
+            f = [x / factor for x in f]
+        elif scaling == "parts":
+            if original is None or original <= 0 or not 0 <= slow < fast < math.inf:
+                raise ValueError("scaling 'parts' needs original > 0 and 0 <= slow < fast")
+            kept = [min(1.0, max(0.0, (original * x / (2 * math.pi) - slow) / (fast - slow))) for x in f]
+            f = [x * (g + (1.0 - g) / factor) for x, g in zip(f, kept)]
+        elif scaling not in (None, "base"):
+            raise ValueError(f"scaling must be None, 'linear', 'base' or 'parts', got {scaling!r}")
+        if not all(math.isfinite(x) for x in f):
+            raise ValueError("base and factor give frequencies that are not finite")
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"expected a GPU device, got {device}")
+    turns = [round(x / (2 * math.pi) % 1.0 * 2.0 ** 64) % (1 << 64) for x in f]
+    turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
+    return RotaryPlan(turns.to(device), dim, bool(interleaved), amplitude)
+
+
+@functools.lru_cache(maxsize=512)
+def _rotary_views(dt, xs, xst, pd, ps, pst, os, ost, dim):
+    """(type code, sizes, stride arrays) of rotary's tensors, checked."""
+    if dt not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"x must be fp16, bf16 or fp32, got {dt}")
+    if len(xs) not in (3, 4):
+        raise ValueError(f"x is [tokens, heads, head_dim] or [B, S, heads, head_dim], got {tuple(xs)}")
+    if pd not in (torch.int32, torch.int64) or ps != xs[:-2]:
+        raise ValueError(f"positions must be int32 or int64 of shape {tuple(xs[:-2])}, got {pd} {tuple(ps)}")
+    D = xs[-1]
+    if D % 2 or not dim <= D <= 512:
+        raise ValueError(f"head_dim must be even, at most 512 and at least the plan's {dim}, got {D}")
+    if os is not None and os != xs:
+        raise ValueError(f"out must have x's shape {tuple(xs)}")
+    if 0 not in xs and (xst[-1] != 1 or (os is not None and ost[-1] != 1)):
+        raise ValueError("head_dim must be the unit-stride dimension of x and out")
+    n = (1,) * (4 - len(xs)) + tuple(xs[:-1])
+    if n[0] * n[1] > 1 << 31 or n[2] > 65535:
+        raise ValueError("too many tokens or heads for one call")
+
+    def strides(st):  # (an axis of one element: its stride does not matter)
+        return tuple(0 if size == 1 else s for size, s in zip(n, (0,) * (4 - len(xs)) + tuple(st)))
+
+    xst = strides(xst[:-1])
+    if os is None:
+        ost = (n[1] * n[2] * D, n[2] * D, D)
+    else:
+        _rows_strides("out", os, ost, 1, written=True)
+        ost = strides(ost[:-1])
+    return _lib.dtype_code(dt), (*n, D), _Arrays(strides(pst)[:2], xst, ost), xst == ost
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: bool = False,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates pairs of each head's elements by ``position * frequency``: (x1, x2) becomes
+    amplitude (x1 cos t - x2 sin t, x2 cos t + x1 sin t). ``x`` is ``[tokens, heads, head_dim]`` or
+    ``[B, S, heads, head_dim]`` (fp16, bf16 or fp32, any strides with a unit one for head_dim; queries and keys that
+    lie side by side are one call), ``positions`` int32 or int64 of its leading shape (a broadcast view will do),
+    of any sign and size. Elements behind the plan's ``dim`` are copied.
+
+    ``inverse`` turns back: with the same amplitude it is the transposed map, so the gradient of x is
+    ``rotary(grad, positions, plan, inverse=True)``. Angles are exact to 2^-31 of a turn at any position; fp32
+    arithmetic, rounded once. ``out`` may be ``x`` itself, and must not share memory with it otherwise. No
+    derivatives."""
+    dev = x.get_device()
+    given = out is not None
+    if dev < 0 or positions.get_device() != dev or plan.turns.get_device() != dev or (given and out.get_device() != dev):
+        _on_gpu(x, positions, plan.turns, out)
+    if torch.is_grad_enabled() and (x.requires_grad or (given and out.requires_grad)):
+        _no_backward(x, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(x, out)
+    if given and out.dtype is not x.dtype:
+        raise TypeError(f"out must be {x.dtype}, got {out.dtype}")
+    code, sizes, (pst, xst, ost), alike = _rotary_views(
+        x.dtype, x.shape, x.stride(), positions.dtype, positions.shape, positions.stride(),
+        out.shape if given else None, out.stride() if given else None, plan.dim)
+    if not given:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    elif out.data_ptr() == x.data_ptr() and alike:
+        _check_apart(out, positions, plan.turns)
+    else:
+        _check_apart(out, x, positions, plan.turns)
+    if out.numel() == 0:
+        return out
+    st = _launch(dev, _lib.lib().mi355_rotary, code, x.data_ptr(), out.data_ptr(), positions.data_ptr(),
+                 positions.dtype is torch.int64, plan.turns.data_ptr(), plan.amplitude, *sizes, plan.dim, pst, xst,
+                 ost, plan.interleaved, inverse)
+    if st:
+        _lib.check("mi355_rotary", st)
+    return out
+
+
+# tokens of a paged cache that share a scale
+PAGED_BLOCK = 16
+
+
+@dataclass(frozen=True, eq=False)
+class PagedCache:
+    """A layer's keys and values in pages, 8 bits each: ``k`` and ``v`` ``[pages, kv_heads, page, head_dim]``
+    float8_e4m3fn, ``k_scale`` and ``v_scale`` ``[pages, kv_heads, page / 16]`` fp32, a power of two for each block of
+    16 tokens and head (element = scale * e4m3). All contiguous; ``page`` is a power of two from 16 to 1024."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    def __post_init__(self):
+        if self.k.dim() != 4 or self.v.shape != self.k.shape:
+            raise ValueError("k and v are [pages, kv_heads, page, head_dim]")
+        pages, kv_heads, page, D = self.k.shape
+        if page not in (16, 32, 64, 128, 256, 512, 1024):
+            raise ValueError(f"page must be a power of two from 16 to 1024, got {page}")
+        if D not in GROUPED_HEAD_DIMS:
+            raise ValueError(f"head_dim {D} is not one of {GROUPED_HEAD_DIMS}")
+        if not 1 <= pages < 1 << 30 or not 1 <= kv_heads <= 65535:
+            raise ValueError(f"{pages} pages and {kv_heads} heads are out of range")
+        shape = (pages, kv_heads, page // PAGED_BLOCK)
+        if tuple(self.k_scale.shape) != shape or tuple(self.v_scale.shape) != shape:
+            raise ValueError(f"the scales must be of shape {shape}")
+        if self.k.dtype != torch.float8_e4m3fn or self.v.dtype != torch.float8_e4m3fn:
+            raise TypeError("k and v must be float8_e4m3fn")
+        if self.k_scale.dtype != torch.float32 or self.v_scale.dtype != torch.float32:
+            raise TypeError("the scales must be fp32")
+        for t in (self.k, self.v, self.k_scale, self.v_scale):
+            if not t.is_contiguous():
+                raise ValueError("k, v and their scales must be contiguous")
+            if t.get_device() != self.k.get_device():
+                raise ValueError("k, v and their scales must be on one device")
+        if (self.k.data_ptr() | self.v.data_ptr()) & 15:
+            _check_aligned(k=self.k.data_ptr(), v=self.v.data_ptr())
+        _check_apart(self.k, self.v, self.k_scale, self.v_scale)
+        _check_apart(self.v, self.k_scale, self.v_scale)
+        _check_apart(self.k_scale, self.v_scale)
+
+
+def paged_cache(pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> PagedCache:
+    """An empty ``PagedCache`` of ``pages`` pages of ``page`` tokens."""
+    k, v = (torch.zeros((pages, kv_heads, page, head_dim), dtype=torch.float8_e4m3fn, device=device) for _ in range(2))
+    ks, vs = (torch.zeros((pages, kv_heads, page // PAGED_BLOCK), dtype=torch.float32, device=device) for _ in range(2))
+    return PagedCache(k, v, ks, vs)
+
+
+@dataclass(frozen=True, eq=False)
+class PagedBatch:
+    """The sequences of a batch and where their tokens are: token p of sequence b is in page ``table[b, p // page]`` of
+    a cache (``table`` int32 ``[B, width]``), ``lens[b]`` (int32) counts its tokens, the newest of this step included and
+    last. The step's tokens are packed: sequence b's are rows ``offsets[b]`` to ``offsets[b + 1]`` (int32 ``[B + 1]``, from 0
+    and not decreasing), ``most`` of one sequence at most; without ``offsets`` every sequence has ``most``. The same
+    batch serves all layers. The kernels read the three tensors when they run, so a captured graph follows their
+    values; a table entry that is no page is one that does not exist, whatever else it is."""
+    table: torch.Tensor
+    lens: torch.Tensor
+    most: int = 1
+    offsets: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        if self.table.dim() != 2 or self.table.dtype != torch.int32:
+            raise ValueError("table must be an int32 tensor [B, width]")
+        B, width = self.table.shape
+        if width > 1 and self.table.stride(1) != 1:
+            raise ValueError("table needs a unit column stride")
+        if self.lens.dtype != torch.int32 or tuple(self.lens.shape) != (B,) or not self.lens.is_contiguous():
+            raise ValueError(f"lens must be a contiguous int32 tensor of shape ({B},)")
+        if self.offsets is not None and (self.offsets.dtype != torch.int32 or tuple(self.offsets.shape) != (B + 1,)
+                                         or not self.offsets.is_contiguous()):
+            raise ValueError(f"offsets must be a contiguous int32 tensor of shape ({B + 1},)")
+        if not 0 <= operator.index(self.most) < 1 << 30 or B > 1 << 20:
+            raise ValueError(f"most = {self.most} or {B} sequences are out of range")
+
+
+@functools.lru_cache(maxsize=512)
+def _paged_views(cache_shape, table_shape, table_stride, most, ragged, names, dtypes, shapes, strides):
+    """(type code, sizes, stride arrays, workspace bytes) of a paged call's tensors (names: those it has), checked."""
+    if dtypes[0] not in _SIXTEEN_BIT:
+        raise TypeError(f"{names[0]} must be fp16 or bf16, got {dtypes[0]}")
+    if len(set(dtypes)) > 1:
+        raise TypeError(f"{', '.join(names)} must share one dtype, got {dtypes}")
+    pages, Hkv, page, D = cache_shape
+    (B, width), T, H = table_shape, None, Hkv
+    for name, shape in zip(names, shapes):
+        if len(shape) != 3 or shape[2] != D or (T is not None and shape[0] != T):
+            raise ValueError(f"{name} must be [{'tokens' if T is None else T}, heads, {D}], got {tuple(shape)}")
+        T = shape[0]
+        if name in ("k", "v") and shape[1] != Hkv:
+            raise ValueError(f"{name} has {shape[1]} heads, the cache {Hkv}")
+        if name == "q":
+            H = shape[1]
+        if name in ("out", "q_out") and tuple(shape) != (T, H, D):
+            raise ValueError(f"{name} must have q's shape {(T, H, D)}")
+    if H == 0 or H > 65535 or H % Hkv:
+        raise ValueError(f"{H} query heads cannot share {Hkv} K/V heads evenly")
+    if not ragged and T != B * most:
+        raise ValueError(f"{B} sequences of {most} new tokens need {B * most} rows, got {T}")
+    if width * page >= 1 << 30 or T >= 1 << 30:
+        raise ValueError("the table holds 2^30 tokens or more of a sequence, or the call has as many rows")
+    if B * most * H >= 1 << 23:
+        raise ValueError(f"{B} sequences of up to {most} new tokens in {H} heads are too many for one call")
+    views = []
+    for name, shape, st in zip(names, shapes, strides):
+        views.append(_rows_strides(name, shape, st, 4 if name == "out" else 8, 0 if name in ("k", "v") else None,
+                                   written=name in ("out", "q_out")))
+    if names[-1] == "q":
+        views.append((H * D, D))
+    need = 0
+    if "k" not in names:
+        need = _lib.lib().mi355_attn_paged_workspace_bytes(B, most, H, Hkv, D, page, width)
+        if need < 0:
+            _lib.check("mi355_attn_paged_workspace_bytes", need)
+    return (_lib.dtype_code(dtypes[0]), (B, most, T, H, Hkv, D, pages, page, width),
+            table_stride[0] if B > 1 else width, _Arrays(*views), need)
+
+
+def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch,
+                 plan: Optional[RotaryPlan] = None, q: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Writes a step's ``k`` and ``v`` ``[tokens, kv_heads, head_dim]`` (fp16 or bf16, packed as ``batch`` says) into
+    their sequences' pages, K rotated by its position on the way (``plan``; its ``dim`` a multiple of 8), and rotates the
+    queries ``q`` ``[tokens, heads, head_dim]`` of the same tokens in the same launch: returned, None without ``q``.
+
+    A block's scale is the least power of two with which its largest new element stays within e4m3's 448 (at least 2^-118),
+    or the one it had where that is larger; when it grows, the block's earlier tokens are rounded to it anew.
+    Elements are rounded to nearest even from fp32, once; infinities and NaN are held as NaN and leave the scale
+    alone. Tokens without a page (a table entry out of range, a position behind the table) are not written. Each page
+    that is written must be one sequence's. ``q_out`` may be ``q``; rows that no sequence has are left
+    in a given ``q_out``, and zeros in a new one. No derivatives."""
+    dev = k.get_device()
+    if dev < 0 or v.get_device() != dev or cache.k.get_device() != dev or batch.table.get_device() != dev or (
+            batch.lens.get_device() != dev) or (batch.offsets is not None and batch.offsets.get_device() != dev) or (
+            plan is not None and plan.turns.get_device() != dev) or (q is not None and q.get_device() != dev) or (
+            q_out is not None and q_out.get_device() != dev):
+        _on_gpu(k, v, cache.k, batch.table, batch.lens, batch.offsets, None if plan is None else plan.turns, q, q_out)
+    if torch.is_grad_enabled():
+        _no_backward(k, v, q, q_out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(k, v, q, q_out)
+    if q is None and q_out is not None:
+        raise ValueError("q_out without q")
+    if q is not None and plan is None:
+        raise ValueError("q is given to be rotated, but no plan")
+    D = cache.k.shape[3]
+    if plan is not None and (plan.dim % 8 or plan.dim > D):
+        raise ValueError(f"the plan rotates {plan.dim} elements: a multiple of 8, at most the head's {D}, is needed")
+    tensors = (k, v) if q is None else (k, v, q) if q_out is None else (k, v, q, q_out)
+    code, sizes, row, strides, _ = _paged_views(
+        cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
+        ("k", "v", "q", "q_out")[:len(tensors)], tuple([t.dtype for t in tensors]), tuple([t.shape for t in tensors]),
+        tuple([t.stride() for t in tensors]))
+    given = q_out is not None
+    if given:
+        if q_out.data_ptr() == q.data_ptr() and strides[2][:] == strides[3][:]:
+            _check_apart(q_out, k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
+        else:
+            _check_apart(q_out, q, k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        _check_apart(t, k, v, q, batch.table, batch.lens, batch.offsets)
+    B, most, T = sizes[:3]
+    if q is not None and not given:
+        q_out = q.new_empty(q.shape) if B * most else q.new_zeros(q.shape)
+    if B * most == 0 or T == 0:
+        return q_out
+    kp, vp, qp, op = k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr()
+    if (kp | vp | qp | op) & 15:
+        _check_aligned(k=kp, v=vp, q=qp, q_out=op)
+    st = _launch(dev, _lib.lib().mi355_paged_append, code, kp, vp, qp, op, cache.k.data_ptr(), cache.v.data_ptr(),
+                 cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), batch.table.data_ptr(), row, batch.lens.data_ptr(),
+                 0 if batch.offsets is None else batch.offsets.data_ptr(), *sizes, strides[0], strides[1],
+                 strides[2] if qp else None, strides[3] if qp else None, 0 if plan is None else plan.turns.data_ptr(),
+                 0 if plan is None else plan.dim, plan is not None and plan.interleaved,
+                 1.0 if plan is None else plan.amplitude, not given)
+    if st:
+        _lib.check("mi355_paged_append", st)
+    return q_out
+
+
+def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Softmax attention of a step's tokens ``q`` ``[tokens, heads, head_dim]`` (fp16 or bf16, packed as ``batch`` says)
+    over the pages of their sequences, which hold the step's own tokens already (``paged_append``): the token at
+    position p of its sequence sees tokens 0 to p. Query head h reads K/V head ``h // (heads // kv_heads)``.
+
+    A token that sees no key gives zeros, one that sees a key without a page (a table entry out of range, a position
+    behind the table) NaN. What the pages hold behind ``lens`` does not matter, and a NaN in a key or value reaches
+    the tokens that see it alone. fp32 scores and statistics; probabilities are held in twice bf16's bits, outputs
+    rounded once. bf16 values are to stay below 2^110 in q and 2^100 in V. ``out`` must not share memory with the
+    inputs; rows that no sequence has are left in a given ``out``, and zeros in a new one. No derivatives."""
+    dev = q.get_device()
+    given = out is not None
+    if dev < 0 or cache.k.get_device() != dev or batch.table.get_device() != dev or batch.lens.get_device() != dev or (
+            batch.offsets is not None and batch.offsets.get_device() != dev) or (given and out.get_device() != dev):
+        _on_gpu(q, cache.k, batch.table, batch.lens, batch.offsets, out)
+    if torch.is_grad_enabled() and (q.requires_grad or (given and out.requires_grad)):
+        _no_backward(q, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent(q, out)
+    code, sizes, row, (qst, ost), need = _paged_views(
+        cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
+        ("q", "out") if given else ("q",), (q.dtype, out.dtype) if given else (q.dtype,),
+        (q.shape, out.shape) if given else (q.shape,), (q.stride(), out.stride()) if given else (q.stride(),))
+    scale = _scale(scale, sizes[5])
+    B, most, T = sizes[:3]
+    if given:
+        _check_apart(out, q, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
+    else:
+        out = q.new_empty(q.shape) if B * most else q.new_zeros(q.shape)
+    if B * most == 0 or T == 0:
+        return out
+    qp, op = q.data_ptr(), out.data_ptr()
+    if qp & 15 or op & 7:
+        _check_aligned(q=qp, out=op)
+    ws = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
+    st = _launch(dev, _lib.lib().mi355_attn_paged, code, qp, cache.k.data_ptr(), cache.v.data_ptr(),
+                 cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), batch.table.data_ptr(), row, batch.lens.data_ptr(),
+                 0 if batch.offsets is None else batch.offsets.data_ptr(), op, *sizes, qst, ost, scale, not given,
+                 ws.data_ptr() if need else 0, need)
+    if st:
+        _lib.check("mi355_attn_paged", st)
     return out
