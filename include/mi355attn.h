@@ -471,24 +471,22 @@ int mi355_linear_i4(int dtype, int out_dtype, const void* X, int64_t ldx, const 
  * the same amplitude: the transposed map, which is the gradient's).
  * frequencies [rot_dim / 2] (device) are fractions of a full turn for each position, times 2^64
  * (modulo 2^64): angles are exact to 2^-31 of a turn at any position. fp32 arithmetic, rounded once.
- * X and Y are [n0, n1, heads, head_dim] views given by element strides {batch, token, head}, the
- * head_dim stride 1; positions [n0, n1] int32 (int64 with positions_64 != 0), strides {batch, token}, any sign.
- * Y may be X with the same strides, and must not overlap it otherwise. dtype F32, F16 or BF16;
- * head_dim even, up to 512, rot_dim even; n0 n1 up to 2^31. Any alignment of whole elements (16-byte runs are faster).
+ * X and Y are [n0, n1, heads, head_dim] views with a head_dim stride of 1, positions [n0, n1] int32
+ * (int64 with positions_64 != 0), of any sign. sizes = {n0, n1, heads, head_dim, rot_dim}; strides = positions'
+ * {batch, token}, X's {batch, token, head}, Y's, in elements. Y may be X with the same strides, and must not
+ * overlap it otherwise. dtype F32, F16 or BF16; head_dim even, up to 512, rot_dim even; n0 n1 up to 2^31. Any
+ * alignment of whole elements (16-byte runs are faster).
  */
 int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int positions_64,
-                 const uint64_t* frequencies, float amplitude, int64_t n0, int64_t n1, int64_t heads,
-                 int64_t head_dim, int64_t rot_dim, const int64_t* position_strides,
-                 const int64_t* x_strides, const int64_t* y_strides, int interleaved, int inverse,
-                 void* stream);
+                 const uint64_t* frequencies, float amplitude, const int64_t* sizes,
+                 const int64_t* strides, int interleaved, int inverse, void* stream);
 
 /*
  * A K/V cache in pages, 8 bits an element:
  *   cache_k, cache_v [pages, kv_heads, page, head_dim] e4m3 (no infinities), contiguous, 16-byte aligned;
  *   k_scale, v_scale [pages, kv_heads, page / 16] fp32 powers of two; an element is its byte's value times the
  *   scale of its block of 16 tokens and head. page: a power of two from 16 to 1024.
- * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32, row stride
- * table_stride). lens [B] counts a sequence's tokens in the cache, its n new ones included, which are the
+ * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32). lens [B] counts a sequence's tokens in the cache, its n new ones included, which are the
  * last. New tokens are packed: sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not
  * decreasing) of Q, K, V and the outputs, `most` at most (those behind it are ignored); offsets NULL:
  * rows b * most .. of `most` each. table, lens and offsets are read on the device, so a captured graph
@@ -511,27 +509,22 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be
  * stream-ordered. Rows behind the last sequence's as above.
  *
- * Both: dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256; strides {token, head} in
- * elements, multiples of 8 with 16-byte aligned bases (O: of 4, 8-byte); rot_dim a multiple of 8; width * page below 2^30;
- * pages, tokens, most and B below 2^30, B most heads below 2^23.
+ * Both: dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256; rot_dim a multiple of 8.
+ * sizes = {B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride}, strides = {token, head} of K,
+ * V, Q and Q_out (of Q and O in the attention) in elements, multiples of 8 with 16-byte aligned bases (O: of 4, 8-byte).
+ * width * page, pages, tokens, most and table_stride below 2^30, B up to 2^20, B most heads below 2^23.
  */
 int mi355_paged_append(int dtype, const void* K, const void* V, const void* Q, void* Q_out,
                        uint8_t* cache_k, uint8_t* cache_v, float* k_scale, float* v_scale,
-                       const int32_t* table, int64_t table_stride, const int32_t* lens,
-                       const int32_t* offsets, int64_t B, int64_t most, int64_t tokens, int64_t heads,
-                       int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page, int64_t width,
-                       const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
-                       const int64_t* out_strides, const uint64_t* frequencies, int64_t rot_dim,
-                       int interleaved, float amplitude, int zero_tail, void* stream);
-int64_t mi355_attn_paged_workspace_bytes(int64_t B, int64_t most, int64_t heads, int64_t kv_heads,
-                                         int64_t head_dim, int64_t page, int64_t width);
+                       const int32_t* table, const int32_t* lens, const int32_t* offsets,
+                       const int64_t* sizes, const int64_t* strides, const uint64_t* frequencies,
+                       int64_t rot_dim, int interleaved, float amplitude, int zero_tail, void* stream);
+int64_t mi355_attn_paged_workspace_bytes(const int64_t* sizes);
 int mi355_attn_paged(int dtype, const void* Q, const uint8_t* cache_k, const uint8_t* cache_v,
                      const float* k_scale, const float* v_scale, const int32_t* table,
-                     int64_t table_stride, const int32_t* lens, const int32_t* offsets, void* O,
-                     int64_t B, int64_t most, int64_t tokens, int64_t heads, int64_t kv_heads,
-                     int64_t head_dim, int64_t pages, int64_t page, int64_t width,
-                     const int64_t* q_strides, const int64_t* o_strides, float scale, int zero_tail,
-                     void* workspace, int64_t workspace_bytes, void* stream);
+                     const int32_t* lens, const int32_t* offsets, void* O, const int64_t* sizes,
+                     const int64_t* strides, float scale, int zero_tail, void* workspace,
+                     int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -58,10 +58,13 @@ def values64(t, s):
     return x.view(t.shape)
 
 
-def attention64(q, cache, table, lens, offsets, scale):
+def attention64(q, cache, table, lens, offsets, scale, most=None):
     """q [tokens, heads, D] over cache (k, v, k_scale, v_scale): (result, error bound). Errors: scores (D + 4) 2^-24 scale
-    sum |q| |k| and exponentials 2^-20, both in numerator and denominator; probabilities as two bf16 terms 2^-16; sums
-    of m terms m 2^-23; the output's rounding."""
+    sum |q| |k| and exponentials 2^-20, both in numerator and denominator; probabilities as two bf16 terms 2^-16, or where
+    `most` new tokens make more than 32 rows, rounded to q's type in numerator and denominator (fp16 ones below 2^-14 by
+    2^-25); sums of m terms m 2^-23; the output's rounding."""
+    rows = (max(b - a for a, b in zip(offsets, offsets[1:])) if most is None else most) * (q.shape[1] // cache[0].shape[1])
+    once = rows > 32
     k, v = values64(cache[0], cache[2]), values64(cache[1], cache[3])
     pages, kv_heads, page, D = k.shape
     T, H, _ = q.shape
@@ -88,9 +91,11 @@ def attention64(q, cache, table, lens, offsets, scale):
                     s = kk[:sees] @ qq * scale
                     w = torch.softmax(s, 0)
                     o = w @ vv[:sees]
-                    rel = 2.0 ** -16 + 2 * (2.0 ** -20 + (D + 4) * 2.0 ** -24 * scale * (kk[:sees].abs() @ qq.abs()).max()) + sees * 2.0 ** -23
+                    rel = (2 * UNIT[q.dtype] if once else 2.0 ** -16) + 2 * (2.0 ** -20 + (D + 4) * 2.0 ** -24 * scale * (kk[:sees].abs() @ qq.abs()).max()) + sees * 2.0 ** -23
                     ref[first + i, x] = o
                     tol[first + i, x] = rel * (w @ vv[:sees].abs()) + UNIT[q.dtype] * o.abs() + 2.0 ** -24
+                    if once and q.dtype == torch.float16:
+                        tol[first + i, x] += sees * 2.0 ** -25 * vv[:sees].abs().amax()
     return ref, tol
 
 

@@ -353,6 +353,7 @@ def test_attention(dtype, case):
         check(got, ref, tol, "attention")
         assert torch.equal(got, ops.attention_paged(q.cuda(), dev, batch))
     more = ops.PagedBatch(table.cuda(), i32(lens), max(new) + 40, i32(offsets))  # `most` need not be exact
+    ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5, max(new) + 40)
     check(ops.attention_paged(q.cuda(), dev, more), ref, tol, "attention")
 
 

@@ -13,68 +13,76 @@ BAD_SIZE, NULL, DTYPE, ALIGN, HEAD, UNSUP = -2, -1, -3, -4, -5, -6
 i64 = _lib.i64_array
 
 
-ROTARY = dict(dtype=F16, X=64, Y=64, pos=64, freqs=64, n0=1, n1=4, heads=2, head_dim=64, rot=64, ps=(0, 1), xs=(0, 128, 64),
-              ys=(0, 128, 64))
+ROTARY = dict(dtype=F16, X=64, Y=64, pos=64, freqs=64, n0=1, n1=4, heads=2, head_dim=64, rot=64, sizes=True,
+              strides=(0, 1, 0, 128, 64, 0, 128, 64))
 
 
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=3), DTYPE), (dict(n0=-1), BAD_SIZE), (dict(n1=1 << 32), BAD_SIZE), (dict(n0=1 << 16, n1=1 << 16), BAD_SIZE),
     (dict(heads=70000), BAD_SIZE), (dict(heads=-1), BAD_SIZE), (dict(head_dim=63), HEAD), (dict(head_dim=514), HEAD),
     (dict(rot=66), HEAD), (dict(rot=0), HEAD), (dict(rot=3), HEAD), (dict(X=0), NULL), (dict(Y=0), NULL), (dict(pos=0), NULL),
-    (dict(freqs=0), NULL), (dict(ps=None), NULL), (dict(xs=None), NULL), (dict(ys=None), NULL), (dict(n1=0), 0), (dict(heads=0), 0)])
+    (dict(freqs=0), NULL), (dict(sizes=False), NULL), (dict(strides=None), NULL), (dict(n1=0), 0), (dict(heads=0), 0)])
 def test_rotary_entry_refusals(kw, status):
     a = {**ROTARY, **kw}
-    arr = [i64(a[k]) if a[k] else None for k in ("ps", "xs", "ys")]
-    assert _lib.lib().mi355_rotary(a["dtype"], a["X"], a["Y"], a["pos"], 1, a["freqs"], 1.0, a["n0"], a["n1"], a["heads"],
-                                   a["head_dim"], a["rot"], *arr, 0, 0, None) == status
+    sizes = i64([a[k] for k in ("n0", "n1", "heads", "head_dim", "rot")])
+    assert _lib.lib().mi355_rotary(a["dtype"], a["X"], a["Y"], a["pos"], 1, a["freqs"], 1.0, sizes if a["sizes"] else None,
+                                   i64(a["strides"]) if a["strides"] else None, 0, 0, None) == status
 
 
 APPEND = dict(dtype=F16, K=64, V=64, Q=64, QO=64, ck=64, cv=64, ks=64, vs=64, table=64, row=4, lens=64, off=64, B=2, most=3,
-              tokens=6, heads=4, kv_heads=2, head_dim=64, pages=9, page=16, width=4, kst=(128, 64), vst=(128, 64),
-              qst=(256, 64), ost=(256, 64), freqs=64, rot=64)
+              tokens=6, heads=4, kv_heads=2, head_dim=64, pages=9, page=16, width=4, strides=(128, 64, 128, 64, 256, 64, 256, 64),
+              freqs=64, rot=64)
+
+
+def sizes_of(a):
+    return i64([a[k] for k in ("B", "most", "tokens", "heads", "kv_heads", "head_dim", "pages", "page", "width", "row")])
+
+
+def strides_but(at, value):
+    return tuple(value if i == at else s for i, s in enumerate(APPEND["strides"]))
+
+
 SIZES = [
     (dict(dtype=F32), DTYPE), (dict(head_dim=40), HEAD), (dict(B=-1), BAD_SIZE), (dict(B=(1 << 20) + 1), BAD_SIZE),
     (dict(most=-1), BAD_SIZE), (dict(tokens=1 << 30), BAD_SIZE), (dict(heads=5), BAD_SIZE), (dict(kv_heads=0), BAD_SIZE),
     (dict(pages=1 << 30), BAD_SIZE), (dict(page=8), BAD_SIZE), (dict(page=48), BAD_SIZE), (dict(page=2048), BAD_SIZE),
-    (dict(width=1 << 26), BAD_SIZE), (dict(width=-1), BAD_SIZE), (dict(off=0, tokens=5), BAD_SIZE)]
+    (dict(width=1 << 26), BAD_SIZE), (dict(width=-1), BAD_SIZE), (dict(off=0, tokens=5), BAD_SIZE),
+    (dict(row=-1), BAD_SIZE), (dict(row=1 << 30), BAD_SIZE), (dict(strides=None), NULL)]
 
 
 @pytest.mark.parametrize("kw,status", SIZES + [
     *[({k: 0}, NULL) for k in ("K", "V", "QO", "ck", "cv", "ks", "vs", "table", "lens", "freqs")],
-    *[({k: None}, NULL) for k in ("kst", "vst", "qst", "ost")],
     (dict(rot=4), HEAD), (dict(rot=72), HEAD), (dict(rot=20), HEAD), (dict(K=72), ALIGN), (dict(V=68), ALIGN), (dict(Q=72), ALIGN),
-    (dict(QO=72), ALIGN), (dict(ck=72), ALIGN), (dict(cv=72), ALIGN), (dict(kst=(132, 64)), ALIGN), (dict(vst=(128, 60)), ALIGN),
-    (dict(qst=(256, 4)), ALIGN), (dict(ost=(257, 64)), ALIGN), (dict(most=1 << 29, B=1 << 10), BAD_SIZE), (dict(B=0), 0),
+    (dict(QO=72), ALIGN), (dict(ck=72), ALIGN), (dict(cv=72), ALIGN), *[(dict(strides=strides_but(i, 132)), ALIGN) for i in range(8)], (dict(most=1 << 29, B=1 << 10), BAD_SIZE), (dict(B=0), 0),
     (dict(tokens=0), 0), (dict(most=0), 0)])
 def test_append_entry_refusals(kw, status):
     a = {**APPEND, **kw}
-    st = [i64(a[k]) if a[k] else None for k in ("kst", "vst", "qst", "ost")]
     assert _lib.lib().mi355_paged_append(
-        a["dtype"], a["K"], a["V"], a["Q"], a["QO"], a["ck"], a["cv"], a["ks"], a["vs"], a["table"], a["row"], a["lens"], a["off"],
-        a["B"], a["most"], a["tokens"], a["heads"], a["kv_heads"], a["head_dim"], a["pages"], a["page"], a["width"], *st, a["freqs"],
-        a["rot"], 0, 1.0, 1, None) == status
+        a["dtype"], a["K"], a["V"], a["Q"], a["QO"], a["ck"], a["cv"], a["ks"], a["vs"], a["table"], a["lens"], a["off"],
+        sizes_of(a), i64(a["strides"]) if a["strides"] else None, a["freqs"], a["rot"], 0, 1.0, 1, None) == status
 
 
 @pytest.mark.parametrize("kw,status", SIZES + [
-    *[({k: 0}, NULL) for k in ("Q", "QO", "ck", "cv", "ks", "vs", "table", "lens")], *[({k: None}, NULL) for k in ("qst", "ost")],
+    *[({k: 0}, NULL) for k in ("Q", "QO", "ck", "cv", "ks", "vs", "table", "lens")],
     (dict(pages=0), BAD_SIZE), (dict(scale=0.0), UNSUP), (dict(scale=-1.0), UNSUP), (dict(scale=math.nan), UNSUP),
     (dict(scale=math.inf), UNSUP), (dict(Q=72), ALIGN), (dict(QO=68), ALIGN), (dict(ck=72), ALIGN), (dict(cv=8), ALIGN),
-    (dict(qst=(252, 64)), ALIGN), (dict(ost=(256, 62)), ALIGN), (dict(width=17, ws=0), BAD_SIZE), (dict(width=17, ws_bytes=64), BAD_SIZE),
+    *[(dict(strides=strides_but(i, 130)), ALIGN) for i in range(4)], (dict(width=17, ws=0), BAD_SIZE), (dict(width=17, ws_bytes=64), BAD_SIZE),
     (dict(width=17, ws=72), BAD_SIZE), (dict(B=1 << 11, most=1 << 10, tokens=1 << 21), BAD_SIZE), (dict(B=0), 0), (dict(tokens=0), 0)])
 def test_attention_entry_refusals(kw, status):
     a = {**APPEND, "scale": 0.125, "ws": 64, "ws_bytes": 1 << 30, **kw}
-    st = [i64(a[k]) if a[k] else None for k in ("qst", "ost")]
     assert _lib.lib().mi355_attn_paged(
-        a["dtype"], a["Q"], a["ck"], a["cv"], a["ks"], a["vs"], a["table"], a["row"], a["lens"], a["off"], a["QO"], a["B"], a["most"],
-        a["tokens"], a["heads"], a["kv_heads"], a["head_dim"], a["pages"], a["page"], a["width"], *st, a["scale"], 1, a["ws"],
-        a["ws_bytes"], None) == status
+        a["dtype"], a["Q"], a["ck"], a["cv"], a["ks"], a["vs"], a["table"], a["lens"], a["off"], a["QO"], sizes_of(a),
+        i64(a["strides"]) if a["strides"] else None, a["scale"], 1, a["ws"], a["ws_bytes"], None) == status
 
 
 def test_attention_workspace():
-    f = _lib.lib().mi355_attn_paged_workspace_bytes
-    assert f(4, 1, 8, 2, 64, 16, 16) == 0  # 256 keys: nothing to share out
-    assert f(4, 1, 8, 2, 64, 16, 17) > 0 and f(4, 1, 8, 2, 64, 16, 17) % 16 == 0
-    assert f(4, 1, 8, 3, 64, 16, 16) == BAD_SIZE and f(4, 1, 8, 2, 40, 16, 16) == HEAD and f(4, 1, 8, 2, 64, 24, 16) == BAD_SIZE
+    def f(**kw):
+        return _lib.lib().mi355_attn_paged_workspace_bytes(sizes_of({**APPEND, "tokens": 0, **kw}))
+
+    assert f(width=16) == 0  # 256 keys: nothing to share out
+    assert f(width=17) > 0 and f(width=17) % 16 == 0
+    assert f(kv_heads=3) == BAD_SIZE and f(head_dim=40) == HEAD and f(page=24) == BAD_SIZE
+    assert _lib.lib().mi355_attn_paged_workspace_bytes(None) == NULL
 
 
 def cache(pages=3, kv_heads=2, page=16, D=64):

@@ -126,20 +126,16 @@ _SIGNATURES = {
         [C.c_int, C.c_int, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P],
     ),
     "mi355_rotary": (
-        C.c_int,
-        [C.c_int, _P, _P, _P, C.c_int, _P, C.c_float, *[_I64] * 5, *[C.POINTER(_I64)] * 3, C.c_int,
-         C.c_int, _P],
+        C.c_int, [C.c_int, _P, _P, _P, C.c_int, _P, C.c_float, C.POINTER(_I64), C.POINTER(_I64), C.c_int, C.c_int, _P],
     ),
     "mi355_paged_append": (
         C.c_int,
-        [C.c_int, *[_P] * 9, _I64, _P, _P, *[_I64] * 9, *[C.POINTER(_I64)] * 4, _P, _I64, C.c_int,
-         C.c_float, C.c_int, _P],
+        [C.c_int, *[_P] * 11, C.POINTER(_I64), C.POINTER(_I64), _P, _I64, C.c_int, C.c_float, C.c_int, _P],
     ),
-    "mi355_attn_paged_workspace_bytes": (_I64, [_I64] * 7),
+    "mi355_attn_paged_workspace_bytes": (_I64, [C.POINTER(_I64)]),
     "mi355_attn_paged": (
         C.c_int,
-        [C.c_int, *[_P] * 6, _I64, *[_P] * 3, *[_I64] * 9, *[C.POINTER(_I64)] * 2, C.c_float, C.c_int,
-         _P, _I64, _P],
+        [C.c_int, *[_P] * 9, C.POINTER(_I64), C.POINTER(_I64), C.c_float, C.c_int, _P, _I64, _P],
     ),
 }
 

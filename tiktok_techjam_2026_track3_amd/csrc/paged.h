@@ -52,20 +52,36 @@ MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
   return s;
 }
 
-// What both entry points refuse.
-inline int check(int dtype, int64_t B, int64_t most, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                 int64_t pages, int64_t page, int64_t width) {
+// The sizes of a call, as both entry points take them.
+struct Sizes {
+  int64_t B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride;
+};
+
+// What both refuse.
+inline int check(int dtype, const Sizes& z) {
+  const auto [B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride] = z;
   if (dtype != MI355_F16 && dtype != MI355_BF16) return MI355_E_BAD_DTYPE;
   switch (head_dim) {
     case 16: case 32: case 48: case 64: case 80: case 96: case 128: case 192: case 256: break;
     default: return MI355_E_HEAD_DIM;
   }
   constexpr int64_t MOST = int64_t(1) << 30;
-  for (const int64_t n : {B, most, tokens, pages, width})
+  for (const int64_t n : {B, most, tokens, pages, width, table_stride})
     if (n < 0 || n >= MOST) return MI355_E_BAD_SIZE;
   if (B > (1 << 20) || heads < 1 || heads > 65535 || kv_heads < 1 || heads % kv_heads) return MI355_E_BAD_SIZE;
   if (page < BLOCK || page > 1024 || (page & (page - 1)) || width * page >= MOST) return MI355_E_BAD_SIZE;
   return MI355_OK;
+}
+
+inline Cache cache_of(const Sizes& z, const uint8_t* k, const uint8_t* v, const float* ks, const float* vs) {
+  return Cache{const_cast<uint8_t*>(k), const_cast<uint8_t*>(v), const_cast<float*>(ks), const_cast<float*>(vs),
+               static_cast<int32_t>(z.pages), static_cast<int32_t>(z.kv_heads), static_cast<int32_t>(z.head_dim),
+               __builtin_ctzll(static_cast<uint64_t>(z.page))};
+}
+
+inline Batch batch_of(const Sizes& z, const int32_t* table, const int32_t* lens, const int32_t* offsets) {
+  return Batch{table, z.table_stride, lens, offsets, static_cast<int32_t>(z.B), static_cast<int32_t>(z.width),
+               static_cast<int32_t>(z.most), static_cast<int32_t>(z.tokens)};
 }
 
 }  // namespace paged

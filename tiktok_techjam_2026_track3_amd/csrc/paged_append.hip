@@ -227,55 +227,51 @@ int launch_dim(const AppendArgs& p, hipStream_t s) {
 
 extern "C" int mi355_paged_append(int dtype, const void* K, const void* V, const void* Q, void* Q_out, uint8_t* cache_k,
                                   uint8_t* cache_v, float* k_scale, float* v_scale, const int32_t* table,
-                                  int64_t table_stride, const int32_t* lens, const int32_t* offsets, int64_t B, int64_t most,
-                                  int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
-                                  int64_t page, int64_t width, const int64_t* k_strides, const int64_t* v_strides,
-                                  const int64_t* q_strides, const int64_t* out_strides, const uint64_t* frequencies,
-                                  int64_t rot_dim, int interleaved, float amplitude, int zero_tail, void* stream) {
-  AppendArgs p{};
-  if (const int st = paged::check(dtype, B, most, tokens, heads, kv_heads, head_dim, pages, page, width)) return st;
-  if (B * most == 0 || tokens == 0) return MI355_OK;
-  if (!K || !V || !lens || !k_strides || !v_strides || (pages > 0 && (!cache_k || !cache_v || !k_scale || !v_scale)) ||
-      (width > 0 && !table))
+                                  const int32_t* lens, const int32_t* offsets, const int64_t* sizes, const int64_t* strides,
+                                  const uint64_t* frequencies, int64_t rot_dim, int interleaved, float amplitude,
+                                  int zero_tail, void* stream) {
+  if (!sizes || !strides) return MI355_E_NULL_POINTER;
+  const paged::Sizes z = *reinterpret_cast<const paged::Sizes*>(sizes);
+  if (const int st = paged::check(dtype, z)) return st;
+  if (z.B * z.most == 0 || z.tokens == 0) return MI355_OK;
+  if (!K || !V || !lens || (z.pages > 0 && (!cache_k || !cache_v || !k_scale || !v_scale)) || (z.width > 0 && !table))
     return MI355_E_NULL_POINTER;
-  if (Q && (!Q_out || !q_strides || !out_strides || !frequencies)) return MI355_E_NULL_POINTER;
-  if (!offsets && B * most > tokens) return MI355_E_BAD_SIZE;
-  if (frequencies && (rot_dim < 8 || rot_dim > head_dim || rot_dim % 8)) return MI355_E_HEAD_DIM;
+  if (Q && (!Q_out || !frequencies)) return MI355_E_NULL_POINTER;
+  if (!offsets && z.B * z.most > z.tokens) return MI355_E_BAD_SIZE;
+  if (frequencies && (rot_dim < 8 || rot_dim > z.head_dim || rot_dim % 8)) return MI355_E_HEAD_DIM;
   const auto even = [](const void* base, const int64_t* st) {
     return aligned16(base) && st[0] % 8 == 0 && st[1] % 8 == 0;
   };
-  if (!even(K, k_strides) || !even(V, v_strides) || (Q && (!even(Q, q_strides) || !even(Q_out, out_strides))) ||
+  if (!even(K, strides) || !even(V, strides + 2) || (Q && (!even(Q, strides + 4) || !even(Q_out, strides + 6))) ||
       !aligned16(cache_k) || !aligned16(cache_v))
     return MI355_E_ALIGNMENT;
-  p.cache = paged::Cache{cache_k, cache_v, k_scale, v_scale, static_cast<int32_t>(pages), static_cast<int32_t>(kv_heads),
-                         static_cast<int32_t>(head_dim), __builtin_ctzll(static_cast<uint64_t>(page))};
-  p.batch = paged::Batch{table, table_stride, lens, offsets, static_cast<int32_t>(B), static_cast<int32_t>(width),
-                         static_cast<int32_t>(most), static_cast<int32_t>(tokens)};
+  AppendArgs p{};
+  p.cache = paged::cache_of(z, cache_k, cache_v, k_scale, v_scale);
+  p.batch = paged::batch_of(z, table, lens, offsets);
   p.k = K;
   p.v = V;
   p.q = Q;
   p.qo = Q_out;
-  p.kt = k_strides[0];
-  p.kh = k_strides[1];
-  p.vt = v_strides[0];
-  p.vh = v_strides[1];
+  p.kt = strides[0];
+  p.kh = strides[1];
+  p.vt = strides[2];
+  p.vh = strides[3];
   if (Q) {
-    p.qt = q_strides[0];
-    p.qh = q_strides[1];
-    p.ot = out_strides[0];
-    p.oh = out_strides[1];
+    p.qt = strides[4];
+    p.qh = strides[5];
+    p.ot = strides[6];
+    p.oh = strides[7];
   }
   p.freqs = frequencies;
   p.amplitude = amplitude;
   p.rot = frequencies ? static_cast<int32_t>(rot_dim) : 0;
   p.interleaved = interleaved;
-  p.heads = static_cast<int32_t>(heads);
+  p.heads = static_cast<int32_t>(z.heads);
   p.zero_tail = Q && zero_tail;
-  p.blocks = static_cast<int32_t>((most + 2 * BLOCK - 2) / BLOCK);
+  p.blocks = static_cast<int32_t>((z.most + 2 * BLOCK - 2) / BLOCK);
   // work-groups that share a block's heads: enough to have two a CU, no more than heads can use
-  const int64_t groups = B * p.blocks;
-  int64_t slices = (512 + groups - 1) / groups;
-  const int64_t useful = (2 * kv_heads + 3) / 4;
+  const int64_t groups = z.B * p.blocks;
+  const int64_t slices = (512 + groups - 1) / groups, useful = (2 * z.kv_heads + 3) / 4;
   p.slices = static_cast<int32_t>(slices < useful ? slices : useful);
   if (groups * p.slices >= (int64_t(1) << 23)) return MI355_E_BAD_SIZE;  // 2^31 threads
   const auto s = static_cast<hipStream_t>(stream);

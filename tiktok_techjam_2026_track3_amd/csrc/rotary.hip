@@ -110,16 +110,18 @@ int launch_vec(RotaryArgs& p, int64_t head_dim, bool interleaved, int vec, hipSt
 }  // namespace
 
 extern "C" int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int positions_64,
-                            const uint64_t* frequencies, float amplitude, int64_t n0, int64_t n1, int64_t heads,
-                            int64_t head_dim, int64_t rot_dim, const int64_t* position_strides, const int64_t* x_strides,
-                            const int64_t* y_strides, int interleaved, int inverse, void* stream) {
+                            const uint64_t* frequencies, float amplitude, const int64_t* sizes, const int64_t* strides,
+                            int interleaved, int inverse, void* stream) {
+  if (!sizes || !strides) return MI355_E_NULL_POINTER;
+  const int64_t n0 = sizes[0], n1 = sizes[1], heads = sizes[2], head_dim = sizes[3], rot_dim = sizes[4];
+  const int64_t *position_strides = strides, *x_strides = strides + 2, *y_strides = strides + 5;
   if (n0 < 0 || n1 < 0 || heads < 0 || n0 > (int64_t(1) << 31) || n1 > (int64_t(1) << 31) || n0 * n1 > (int64_t(1) << 31) ||
       heads > 65535)
     return MI355_E_BAD_SIZE;
   if (head_dim < 2 || head_dim > 512 || head_dim % 2 || rot_dim < 2 || rot_dim > head_dim || rot_dim % 2) return MI355_E_HEAD_DIM;
   if (dtype != MI355_F32 && dtype != MI355_F16 && dtype != MI355_BF16) return MI355_E_BAD_DTYPE;
   if (n0 * n1 * heads == 0) return MI355_OK;
-  if (!X || !Y || !positions || !frequencies || !position_strides || !x_strides || !y_strides) return MI355_E_NULL_POINTER;
+  if (!X || !Y || !positions || !frequencies) return MI355_E_NULL_POINTER;
   RotaryArgs p{};
   p.x = X;
   p.y = Y;

@@ -1092,7 +1092,8 @@ def _rotary_views(dt, xs, xst, pd, ps, pst, os, ost, dim):
     else:
         _rows_strides("out", os, ost, 1, written=True)
         ost = strides(ost[:-1])
-    return _lib.dtype_code(dt), (*n, D), _Arrays(strides(pst)[:2], xst, ost), xst == ost
+    return (_lib.dtype_code(dt), _lib.i64_array((*n, D, dim)), _lib.i64_array((*strides(pst)[:2], *xst, *ost)),
+            xst == ost)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: bool = False,
@@ -1117,11 +1118,11 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: 
         _no_tangent(x, out)
     if given and out.dtype is not x.dtype:
         raise TypeError(f"out must be {x.dtype}, got {out.dtype}")
-    code, sizes, (pst, xst, ost), alike = _rotary_views(
+    code, sizes, strides, alike = _rotary_views(
         x.dtype, x.shape, x.stride(), positions.dtype, positions.shape, positions.stride(),
         out.shape if given else None, out.stride() if given else None, plan.dim)
     if not given:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = x.new_empty(x.shape)
     elif out.data_ptr() == x.data_ptr() and alike:
         _check_apart(out, positions, plan.turns)
     else:
@@ -1129,8 +1130,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: 
     if out.numel() == 0:
         return out
     st = _launch(dev, _lib.lib().mi355_rotary, code, x.data_ptr(), out.data_ptr(), positions.data_ptr(),
-                 positions.dtype is torch.int64, plan.turns.data_ptr(), plan.amplitude, *sizes, plan.dim, pst, xst,
-                 ost, plan.interleaved, inverse)
+                 positions.dtype is torch.int64, plan.turns.data_ptr(), plan.amplitude, sizes, strides,
+                 plan.interleaved, inverse)
     if st:
         _lib.check("mi355_rotary", st)
     return out
@@ -1177,6 +1178,8 @@ class PagedCache:
         _check_apart(self.k, self.v, self.k_scale, self.v_scale)
         _check_apart(self.v, self.k_scale, self.v_scale)
         _check_apart(self.k_scale, self.v_scale)
+        object.__setattr__(self, "spans", tuple(_bytes(t.shape, t.stride(), t.dtype)
+                                                for t in (self.k, self.v, self.k_scale, self.v_scale)))
 
 
 def paged_cache(pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> PagedCache:
@@ -1216,7 +1219,8 @@ class PagedBatch:
 
 @functools.lru_cache(maxsize=512)
 def _paged_views(cache_shape, table_shape, table_stride, most, ragged, names, dtypes, shapes, strides):
-    """(type code, sizes, stride arrays, workspace bytes) of a paged call's tensors (names: those it has), checked."""
+    """(type code, arrays of sizes and strides, workspace bytes, bytes of each tensor, whether there is nothing to do,
+    whether the last two have the same strides) of a paged call's tensors (names: those it has), checked."""
     if dtypes[0] not in _SIXTEEN_BIT:
         raise TypeError(f"{names[0]} must be fp16 or bf16, got {dtypes[0]}")
     if len(set(dtypes)) > 1:
@@ -1247,13 +1251,15 @@ def _paged_views(cache_shape, table_shape, table_stride, most, ragged, names, dt
                                    written=name in ("out", "q_out")))
     if names[-1] == "q":
         views.append((H * D, D))
+    sizes = _lib.i64_array((B, most, T, H, Hkv, D, pages, page, width, table_stride[0] if B > 1 else width))
     need = 0
     if "k" not in names:
-        need = _lib.lib().mi355_attn_paged_workspace_bytes(B, most, H, Hkv, D, page, width)
+        need = _lib.lib().mi355_attn_paged_workspace_bytes(sizes)
         if need < 0:
             _lib.check("mi355_attn_paged_workspace_bytes", need)
-    return (_lib.dtype_code(dtypes[0]), (B, most, T, H, Hkv, D, pages, page, width),
-            table_stride[0] if B > 1 else width, _Arrays(*views), need)
+    # bytes from each tensor's first element to behind its last, for the overlap checks
+    spans = tuple(_bytes(shape, st, dt) for shape, st, dt in zip(shapes, strides, dtypes))
+    return _lib.dtype_code(dtypes[0]), sizes, _lib.i64_array(sum(views, ())), need, spans, B * most * T == 0, views[-1] == views[-2]
 
 
 def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch,
@@ -1287,32 +1293,35 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: Pag
     if plan is not None and (plan.dim % 8 or plan.dim > D):
         raise ValueError(f"the plan rotates {plan.dim} elements: a multiple of 8, at most the head's {D}, is needed")
     tensors = (k, v) if q is None else (k, v, q) if q_out is None else (k, v, q, q_out)
-    code, sizes, row, strides, _ = _paged_views(
+    code, sizes, strides, _, spans, empty, alike = _paged_views(
         cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
         ("k", "v", "q", "q_out")[:len(tensors)], tuple([t.dtype for t in tensors]), tuple([t.shape for t in tensors]),
         tuple([t.stride() for t in tensors]))
     given = q_out is not None
-    if given:
-        if q_out.data_ptr() == q.data_ptr() and strides[2][:] == strides[3][:]:
-            _check_apart(q_out, k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
-        else:
-            _check_apart(q_out, q, k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
-    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
-        _check_apart(t, k, v, q, batch.table, batch.lens, batch.offsets)
-    B, most, T = sizes[:3]
     if q is not None and not given:
-        q_out = q.new_empty(q.shape) if B * most else q.new_zeros(q.shape)
-    if B * most == 0 or T == 0:
+        q_out = q.new_zeros(q.shape) if empty else q.new_empty(q.shape)
+    if empty:
         return q_out
-    kp, vp, qp, op = k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr(), 0 if q is None else q_out.data_ptr()
+    held = (cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr())
+    at = [t.data_ptr() for t in tensors]
+    for start, size in zip(at, spans):
+        for begin, length in zip(held, cache.spans):
+            if start < begin + length and begin < start + size:
+                raise ValueError("k, v or q shares memory with the cache")
+    if given:
+        _check_apart(q_out, k, v, batch.table, batch.lens, batch.offsets)
+        if at[2] != at[3] or not alike:
+            _check_apart(q_out, q)
+    kp, vp, qp, op = at[0], at[1], 0 if q is None else at[2], 0 if q is None else q_out.data_ptr()
     if (kp | vp | qp | op) & 15:
         _check_aligned(k=kp, v=vp, q=qp, q_out=op)
-    st = _launch(dev, _lib.lib().mi355_paged_append, code, kp, vp, qp, op, cache.k.data_ptr(), cache.v.data_ptr(),
-                 cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), batch.table.data_ptr(), row, batch.lens.data_ptr(),
-                 0 if batch.offsets is None else batch.offsets.data_ptr(), *sizes, strides[0], strides[1],
-                 strides[2] if qp else None, strides[3] if qp else None, 0 if plan is None else plan.turns.data_ptr(),
-                 0 if plan is None else plan.dim, plan is not None and plan.interleaved,
-                 1.0 if plan is None else plan.amplitude, not given)
+    if plan is None:
+        st = _launch(dev, _lib.lib().mi355_paged_append, code, kp, vp, qp, op, *held, batch.table.data_ptr(), batch.lens.data_ptr(),
+                     0 if batch.offsets is None else batch.offsets.data_ptr(), sizes, strides, 0, 0, False, 1.0, False)
+    else:
+        st = _launch(dev, _lib.lib().mi355_paged_append, code, kp, vp, qp, op, *held, batch.table.data_ptr(), batch.lens.data_ptr(),
+                     0 if batch.offsets is None else batch.offsets.data_ptr(), sizes, strides, plan.turns.data_ptr(),
+                     plan.dim, plan.interleaved, plan.amplitude, not given)
     if st:
         _lib.check("mi355_paged_append", st)
     return q_out
@@ -1338,25 +1347,24 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale
         _no_backward(q, out)
     if forward_ad._current_level >= 0:
         _no_tangent(q, out)
-    code, sizes, row, (qst, ost), need = _paged_views(
+    code, sizes, strides, need, _, empty, _ = _paged_views(
         cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
         ("q", "out") if given else ("q",), (q.dtype, out.dtype) if given else (q.dtype,),
         (q.shape, out.shape) if given else (q.shape,), (q.stride(), out.stride()) if given else (q.stride(),))
-    scale = _scale(scale, sizes[5])
-    B, most, T = sizes[:3]
+    scale = _scale(scale, cache.k.shape[3])
     if given:
         _check_apart(out, q, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
     else:
-        out = q.new_empty(q.shape) if B * most else q.new_zeros(q.shape)
-    if B * most == 0 or T == 0:
+        out = q.new_zeros(q.shape) if empty else q.new_empty(q.shape)
+    if empty:
         return out
     qp, op = q.data_ptr(), out.data_ptr()
     if qp & 15 or op & 7:
         _check_aligned(q=qp, out=op)
     ws = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
     st = _launch(dev, _lib.lib().mi355_attn_paged, code, qp, cache.k.data_ptr(), cache.v.data_ptr(),
-                 cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), batch.table.data_ptr(), row, batch.lens.data_ptr(),
-                 0 if batch.offsets is None else batch.offsets.data_ptr(), op, *sizes, qst, ost, scale, not given,
+                 cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), batch.table.data_ptr(), batch.lens.data_ptr(),
+                 0 if batch.offsets is None else batch.offsets.data_ptr(), op, sizes, strides, scale, not given,
                  ws.data_ptr() if need else 0, need)
     if st:
         _lib.check("mi355_attn_paged", st)
