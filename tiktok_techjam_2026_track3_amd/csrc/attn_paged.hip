@@ -18,6 +18,7 @@
 // Work is dealt out evenly: the units of 32 keys of all (sequence, K/V head, tile of rows), in this order, are cut into
 // as many equal runs as there are work-groups. A work-group's first and last job may be parts of one; those leave partial
 // results, and a second launch joins them. So lengths that differ, and one long sequence, fill the GPU alike.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.h"
@@ -163,7 +164,7 @@ MI355_DEVINL int64_t wave_sum(int64_t v) {
 }
 
 // Work-groups that a CU's registers hold.
-constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : many || nr > 1 ? 2 : 3; }
+constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : dw == 1 ? 5 - nr : many || nr > 1 ? 2 : 3; }
 
 // DW: dwords that a lane has of a V row, head_dim / 64 rounded up to 1, 2, 3 or 4 (dims behind head_dim are loaded from
 // its start: Q is 0 there, and those output rows are not stored). NR: groups of 16 rows of a wave.
@@ -688,52 +689,76 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
   if (threadIdx.x == 0) p.joins[w] = head;
 }
 
-// Joins the parts of the jobs that several work-groups had: (work-group with a first part, row) to a work-group. Its four
-// waves take every fourth part; lanes have runs of four dims.
-template <typename T>
+// Joins the parts of the jobs that several work-groups had: a work-group with a first part (blockIdx.x) and a row of its
+// job's tile, or WAVES = 1 four rows. A row's waves take every WAVES-th part, eight requested at a time; lanes have runs
+// of four dims. Few rows have many parts, tiles of many rows few.
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_tile) {
-  __shared__ float lds[4][256];
+  __shared__ float lds[WAVES][256];
   __shared__ float lds_ml[4][2];
-  const int w = blockIdx.x, in_tile = blockIdx.y, hd = p.cache.head_dim, G = p.G;
+  constexpr int AHEAD = 8;
+  const int w = blockIdx.x, hd = p.cache.head_dim, G = p.G;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int in_tile = WAVES == 1 ? blockIdx.y * 4 + wave : blockIdx.y;
   const Head j = p.joins[w];
   if (j.parts == 0) return;
   const Rows rows = rows_of(p, j.b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = j.tile * rows_of_tile + in_tile;
-  if (r >= rows.nrows) return;
+  const int r = j.tile * rows_of_tile + in_tile, r_loaded = r < rows.nrows && in_tile < rows_of_tile ? in_tile : 0;
   // part 0: the work-group's last job; part k: the first one of the k-th after it
   const auto slot = [&](int k) MI355_LAMBDA_INLINE {
     const int64_t s = k == 0 ? 2 * static_cast<int64_t>(w) + 1 : 2 * (static_cast<int64_t>(w) + k);
-    return s * rows_of_tile + in_tile;
+    return s * rows_of_tile + r_loaded;
   };
-  const int parts = j.parts < p.groups - w ? j.parts : p.groups - 1 - w;
+  const int parts = (j.parts < p.groups - w ? j.parts : p.groups - 1 - w) + 1;
   float m = NEG_INF;
-  for (int k = threadIdx.x; k <= parts; k += 256) m = fmaxf(m, p.ml[2 * slot(k)]);
+  for (int k = WAVES == 1 ? lane : static_cast<int>(threadIdx.x); k < parts; k += 64 * WAVES) m = fmaxf(m, p.ml[2 * slot(k)]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  if (lane == 0) lds_ml[wave][0] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(lds_ml[0][0], lds_ml[1][0]), fmaxf(lds_ml[2][0], lds_ml[3][0]));
+  if constexpr (WAVES == 4) {
+    if (lane == 0) lds_ml[wave][0] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(lds_ml[0][0], lds_ml[1][0]), fmaxf(lds_ml[2][0], lds_ml[3][0]));
+  }
   const auto factor = [&](float t) MI355_LAMBDA_INLINE { return t == NEG_INF ? 1.0f : fast_exp2(t - m); };
   float z = 0.0f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int k = wave; k <= parts; k += 4) {
-    const int64_t at = slot(k);
-    const float f = factor(p.ml[2 * at]);
-    z += p.ml[2 * at + 1] * f;
-    if (4 * lane < hd) a += *reinterpret_cast<const f32x4*>(p.part + at * hd + 4 * lane) * f;
+  const int d4 = 4 * lane < hd ? 4 * lane : 0;
+  for (int k0 = WAVES == 1 ? 0 : wave; k0 < parts; k0 += WAVES * AHEAD) {
+    f32x4 v[AHEAD];
+    float top[AHEAD], sum[AHEAD];
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      const int64_t at = slot(k0 + WAVES * x < parts ? k0 + WAVES * x : k0);
+      v[x] = *reinterpret_cast<const f32x4*>(p.part + at * hd + d4);
+      top[x] = p.ml[2 * at];
+      sum[x] = p.ml[2 * at + 1];
+    }
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      if (k0 + WAVES * x >= parts) break;
+      const float f = factor(top[x]);
+      z += sum[x] * f;
+      a += v[x] * f;
+    }
   }
-  *reinterpret_cast<f32x4*>(&lds[wave][4 * lane]) = a;
-  if (lane == 0) lds_ml[wave][1] = z;
-  __syncthreads();
-  z = lds_ml[0][1] + lds_ml[1][1] + lds_ml[2][1] + lds_ml[3][1];
+  if constexpr (WAVES == 4) {
+    *reinterpret_cast<f32x4*>(&lds[wave][4 * lane]) = a;
+    if (lane == 0) lds_ml[wave][1] = z;
+    __syncthreads();
+    if (wave != 0) return;
+    z = lds_ml[0][1] + lds_ml[1][1] + lds_ml[2][1] + lds_ml[3][1];
+    a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a += *reinterpret_cast<const f32x4*>(&lds[k][4 * lane]);
+  }
+  if (r >= rows.nrows || in_tile >= rows_of_tile || 4 * lane >= hd) return;
   const int limit = rows.lim(r, G);
   float inv = z > 0.0f ? 1.0f / z : (z == 0.0f && limit == 0 ? 0.0f : __builtin_nanf(""));
   if (limit > rows.keys) inv = __builtin_nanf("");
-  const int t = r / G, d = threadIdx.x;
-  if (d < hd)
-    static_cast<T*>(p.o)[(rows.s.first + static_cast<int64_t>(t)) * p.ot + (j.h * G + r - t * G) * p.oh + d] =
-        from_f32<T>((lds[0][d] + lds[1][d] + lds[2][d] + lds[3][d]) * inv);
+  const int t = r / G;
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<V4*>(static_cast<T*>(p.o) + (rows.s.first + static_cast<int64_t>(t)) * p.ot + (j.h * G + r - t * G) * p.oh + 4 * lane) =
+      V4{from_f32<T>(a[0] * inv), from_f32<T>(a[1] * inv), from_f32<T>(a[2] * inv), from_f32<T>(a[3] * inv)};
 }
 
 // Largest room (in tokens) that one work-group walks alone, without a second launch.
@@ -765,7 +790,11 @@ template <typename T, int DW, int NR, bool MANY>
 int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
   attn_paged_kernel<T, DW, NR, MANY><<<static_cast<uint32_t>(l.grid), 256, 0, s>>>(p);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || l.groups == 0) return static_cast<int>(e);
-  attn_paged_join<T><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>(l.rows)), 256, 0, s>>>(p, l.rows);
+  const int64_t rows = std::min<int64_t>(l.rows, p.batch.most * static_cast<int64_t>(p.G));
+  if constexpr (MANY)
+    attn_paged_join<T, 1><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(p, l.rows);
+  else
+    attn_paged_join<T, 4><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>(rows)), 256, 0, s>>>(p, l.rows);
   return static_cast<int>(hipGetLastError());
 }
 

@@ -15,6 +15,7 @@
 namespace {
 
 using paged::BLOCK;
+constexpr int AHEAD = 4;  // rows of queries whose loads a thread has under way
 
 struct AppendArgs {
   paged::Cache cache;
@@ -76,7 +77,8 @@ MI355_DEVINL void load8(const T* row, int first, int second, float (&x)[8]) {
   }
 }
 
-// UNITS: units of 8 elements that a lane has at most, head_dim / 32 of a whole block.
+// UNITS: units of 8 elements that a lane has at most. A wave takes 64 / (head_dim / 8) rows of a head at a time (lanes that
+// are left over idle), so that a lane's unit of a row is the same in all of them.
 template <typename T, int UNITS, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   extern __shared__ float2 angles[];  // [16][rot / 2] of the new tokens
@@ -113,6 +115,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   int page = -1;
   if (block >= 0 && (base >> p.cache.page_shift) < p.batch.width) page = p.batch.table[b * p.batch.table_stride + (base >> p.cache.page_shift)];
   if (page >= 0 && page < p.cache.pages) {
+    const int per = 64 / hu, row0 = lane / hu, c = lane - row0 * hu;
     const int in_page = static_cast<int>(base & ((1 << p.cache.page_shift) - 1));
     for (int item = wave + 4 * slice; item < 2 * p.cache.kv_heads; item += 4 * p.slices) {
       const bool is_v = item >= p.cache.kv_heads;
@@ -126,12 +129,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
       const bool turn = !is_v && p.freqs != nullptr;
       const int rot = turn ? p.rot : 0;
       float x[UNITS][8], top = 0.0f;
+      int first, second;
+      runs_of<INTERLEAVED>(c, rot, first, second);
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
-        int first, second;
-        runs_of<INTERLEAVED>(c, rot, first, second);
-        if (t < nt) {
+        const int t = row0 + per * u;
+        if (row0 < per && t < nt) {
           load8(src + (token0 + t0 + t) * ts, first, second, x[u]);
         } else {
 #pragma unroll
@@ -140,8 +143,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
       }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
-        if (t < nt && c < rot / 8) rotate8<INTERLEAVED>(x[u], angles + t * half + 4 * c);
+        const int t = row0 + per * u;
+        if (c < rot / 8 && row0 < per && t < nt) rotate8<INTERLEAVED>(x[u], angles + t * half + 4 * c);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float m = __builtin_fabsf(x[u][e]);
@@ -169,10 +172,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
       }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int i = lane + 64 * u, t = i / hu, c = i - t * hu;
-        int first, second;
-        runs_of<INTERLEAVED>(c, rot, first, second);
-        if (t < nt) {
+        const int t = row0 + per * u;
+        if (row0 < per && t < nt) {
           float y[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {  // (an infinity to NaN: inf - inf)
@@ -190,17 +191,39 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
 
   if (p.q != nullptr) {
     typedef T V4 __attribute__((ext_vector_type(4)));
-    const int units = nt * p.heads * hu;
-    for (int i = tid + 256 * slice; i < units; i += 256 * p.slices) {
-      const int th = i / hu, c = i - th * hu, t = th / p.heads, h = th - t * p.heads;
-      int first, second;
-      runs_of<INTERLEAVED>(c, p.rot, first, second);
-      float x[8];
-      load8(static_cast<const T*>(p.q) + (token0 + t0 + t) * p.qt + h * p.qh, first, second, x);
-      if (c < p.rot / 8) rotate8<INTERLEAVED>(x, angles + t * half + 4 * c);
-      T* row = static_cast<T*>(p.qo) + (token0 + t0 + t) * p.ot + h * p.oh;
-      *reinterpret_cast<V4*>(row + first) = V4{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
-      *reinterpret_cast<V4*>(row + second) = V4{from_f32<T>(x[4]), from_f32<T>(x[5]), from_f32<T>(x[6]), from_f32<T>(x[7])};
+    const int per = 256 / hu, row0 = tid / hu, c = tid - row0 * hu;
+    if (row0 >= per) return;
+    int first, second;
+    runs_of<INTERLEAVED>(c, p.rot, first, second);
+    const bool turn = c < p.rot / 8;
+    // rows (token, head) of the block's new tokens, heads fastest: AHEAD of them under way
+    const int rows = nt * p.heads, step = per * p.slices;
+    for (int row = row0 + per * slice; row < rows; row += AHEAD * step) {
+      V4 a[AHEAD], b4[AHEAD];
+      int t[AHEAD], h[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = row + k * step < rows ? row + k * step : row;
+        t[k] = r / p.heads;
+        h[k] = r - t[k] * p.heads;
+        const T* src = static_cast<const T*>(p.q) + (token0 + t0 + t[k]) * p.qt + h[k] * p.qh;
+        a[k] = *reinterpret_cast<const V4*>(src + first);
+        b4[k] = *reinterpret_cast<const V4*>(src + second);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (row + k * step >= rows) break;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = to_f32(static_cast<T>(a[k][i]));
+          x[4 + i] = to_f32(static_cast<T>(b4[k][i]));
+        }
+        if (turn) rotate8<INTERLEAVED>(x, angles + t[k] * half + 4 * c);
+        T* dst = static_cast<T*>(p.qo) + (token0 + t0 + t[k]) * p.ot + h[k] * p.oh;
+        *reinterpret_cast<V4*>(dst + first) = V4{from_f32<T>(x[0]), from_f32<T>(x[1]), from_f32<T>(x[2]), from_f32<T>(x[3])};
+        *reinterpret_cast<V4*>(dst + second) = V4{from_f32<T>(x[4]), from_f32<T>(x[5]), from_f32<T>(x[6]), from_f32<T>(x[7])};
+      }
     }
   }
 }
@@ -271,7 +294,7 @@ extern "C" int mi355_paged_append(int dtype, const void* K, const void* V, const
   p.blocks = static_cast<int32_t>((z.most + 2 * BLOCK - 2) / BLOCK);
   // work-groups that share a block's heads: enough to have two a CU, no more than heads can use
   const int64_t groups = z.B * p.blocks;
-  const int64_t slices = (512 + groups - 1) / groups, useful = (2 * z.kv_heads + 3) / 4;
+  const int64_t slices = (8192 + groups - 1) / groups, useful = (2 * z.kv_heads + 3) / 4;
   p.slices = static_cast<int32_t>(slices < useful ? slices : useful);
   if (groups * p.slices >= (int64_t(1) << 23)) return MI355_E_BAD_SIZE;  // 2^31 threads
   const auto s = static_cast<hipStream_t>(stream);

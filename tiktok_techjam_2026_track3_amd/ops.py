@@ -1122,7 +1122,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: 
         x.dtype, x.shape, x.stride(), positions.dtype, positions.shape, positions.stride(),
         out.shape if given else None, out.stride() if given else None, plan.dim)
     if not given:
-        out = x.new_empty(x.shape)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.data_ptr() == x.data_ptr() and alike:
         _check_apart(out, positions, plan.turns)
     else:
@@ -1215,6 +1215,9 @@ class PagedBatch:
             raise ValueError(f"offsets must be a contiguous int32 tensor of shape ({B + 1},)")
         if not 0 <= operator.index(self.most) < 1 << 30 or B > 1 << 20:
             raise ValueError(f"most = {self.most} or {B} sequences are out of range")
+        for t in (self.lens, self.offsets):
+            if t is not None and t.get_device() != self.table.get_device():
+                raise ValueError("table, lens and offsets must be on one device")
 
 
 @functools.lru_cache(maxsize=512)
@@ -1275,39 +1278,46 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: Pag
     alone. Tokens without a page (a table entry out of range, a position behind the table) are not written. Each page
     that is written must be one sequence's. ``q_out`` may be ``q``; rows that no sequence has are left
     in a given ``q_out``, and zeros in a new one. No derivatives."""
-    dev = k.get_device()
-    if dev < 0 or v.get_device() != dev or cache.k.get_device() != dev or batch.table.get_device() != dev or (
-            batch.lens.get_device() != dev) or (batch.offsets is not None and batch.offsets.get_device() != dev) or (
+    dev, held_k, given = k.get_device(), cache.k, q_out is not None
+    if dev < 0 or v.get_device() != dev or held_k.get_device() != dev or batch.table.get_device() != dev or (
             plan is not None and plan.turns.get_device() != dev) or (q is not None and q.get_device() != dev) or (
-            q_out is not None and q_out.get_device() != dev):
-        _on_gpu(k, v, cache.k, batch.table, batch.lens, batch.offsets, None if plan is None else plan.turns, q, q_out)
+            given and q_out.get_device() != dev):
+        _on_gpu(k, v, held_k, batch.table, None if plan is None else plan.turns, q, q_out)
     if torch.is_grad_enabled():
         _no_backward(k, v, q, q_out)
     if forward_ad._current_level >= 0:
         _no_tangent(k, v, q, q_out)
-    if q is None and q_out is not None:
-        raise ValueError("q_out without q")
-    if q is not None and plan is None:
-        raise ValueError("q is given to be rotated, but no plan")
-    D = cache.k.shape[3]
-    if plan is not None and (plan.dim % 8 or plan.dim > D):
-        raise ValueError(f"the plan rotates {plan.dim} elements: a multiple of 8, at most the head's {D}, is needed")
-    tensors = (k, v) if q is None else (k, v, q) if q_out is None else (k, v, q, q_out)
+    if plan is None:
+        if q is not None or given:
+            raise ValueError("queries are given to be rotated, but no plan")
+    elif plan.dim % 8 or plan.dim > held_k.shape[3]:
+        raise ValueError(f"the plan rotates {plan.dim} elements: a multiple of 8, at most the head's {held_k.shape[3]}, is needed")
+    if q is None:
+        if given:
+            raise ValueError("q_out without q")
+        names, tensors = ("k", "v"), (k, v)
+        views = (k.dtype, v.dtype), (k.shape, v.shape), (k.stride(), v.stride())
+    elif not given:
+        names, tensors = ("k", "v", "q"), (k, v, q)
+        views = (k.dtype, v.dtype, q.dtype), (k.shape, v.shape, q.shape), (k.stride(), v.stride(), q.stride())
+    else:
+        names, tensors = ("k", "v", "q", "q_out"), (k, v, q, q_out)
+        views = ((k.dtype, v.dtype, q.dtype, q_out.dtype), (k.shape, v.shape, q.shape, q_out.shape),
+                 (k.stride(), v.stride(), q.stride(), q_out.stride()))
     code, sizes, strides, _, spans, empty, alike = _paged_views(
-        cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
-        ("k", "v", "q", "q_out")[:len(tensors)], tuple([t.dtype for t in tensors]), tuple([t.shape for t in tensors]),
-        tuple([t.stride() for t in tensors]))
-    given = q_out is not None
+        held_k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None, names, *views)
     if q is not None and not given:
-        q_out = q.new_zeros(q.shape) if empty else q.new_empty(q.shape)
+        q_out = q.new_zeros(q.shape) if empty else torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:
         return q_out
-    held = (cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr())
+    ck, cv, cks, cvs = held = (held_k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr())
+    nk, nv, nks, nvs = cache.spans
     at = [t.data_ptr() for t in tensors]
     for start, size in zip(at, spans):
-        for begin, length in zip(held, cache.spans):
-            if start < begin + length and begin < start + size:
-                raise ValueError("k, v or q shares memory with the cache")
+        end = start + size
+        if (start < ck + nk and ck < end) or (start < cv + nv and cv < end) or (start < cks + nks and cks < end) or (
+                start < cvs + nvs and cvs < end):
+            raise ValueError("k, v or q shares memory with the cache")
     if given:
         _check_apart(q_out, k, v, batch.table, batch.lens, batch.offsets)
         if at[2] != at[3] or not alike:
@@ -1340,9 +1350,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale
     inputs; rows that no sequence has are left in a given ``out``, and zeros in a new one. No derivatives."""
     dev = q.get_device()
     given = out is not None
-    if dev < 0 or cache.k.get_device() != dev or batch.table.get_device() != dev or batch.lens.get_device() != dev or (
-            batch.offsets is not None and batch.offsets.get_device() != dev) or (given and out.get_device() != dev):
-        _on_gpu(q, cache.k, batch.table, batch.lens, batch.offsets, out)
+    if dev < 0 or cache.k.get_device() != dev or batch.table.get_device() != dev or (given and out.get_device() != dev):
+        _on_gpu(q, cache.k, batch.table, out)
     if torch.is_grad_enabled() and (q.requires_grad or (given and out.requires_grad)):
         _no_backward(q, out)
     if forward_ad._current_level >= 0:
@@ -1355,7 +1364,7 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale
     if given:
         _check_apart(out, q, cache.k, cache.v, cache.k_scale, cache.v_scale, batch.table, batch.lens, batch.offsets)
     else:
-        out = q.new_zeros(q.shape) if empty else q.new_empty(q.shape)
+        out = q.new_zeros(q.shape) if empty else torch.empty_like(q, memory_format=torch.contiguous_format)
     if empty:
         return out
     qp, op = q.data_ptr(), out.data_ptr()
