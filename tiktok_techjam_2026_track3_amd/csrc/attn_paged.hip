@@ -59,11 +59,15 @@ struct PagedArgs {
 
 MI355_DEVINL f32x4 mma32(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 MI355_DEVINL f32x4 mma32(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// IEEE maximum (NaN-propagating): gfx950 v_maximum3_f32, no operand canonicalisation needed
+MI355_DEVINL float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 MI355_DEVINL float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 // reductions over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a row
 MI355_DEVINL float row_max(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return pair_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  v = vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return vmax(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 MI355_DEVINL float row_sum(float v) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -109,8 +113,9 @@ MI355_DEVINL void run_of(uint32_t (&v)[DW], __amdgpu_buffer_rsrc_t src, uint32_t
   }
 }
 
-// 0x80 in each byte of w that is a NaN
+// 0x80 in each byte of w that is a NaN, and w with zeros for those
 MI355_DEVINL uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+MI355_DEVINL uint32_t without(uint32_t w, uint32_t nans) { return w & ~((nans >> 7) * 0xffu); }
 
 MI355_DEVINL float lane_of(float v, int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)); }
 
@@ -128,10 +133,21 @@ struct Rows {
     const int64_t n = see0 + r / G;
     return static_cast<int>(n < 0 ? 0 : n);
   }
+  // keys that rows below `stop` see
+  MI355_DEVINL int sees(int stop, int G) const {
+    const int last = lim((stop < nrows ? stop : nrows) - 1, G);
+    return last < keys ? last : keys;
+  }
   // units of the tile that ends before row `stop`; one where it sees nothing, to write its zeros
   MI355_DEVINL int units(int stop, int G) const {
-    const int last = lim((stop < nrows ? stop : nrows) - 1, G), n = last < keys ? last : keys;
+    const int n = sees(stop, G);
     return n > 0 ? (n + UNIT - 1) / UNIT : 1;
+  }
+  // What a row's outputs are multiplied by. No key: zeros. Keys whose scores were all -inf, and a key that it sees
+  // behind the table's end: NaN.
+  MI355_DEVINL float inverse(float sum, int limit) const {
+    if (limit > keys) return __builtin_nanf("");
+    return sum > 0.0f ? 1.0f / sum : (sum == 0.0f && limit == 0 ? 0.0f : __builtin_nanf(""));
   }
 };
 
@@ -166,259 +182,101 @@ MI355_DEVINL int64_t wave_sum(int64_t v) {
 // Work-groups that a CU's registers hold.
 constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : dw == 1 ? 5 - nr : many || nr > 1 ? 2 : 3; }
 
+// A wave's rows: NR groups of 16, their queries, statistics and outputs.
 // DW: dwords that a lane has of a V row, head_dim / 64 rounded up to 1, 2, 3 or 4 (dims behind head_dim are loaded from
-// its start: Q is 0 there, and those output rows are not stored). NR: groups of 16 rows of a wave.
-// MANY = false, up to 16 NR rows: the four waves have the same rows and a quarter of the keys each, and are joined
-//   through LDS. K and V are waited for. A probability enters P·V as two bf16 terms, off by at most 2^-16 of it: free here.
-// MANY = true: each wave has 16 NR rows of its own, all walk over the same keys (which the CU's L1 holds for the four
-//   of them), and there is neither LDS nor a barrier. Probabilities are rounded to the type of q once.
-//   fp16: the scales of V are taken relative to the largest so far, so that a block's V fits the type; blocks down to
-//   2^-21 of that are exact.
-template <typename T, int DW, int NR, bool MANY>
-struct Kernel {
-  using TP = std::conditional_t<MANY, T, __bf16>;  // type of P and V
+// its start: Q is 0 there, and those output rows are not stored).
+// TERMS: a probability enters P·V as that many. Two bf16 terms, off by at most 2^-16 of it, where K and V are waited for
+// and they cost nothing; where rows are many enough to be matrix work, one of the type of q.
+template <typename T, int DW, int NR, int TERMS>
+struct Tile {
+  using TP = std::conditional_t<TERMS == 1, T, __bf16>;  // type of P and V
   using frag = typename Mfma<T>::frag;
   using pfrag = typename Mfma<TP>::frag;
-  static constexpr int DP = 64 * DW, ME = 4 * DW, ROWS = 16 * NR * (MANY ? 4 : 1);
-  static constexpr int KS = 2 * DW;  // MFMAs of S^T, 32 dims each
-  static constexpr bool RELATIVE = MANY && __is_same(T, _Float16);
+  static constexpr int KS = 2 * DW, ME = 4 * DW;  // MFMAs of S^T (32 dims each) and of O^T (16) for a group
   typedef T V4 __attribute__((ext_vector_type(4)));
 
-  struct Lds {
-    float o[2][16 * NR * DP];
-    float ml[4][16 * NR][2];
-  };
+  frag qf[NR][KS];
+  int limit[NR];  // keys that the lane's rows see
+  f32x4 acc[NR][ME];
+  float top[NR], sum[NR];  // top: in log2 units
+  bool far;
 
-  // One job, or a part of one: units [u0, u1) of its tile's keys. slot < 0: the rows' outputs, otherwise partial results.
-  static MI355_DEVINL void run(const PagedArgs& p, Lds* lds, const Rows& rows, int b, int h, int tile, int u0, int u1,
-                               int64_t slot) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, l16 = lane & 15;
-    const int hd = p.cache.head_dim, G = p.G, kvh = p.cache.kv_heads, shift = p.cache.page_shift;
-    const int row0 = tile * ROWS + (MANY ? wave * 16 * NR : 0), nrows = rows.nrows;
-
-    int k0 = u0 * UNIT, k1, fewest;
-    if (MANY && row0 >= nrows) return;
-    {
-      const int last = row0 + 16 * NR < nrows ? row0 + 16 * NR - 1 : nrows - 1;
-      const int sees = rows.lim(last, G) < rows.keys ? rows.lim(last, G) : rows.keys;
-      k1 = u1 * UNIT < sees ? u1 * UNIT : sees;
-      if (!MANY) {  // the wave's quarter
-        const int each = (u1 - u0 + 3) / 4 * UNIT;
-        k0 += wave * each;
-        k1 = k0 + each < k1 ? k0 + each : k1;
-      }
-      fewest = rows.lim(row0, G);
-    }
-    k0 = __builtin_amdgcn_readfirstlane(k0);
-    k1 = __builtin_amdgcn_readfirstlane(k1);
-    fewest = __builtin_amdgcn_readfirstlane(fewest < k1 ? fewest : k1);
-
-    frag qf[NR][KS];
-    int limit[NR];
+  MI355_DEVINL void start(const PagedArgs& p, const Rows& rows, int h, int row0, int lane) {
+    const int l16 = lane & 15, g = lane >> 4, hd = p.cache.head_dim;
+    far = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int r = row0 + 16 * n + l16 < nrows ? row0 + 16 * n + l16 : nrows - 1;
-      limit[n] = rows.lim(r, G);
-      const int t = r / G;
-      const T* src = static_cast<const T*>(p.q) + (rows.s.first + static_cast<int64_t>(t)) * p.qt + (h * G + r - t * G) * p.qh;
+      const int r = row0 + 16 * n + l16 < rows.nrows ? row0 + 16 * n + l16 : rows.nrows - 1;
+      limit[n] = rows.lim(r, p.G);
+      const int t = r / p.G;
+      const T* src = static_cast<const T*>(p.q) + (rows.s.first + static_cast<int64_t>(t)) * p.qt + (h * p.G + r - t * p.G) * p.qh;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int d = 64 * (k >> 1) + 16 * g + 8 * (k & 1);
         const u32x4 v = *reinterpret_cast<const u32x4*>(src + (d < hd ? d : 0));
         qf[n][k] = __builtin_bit_cast(frag, d < hd ? v : u32x4{0u, 0u, 0u, 0u});
       }
-    }
-
-    f32x4 acc[NR][ME];
-    float top[NR], sum[NR];  // top: in log2 units
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
       top[n] = NEG_INF;
       sum[n] = 0.0f;
 #pragma unroll
       for (int e = 0; e < ME; ++e) acc[n][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float c2 = p.scale * LOG2E;
-    bool far = false;
-    float v_top = 0.0f;  // RELATIVE: the largest V scale so far
+  }
 
-    // offsets within a block of 16 keys
-    uint32_t k_at[DW], v_at[4];
-#pragma unroll
-    for (int c = 0; c < DW; ++c) k_at[c] = l16 * hd + (64 * c + 16 * g < hd ? 64 * c + 16 * g : 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * hd + (l16 * 4 * DW < hd ? l16 * 4 * DW : 0);
+  // 16 bytes of K as the operands of MFMAs 2 c and 2 c + 1
+  static MI355_DEVINL u32x4 k_operand(uint32_t x, uint32_t y) {
+    return u32x4{two_of<T, false>(x, 1.0f), two_of<T, true>(x, 1.0f), two_of<T, false>(y, 1.0f), two_of<T, true>(y, 1.0f)};
+  }
 
-    // lane l knows block l of a window of 64, in order of position: its page, and the factors of its scores (in log2
-    // units) and V (a page that does not exist: NaN for the rows that see its keys, and page 0 is read in its place)
-    int page = 0, from = k0;
-    float kf = 0.0f, vf = 0.0f;
-    const auto window = [&](int at0) MI355_LAMBDA_INLINE {
-      from = at0;
-      const int at = from + lane * BLOCK;
-      page = 0;
-      kf = vf = 0.0f;
-      if (at < k1) {
-        const int id = p.batch.table[b * p.batch.table_stride + (at >> shift)];
-        const bool ok = id >= 0 && id < p.cache.pages;
-        page = ok ? id : 0;
-        const int64_t si = ((static_cast<int64_t>(page) * kvh + h) << (shift - 4)) + ((at & ((1 << shift) - 1)) >> 4);
-        kf = ok ? p.cache.ks[si] * c2 : __builtin_nanf("");
-        vf = ok ? p.cache.vs[si] : 0.0f;
-      }
-    };
+  // Row n's lane sees key `at` + 16 (r / 4) + 4 g + r % 4 of a unit where that offset less 4 g is below this.
+  MI355_DEVINL int seen_below(int n, int at, int k1, int g) const { return (limit[n] < k1 ? limit[n] : k1) - at - 4 * g; }
 
-    struct KUnit {
-      u32x4 v[2][DW];
-      float a[2];
-    };
-    struct VUnit {
-      uint32_t v[2][4][DW];
-      float s[2];
-    };
-    const auto block_at = [&](int at, int l) MI355_LAMBDA_INLINE {  // byte offset of the block at key `at`, lane l's
-      const int id = __builtin_amdgcn_readlane(page, l);
-      return (((static_cast<int64_t>(id) * kvh + h) << shift) + (at & ((1 << shift) - 1))) * hd;
-    };
-    const auto load_k = [&](KUnit& u, int at) MI355_LAMBDA_INLINE {
-      const int l = (at - from) >> 4;
+  // Scores of a unit that some row does not see whole: scaled, -inf where not seen.
+  MI355_DEVINL void mask(f32x4 (&sc)[NR][2], float (&a)[2], int at, int k1, int g) const {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const auto src = raw_rsrc(uniform_ptr(p.cache.k + block_at(at + BLOCK * t, l + t)), BLOCK * hd);
+    for (int n = 0; n < NR; ++n) {
+      const int stop = seen_below(n, at, k1, g);
 #pragma unroll
-        for (int c = 0; c < DW; ++c) u.v[t][c] = __builtin_amdgcn_raw_buffer_load_b128(src, k_at[c], 0, 0);
-        u.a[t] = lane_of(kf, l + t);
-      }
-    };
-    const auto load_v = [&](VUnit& u, int at) MI355_LAMBDA_INLINE {
-      const int l = (at - from) >> 4;
+      for (int r = 0; r < 8; ++r)
+        sc[n][r >> 2][r & 3] = BLOCK * (r >> 2) + (r & 3) < stop ? sc[n][r >> 2][r & 3] * a[r >> 2] : NEG_INF;
+    }
+    a[0] = a[1] = 1.0f;
+  }
+
+  // Probabilities of a unit from its scores (a: their factors, in log2 units), and what they do to the statistics.
+  MI355_DEVINL void softmax(const f32x4 (&sc)[NR][2], const float (&a)[2], pfrag (&hi)[NR], pfrag (&lo)[NR]) {
+    float most[NR];
+    bool moves = false;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const auto src = raw_rsrc(uniform_ptr(p.cache.v + block_at(at + BLOCK * t, l + t)), BLOCK * hd);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) run_of<DW>(u.v[t][i], src, v_at[i]);
-        u.s[t] = lane_of(vf, l + t);
-      }
-    };
-    const auto scores = [&](f32x4 (&sc)[NR][2], const KUnit& u) MI355_LAMBDA_INLINE {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) sc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < DW; ++c)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t x = u.v[t][c][2 * half], y = u.v[t][c][2 * half + 1];
-            const u32x4 k = {two_of<T, false>(x, 1.0f), two_of<T, true>(x, 1.0f), two_of<T, false>(y, 1.0f), two_of<T, true>(y, 1.0f)};
-#pragma unroll
-            for (int n = 0; n < NR; ++n) sc[n][t] = mma32(__builtin_bit_cast(frag, k), qf[n][2 * c + half], sc[n][t]);
-          }
-      }
-    };
-    const auto pairs_of = [&](const uint32_t (&a)[2][4][DW], int c, int half, int k) MI355_LAMBDA_INLINE {
-      return __builtin_amdgcn_perm(a[k >> 1][(k & 1) * 2 + 1][c], a[k >> 1][(k & 1) * 2][c], half ? 0x07030602u : 0x05010400u);
-    };
-    // The rest of a unit's work, from its scores: keys at .. at + 31.
-    const auto finish = [&](f32x4 (&sc)[NR][2], float (&a)[2], VUnit& u, int at) MI355_LAMBDA_INLINE {
-      if (at + UNIT > fewest) {
-        // Some row does not see all of the keys. Scores that it does not see: -inf. V that no row sees: zeros.
-        // NaN in V that only some rows see: the outputs that they reach (a row that sees a NaN in a dim: counted by
-        // MFMAs) become NaN here, and the NaN zeros.
-        const int stop0 = k1 - at - 4 * g;
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          const int stop = (limit[n] < k1 ? limit[n] : k1) - at - 4 * g;
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            sc[n][r >> 2][r & 3] = BLOCK * (r >> 2) + (r & 3) < stop ? sc[n][r >> 2][r & 3] * a[r >> 2] : NEG_INF;
-        }
-        a[0] = a[1] = 1.0f;
-        uint32_t any = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < DW; ++c) {
-              u.v[t][i][c] = BLOCK * t + i < stop0 ? u.v[t][i][c] : 0u;
-              any |= nan_bytes(u.v[t][i][c]);
-            }
-        if (__ballot(any != 0)) {
-          const uint32_t unit = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<TP>(1.0f)));
-          uint32_t is_nan[2][4][DW];
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int c = 0; c < DW; ++c) {
-                is_nan[t][i][c] = nan_bytes(u.v[t][i][c]);
-                u.v[t][i][c] &= ~((is_nan[t][i][c] >> 7) * 0xffu);
-              }
-#pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            const int stop = (limit[n] < k1 ? limit[n] : k1) - at - 4 * g;
-            pfrag seen;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) seen[r] = static_cast<TP>(BLOCK * (r >> 2) + (r & 3) < stop ? 1.0f : 0.0f);
-#pragma unroll
-            for (int c = 0; c < DW; ++c)
-#pragma unroll
-              for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                  u32x4 one;
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    const uint32_t w2 = pairs_of(is_nan, c, half, k) >> (16 * odd);
-                    one[k] = ((w2 >> 7) & 1) * unit | ((w2 >> 15) & 1) * (unit << 16);
-                  }
-                  const f32x4 hits = mma32(__builtin_bit_cast(pfrag, one), seen, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    if (hits[i] > 0.0f) acc[n][4 * c + 2 * half + odd][i] = __builtin_nanf("");
-                }
-          }
-        }
-      }
-      float most[NR];
-      bool moves = false;
+    for (int n = 0; n < NR; ++n) {
+      const auto four = [&](const f32x4& x) MI355_LAMBDA_INLINE { return vmax(vmax(vmax(x[0], x[1]), x[2]), x[3]); };
+      most[n] = vmax(four(sc[n][0]) * a[0], four(sc[n][1]) * a[1]);
+      moves = moves || most[n] > top[n] + SLACK;
+    }
+    if (__ballot(moves)) {
+      bool beyond = false;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const auto four = [&](const f32x4& x) MI355_LAMBDA_INLINE { return fmaxf(fmaxf(fmaxf(x[0], x[1]), x[2]), x[3]); };
-        most[n] = fmaxf(four(sc[n][0]) * a[0], four(sc[n][1]) * a[1]);
-        moves = moves || most[n] > top[n] + SLACK;
-      }
-      if (__ballot(moves)) {
-        bool beyond = false;
+        const float now = vmax(top[n], row_max(most[n]));
+        const float keep = top[n] == NEG_INF ? 0.0f : fast_exp2(top[n] - now);
+        top[n] = now;
+        beyond = beyond || __builtin_fabsf(now) >= FAR;  // (rows that have seen nothing take that way too)
+        sum[n] *= keep;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          const float now = fmaxf(top[n], row_max(most[n]));
-          const float keep = top[n] == NEG_INF ? 0.0f : fast_exp2(top[n] - now);
-          top[n] = now;
-          beyond = beyond || __builtin_fabsf(now) >= FAR;  // (rows that have seen nothing take that way too)
-          sum[n] *= keep;
-#pragma unroll
-          for (int e = 0; e < ME; ++e) acc[n][e] *= keep;
-        }
-        far = __ballot(beyond) != 0;
+        for (int e = 0; e < ME; ++e) acc[n][e] *= keep;
       }
-      pfrag hi[NR], lo[NR];
+      far = __ballot(beyond) != 0;
+    }
+    const auto rest = [&](auto rounded) MI355_LAMBDA_INLINE {
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const float ref = top[n] == NEG_INF ? 0.0f : top[n];
         float e[8];
-        if (far) {
 #pragma unroll
-          for (int r = 0; r < 8; ++r) e[r] = fast_exp2(sc[n][r >> 2][r & 3] * a[r >> 2] - ref);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) e[r] = fast_exp2(__builtin_fmaf(sc[n][r >> 2][r & 3], a[r >> 2], -ref));
-        }
-        if constexpr (MANY) {
+        for (int r = 0; r < 8; ++r)
+          e[r] = fast_exp2(decltype(rounded)::value ? sc[n][r >> 2][r & 3] * a[r >> 2] - ref
+                                                    : __builtin_fmaf(sc[n][r >> 2][r & 3], a[r >> 2], -ref));
+        if constexpr (TERMS == 1) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) hi[n][r] = static_cast<TP>(e[r]);
           sum[n] = prob_sum(hi[n], sum[n]);
@@ -432,140 +290,62 @@ struct Kernel {
           }
         }
       }
-      float vs[2] = {u.s[0], u.s[1]};
-      if constexpr (RELATIVE) {
-        const float now = fmaxf(vs[0], vs[1]);
-        if (now > v_top) {
-          const float keep = v_top / now;
-          v_top = now;
-#pragma unroll
-          for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int e = 0; e < ME; ++e) acc[n][e] *= keep;
-        }
-        const float r = v_top > 0.0f ? 64.0f / v_top : 1.0f;
-        vs[0] *= r;
-        vs[1] *= r;
-      }
-#pragma unroll
-      for (int c = 0; c < DW; ++c)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          u32x4 even, odd;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t pr = pairs_of(u.v, c, half, k);
-            even[k] = two_of<TP, false>(pr, vs[k >> 1]);
-            odd[k] = two_of<TP, true>(pr, vs[k >> 1]);
-          }
-#pragma unroll
-          for (int n = 0; n < NR; ++n) {
-            f32x4& a0 = acc[n][4 * c + 2 * half];
-            f32x4& a1 = acc[n][4 * c + 2 * half + 1];
-            a0 = mma32(__builtin_bit_cast(pfrag, even), hi[n], a0);
-            a1 = mma32(__builtin_bit_cast(pfrag, odd), hi[n], a1);
-            if constexpr (!MANY) {
-              a0 = mma32(__builtin_bit_cast(pfrag, even), lo[n], a0);
-              a1 = mma32(__builtin_bit_cast(pfrag, odd), lo[n], a1);
-            }
-          }
-        }
     };
+    if (far)
+      rest(std::true_type{});
+    else
+      rest(std::false_type{});
+  }
 
-    // A unit's bytes are requested as soon as the registers of those before it are free. Loads of what lies behind the
-    // window's end are of its last unit again.
-    for (int w0 = k0; w0 < k1; w0 += 64 * BLOCK) {
-      window(w0);
-      const int stop = k1 < w0 + 64 * BLOCK ? k1 : w0 + 64 * BLOCK;
-      KUnit ku;
-      VUnit vu;
-      load_k(ku, w0);
-      load_v(vu, w0);
-      for (int at = w0; at < stop; at += UNIT) {
-        const int next = at + UNIT < stop ? at + UNIT : at;
-        f32x4 sc[NR][2];
-        scores(sc, ku);
-        float a[2] = {ku.a[0], ku.a[1]};
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(ku, next);
-        __builtin_amdgcn_sched_barrier(0);
-        finish(sc, a, vu, at);
-        __builtin_amdgcn_sched_barrier(0);
-        load_v(vu, next);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-
-    float all_top[NR], all_sum[NR];
+  // Outputs e: += V^T · P^T
+  MI355_DEVINL void add(int e, u32x4 v, const pfrag (&hi)[NR], const pfrag (&lo)[NR]) {
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      all_top[n] = top[n];
-      all_sum[n] = sum[n] = row_sum(sum[n]);
+      acc[n][e] = mma32(__builtin_bit_cast(pfrag, v), hi[n], acc[n][e]);
+      if constexpr (TERMS == 2) acc[n][e] = mma32(__builtin_bit_cast(pfrag, v), lo[n], acc[n][e]);
     }
-    if constexpr (RELATIVE) {
-      const float back = v_top > 0.0f ? v_top / 64.0f : 1.0f;
-#pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int e = 0; e < ME; ++e) acc[n][e] *= back;
-    }
-    if constexpr (!MANY) {
-      // the four waves' results: factors of a row from their maxima, then pairs of waves added up in LDS
-      if (g == 0)
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          lds->ml[wave][16 * n + l16][0] = top[n];
-          lds->ml[wave][16 * n + l16][1] = sum[n];
-        }
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        float m = NEG_INF;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m = fmaxf(m, lds->ml[k][16 * n + l16][0]);
-        const auto factor = [&](float t) MI355_LAMBDA_INLINE { return t == NEG_INF ? 1.0f : fast_exp2(t - m); };
-        float z = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z += lds->ml[k][16 * n + l16][1] * factor(lds->ml[k][16 * n + l16][0]);
-        all_top[n] = m;
-        all_sum[n] = z;
-        const float f = factor(top[n]);
-#pragma unroll
-        for (int e = 0; e < ME; ++e) acc[n][e] *= f;
-      }
-      const auto put = [&](float* dst) MI355_LAMBDA_INLINE {
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int e = 0; e < ME; ++e) *reinterpret_cast<f32x4*>(dst + ((n * ME + e) * 64 + lane) * 4) = acc[n][e];
-      };
-      const auto add = [&](const float* src) MI355_LAMBDA_INLINE {
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-#pragma unroll
-          for (int e = 0; e < ME; ++e) acc[n][e] += *reinterpret_cast<const f32x4*>(src + ((n * ME + e) * 64 + lane) * 4);
-      };
-      if (wave >= 2) put(lds->o[wave - 2]);
-      __syncthreads();
-      if (wave < 2) add(lds->o[wave]);
-      __syncthreads();
-      if (wave == 1) put(lds->o[0]);
-      __syncthreads();
-      if (wave == 0) add(lds->o[0]);
-      __syncthreads();  // (the next job's waves write there again)
-      if (wave != 0) return;
-    }
+  }
 
-    // lane (row l16, g) has dims 16 DW g + 4 DW i + e of its row
+  // Outputs e of a unit that some row does not see whole, whose V had NaN (zeros by now: 0 · NaN would be NaN in rows that
+  // do not see it): NaN where a row sees one. count: V^T with 1 for each. MFMAs count what a row sees.
+  MI355_DEVINL void inject(int e, u32x4 count, int at, int k1, int g) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      int stop = seen_below(n, at, k1, g);
+      asm volatile("" : "+v"(stop));  // (worked out here, not kept in registers for all e)
+      pfrag seen;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) seen[r] = static_cast<TP>(BLOCK * (r >> 2) + (r & 3) < stop ? 1.0f : 0.0f);
+      const f32x4 hits = mma32(__builtin_bit_cast(pfrag, count), seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][e][i] += hits[i] > 0.0f ? __builtin_nanf("") : 0.0f;
+    }
+  }
+  // V^T with 1 for each NaN, of outputs 2 x and 2 x + 1: from bytes of V with 0x80 for each, as `pair` puts them together
+  template <typename F>
+  static MI355_DEVINL void counts(F pair, u32x4& even, u32x4& odd) {
+    constexpr uint32_t one = __is_same(TP, _Float16) ? 0x3c00u : 0x3f80u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = pair(k);
+      even[k] = ((w >> 7) & 1) * one | ((w >> 15) & 1) * (one << 16);
+      odd[k] = ((w >> 23) & 1) * one | (w >> 31) * (one << 16);
+    }
+  }
+
+  // The rows' outputs, or with slot >= 0 partial results of a tile of `rows_of_tile` rows from `tile0` on. top and
+  // sum are the row's. Lane (row l16, g) has dims 16 DW g + 4 DW i + e of its row.
+  MI355_DEVINL void write(const PagedArgs& p, const Rows& rows, int h, int row0, int tile0, int rows_of_tile, int64_t slot, int lane) {
+    const int l16 = lane & 15, g = lane >> 4, hd = p.cache.head_dim;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = row0 + 16 * n + l16;
-      if (r >= nrows) continue;
+      if (r >= rows.nrows) continue;
       if (slot >= 0) {
-        const int64_t at = slot * ROWS + (r - tile * ROWS);
+        const int64_t at = slot * rows_of_tile + (r - tile0);
         if (g == 0) {
-          p.ml[2 * at] = all_top[n];
-          p.ml[2 * at + 1] = all_sum[n];
+          p.ml[2 * at] = top[n];
+          p.ml[2 * at + 1] = sum[n];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -577,11 +357,9 @@ struct Kernel {
                   f32x4{acc[n][4 * c][i], acc[n][4 * c + 1][i], acc[n][4 * c + 2][i], acc[n][4 * c + 3][i]};
         }
       } else {
-        // no key: zeros; keys whose scores were all -inf, and keys behind the table's end: NaN
-        float inv = all_sum[n] > 0.0f ? 1.0f / all_sum[n] : (all_sum[n] == 0.0f && limit[n] == 0 ? 0.0f : __builtin_nanf(""));
-        if (limit[n] > rows.keys) inv = __builtin_nanf("");
-        const int t = r / G;
-        T* dst = static_cast<T*>(p.o) + (rows.s.first + static_cast<int64_t>(t)) * p.ot + (h * G + r - t * G) * p.oh;
+        const float inv = rows.inverse(sum[n], limit[n]);
+        const int t = r / p.G;
+        T* dst = static_cast<T*>(p.o) + (rows.s.first + static_cast<int64_t>(t)) * p.ot + (h * p.G + r - t * p.G) * p.oh;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = 16 * DW * g + 4 * DW * i;
@@ -597,11 +375,450 @@ struct Kernel {
   }
 };
 
+// 64 blocks of a sequence's keys from `from` on, one to a lane: where it is in the pools, and the factors of its scores
+// (in log2 units) and V. A page that does not exist: NaN for the rows that see its keys, and page 0 is read in its place. Blocks
+// behind `stop`: likewise page 0, with zeros.
+struct Window {
+  int from;
+  uint32_t lo, hi;  // byte offset
+  float kf, vf;
+  MI355_DEVINL void fill(const PagedArgs& p, int b, int h, int at0, int stop, int lane) {
+    const int at = at0 + lane * BLOCK, shift = p.cache.page_shift;
+    from = at0;
+    int64_t row = 0;
+    kf = vf = 0.0f;
+    if (at < stop) {
+      const int id = p.batch.table[b * p.batch.table_stride + (at >> shift)];
+      const bool ok = id >= 0 && id < p.cache.pages;
+      row = ((static_cast<int64_t>(ok ? id : 0) * p.cache.kv_heads + h) << shift) + (at & ((1 << shift) - 1));
+      kf = ok ? p.cache.ks[row / BLOCK] * (p.scale * LOG2E) : __builtin_nanf("");
+      vf = ok ? p.cache.vs[row / BLOCK] : 0.0f;
+    }
+    row *= p.cache.head_dim;
+    lo = static_cast<uint32_t>(row);
+    hi = static_cast<uint32_t>(row >> 32);
+  }
+  MI355_DEVINL int64_t offset(int at) const {
+    const int l = (at - from) >> 4;
+    const uint64_t a = static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, l)), b = static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, l));
+    return static_cast<int64_t>(a | (b << 32));
+  }
+  // The block with key `at`, of K or V
+  MI355_DEVINL __amdgpu_buffer_rsrc_t block(const PagedArgs& p, const uint8_t* pool, int at) const {
+    return raw_rsrc(uniform_ptr(pool + offset(at)), BLOCK * p.cache.head_dim);
+  }
+  MI355_DEVINL float k_factor(int at) const { return lane_of(kf, (at - from) >> 4); }
+  MI355_DEVINL float v_factor(int at) const { return lane_of(vf, (at - from) >> 4); }
+};
+
+// Up to 16 NR rows: the four waves have the same rows and a quarter of the keys each, and are joined through LDS. K and V
+// are waited for; a unit's bytes are requested as soon as the registers of those before it are free.
+template <typename T, int DW, int NR>
+struct Few {
+  using Own = Tile<T, DW, NR, 2>;
+  using TP = typename Own::TP;
+  using pfrag = typename Own::pfrag;
+  static constexpr int ME = Own::ME, ROWS = 16 * NR;
+  struct Lds {
+    float o[2][16 * NR * 64 * DW];
+    float ml[4][16 * NR][2];
+  };
+
+  // One job, or a part of one: units [u0, u1) of its tile's keys. slot < 0: the rows' outputs, otherwise partial results.
+  static MI355_DEVINL void run(const PagedArgs& p, Lds& lds, const Rows& rows, int b, int h, int tile, int u0, int u1,
+                               int64_t slot) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, l16 = lane & 15, hd = p.cache.head_dim, row0 = tile * ROWS;
+    const int sees = rows.sees(row0 + ROWS, p.G), each = (u1 - u0 + 3) / 4 * UNIT;
+    int k1 = u1 * UNIT < sees ? u1 * UNIT : sees, k0 = u0 * UNIT + wave * each;
+    k1 = __builtin_amdgcn_readfirstlane(k0 + each < k1 ? k0 + each : k1);
+    k0 = __builtin_amdgcn_readfirstlane(k0);
+    const int first = rows.lim(row0, p.G), fewest = __builtin_amdgcn_readfirstlane(first < k1 ? first : k1);
+    Own own;
+    own.start(p, rows, h, row0, lane);
+
+    // offsets within a block of 16 keys
+    uint32_t k_at[DW], v_at[4];
+#pragma unroll
+    for (int c = 0; c < DW; ++c) k_at[c] = l16 * hd + (64 * c + 16 * g < hd ? 64 * c + 16 * g : 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * hd + (l16 * 4 * DW < hd ? l16 * 4 * DW : 0);
+    u32x4 ku[2][DW];
+    uint32_t vu[2][4][DW];
+    float ka[2], va[2];
+    Window win;
+    const auto load_k = [&](int at) MI355_LAMBDA_INLINE {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const auto src = win.block(p, p.cache.k, at + BLOCK * t);
+#pragma unroll
+        for (int c = 0; c < DW; ++c) ku[t][c] = __builtin_amdgcn_raw_buffer_load_b128(src, k_at[c], 0, 0);
+        ka[t] = win.k_factor(at + BLOCK * t);
+      }
+    };
+    const auto load_v = [&](int at) MI355_LAMBDA_INLINE {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const auto src = win.block(p, p.cache.v, at + BLOCK * t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) run_of<DW>(vu[t][i], src, v_at[i]);
+        va[t] = win.v_factor(at + BLOCK * t);
+      }
+    };
+    // byte pairs of two keys for outputs 4 c + 2 half and the next one
+    const auto pair_of = [&](const uint32_t (&v)[2][4][DW], int x, int k) MI355_LAMBDA_INLINE {
+      return __builtin_amdgcn_perm(v[k >> 1][(k & 1) * 2 + 1][x >> 1], v[k >> 1][(k & 1) * 2][x >> 1], x & 1 ? 0x07030602u : 0x05010400u);
+    };
+
+    for (int w0 = k0; w0 < k1; w0 += 64 * BLOCK) {
+      win.fill(p, b, h, w0, k1, lane);
+      const int stop = k1 < w0 + 64 * BLOCK ? k1 : w0 + 64 * BLOCK;
+      load_k(w0);
+      __builtin_amdgcn_sched_barrier(0);  // (K first, as in the loop: it waits for K, not for V)
+      load_v(w0);
+      __builtin_amdgcn_sched_barrier(0);
+      for (int at = w0; at < stop; at += UNIT) {
+        const int next = at + UNIT < stop ? at + UNIT : at;
+        f32x4 sc[NR][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n) sc[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2 * DW; ++k) {
+            const u32x4 x = Own::k_operand(ku[t][k >> 1][2 * (k & 1)], ku[t][k >> 1][2 * (k & 1) + 1]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) sc[n][t] = mma32(__builtin_bit_cast(typename Own::frag, x), own.qf[n][k], sc[n][t]);
+          }
+        }
+        float a[2] = {ka[0], ka[1]};
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (at + UNIT > fewest) {  // some row does not see all of the keys
+          own.mask(sc, a, at, k1, g);
+          uint32_t any = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int c = 0; c < DW; ++c) {
+                vu[t][i][c] = BLOCK * t + i < k1 - at - 4 * g ? vu[t][i][c] : 0u;
+                any |= nan_bytes(vu[t][i][c]);
+              }
+          if (__ballot(any != 0)) {
+            uint32_t nans[2][4][DW];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < DW; ++c) {
+                  nans[t][i][c] = nan_bytes(vu[t][i][c]);
+                  vu[t][i][c] = without(vu[t][i][c], nans[t][i][c]);
+                }
+#pragma unroll
+            for (int x = 0; x < 2 * DW; ++x) {
+              u32x4 even, odd;
+              Own::counts([&](int k) MI355_LAMBDA_INLINE { return pair_of(nans, x, k); }, even, odd);
+              own.inject(2 * x, even, at, k1, g);
+              own.inject(2 * x + 1, odd, at, k1, g);
+            }
+          }
+        }
+        pfrag hi[NR], lo[NR];
+        own.softmax(sc, a, hi, lo);
+#pragma unroll
+        for (int x = 0; x < 2 * DW; ++x) {
+          u32x4 even, odd;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t pr = pair_of(vu, x, k);
+            even[k] = two_of<TP, false>(pr, va[k >> 1]);
+            odd[k] = two_of<TP, true>(pr, va[k >> 1]);
+          }
+          own.add(2 * x, even, hi, lo);
+          own.add(2 * x + 1, odd, hi, lo);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+
+    // the four waves' results: factors of a row from their maxima, then pairs of waves added up in LDS
+#pragma unroll
+    for (int n = 0; n < NR; ++n) own.sum[n] = row_sum(own.sum[n]);
+    if (g == 0)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        lds.ml[wave][16 * n + l16][0] = own.top[n];
+        lds.ml[wave][16 * n + l16][1] = own.sum[n];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float m = NEG_INF;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = fmaxf(m, lds.ml[k][16 * n + l16][0]);
+      const auto factor = [&](float t) MI355_LAMBDA_INLINE { return t == NEG_INF ? 1.0f : fast_exp2(t - m); };
+      float z = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z += lds.ml[k][16 * n + l16][1] * factor(lds.ml[k][16 * n + l16][0]);
+      const float f = factor(own.top[n]);
+      own.top[n] = m;
+      own.sum[n] = z;
+#pragma unroll
+      for (int e = 0; e < ME; ++e) own.acc[n][e] *= f;
+    }
+    const auto put = [&](float* dst) MI355_LAMBDA_INLINE {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < ME; ++e) *reinterpret_cast<f32x4*>(dst + ((n * ME + e) * 64 + lane) * 4) = own.acc[n][e];
+    };
+    const auto add = [&](const float* src) MI355_LAMBDA_INLINE {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < ME; ++e) own.acc[n][e] += *reinterpret_cast<const f32x4*>(src + ((n * ME + e) * 64 + lane) * 4);
+    };
+    if (wave >= 2) put(lds.o[wave - 2]);
+    __syncthreads();
+    if (wave < 2) add(lds.o[wave]);
+    __syncthreads();
+    if (wave == 1) put(lds.o[0]);
+    __syncthreads();
+    if (wave == 0) add(lds.o[0]);
+    __syncthreads();  // (the next job's waves write there again)
+    if (wave == 0) own.write(p, rows, h, row0, row0, ROWS, slot, lane);
+  }
+};
+
+template <int N, typename F>
+MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
+  if constexpr (N > 0) {
+    for_each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
+// More rows: each wave has 16 NR of its own. A unit's K and V are converted once for the four of them, a quarter by
+// each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
+// buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit.
+// fp16: V's scales are taken relative to the largest so far, so that a block's V fits the type; blocks down to
+// 2^-21 of that are exact.
+template <typename T, int DW, int NR>
+struct Many {
+  using Own = Tile<T, DW, NR, 1>;
+  using pfrag = typename Own::pfrag;
+  static constexpr int ME = Own::ME, ROWS = 64 * NR;
+  static constexpr bool RELATIVE = __is_same(T, _Float16);
+  struct Lds {
+    u32x4 k[2][4 * DW][64];  // [buffer][MFMA of S^T: (tile of 16 keys, 32 dims)][lane]
+    u32x4 v[2][4 * DW][64];  // [buffer][output e][lane]
+    u32x4 nans[2][4 * DW][64];  // 1 for each NaN of V, where flag says that a wave found one
+    int flag[2][4];
+  };
+  // A wave's part of a unit: of its 2 DW pieces of K (16 keys, 64 dims) and 2 DW of V (two outputs) those with number
+  // wave + 4 s, as bytes.
+  struct Stage {
+    uint32_t r[DW][8];
+    float vs[2];
+  };
+
+  static MI355_DEVINL void run(const PagedArgs& p, Lds& lds, const Rows& rows, int b, int h, int tile, int u0, int u1,
+                               int64_t slot) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, l16 = lane & 15, hd = p.cache.head_dim, row0 = tile * ROWS + wave * 16 * NR;
+    const bool active = row0 < rows.nrows;
+    const int all = rows.sees(tile * ROWS + ROWS, p.G), k0 = u0 * UNIT;
+    const int stop = __builtin_amdgcn_readfirstlane(u1 * UNIT < all ? u1 * UNIT : all);  // keys that any row sees
+    const int mine = active ? rows.sees(row0 + 16 * NR, p.G) : 0, first = rows.lim(tile * ROWS, p.G);
+    const int k1 = __builtin_amdgcn_readfirstlane(mine < stop ? mine : stop);        // ... that the wave's rows see
+    const int all_see = __builtin_amdgcn_readfirstlane(first < stop ? first : stop);  // ... that all rows see
+    Own own;
+    if (active) own.start(p, rows, h, row0, lane);
+
+    Window win, ahead;  // blocks of the units worked on, and those after them
+    // whether slot s of a wave is a piece of K: for all waves, none, or the first 2 DW - 4 s
+    const auto is_k = [&](auto s) MI355_LAMBDA_INLINE {
+      constexpr int left = 2 * DW - 4 * decltype(s)::value;
+      return left >= 4 ? true : left <= 0 ? false : wave < left;
+    };
+    const auto load = [&](Stage& st, int at) MI355_LAMBDA_INLINE {
+      const bool now = at - win.from < 64 * BLOCK;
+      Window w;
+      w.from = now ? win.from : ahead.from;
+      w.lo = now ? win.lo : ahead.lo;
+      w.hi = now ? win.hi : ahead.hi;
+      w.vf = now ? win.vf : ahead.vf;
+      for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
+        constexpr int S = decltype(s)::value;
+        const int piece = wave + 4 * S;
+        if (is_k(s)) {
+          const int t = piece / DW, c = piece - t * DW;
+          const auto src = w.block(p, p.cache.k, at + BLOCK * t);
+          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(src, l16 * hd + (64 * c + 16 * g < hd ? 64 * c + 16 * g : 0), 0, 0);
+          st.r[S][0] = x[0], st.r[S][1] = x[1], st.r[S][2] = x[2], st.r[S][3] = x[3];
+        } else {
+          const uint32_t run = (l16 * 4 * DW < hd ? l16 * 4 * DW : 0) + 4 * ((piece - 2 * DW) >> 1);
+          for_each<8>([&](auto i) MI355_LAMBDA_INLINE {
+            constexpr int I = decltype(i)::value;
+            st.r[S][I] = __builtin_amdgcn_raw_buffer_load_b32(w.block(p, p.cache.v, at + BLOCK * (I / 4)), (4 * g + I % 4) * hd + run, 0, 0);
+          });
+        }
+      });
+      st.vs[0] = w.v_factor(at);
+      st.vs[1] = w.v_factor(at + BLOCK);
+    };
+    float v_top = 0.0f, v_of[2] = {0.0f, 0.0f}, v_acc = 0.0f;  // RELATIVE: largest V scale so far, of the buffers, of the outputs
+    const auto convert = [&](Stage& st, int at, auto buffer) MI355_LAMBDA_INLINE {
+      constexpr int buf = decltype(buffer)::value;
+      float vs[2] = {st.vs[0], st.vs[1]};
+      if constexpr (RELATIVE) {
+        v_top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
+        v_of[buf] = v_top;
+        const float r = v_top > 0.0f ? 64.0f / v_top : 1.0f;
+        vs[0] *= r;
+        vs[1] *= r;
+      }
+      const bool masked = at + UNIT > all_see;  // some row does not see all of the keys
+      bool found = false;
+      for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
+        constexpr int S = decltype(s)::value;
+        const int piece = wave + 4 * S;
+        if (is_k(s)) {
+          lds.k[buf][2 * piece][lane] = Own::k_operand(st.r[S][0], st.r[S][1]);
+          lds.k[buf][2 * piece + 1][lane] = Own::k_operand(st.r[S][2], st.r[S][3]);
+        } else {
+          const int e = 2 * (piece - 2 * DW);
+          const uint32_t half = piece & 1 ? 0x07030602u : 0x05010400u;  // the two outputs' bytes of a dword
+          if (masked) {  // zeros for V that no row sees, and for NaN
+            uint32_t nans[8], any = 0;
+            for_each<8>([&](auto i) MI355_LAMBDA_INLINE {
+              constexpr int I = decltype(i)::value;
+              const uint32_t v = BLOCK * (I / 4) + I % 4 < stop - at - 4 * g ? st.r[S][I] : 0u;
+              nans[I] = nan_bytes(v);
+              st.r[S][I] = without(v, nans[I]);
+              any |= nans[I];
+            });
+            found = found || __ballot(any != 0) != 0;
+            u32x4 even, odd;
+            Own::counts([&](int k) MI355_LAMBDA_INLINE { return __builtin_amdgcn_perm(nans[2 * k + 1], nans[2 * k], half); }, even, odd);
+            lds.nans[buf][e][lane] = even;
+            lds.nans[buf][e + 1][lane] = odd;
+          }
+          u32x4 even, odd;
+          for_each<4>([&](auto k) MI355_LAMBDA_INLINE {
+            constexpr int K = decltype(k)::value;
+            const uint32_t pr = __builtin_amdgcn_perm(st.r[S][2 * K + 1], st.r[S][2 * K], half);
+            even[K] = two_of<T, false>(pr, vs[K / 2]);
+            odd[K] = two_of<T, true>(pr, vs[K / 2]);
+          });
+          lds.v[buf][e][lane] = even;
+          lds.v[buf][e + 1][lane] = odd;
+        }
+      });
+      if (masked && lane == 0) lds.flag[buf][wave] = found;
+    };
+    const auto barrier = [&]() MI355_LAMBDA_INLINE { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // Operands are read well before their MFMAs: K's while the next unit is converted, V's during the softmax.
+    u32x4 operand[4 * DW];
+    const auto read = [&](const u32x4 (&from)[4 * DW][64]) MI355_LAMBDA_INLINE {
+#pragma unroll
+      for (int e = 0; e < 4 * DW; ++e) operand[e] = from[e][lane];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto work = [&](int at, auto buffer) MI355_LAMBDA_INLINE {
+      constexpr int buf = decltype(buffer)::value;
+      f32x4 sc[NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 2 * DW; ++k)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+            sc[n][t] = mma32(__builtin_bit_cast(typename Own::frag, operand[2 * DW * t + k]), own.qf[n][k], sc[n][t]);
+      read(lds.v[buf]);
+      float a[2] = {win.k_factor(at), win.k_factor(at + BLOCK)};
+      if (at + UNIT > all_see) {
+        own.mask(sc, a, at, k1, g);
+        if (lds.flag[buf][0] | lds.flag[buf][1] | lds.flag[buf][2] | lds.flag[buf][3])
+#pragma unroll
+          for (int e = 0; e < ME; ++e) own.inject(e, lds.nans[buf][e][lane], at, k1, g);
+      }
+      pfrag hi[NR], lo[NR];
+      own.softmax(sc, a, hi, lo);
+      if constexpr (RELATIVE)
+        if (v_of[buf] != v_acc) {
+          const float keep = v_acc / v_of[buf];
+          v_acc = v_of[buf];
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < ME; ++e) own.acc[n][e] *= keep;
+        }
+#pragma unroll
+      for (int e = 0; e < ME; ++e) own.add(e, operand[e], hi, lo);
+    };
+
+    const int n = u1 - u0;
+    const auto key = [&](int i) MI355_LAMBDA_INLINE { return k0 + (i < n ? i : n - 1) * UNIT; };
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
+    Stage even, odd;
+    win.fill(p, b, h, k0, stop, lane);
+    ahead.fill(p, b, h, k0 + 64 * BLOCK, stop, lane);
+    const auto fence = [&]() MI355_LAMBDA_INLINE { __builtin_amdgcn_sched_barrier(0); };  // (loads stay in this order)
+    load(even, key(0));
+    fence();
+    load(odd, key(1));
+    fence();
+    convert(even, key(0), Even{});
+    load(even, key(2));
+    fence();
+    barrier();
+    for (int i = 0; i < n; i += 2) {
+      if (k0 + i * UNIT >= win.from + 64 * BLOCK) {
+        win = ahead;
+        ahead.fill(p, b, h, win.from + 64 * BLOCK, stop, lane);
+      }
+      read(lds.k[0]);
+      convert(odd, key(i + 1), Odd{});
+      load(odd, key(i + 3));
+      fence();
+      if (k0 + i * UNIT < k1) work(k0 + i * UNIT, Even{});
+      barrier();
+      if (i + 1 >= n) break;
+      read(lds.k[1]);
+      convert(even, key(i + 2), Even{});
+      load(even, key(i + 4));
+      fence();
+      if (k0 + (i + 1) * UNIT < k1) work(k0 + (i + 1) * UNIT, Odd{});
+      barrier();
+    }
+    if (!active) return;
+    if constexpr (RELATIVE) {
+      const float back = v_acc > 0.0f ? v_acc / 64.0f : 1.0f;
+#pragma unroll
+      for (int m = 0; m < NR; ++m)
+#pragma unroll
+        for (int e = 0; e < ME; ++e) own.acc[m][e] *= back;
+    }
+#pragma unroll
+    for (int m = 0; m < NR; ++m) own.sum[m] = row_sum(own.sum[m]);
+    own.write(p, rows, h, row0, tile * ROWS, ROWS, slot, lane);
+  }
+};
+
 template <typename T, int DW, int NR, bool MANY>
 __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel(PagedArgs p) {
-  using K = Kernel<T, DW, NR, MANY>;
-  __shared__ std::conditional_t<MANY, char, typename K::Lds> lds_mem;
-  typename K::Lds* lds = reinterpret_cast<typename K::Lds*>(&lds_mem);
+  using K = std::conditional_t<MANY, Many<T, DW, NR>, Few<T, DW, NR>>;
+  __shared__ typename K::Lds lds;
   const int lane = threadIdx.x & 63, kvh = p.cache.kv_heads, G = p.G;
 
   if (p.zero_tail) {  // rows that no sequence has, shared out by work-group
@@ -752,9 +969,7 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
     for (int k = 0; k < 4; ++k) a += *reinterpret_cast<const f32x4*>(&lds[k][4 * lane]);
   }
   if (r >= rows.nrows || in_tile >= rows_of_tile || 4 * lane >= hd) return;
-  const int limit = rows.lim(r, G);
-  float inv = z > 0.0f ? 1.0f / z : (z == 0.0f && limit == 0 ? 0.0f : __builtin_nanf(""));
-  if (limit > rows.keys) inv = __builtin_nanf("");
+  const float inv = rows.inverse(z, rows.lim(r, G));
   const int t = r / G;
   typedef T V4 __attribute__((ext_vector_type(4)));
   *reinterpret_cast<V4*>(static_cast<T*>(p.o) + (rows.s.first + static_cast<int64_t>(t)) * p.ot + (j.h * G + r - t * G) * p.oh + 4 * lane) =
