@@ -180,7 +180,7 @@ MI355_DEVINL int64_t wave_sum(int64_t v) {
 }
 
 // Work-groups that a CU's registers hold.
-constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : dw == 1 ? 5 - nr : many || nr > 1 ? 2 : 3; }
+constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : many ? 2 : dw == 1 ? 5 - nr : 4 - nr; }
 
 // A wave's rows: NR groups of 16, their queries, statistics and outputs.
 // DW: dwords that a lane has of a V row, head_dim / 64 rounded up to 1, 2, 3 or 4 (dims behind head_dim are loaded from
@@ -321,16 +321,11 @@ struct Tile {
       for (int i = 0; i < 4; ++i) acc[n][e][i] += hits[i] > 0.0f ? __builtin_nanf("") : 0.0f;
     }
   }
-  // V^T with 1 for each NaN, of outputs 2 x and 2 x + 1: from bytes of V with 0x80 for each, as `pair` puts them together
-  template <typename F>
-  static MI355_DEVINL void counts(F pair, u32x4& even, u32x4& odd) {
+  // Two elements of V^T with 1 for each NaN, of an output and the next one: from bytes with 0x80 for each, pairs of two keys
+  static MI355_DEVINL void count(uint32_t w, uint32_t& even, uint32_t& odd) {
     constexpr uint32_t one = __is_same(TP, _Float16) ? 0x3c00u : 0x3f80u;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t w = pair(k);
-      even[k] = ((w >> 7) & 1) * one | ((w >> 15) & 1) * (one << 16);
-      odd[k] = ((w >> 23) & 1) * one | (w >> 31) * (one << 16);
-    }
+    even = ((w >> 7) & 1) * one | ((w >> 15) & 1) * (one << 16);
+    odd = ((w >> 23) & 1) * one | (w >> 31) * (one << 16);
   }
 
   // The rows' outputs, or with slot >= 0 partial results of a tile of `rows_of_tile` rows from `tile0` on. top and
@@ -521,7 +516,13 @@ struct Few {
 #pragma unroll
             for (int x = 0; x < 2 * DW; ++x) {
               u32x4 even, odd;
-              Own::counts([&](int k) MI355_LAMBDA_INLINE { return pair_of(nans, x, k); }, even, odd);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t a2, b2;
+                Own::count(pair_of(nans, x, k), a2, b2);
+                even[k] = a2;
+                odd[k] = b2;
+              }
               own.inject(2 * x, even, at, k1, g);
               own.inject(2 * x + 1, odd, at, k1, g);
             }
@@ -621,10 +622,10 @@ struct Many {
     u32x4 nans[2][4 * DW][64];  // 1 for each NaN of V, where flag says that a wave found one
     int flag[2][4];
   };
-  // A wave's part of a unit: of its 2 DW pieces of K (16 keys, 64 dims) and 2 DW of V (two outputs) those with number
-  // wave + 4 s, as bytes.
+  // A wave's part of a unit: of its 2 DW pieces of K (16 keys, 64 dims) and 2 DW of V (16 keys, four outputs) those with
+  // number wave + 4 s, as bytes.
   struct Stage {
-    uint32_t r[DW][8];
+    uint32_t r[DW][4];
     float vs[2];
   };
 
@@ -663,10 +664,12 @@ struct Many {
           const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(src, l16 * hd + (64 * c + 16 * g < hd ? 64 * c + 16 * g : 0), 0, 0);
           st.r[S][0] = x[0], st.r[S][1] = x[1], st.r[S][2] = x[2], st.r[S][3] = x[3];
         } else {
-          const uint32_t run = (l16 * 4 * DW < hd ? l16 * 4 * DW : 0) + 4 * ((piece - 2 * DW) >> 1);
-          for_each<8>([&](auto i) MI355_LAMBDA_INLINE {
+          const int t = (piece - 2 * DW) / DW, c = piece - 2 * DW - t * DW;
+          const auto src = w.block(p, p.cache.v, at + BLOCK * t);
+          const uint32_t run = (l16 * 4 * DW < hd ? l16 * 4 * DW : 0) + 4 * c;
+          for_each<4>([&](auto i) MI355_LAMBDA_INLINE {
             constexpr int I = decltype(i)::value;
-            st.r[S][I] = __builtin_amdgcn_raw_buffer_load_b32(w.block(p, p.cache.v, at + BLOCK * (I / 4)), (4 * g + I % 4) * hd + run, 0, 0);
+            st.r[S][I] = __builtin_amdgcn_raw_buffer_load_b32(src, (4 * g + I) * hd + run, 0, 0);
           });
         }
       });
@@ -693,32 +696,39 @@ struct Many {
           lds.k[buf][2 * piece][lane] = Own::k_operand(st.r[S][0], st.r[S][1]);
           lds.k[buf][2 * piece + 1][lane] = Own::k_operand(st.r[S][2], st.r[S][3]);
         } else {
-          const int e = 2 * (piece - 2 * DW);
-          const uint32_t half = piece & 1 ? 0x07030602u : 0x05010400u;  // the two outputs' bytes of a dword
+          // operands 2 t, 2 t + 1 of a lane's four, of outputs 4 c ..
+          const int t = (piece - 2 * DW) / DW, e = 4 * (piece - 2 * DW - t * DW);
+          const auto put = [&](u32x4 (&to)[4 * DW][64], int x, uint32_t a, uint32_t b) MI355_LAMBDA_INLINE {
+            *(reinterpret_cast<u32x2*>(&to[e + x][lane]) + t) = u32x2{a, b};
+          };
           if (masked) {  // zeros for V that no row sees, and for NaN
-            uint32_t nans[8], any = 0;
-            for_each<8>([&](auto i) MI355_LAMBDA_INLINE {
+            uint32_t nans[4], any = 0;
+            for_each<4>([&](auto i) MI355_LAMBDA_INLINE {
               constexpr int I = decltype(i)::value;
-              const uint32_t v = BLOCK * (I / 4) + I % 4 < stop - at - 4 * g ? st.r[S][I] : 0u;
+              const uint32_t v = BLOCK * t + I < stop - at - 4 * g ? st.r[S][I] : 0u;
               nans[I] = nan_bytes(v);
               st.r[S][I] = without(v, nans[I]);
               any |= nans[I];
             });
             found = found || __ballot(any != 0) != 0;
-            u32x4 even, odd;
-            Own::counts([&](int k) MI355_LAMBDA_INLINE { return __builtin_amdgcn_perm(nans[2 * k + 1], nans[2 * k], half); }, even, odd);
-            lds.nans[buf][e][lane] = even;
-            lds.nans[buf][e + 1][lane] = odd;
+            for_each<2>([&](auto half) MI355_LAMBDA_INLINE {
+              constexpr int H = decltype(half)::value;
+              const uint32_t sel = H ? 0x07030602u : 0x05010400u;
+              uint32_t even[2], odd[2];
+              Own::count(__builtin_amdgcn_perm(nans[1], nans[0], sel), even[0], odd[0]);
+              Own::count(__builtin_amdgcn_perm(nans[3], nans[2], sel), even[1], odd[1]);
+              put(lds.nans[buf], 2 * H, even[0], even[1]);
+              put(lds.nans[buf], 2 * H + 1, odd[0], odd[1]);
+            });
           }
-          u32x4 even, odd;
-          for_each<4>([&](auto k) MI355_LAMBDA_INLINE {
-            constexpr int K = decltype(k)::value;
-            const uint32_t pr = __builtin_amdgcn_perm(st.r[S][2 * K + 1], st.r[S][2 * K], half);
-            even[K] = two_of<T, false>(pr, vs[K / 2]);
-            odd[K] = two_of<T, true>(pr, vs[K / 2]);
+          const float f = t ? vs[1] : vs[0];
+          for_each<2>([&](auto half) MI355_LAMBDA_INLINE {
+            constexpr int H = decltype(half)::value;
+            const uint32_t sel = H ? 0x07030602u : 0x05010400u;
+            const uint32_t a = __builtin_amdgcn_perm(st.r[S][1], st.r[S][0], sel), b = __builtin_amdgcn_perm(st.r[S][3], st.r[S][2], sel);
+            put(lds.v[buf], 2 * H, two_of<T, false>(a, f), two_of<T, false>(b, f));
+            put(lds.v[buf], 2 * H + 1, two_of<T, true>(a, f), two_of<T, true>(b, f));
           });
-          lds.v[buf][e][lane] = even;
-          lds.v[buf][e + 1][lane] = odd;
         }
       });
       if (masked && lane == 0) lds.flag[buf][wave] = found;
@@ -752,7 +762,10 @@ struct Many {
           for (int e = 0; e < ME; ++e) own.inject(e, lds.nans[buf][e][lane], at, k1, g);
       }
       pfrag hi[NR], lo[NR];
+      // the SIMD's other wave has its matrix instructions first meanwhile
+      __builtin_amdgcn_s_setprio(0);
       own.softmax(sc, a, hi, lo);
+      __builtin_amdgcn_s_setprio(1);
       if constexpr (RELATIVE)
         if (v_of[buf] != v_acc) {
           const float keep = v_acc / v_of[buf];
