@@ -643,6 +643,10 @@ struct Many {
     if (active) own.start(p, rows, h, row0, lane);
 
     Window win, ahead;  // blocks of the units worked on, and those after them
+    // half t of a lane's operand (the keys of tile t)
+    const auto put = [&](u32x4 (&to)[64], int t, uint32_t a, uint32_t b) MI355_LAMBDA_INLINE {
+      *(reinterpret_cast<u32x2*>(&to[lane]) + t) = u32x2{a, b};
+    };
     // whether slot s of a wave is a piece of K: for all waves, none, or the first 2 DW - 4 s
     const auto is_k = [&](auto s) MI355_LAMBDA_INLINE {
       constexpr int left = 2 * DW - 4 * decltype(s)::value;
@@ -677,7 +681,38 @@ struct Many {
       st.vs[1] = w.v_factor(at + BLOCK);
     };
     float v_top = 0.0f, v_of[2] = {0.0f, 0.0f}, v_acc = 0.0f;  // RELATIVE: largest V scale so far, of the buffers, of the outputs
-    const auto convert = [&](Stage& st, int at, auto buffer) MI355_LAMBDA_INLINE {
+    // A unit that goes into buffer `buf`, where some row does not see all of its keys: zeros for V that no row sees and for
+    // NaN, whose places are noted.
+    const auto sanitize = [&](Stage& st, int at, auto buffer) MI355_LAMBDA_INLINE {
+      constexpr int buf = decltype(buffer)::value;
+      if (at + UNIT <= all_see) return;
+      bool found = false;
+      for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
+        constexpr int S = decltype(s)::value;
+        if (is_k(s)) return;
+        const int piece = wave + 4 * S - 2 * DW, t = piece / DW, e = 4 * (piece - t * DW);
+        uint32_t nans[4], any = 0;
+        for_each<4>([&](auto i) MI355_LAMBDA_INLINE {
+          constexpr int I = decltype(i)::value;
+          const uint32_t v = BLOCK * t + I < stop - at - 4 * g ? st.r[S][I] : 0u;
+          nans[I] = nan_bytes(v);
+          st.r[S][I] = without(v, nans[I]);
+          any |= nans[I];
+        });
+        found = found || __ballot(any != 0) != 0;
+        for_each<2>([&](auto half) MI355_LAMBDA_INLINE {
+          constexpr int H = decltype(half)::value;
+          const uint32_t sel = H ? 0x07030602u : 0x05010400u;
+          uint32_t even[2], odd[2];
+          Own::count(__builtin_amdgcn_perm(nans[1], nans[0], sel), even[0], odd[0]);
+          Own::count(__builtin_amdgcn_perm(nans[3], nans[2], sel), even[1], odd[1]);
+          put(lds.nans[buf][e + 2 * H], t, even[0], even[1]);
+          put(lds.nans[buf][e + 2 * H + 1], t, odd[0], odd[1]);
+        });
+      });
+      if (lane == 0) lds.flag[buf][wave] = found;
+    };
+    const auto convert = [&](Stage& st, auto buffer) MI355_LAMBDA_INLINE {
       constexpr int buf = decltype(buffer)::value;
       float vs[2] = {st.vs[0], st.vs[1]};
       if constexpr (RELATIVE) {
@@ -687,111 +722,110 @@ struct Many {
         vs[0] *= r;
         vs[1] *= r;
       }
-      const bool masked = at + UNIT > all_see;  // some row does not see all of the keys
-      bool found = false;
       for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
         constexpr int S = decltype(s)::value;
-        const int piece = wave + 4 * S;
+        int piece = wave + 4 * S;
         if (is_k(s)) {
           lds.k[buf][2 * piece][lane] = Own::k_operand(st.r[S][0], st.r[S][1]);
           lds.k[buf][2 * piece + 1][lane] = Own::k_operand(st.r[S][2], st.r[S][3]);
         } else {
-          // operands 2 t, 2 t + 1 of a lane's four, of outputs 4 c ..
-          const int t = (piece - 2 * DW) / DW, e = 4 * (piece - 2 * DW - t * DW);
-          const auto put = [&](u32x4 (&to)[4 * DW][64], int x, uint32_t a, uint32_t b) MI355_LAMBDA_INLINE {
-            *(reinterpret_cast<u32x2*>(&to[e + x][lane]) + t) = u32x2{a, b};
-          };
-          if (masked) {  // zeros for V that no row sees, and for NaN
-            uint32_t nans[4], any = 0;
-            for_each<4>([&](auto i) MI355_LAMBDA_INLINE {
-              constexpr int I = decltype(i)::value;
-              const uint32_t v = BLOCK * t + I < stop - at - 4 * g ? st.r[S][I] : 0u;
-              nans[I] = nan_bytes(v);
-              st.r[S][I] = without(v, nans[I]);
-              any |= nans[I];
-            });
-            found = found || __ballot(any != 0) != 0;
-            for_each<2>([&](auto half) MI355_LAMBDA_INLINE {
-              constexpr int H = decltype(half)::value;
-              const uint32_t sel = H ? 0x07030602u : 0x05010400u;
-              uint32_t even[2], odd[2];
-              Own::count(__builtin_amdgcn_perm(nans[1], nans[0], sel), even[0], odd[0]);
-              Own::count(__builtin_amdgcn_perm(nans[3], nans[2], sel), even[1], odd[1]);
-              put(lds.nans[buf], 2 * H, even[0], even[1]);
-              put(lds.nans[buf], 2 * H + 1, odd[0], odd[1]);
-            });
-          }
+          piece -= 2 * DW;
+          const int t = piece / DW, e = 4 * (piece - t * DW);
           const float f = t ? vs[1] : vs[0];
           for_each<2>([&](auto half) MI355_LAMBDA_INLINE {
             constexpr int H = decltype(half)::value;
             const uint32_t sel = H ? 0x07030602u : 0x05010400u;
             const uint32_t a = __builtin_amdgcn_perm(st.r[S][1], st.r[S][0], sel), b = __builtin_amdgcn_perm(st.r[S][3], st.r[S][2], sel);
-            put(lds.v[buf], 2 * H, two_of<T, false>(a, f), two_of<T, false>(b, f));
-            put(lds.v[buf], 2 * H + 1, two_of<T, true>(a, f), two_of<T, true>(b, f));
+            put(lds.v[buf][e + 2 * H], t, two_of<T, false>(a, f), two_of<T, false>(b, f));
+            put(lds.v[buf][e + 2 * H + 1], t, two_of<T, true>(a, f), two_of<T, true>(b, f));
           });
         }
       });
-      if (masked && lane == 0) lds.flag[buf][wave] = found;
     };
     const auto barrier = [&]() MI355_LAMBDA_INLINE { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    // Operands are read well before their MFMAs: K's while the next unit is converted, V's during the softmax.
+    const int n = u1 - u0;
+    const auto key = [&](int i) MI355_LAMBDA_INLINE { return k0 + (i < n ? i : n - 1) * UNIT; };
+    const auto fence = [&]() MI355_LAMBDA_INLINE { __builtin_amdgcn_sched_barrier(0); };
+    // MFMAs with this many of the region's other instructions after each
+    const auto spread = [&](auto count, auto others) MI355_LAMBDA_INLINE {
+      for_each<decltype(count)::value>([&](auto) MI355_LAMBDA_INLINE {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x6 | 0x200 | 0x20, decltype(others)::value, 0);  // ALU, LDS writes, loads
+      });
+      fence();
+    };
     u32x4 operand[4 * DW];
     const auto read = [&](const u32x4 (&from)[4 * DW][64]) MI355_LAMBDA_INLINE {
 #pragma unroll
       for (int e = 0; e < 4 * DW; ++e) operand[e] = from[e][lane];
-      __builtin_amdgcn_sched_barrier(0);
+      fence();
     };
-    const auto work = [&](int at, auto buffer) MI355_LAMBDA_INLINE {
+    // Unit i, and the conversion of unit i + 1 from st. Operands are read well before their MFMAs, K's at once, V's
+    // before the softmax; the conversion and the next loads go between the MFMAs.
+    const auto step = [&](int i, auto buffer, Stage& st) MI355_LAMBDA_INLINE {
       constexpr int buf = decltype(buffer)::value;
-      f32x4 sc[NR][2];
+      using Next = std::integral_constant<int, 1 - buf>;
+      const int at = k0 + i * UNIT;
+      read(lds.k[buf]);
+      sanitize(st, key(i + 1), Next{});
+      if (at < k1) {
+        f32x4 sc[NR][2];
 #pragma unroll
-      for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < NR; ++m) sc[m][0] = sc[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < 2 * DW; ++k)
+        for (int k = 0; k < 2 * DW; ++k)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int n = 0; n < NR; ++n)
-            sc[n][t] = mma32(__builtin_bit_cast(typename Own::frag, operand[2 * DW * t + k]), own.qf[n][k], sc[n][t]);
-      read(lds.v[buf]);
-      float a[2] = {win.k_factor(at), win.k_factor(at + BLOCK)};
-      if (at + UNIT > all_see) {
-        own.mask(sc, a, at, k1, g);
-        if (lds.flag[buf][0] | lds.flag[buf][1] | lds.flag[buf][2] | lds.flag[buf][3])
+            for (int m = 0; m < NR; ++m)
+              sc[m][t] = mma32(__builtin_bit_cast(typename Own::frag, operand[2 * DW * t + k]), own.qf[m][k], sc[m][t]);
+        convert(st, Next{});
+        spread(std::integral_constant<int, 4 * DW * NR>{}, std::integral_constant<int, 3>{});
+        read(lds.v[buf]);
+        float a[2] = {win.k_factor(at), win.k_factor(at + BLOCK)};
+        if (at + UNIT > all_see) {
+          own.mask(sc, a, at, k1, g);
+          if (lds.flag[buf][0] | lds.flag[buf][1] | lds.flag[buf][2] | lds.flag[buf][3])
 #pragma unroll
-          for (int e = 0; e < ME; ++e) own.inject(e, lds.nans[buf][e][lane], at, k1, g);
-      }
-      pfrag hi[NR], lo[NR];
-      // the SIMD's other wave has its matrix instructions first meanwhile
-      __builtin_amdgcn_s_setprio(0);
-      own.softmax(sc, a, hi, lo);
-      __builtin_amdgcn_s_setprio(1);
-      if constexpr (RELATIVE)
-        if (v_of[buf] != v_acc) {
-          const float keep = v_acc / v_of[buf];
-          v_acc = v_of[buf];
-#pragma unroll
-          for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int e = 0; e < ME; ++e) own.acc[n][e] *= keep;
+            for (int e = 0; e < ME; ++e) own.inject(e, lds.nans[buf][e][lane], at, k1, g);
         }
+        pfrag hi[NR], lo[NR];
+        // the SIMD's other wave has its matrix instructions first meanwhile
+        __builtin_amdgcn_s_setprio(0);
+        own.softmax(sc, a, hi, lo);
+        __builtin_amdgcn_s_setprio(1);
+        if constexpr (RELATIVE)
+          if (v_of[buf] != v_acc) {
+            const float keep = v_acc / v_of[buf];
+            v_acc = v_of[buf];
 #pragma unroll
-      for (int e = 0; e < ME; ++e) own.add(e, operand[e], hi, lo);
+            for (int m = 0; m < NR; ++m)
+#pragma unroll
+              for (int e = 0; e < ME; ++e) own.acc[m][e] *= keep;
+          }
+        fence();
+#pragma unroll
+        for (int e = 0; e < ME; ++e) own.add(e, operand[e], hi, lo);
+        load(st, key(i + 3));
+        spread(std::integral_constant<int, ME * NR>{}, std::integral_constant<int, 4>{});
+      } else {
+        convert(st, Next{});
+        load(st, key(i + 3));
+      }
+      barrier();
     };
 
-    const int n = u1 - u0;
-    const auto key = [&](int i) MI355_LAMBDA_INLINE { return k0 + (i < n ? i : n - 1) * UNIT; };
     using Even = std::integral_constant<int, 0>;
     using Odd = std::integral_constant<int, 1>;
     Stage even, odd;
     win.fill(p, b, h, k0, stop, lane);
     ahead.fill(p, b, h, k0 + 64 * BLOCK, stop, lane);
-    const auto fence = [&]() MI355_LAMBDA_INLINE { __builtin_amdgcn_sched_barrier(0); };  // (loads stay in this order)
     load(even, key(0));
-    fence();
+    fence();  // (loads stay in order: waits are for the older ones)
     load(odd, key(1));
     fence();
-    convert(even, key(0), Even{});
+    sanitize(even, key(0), Even{});
+    convert(even, Even{});
     load(even, key(2));
     fence();
     barrier();
@@ -800,19 +834,8 @@ struct Many {
         win = ahead;
         ahead.fill(p, b, h, win.from + 64 * BLOCK, stop, lane);
       }
-      read(lds.k[0]);
-      convert(odd, key(i + 1), Odd{});
-      load(odd, key(i + 3));
-      fence();
-      if (k0 + i * UNIT < k1) work(k0 + i * UNIT, Even{});
-      barrier();
-      if (i + 1 >= n) break;
-      read(lds.k[1]);
-      convert(even, key(i + 2), Even{});
-      load(even, key(i + 4));
-      fence();
-      if (k0 + (i + 1) * UNIT < k1) work(k0 + (i + 1) * UNIT, Odd{});
-      barrier();
+      step(i, Even{}, odd);
+      if (i + 1 < n) step(i + 1, Odd{}, even);
     }
     if (!active) return;
     if constexpr (RELATIVE) {
