@@ -36,8 +36,9 @@ constexpr float FAR = 0x1p24f;
 constexpr int UNIT = 32;
 
 // What a work-group leaves for the second launch: a job whose first part it has.
-struct Head {
-  int32_t b, h, tile, parts;  // parts: work-groups after it that have more of the job; 0: there is nothing to join
+struct alignas(16) Head {
+  paged::Sequence s;
+  int32_t h, tile, parts;  // parts: work-groups after it that have more of the job; 0: there is nothing to join
 };
 
 struct PagedArgs {
@@ -151,13 +152,26 @@ struct Rows {
   }
 };
 
-MI355_DEVINL Rows rows_of(const PagedArgs& p, int b) {
+MI355_DEVINL Rows rows_of(const PagedArgs& p, paged::Sequence s) {
   Rows r;
-  r.s = paged::sequence_of(p.batch, b);
-  r.nrows = r.s.n * p.G;
-  r.keys = keys_of(p, r.s.len);
-  r.see0 = static_cast<int64_t>(r.s.len) - r.s.n + 1;
+  r.s = s;
+  r.nrows = s.n * p.G;
+  r.keys = keys_of(p, s.len);
+  r.see0 = static_cast<int64_t>(s.len) - s.n + 1;
   return r;
+}
+
+// Sequence b's, of which lane b of `near` has the numbers if b < 64.
+MI355_DEVINL Rows rows_at(const PagedArgs& p, const paged::Sequence& near, int b) {
+  if (b >= 64) return rows_of(p, paged::sequence_of(p.batch, b));
+  return rows_of(p, paged::Sequence{static_cast<int32_t>(__builtin_amdgcn_readlane(near.first, b)),
+                                    static_cast<int32_t>(__builtin_amdgcn_readlane(near.n, b)),
+                                    static_cast<int32_t>(__builtin_amdgcn_readlane(near.len, b))});
+}
+
+MI355_DEVINL int64_t quotient(int64_t n, int64_t d) {  // of what is not negative, mostly of 32 bits
+  if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
 }
 
 // units of all tiles of `rows` rows of a sequence, for one head
@@ -171,12 +185,6 @@ MI355_DEVINL int64_t first_lane(int64_t v) {  // of the wave, in scalar register
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-
-MI355_DEVINL int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-  return first_lane(v);
 }
 
 // Work-groups that a CU's registers hold.
@@ -864,27 +872,46 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
         static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
   }
 
-  // the work-group's run of units: [x, end) of all, or one job whole
-  int b, h, tile, u0, w = blockIdx.x;
+  // the work-group's run of units: [x, x + left) of all, or one job whole
+  int b = 0, h, tile, u0, w = blockIdx.x;
   int64_t each = 0, left;
   Rows rows;
-  Head head{0, 0, 0, 0};
+  Head head{{0, 0, 0}, 0, 0, 0};
+  paged::Sequence near{0, 0, 0};  // lane l has sequence l
   if (p.groups == 0) {
     tile = w % p.row_tiles;
     h = (w / p.row_tiles) % kvh;
     b = w / p.row_tiles / kvh;
-    rows = rows_of(p, b);
+    rows = rows_of(p, paged::sequence_of(p.batch, b));
     if (tile * K::ROWS >= rows.nrows) return;
     u0 = 0;
     left = rows.units((tile + 1) * K::ROWS, G);
   } else {
     // work-groups of one XCD (every eighth) have neighbouring runs: jobs there share keys
     w = blockIdx.x % 8 * (p.groups / 8) + blockIdx.x / 8;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < p.batch.B; b0 += 64)
-      total += b0 + lane < p.batch.B ? all_units(rows_of(p, b0 + lane), K::ROWS, G) * kvh : 0;
-    total = wave_sum(total);
-    each = (total + p.groups - 1) / p.groups;
+    // units of the sequences for one head, 64 at a time: of the lane's, and up to it
+    int64_t mine = 0, upto;
+    const auto scan = [&](int b0) MI355_LAMBDA_INLINE {
+      paged::Sequence s{0, 0, 0};
+      if (b0 + lane < p.batch.B) s = paged::sequence_of(p.batch, b0 + lane);
+      mine = b0 + lane < p.batch.B ? all_units(rows_of(p, s), K::ROWS, G) : 0;
+      upto = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int64_t v = __shfl_up(upto, off);
+        if (lane >= off) upto += v;
+      }
+      return s;
+    };
+    near = scan(0);
+    const int64_t mine0 = mine, upto0 = upto;
+    int64_t total = first_lane(__shfl(upto, 63));
+    for (int b0 = 64; b0 < p.batch.B; b0 += 64) {
+      scan(b0);
+      total += first_lane(__shfl(upto, 63));
+    }
+    total *= kvh;
+    each = quotient(total + p.groups - 1, p.groups);
     each = each > p.least ? each : p.least;
     const int64_t x = w * each;
     left = x + each < total ? each : total - x;
@@ -893,28 +920,28 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
       return;
     }
     // the sequence with unit x, and the unit within it
-    int64_t rest = x;
-    b = 0;
-    for (int b0 = 0; b0 < p.batch.B; b0 += 64) {
-      const int64_t mine = b0 + lane < p.batch.B ? all_units(rows_of(p, b0 + lane), K::ROWS, G) * kvh : 0;
-      int64_t upto = mine;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int64_t v = __shfl_up(upto, off);
-        if (lane >= off) upto += v;
-      }
-      const uint64_t hit = __ballot(rest < upto);
+    int64_t rest = x, per_head = 1;
+    mine = mine0;
+    upto = upto0;
+    for (;;) {
+      const uint64_t hit = __ballot(rest < upto * kvh);
       if (hit) {
         const int l = __builtin_ctzll(hit);
-        b = b0 + l;
-        rest -= first_lane(__shfl(upto - mine, l));
+        b += l;
+        per_head = first_lane(__shfl(mine, l));
+        rest -= (first_lane(__shfl(upto, l)) - per_head) * kvh;
         break;
       }
-      rest -= first_lane(__shfl(upto, 63));
+      rest -= first_lane(__shfl(upto, 63)) * kvh;
+      b += 64;
+      if (b >= p.batch.B) {  // (there is one)
+        if (threadIdx.x == 0) p.joins[w] = head;
+        return;
+      }
+      scan(b);
     }
-    rows = rows_of(p, b);
-    const int64_t per_head = all_units(rows, K::ROWS, G);
-    h = static_cast<int>(rest / per_head);
+    rows = rows_at(p, near, b);
+    h = static_cast<int>(quotient(rest, per_head));
     tile = 0;
     rest -= h * per_head;
     while (rest >= rows.units((tile + 1) * K::ROWS, G)) rest -= rows.units(++tile * K::ROWS, G);
@@ -924,7 +951,7 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
     const int all = rows.units((tile + 1) * K::ROWS, G);
     const int u1 = all - u0 < left ? all : u0 + static_cast<int>(left);
     const bool whole = u0 == 0 && u1 == all;
-    if (u0 == 0 && !whole) head = Head{b, h, tile, static_cast<int32_t>((all - u1 + each - 1) / each)};
+    if (u0 == 0 && !whole) head = Head{rows.s, h, tile, static_cast<int32_t>(quotient(all - u1 + each - 1, each))};
     K::run(p, lds, rows, b, h, tile, u0, u1, whole ? -1 : 2 * static_cast<int64_t>(w) + (u0 == 0));
     left -= u1 - u0;
     if (left <= 0) break;
@@ -934,7 +961,7 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
     if (++h < kvh) continue;
     h = 0;
     do  // (there is one with rows: units are left)
-      rows = ++b < p.batch.B ? rows_of(p, b) : Rows{};
+      rows = ++b < p.batch.B ? rows_at(p, near, b) : Rows{};
     while (rows.nrows == 0 && b < p.batch.B);
     if (rows.nrows == 0) break;
   }
@@ -943,26 +970,40 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
 }
 
 // Joins the parts of the jobs that several work-groups had: a work-group with a first part (blockIdx.x) and a row of its
-// job's tile, or WAVES = 1 four rows. A row's waves take every WAVES-th part, eight requested at a time; lanes have runs
+// job's tile, or WAVES = 1 four rows. A row's waves take every WAVES-th part, several requested at a time; lanes have runs
 // of four dims. Few rows have many parts, tiles of many rows few.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_tile) {
   __shared__ float lds[WAVES][256];
   __shared__ float lds_ml[4][2];
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = WAVES == 1 ? 4 : 8;
   const int w = blockIdx.x, hd = p.cache.head_dim, G = p.G;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int in_tile = WAVES == 1 ? blockIdx.y * 4 + wave : blockIdx.y;
   const Head j = p.joins[w];
   if (j.parts == 0) return;
-  const Rows rows = rows_of(p, j.b);
-  const int r = j.tile * rows_of_tile + in_tile, r_loaded = r < rows.nrows && in_tile < rows_of_tile ? in_tile : 0;
+  const Rows rows = rows_of(p, j.s);
+  const int r = j.tile * rows_of_tile + in_tile, in_ws = in_tile < rows_of_tile ? in_tile : 0;
   // part 0: the work-group's last job; part k: the first one of the k-th after it
   const auto slot = [&](int k) MI355_LAMBDA_INLINE {
     const int64_t s = k == 0 ? 2 * static_cast<int64_t>(w) + 1 : 2 * (static_cast<int64_t>(w) + k);
-    return s * rows_of_tile + r_loaded;
+    return s * rows_of_tile + in_ws;
   };
   const int parts = (j.parts < p.groups - w ? j.parts : p.groups - 1 - w) + 1;
+  const int first = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(wave), d4 = 4 * lane < hd ? 4 * lane : 0;
+  f32x4 v[AHEAD];
+  float top[AHEAD], sum[AHEAD];
+  const auto fetch = [&](int k0) MI355_LAMBDA_INLINE {
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) {
+      if (k0 + WAVES * x >= parts) break;
+      const int64_t at = slot(k0 + WAVES * x);
+      v[x] = *reinterpret_cast<const f32x4*>(p.part + at * hd + d4);
+      top[x] = p.ml[2 * at];
+      sum[x] = p.ml[2 * at + 1];
+    }
+  };
+  fetch(first);  // (under way while the maximum is made)
   float m = NEG_INF;
   for (int k = WAVES == 1 ? lane : static_cast<int>(threadIdx.x); k < parts; k += 64 * WAVES) m = fmaxf(m, p.ml[2 * slot(k)]);
 #pragma unroll
@@ -975,17 +1016,8 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
   const auto factor = [&](float t) MI355_LAMBDA_INLINE { return t == NEG_INF ? 1.0f : fast_exp2(t - m); };
   float z = 0.0f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  const int d4 = 4 * lane < hd ? 4 * lane : 0;
-  for (int k0 = WAVES == 1 ? 0 : wave; k0 < parts; k0 += WAVES * AHEAD) {
-    f32x4 v[AHEAD];
-    float top[AHEAD], sum[AHEAD];
-#pragma unroll
-    for (int x = 0; x < AHEAD; ++x) {
-      const int64_t at = slot(k0 + WAVES * x < parts ? k0 + WAVES * x : k0);
-      v[x] = *reinterpret_cast<const f32x4*>(p.part + at * hd + d4);
-      top[x] = p.ml[2 * at];
-      sum[x] = p.ml[2 * at + 1];
-    }
+  for (int k0 = first; k0 < parts; k0 += WAVES * AHEAD) {
+    if (k0 != first) fetch(k0);
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x) {
       if (k0 + WAVES * x >= parts) break;
