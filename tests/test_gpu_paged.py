@@ -32,6 +32,12 @@ def tables(lens, page, seed, spare=3):
     return torch.randperm(pages, generator=g)[:len(lens) * width].to(torch.int32).view(len(lens), width), pages
 
 
+def widened(table, page):
+    """The table with room for 2^17 tokens, of pages that do not exist: a call whose work is shared out evenly, whatever
+    the lengths are."""
+    return torch.cat((table, torch.full((table.shape[0], (1 << 17) // page - table.shape[1]), -1, dtype=torch.int32)), 1)
+
+
 # rotary
 
 @pytest.mark.parametrize("dtype", [*DTYPES, torch.float32])
@@ -333,16 +339,23 @@ ATTENDS = [
     ([100], [150], 2, 1, 64, 1024),
     ([1, 1], [0, 4], 2, 2, 64, 16),           # an empty sequence
     ([40, 1], [300, 1300], 8, 2, 256, 64),
+    ([70, 3, 0, 41], [70, 900, 5, 1500], 6, 2, 128, 64),
+    ([33], [5000], 1, 1, 192, 128),
+    ([1] * 3, [5000, 40, 1024], 12, 3, 80, 16),
+    ([200], [200], 4, 4, 48, 32),
+    ([9, 1], [1100, 2080], 16, 4, 96, 256),
 ]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("case", ATTENDS)
-def test_attention(dtype, case):
+def test_attention(dtype, case, wide):
     new, lens, H, kvh, D, page = case
     ops = _ops()
     offsets = packed(new)
     table, pages = tables(lens, page, sum(lens))
+    table = widened(table, page) if wide else table
     cache = empty_cache(pages, kvh, page, D, seed=5)
     q = rand((offsets[-1], H, D), dtype, 6, 1.5)
     ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5)
@@ -375,26 +388,31 @@ def test_attention_views(dtype):
     assert not out[:, 4].any() and not out[:, :, D:].any()
 
 
-@pytest.mark.parametrize("D", [64, 128, 256])
-def test_attention_what_is_not_seen(D):
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D", [64, 80, 128, 192, 256])
+def test_attention_what_is_not_seen(D, wide, many):
     """Stale bytes behind a sequence's end and NaN in keys and values: only the tokens that see them change."""
     ops = _ops()
     page, lens, new = 16, [50, 700, 33], [3, 4, 2]
     table, pages = tables(lens, page, 12)
+    own = table.shape[1]
+    table = widened(table, page) if wide else table
     offsets = packed(new)
     cache = empty_cache(pages, 2, page, D, seed=13)
     q = rand((offsets[-1], 4, D), torch.bfloat16, 14)
     dev = on_gpu(cache)
-    batch = ops.PagedBatch(table.cuda(), i32(lens), 4, i32(offsets))
+    most = 40 if many else 4  # (more than 32 rows: another kernel)
+    batch = ops.PagedBatch(table.cuda(), i32(lens), most, i32(offsets))
     clean = ops.attention_paged(q.cuda(), dev, batch)
-    ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5)
+    ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5, most)
     check(clean, ref, tol)
     for b, m in enumerate(lens):
-        for p in range(m, table.shape[1] * page):
+        for p in range(m, own * page):
             for t in (dev.k, dev.v):
                 t.view(torch.uint8)[int(table[b, p // page]), :, p % page] = 0x7f
         last = -(-m // BLOCK) * BLOCK  # scales of blocks behind the end
-        for p in range(last, table.shape[1] * page, BLOCK):
+        for p in range(last, own * page, BLOCK):
             dev.k_scale[int(table[b, p // page]), :, p % page // BLOCK] = math.nan
             dev.v_scale[int(table[b, p // page]), :, p % page // BLOCK] = math.inf
     assert torch.equal(ops.attention_paged(q.cuda(), dev, batch), clean)
@@ -419,7 +437,8 @@ def test_attention_what_is_not_seen(D):
     assert got[3:7, 2:, 7].isnan().all() and not got[3:6, :2].isnan().any() and not got[0:2].isnan().any()
 
 
-def test_attention_pages_that_do_not_exist():
+@pytest.mark.parametrize("most", [6, 40])
+def test_attention_pages_that_do_not_exist(most):
     ops = _ops()
     D, page, lens, new = 64, 16, [40, 40, 130, 30], [2, 2, 1, 6]
     table, pages = tables([64] * 4, page, 15)  # room for 80 tokens: the third sequence's 130 do not fit
@@ -428,14 +447,15 @@ def test_attention_pages_that_do_not_exist():
     lens[3] = 18  # tokens at positions 12 to 17: two of them see the page that is missing
     cache = empty_cache(pages, 2, page, D, seed=16)
     q = rand((offsets[-1], 2, D), torch.float16, 17)
-    ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5)
+    ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5, most)
     assert ref[:2].isnan().all() and not ref[2:4].isnan().any() and ref[4].isnan().all() and ref[9:].isnan().all()
-    got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(table.cuda(), i32(lens), 6, i32(offsets)))
+    got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(table.cuda(), i32(lens), most, i32(offsets)))
     check(got, ref, tol)
 
 
+@pytest.mark.parametrize("most", [1, 40])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_large_scores(dtype):
+def test_attention_large_scores(dtype, most):
     """Scores far apart, all far from zero, and one that takes everything."""
     ops = _ops()
     D, page, lens = 64, 32, [600, 900]
@@ -443,15 +463,17 @@ def test_attention_large_scores(dtype):
     cache = empty_cache(pages, 1, page, D, seed=19)
     for factor in (30.0, 3000.0):
         q = rand((2, 4, D), dtype, 20, factor)
-        ref, tol = attention64(q, cache, table, lens, packed([1, 1]), D ** -0.5)
-        got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(table.cuda(), i32(lens)))
-        check(got, ref, tol)
+        ref, tol = attention64(q, cache, table, lens, packed([1, 1]), D ** -0.5, most)
+        for t in (table, widened(table, page)):
+            got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(t.cuda(), i32(lens), most, i32([0, 1, 2])))
+            check(got, ref, tol)
 
 
 # together
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_generation_steps(dtype):
+def test_generation_steps(dtype, wide):
     """Two prompts admitted into the cache, then steps of both (and a graph of one step, replayed with lengths that grow on
     the device), each against 64 bits over what the cache holds."""
     ops = _ops()
@@ -459,6 +481,7 @@ def test_generation_steps(dtype):
     prompts = [37, 90]
     plan = ops.rotary_plan(rot)
     table, pages = tables([200, 200], page, 21)
+    table = widened(table, page) if wide else table
     cache = ops.paged_cache(pages, kvh, D, page)
     table_gpu, lens = table.cuda(), i32(prompts)
     offsets = packed(prompts)
@@ -514,10 +537,12 @@ def test_generation_steps(dtype):
         assert torch.equal(eager, o)
 
 
-def test_side_stream_and_two_at_once():
+@pytest.mark.parametrize("wide", [False, True])
+def test_side_stream_and_two_at_once(wide):
     ops = _ops()
     lens, D, page = [3000, 1000], 128, 64
     table, pages = tables(lens, page, 23)
+    table = widened(table, page) if wide else table
     dev = on_gpu(empty_cache(pages, 2, page, D, seed=24))
     batch = ops.PagedBatch(table.cuda(), i32(lens))
     q = [rand((2, 8, D), torch.bfloat16, 25 + i).cuda() for i in range(2)]

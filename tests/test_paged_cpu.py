@@ -66,8 +66,8 @@ def test_append_entry_refusals(kw, status):
     *[({k: 0}, NULL) for k in ("Q", "QO", "ck", "cv", "ks", "vs", "table", "lens")],
     (dict(pages=0), BAD_SIZE), (dict(scale=0.0), UNSUP), (dict(scale=-1.0), UNSUP), (dict(scale=math.nan), UNSUP),
     (dict(scale=math.inf), UNSUP), (dict(Q=72), ALIGN), (dict(QO=68), ALIGN), (dict(ck=72), ALIGN), (dict(cv=8), ALIGN),
-    *[(dict(strides=strides_but(i, 130)), ALIGN) for i in range(4)], (dict(width=17, ws=0), BAD_SIZE), (dict(width=17, ws_bytes=64), BAD_SIZE),
-    (dict(width=17, ws=72), BAD_SIZE), (dict(B=1 << 11, most=1 << 10, tokens=1 << 21), BAD_SIZE), (dict(B=0), 0), (dict(tokens=0), 0)])
+    *[(dict(strides=strides_but(i, 130)), ALIGN) for i in range(4)], (dict(width=129, ws=0), BAD_SIZE), (dict(width=129, ws_bytes=64), BAD_SIZE),
+    (dict(width=129, ws=72), BAD_SIZE), (dict(B=1 << 11, most=1 << 10, tokens=1 << 21), BAD_SIZE), (dict(B=0), 0), (dict(tokens=0), 0)])
 def test_attention_entry_refusals(kw, status):
     a = {**APPEND, "scale": 0.125, "ws": 64, "ws_bytes": 1 << 30, **kw}
     assert _lib.lib().mi355_attn_paged(
@@ -79,8 +79,8 @@ def test_attention_workspace():
     def f(**kw):
         return _lib.lib().mi355_attn_paged_workspace_bytes(sizes_of({**APPEND, "tokens": 0, **kw}))
 
-    assert f(width=16) == 0  # 256 keys: nothing to share out
-    assert f(width=17) > 0 and f(width=17) % 16 == 0
+    assert f(width=128) == 0  # 2048 keys: a work-group for each job
+    assert f(width=129) > 0 and f(width=129) % 16 == 0
     assert f(kv_heads=3) == BAD_SIZE and f(head_dim=40) == HEAD and f(page=24) == BAD_SIZE
     assert _lib.lib().mi355_attn_paged_workspace_bytes(None) == NULL
 

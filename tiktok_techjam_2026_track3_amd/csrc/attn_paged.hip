@@ -879,9 +879,10 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
   Head head{{0, 0, 0}, 0, 0, 0};
   paged::Sequence near{0, 0, 0};  // lane l has sequence l
   if (p.groups == 0) {
-    tile = w % p.row_tiles;
-    h = (w / p.row_tiles) % kvh;
-    b = w / p.row_tiles / kvh;
+    const int heads = p.batch.B * kvh;  // (later tiles see more keys: they come first)
+    tile = p.row_tiles - 1 - w / heads;
+    h = w % heads % kvh;
+    b = w % heads / kvh;
     rows = rows_of(p, paged::sequence_of(p.batch, b));
     if (tile * K::ROWS >= rows.nrows) return;
     u0 = 0;
@@ -1044,9 +1045,6 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
       V4{from_f32<T>(a[0] * inv), from_f32<T>(a[1] * inv), from_f32<T>(a[2] * inv), from_f32<T>(a[3] * inv)};
 }
 
-// Largest room (in tokens) that one work-group walks alone, without a second launch.
-constexpr int64_t ALONE = 256;
-
 struct Launch {
   bool many;
   int nr, rows;               // groups of 16 rows of a wave, rows of a tile
@@ -1061,8 +1059,17 @@ Launch launch_of(const paged::Sizes& z) {
   l.rows = 16 * l.nr * (l.many ? 4 : 1);
   l.row_tiles = (rows + l.rows - 1) / l.rows;
   const int64_t jobs = z.B * z.kv_heads * l.row_tiles;
-  // as many work-groups as the GPU's 256 CUs hold at a time (per_cu)
-  l.groups = z.width * z.page <= ALONE ? 0 : 256 * per_cu(dw, l.nr, l.many);
+  // Sharing the work out evenly takes as many work-groups as the GPU's 256 CUs hold at a time (per_cu), partial results and
+  // a second launch. A work-group for each job instead where the longest that the table allows is short, or jobs fill
+  // the GPU. Measured (us, shared out / a job each; bf16, 8 K/V heads of 128, groups of 4, K and V in the last-level cache
+  // but for the largest): one new token, sequences of one length, then of 10 to 100% of it: 2 sequences of 1024 keys 14.5 / 11.3, 2048
+  // 17.4 / 16.7, 4096 18.6 / 27.2; 8: 2048 20.2 / 17.8 and 21.0 / 14.8, 4096 25.1 / 28.5 and 21.7 / 23.6; 16: 4096 33.7 / 29.0 and
+  // 23.9 / 26.6, 8192 51.4 / 54.4 and 32.1 / 47.1; 64: 4096 110 / 98 and 56 / 59, 8192 201 / 187 and 110 / 130. Many rows: a
+  // prompt of 2048 121 / 69, 8192 684 / 554; 512 tokens against 2048 63 / 63, 4096 75 / 117; 1024 against 16384 (256 jobs) 298 / 452;
+  // 2048 against 16384 (512) 550 / 507.
+  const int64_t room = z.width * z.page;
+  const bool each = l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048);
+  l.groups = each ? 0 : 256 * per_cu(dw, l.nr, l.many);
   l.least = 8;
   l.grid = l.groups ? l.groups : jobs;
   l.ws = l.groups * (2 * l.rows * (z.head_dim + 2) * 4 + static_cast<int64_t>(sizeof(Head)));
