@@ -123,6 +123,23 @@ def test_rotary_views(dtype):
     assert ops.rotary(x[:0], positions[:0], plan).shape == (0, 3, 2, 32)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_larger_than_the_caches(interleaved):
+    """Outputs of 32 MiB and more are stored another way; the append's queries likewise, and to the same bits."""
+    ops = _ops()
+    T, H, D = 4100, 34, 128
+    x = rand((T, H, D), torch.bfloat16, 50)
+    positions = torch.arange(T) + 77
+    plan = ops.rotary_plan(96, interleaved=interleaved)
+    ref, tol = rotate64(x, positions, frequencies(96), interleaved)
+    got = ops.rotary(x.cuda(), positions.cuda(), plan)
+    check(got, ref, tol + UNIT[torch.bfloat16] * ref.abs())
+    k = rand((T, 2, D), torch.bfloat16, 51).cuda()
+    table = torch.arange(5, dtype=torch.int32, device="cuda")[None]
+    cache = ops.paged_cache(5, 2, D, 1024)
+    assert torch.equal(ops.paged_append(cache, k, k, ops.PagedBatch(table, i32([T + 77]), T), plan, x.cuda()), got)
+
+
 def test_rotary_is_its_own_gradient():
     """The inverse is the transposed map: differences of sum(w y), and against autograd of the formula."""
     ops = _ops()

@@ -97,19 +97,20 @@ MI355_DEVINL uint32_t two_of(uint32_t w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, WORD));
 }
 
-// DW dwords at `at`
-template <int DW>
+// DW dwords at `at`; AUX: cache policy of the load (0, or PAST: not kept)
+constexpr int PAST = 2;
+template <int DW, int AUX>
 MI355_DEVINL void run_of(uint32_t (&v)[DW], __amdgpu_buffer_rsrc_t src, uint32_t at) {
   if constexpr (DW == 1) {
-    v[0] = __builtin_amdgcn_raw_buffer_load_b32(src, at, 0, 0);
+    v[0] = __builtin_amdgcn_raw_buffer_load_b32(src, at, 0, AUX);
   } else if constexpr (DW == 2) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b64(src, at, 0, 0);
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(src, at, 0, AUX);
     v[0] = x[0], v[1] = x[1];
   } else if constexpr (DW == 3) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b96(src, at, 0, 0);
+    const auto x = __builtin_amdgcn_raw_buffer_load_b96(src, at, 0, AUX);
     v[0] = x[0], v[1] = x[1], v[2] = x[2];
   } else {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b128(src, at, 0, 0);
+    const auto x = __builtin_amdgcn_raw_buffer_load_b128(src, at, 0, AUX);
     v[0] = x[0], v[1] = x[1], v[2] = x[2], v[3] = x[3];
   }
 }
@@ -416,7 +417,7 @@ struct Window {
 
 // Up to 16 NR rows: the four waves have the same rows and a quarter of the keys each, and are joined through LDS. K and V
 // are waited for; a unit's bytes are requested as soon as the registers of those before it are free.
-template <typename T, int DW, int NR>
+template <typename T, int DW, int NR, int AUX>
 struct Few {
   using Own = Tile<T, DW, NR, 2>;
   using TP = typename Own::TP;
@@ -455,7 +456,7 @@ struct Few {
       for (int t = 0; t < 2; ++t) {
         const auto src = win.block(p, p.cache.k, at + BLOCK * t);
 #pragma unroll
-        for (int c = 0; c < DW; ++c) ku[t][c] = __builtin_amdgcn_raw_buffer_load_b128(src, k_at[c], 0, 0);
+        for (int c = 0; c < DW; ++c) ku[t][c] = __builtin_amdgcn_raw_buffer_load_b128(src, k_at[c], 0, AUX);
         ka[t] = win.k_factor(at + BLOCK * t);
       }
     };
@@ -464,7 +465,7 @@ struct Few {
       for (int t = 0; t < 2; ++t) {
         const auto src = win.block(p, p.cache.v, at + BLOCK * t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) run_of<DW>(vu[t][i], src, v_at[i]);
+        for (int i = 0; i < 4; ++i) run_of<DW, AUX>(vu[t][i], src, v_at[i]);
         va[t] = win.v_factor(at + BLOCK * t);
       }
     };
@@ -859,9 +860,9 @@ struct Many {
   }
 };
 
-template <typename T, int DW, int NR, bool MANY>
+template <typename T, int DW, int NR, bool MANY, int AUX>
 __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel(PagedArgs p) {
-  using K = std::conditional_t<MANY, Many<T, DW, NR>, Few<T, DW, NR>>;
+  using K = std::conditional_t<MANY, Many<T, DW, NR>, Few<T, DW, NR, AUX>>;
   __shared__ typename K::Lds lds;
   const int lane = threadIdx.x & 63, kvh = p.cache.kv_heads, G = p.G;
 
@@ -1046,7 +1047,7 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
 }
 
 struct Launch {
-  bool many;
+  bool many, past;
   int nr, rows;               // groups of 16 rows of a wave, rows of a tile
   int64_t row_tiles, groups, least, grid, ws;
 };
@@ -1059,8 +1060,8 @@ Launch launch_of(const paged::Sizes& z) {
   l.rows = 16 * l.nr * (l.many ? 4 : 1);
   l.row_tiles = (rows + l.rows - 1) / l.rows;
   const int64_t jobs = z.B * z.kv_heads * l.row_tiles;
-  // Sharing the work out evenly takes as many work-groups as the GPU's 256 CUs hold at a time (per_cu), partial results and
-  // a second launch. A work-group for each job instead where the longest that the table allows is short, or jobs fill
+  // Sharing the work out evenly takes two work-groups a CU (one above head dim 128, whose registers allow no more; three
+  // or four where they do: 200000 keys of one sequence 92 us instead of 86), partial results and a second launch. A work-group for each job instead where the longest that the table allows is short, or jobs fill
   // the GPU. Measured (us, shared out / a job each; bf16, 8 K/V heads of 128, groups of 4, K and V in the last-level cache
   // but for the largest): one new token, sequences of one length, then of 10 to 100% of it: 2 sequences of 1024 keys 14.5 / 11.3, 2048
   // 17.4 / 16.7, 4096 18.6 / 27.2; 8: 2048 20.2 / 17.8 and 21.0 / 14.8, 4096 25.1 / 28.5 and 21.7 / 23.6; 16: 4096 33.7 / 29.0 and
@@ -1068,8 +1069,12 @@ Launch launch_of(const paged::Sizes& z) {
   // prompt of 2048 121 / 69, 8192 684 / 554; 512 tokens against 2048 63 / 63, 4096 75 / 117; 1024 against 16384 (256 jobs) 298 / 452;
   // 2048 against 16384 (512) 550 / 507.
   const int64_t room = z.width * z.page;
+  // Few rows read K and V once. Where the tables allow more of them than the last-level cache holds (256 MiB), they are loaded
+  // as what is not kept (us, so / as what is): 64 sequences of up to 9000 keys (655 MB) 121 / 129, 200000 keys (409 MB) 79.4 / 86.0,
+  // 128 sequences of 2048 keys (537 MB) 91.5 / 97.6; 1024 keys (268 MB, in that cache) 50.1 / 43.4.
+  l.past = !l.many && z.B * room * z.kv_heads * z.head_dim * 2 > int64_t(320) << 20;
   const bool each = l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048);
-  l.groups = each ? 0 : 256 * per_cu(dw, l.nr, l.many);
+  l.groups = each ? 0 : 256 * (dw > 2 ? 1 : 2);
   l.least = 8;
   l.grid = l.groups ? l.groups : jobs;
   l.ws = l.groups * (2 * l.rows * (z.head_dim + 2) * 4 + static_cast<int64_t>(sizeof(Head)));
@@ -1078,7 +1083,10 @@ Launch launch_of(const paged::Sizes& z) {
 
 template <typename T, int DW, int NR, bool MANY>
 int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
-  attn_paged_kernel<T, DW, NR, MANY><<<static_cast<uint32_t>(l.grid), 256, 0, s>>>(p);
+  const auto grid = static_cast<uint32_t>(l.grid);
+  if constexpr (!MANY)
+    if (l.past) attn_paged_kernel<T, DW, NR, false, PAST><<<grid, 256, 0, s>>>(p);
+  if (!l.past) attn_paged_kernel<T, DW, NR, MANY, 0><<<grid, 256, 0, s>>>(p);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || l.groups == 0) return static_cast<int>(e);
   const int64_t rows = std::min<int64_t>(l.rows, p.batch.most * static_cast<int64_t>(p.G));
   if constexpr (MANY)

@@ -29,7 +29,8 @@ struct alignas(sizeof(T) * N) Vec {
 
 // A thread: VEC pairs of a token in `per` heads. The two halves of a unit's elements are VEC neighbours at first and at
 // second; pairs that are neighbours come as one run of 2 VEC, like the elements that are copied.
-template <typename T, int VEC, bool INTERLEAVED>
+// PAST: 16-byte stores past the L2s, for outputs larger than those (PAST_CACHES).
+template <typename T, int VEC, bool INTERLEAVED, bool PAST>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
   const int unit = static_cast<int>(threadIdx.x) % p.units;
   const int local = static_cast<int>(threadIdx.x) / p.units, tpb = 256 / p.units;
@@ -77,12 +78,22 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
           }
         }
         T* row = y + (h + k) * p.ys2;
-        *reinterpret_cast<Vec<T, VEC>*>(row + first) = u[k][0];
-        *reinterpret_cast<Vec<T, VEC>*>(row + second) = u[k][1];
+        if constexpr (PAST) {
+          __builtin_nontemporal_store(__builtin_bit_cast(u32x4, u[k][0]), reinterpret_cast<u32x4*>(row + first));
+          __builtin_nontemporal_store(__builtin_bit_cast(u32x4, u[k][1]), reinterpret_cast<u32x4*>(row + second));
+        } else {
+          *reinterpret_cast<Vec<T, VEC>*>(row + first) = u[k][0];
+          *reinterpret_cast<Vec<T, VEC>*>(row + second) = u[k][1];
+        }
       }
     }
   }
 }
+
+// Outputs of this many bytes and more are stored past the L2s, which hold 32 MiB together and would be written back at the
+// kernel's end. Measured (us, past them / through them): 84 MB (8192 tokens, 40 heads of 128) 28.3 / 37.4, 16.8 MB 9.1 / 9.0,
+// 9.6 MB 9.9 / 8.2. (x past them as well: 35.0 and 17.6 where it is in the last-level cache from before.)
+constexpr int64_t PAST_CACHES = int64_t(32) << 20;
 
 template <typename T, int VEC>
 int launch(RotaryArgs& p, int64_t head_dim, bool interleaved, hipStream_t s) {
@@ -93,10 +104,16 @@ int launch(RotaryArgs& p, int64_t head_dim, bool interleaved, hipStream_t s) {
   p.per = 8;
   while (p.per > 1 && rows * ((p.heads + p.per - 1) / p.per) < 1024) p.per /= 2;
   const dim3 grid(static_cast<uint32_t>(rows < (1 << 20) ? rows : (1 << 20)), static_cast<uint32_t>((p.heads + p.per - 1) / p.per));
-  if (interleaved)
-    rotary_kernel<T, VEC, true><<<grid, 256, 0, s>>>(p);
+  const bool past = sizeof(T) * VEC == 16 && p.tokens * p.heads * head_dim * static_cast<int64_t>(sizeof(T)) >= PAST_CACHES;
+  constexpr bool WHOLE = sizeof(T) * VEC == 16;
+  if (past && interleaved)
+    rotary_kernel<T, VEC, true, WHOLE><<<grid, 256, 0, s>>>(p);
+  else if (past)
+    rotary_kernel<T, VEC, false, WHOLE><<<grid, 256, 0, s>>>(p);
+  else if (interleaved)
+    rotary_kernel<T, VEC, true, false><<<grid, 256, 0, s>>>(p);
   else
-    rotary_kernel<T, VEC, false><<<grid, 256, 0, s>>>(p);
+    rotary_kernel<T, VEC, false, false><<<grid, 256, 0, s>>>(p);
   return static_cast<int>(hipGetLastError());
 }
 
