@@ -486,6 +486,132 @@ def test_attention_large_scores(dtype, most):
             check(got, ref, tol)
 
 
+@pytest.mark.parametrize("most", [1, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_rows_beside_bad_ones(dtype, most):
+    """Queries with NaN and infinities: their own outputs alone are NaN, and the other rows keep their bits."""
+    ops = _ops()
+    D, page, lens = 128, 32, [90, 1200]
+    table, pages = tables(lens, page, 30)
+    dev = on_gpu(empty_cache(pages, 2, page, D, seed=31))
+    q = rand((2, 8, D), dtype, 32)
+    for t in (table, widened(table, page)):
+        batch = ops.PagedBatch(t.cuda(), i32(lens), most, i32([0, 1, 2]))
+        clean = ops.attention_paged(q.cuda(), dev, batch)
+        bad = q.clone()
+        bad[0, 1, 3], bad[1, 4, 0], bad[1, 7, 127] = math.nan, math.inf, -math.inf
+        got = ops.attention_paged(bad.cuda(), dev, batch)
+        for r in ((0, 1), (1, 4), (1, 7)):
+            assert got[r].isnan().all()
+            got[r] = clean[r]
+        assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("most", [2, 40])
+def test_lengths_and_offsets_that_make_no_sense(most):
+    """Read on the device, checked there: nothing outside the tensors is touched, and a sequence that makes sense is right."""
+    ops = _ops()
+    D, page, lens = 64, 16, [2 ** 31 - 1, -2 ** 31, 60, -5, 2 ** 31 - 1]
+    table, pages = tables([60] * 5, page, 33)
+    table[4] = torch.tensor([2 ** 31 - 1, -2 ** 31, pages, -1, 2 ** 30])
+    cache = empty_cache(pages, 2, page, D, seed=34)
+    q, k = rand((9, 4, D), torch.float16, 35), rand((9, 2, D), torch.float16, 36)
+    for offsets in ([-7, 2, 3, 5, 4, 2 ** 31 - 1], [0, 2, 3, 5, 7, 9], [2 ** 31 - 1, 0, 3, 5, -2 ** 31, 9]):
+        # a row that two sequences name holds either's result (a start below 0 counts as 0)
+        own = [r for r in (3, 4) if sum(max(a, 0) <= r < min(b, max(a, 0) + most) for a, b in zip(offsets, offsets[1:])) == 1]
+        rows = [r - 3 for r in own]
+        for t in (table, widened(table, page)):
+            batch = ops.PagedBatch(t.cuda(), i32(lens), most, i32(offsets))
+            dev = on_gpu(cache)
+            got = ops.attention_paged(q.cuda(), dev, batch)
+            ref, tol = attention64(q[3:5], cache, table[2:3], [60], [0, 2], D ** -0.5, most)
+            check(got[own], ref[rows], tol[rows])
+            turned = ops.paged_append(dev, k.cuda(), k.cuda(), batch, ops.rotary_plan(D), q.cuda())
+            ref, tol = rotate64(q[3:5], torch.tensor([58, 59]), frequencies(D))
+            check(turned[own], ref[rows], (tol + UNIT[torch.float16] * ref.abs())[rows])
+            one = on_gpu(cache)
+            ops.paged_append(one, k[3:5].cuda(), k[3:5].cuda(), ops.PagedBatch(table[2:3].cuda(), i32([60]), 2), ops.rotary_plan(D))
+            at = int(table[2, 3])
+            assert torch.equal(dev.k.view(torch.uint8)[at], one.k.view(torch.uint8)[at])
+
+
+def test_many_sequences():
+    """More than 64, and more than 1024, sequences; some without a token."""
+    ops = _ops()
+    D, page = 32, 16
+    g = torch.Generator().manual_seed(37)
+    for B in (130, 1500):
+        new = torch.randint(0, 3, (B,), generator=g).tolist()
+        lens = [n + int(torch.randint(0, 60, (1,), generator=g)) for n in new]
+        offsets = packed(new)
+        table, pages = tables(lens, page, B)
+        cache = empty_cache(pages, 1, page, D, seed=38)
+        q = rand((offsets[-1], 2, D), torch.bfloat16, 39)
+        ref, tol = attention64(q, cache, table, lens, offsets, D ** -0.5)
+        for t in (table, widened(table, page)) if B < 1000 else (table,):
+            check(ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(t.cuda(), i32(lens), 2, i32(offsets))), ref, tol)
+
+
+def test_append_in_place_on_a_packed_projection():
+    """q, k and v as views of one buffer: queries rotated in place are refused only where they share elements."""
+    ops = _ops()
+    D, page = 64, 16
+    table, pages = tables([40], page, 41)
+    cache = on_gpu(empty_cache(pages, 2, page, D))
+    plan = ops.rotary_plan(D)
+    qkv = rand((5, 8, D), torch.bfloat16, 42).cuda()
+    batch = ops.PagedBatch(table.cuda(), i32([40]), 5)
+    want = ops.paged_append(cache, qkv[:, 4:6], qkv[:, 6:], batch, plan, qkv[:, :4])
+    bytes_ = cache.k.view(torch.uint8).clone()
+    keep = qkv[:, 4:].clone()
+    ops.paged_append(cache, qkv[:, 4:6], qkv[:, 6:], batch, plan, qkv[:, :4], q_out=qkv[:, :4])
+    assert torch.equal(qkv[:, :4], want) and torch.equal(qkv[:, 4:], keep) and torch.equal(cache.k.view(torch.uint8), bytes_)
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.paged_append(cache, qkv[:, 3:5], qkv[:, 6:], batch, plan, qkv[:, :4], q_out=qkv[:, :4])
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.paged_append(cache, qkv[:, 4:6], qkv[:, 6:], batch, plan, qkv[:, 1:5], q_out=qkv[:, :4])
+
+
+def test_refusals_on_the_gpu():
+    ops = _ops()
+    D = 64
+    cache = ops.paged_cache(4, 2, D, 16)
+    x, kv = torch.zeros(2, 4, D, dtype=torch.float16, device="cuda"), torch.zeros(2, 2, D, dtype=torch.float16, device="cuda")
+    batch = ops.PagedBatch(i32([[0], [1]]), i32([3, 4]))
+    plan = ops.rotary_plan(D)
+    cases = [
+        (TypeError, lambda: ops.attention_paged(x.float(), cache, batch)),
+        (ValueError, lambda: ops.attention_paged(x[:1], cache, batch)),
+        (ValueError, lambda: ops.attention_paged(x, cache, batch, scale=0.0)),
+        (ValueError, lambda: ops.attention_paged(x, cache, batch, out=x)),
+        (ValueError, lambda: ops.attention_paged(x[..., :32], cache, batch)),
+        (ValueError, lambda: ops.attention_paged(x.clone().requires_grad_(), cache, batch)),
+        (ValueError, lambda: ops.attention_paged(x.cpu(), cache, batch)),
+        (ValueError, lambda: ops.paged_append(cache, kv, kv, batch, None, x)),
+        (ValueError, lambda: ops.paged_append(cache, kv, kv, batch, ops.rotary_plan(20), x)),
+        (ValueError, lambda: ops.paged_append(cache, kv, kv, batch, ops.rotary_plan(128), x)),
+        (ValueError, lambda: ops.paged_append(cache, kv, kv, batch, plan, q_out=x)),
+        (ValueError, lambda: ops.paged_append(cache, kv, kv, batch, plan, x, q_out=x.transpose(0, 1))),
+        (ValueError, lambda: ops.paged_append(cache, x, kv, batch)),
+        (TypeError, lambda: ops.paged_append(cache, kv, kv.bfloat16(), batch)),
+        (ValueError, lambda: ops.paged_append(cache, cache.k.view(torch.float16)[0, :, :2].transpose(0, 1)[..., :32].repeat(1, 1, 2), kv.requires_grad_(), batch)),
+        (ValueError, lambda: ops.rotary(x, torch.arange(2, device="cuda"), plan, out=x[:, :, :].flip(0)[:1])),
+        (ValueError, lambda: ops.rotary(x, torch.arange(3, device="cuda"), plan)),
+        (ValueError, lambda: ops.rotary(x, torch.arange(2), plan)),
+        (TypeError, lambda: ops.rotary(x, torch.arange(2, device="cuda"), plan, out=x.float())),
+    ]
+    for i, (error, call) in enumerate(cases):
+        with pytest.raises(error):
+            call()
+            print("case", i)
+    long = torch.zeros(3, 4, D, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.rotary(long[:2], torch.arange(2, device="cuda"), plan, out=long[1:])
+    whole = cache.k.view(torch.float16).view(-1)[:2 * 2 * D].view(2, 2, D)  # the cache's own bytes
+    with pytest.raises(ValueError, match="shares memory"):
+        ops.paged_append(cache, whole, torch.zeros_like(whole), batch)
+
+
 # together
 
 @pytest.mark.parametrize("wide", [False, True])

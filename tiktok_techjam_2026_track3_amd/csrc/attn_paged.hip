@@ -1073,7 +1073,8 @@ Launch launch_of(const paged::Sizes& z) {
   // as what is not kept (us, so / as what is): 64 sequences of up to 9000 keys (655 MB) 121 / 129, 200000 keys (409 MB) 79.4 / 86.0,
   // 128 sequences of 2048 keys (537 MB) 91.5 / 97.6; 1024 keys (268 MB, in that cache) 50.1 / 43.4.
   l.past = !l.many && z.B * room * z.kv_heads * z.head_dim * 2 > int64_t(320) << 20;
-  const bool each = l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048);
+  // (More than 1024 sequences fill the GPU by themselves, and each work-group would go through all their lengths.)
+  const bool each = z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048));
   l.groups = each ? 0 : 256 * (dw > 2 ? 1 : 2);
   l.least = 8;
   l.grid = l.groups ? l.groups : jobs;

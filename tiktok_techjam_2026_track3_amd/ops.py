@@ -1220,6 +1220,22 @@ class PagedBatch:
                 raise ValueError("table, lens and offsets must be on one device")
 
 
+def _check_rows_apart(out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Refuses an ``out`` [tokens, heads, head_dim] that shares memory with an input of that form. Views of one buffer are
+    apart where their tokens are equally far from each other and each token's rows lie beside the other's."""
+    for t in inputs:
+        try:
+            _check_apart(out, t)
+        except ValueError:
+            step = out.stride(0) * out.element_size()
+            if t.stride(0) != out.stride(0) or out.shape[0] < 2 or t.shape[0] < 2:
+                raise
+            mine, other = _bytes(out.shape[1:], out.stride()[1:], out.dtype), _bytes(t.shape[1:], t.stride()[1:], t.dtype)
+            at = (t.data_ptr() - out.data_ptr()) % step
+            if at < mine or at + other > step:
+                raise
+
+
 @functools.lru_cache(maxsize=512)
 def _paged_views(cache_shape, table_shape, table_stride, most, ragged, names, dtypes, shapes, strides):
     """(type code, arrays of sizes and strides, workspace bytes, bytes of each tensor, whether there is nothing to do,
@@ -1319,9 +1335,10 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: Pag
                 start < cvs + nvs and cvs < end):
             raise ValueError("k, v or q shares memory with the cache")
     if given:
-        _check_apart(q_out, k, v, batch.table, batch.lens, batch.offsets)
+        _check_apart(q_out, batch.table, batch.lens, batch.offsets)
+        _check_rows_apart(q_out, k, v)
         if at[2] != at[3] or not alike:
-            _check_apart(q_out, q)
+            _check_rows_apart(q_out, q)
     kp, vp, qp, op = at[0], at[1], 0 if q is None else at[2], 0 if q is None else q_out.data_ptr()
     if (kp | vp | qp | op) & 15:
         _check_aligned(k=kp, v=vp, q=qp, q_out=op)
