@@ -535,6 +535,61 @@ def test_lengths_and_offsets_that_make_no_sense(most):
             assert torch.equal(dev.k.view(torch.uint8)[at], one.k.view(torch.uint8)[at])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_prompt_rows_and_later_scales(D, dtype):
+    """V far larger in later blocks, of the same 32 keys and behind them: rows that do not see those keep their digits."""
+    ops = _ops()
+    page, lens = 64, [80]
+    table, pages = tables(lens, page, 43)
+    cache = empty_cache(pages, 1, page, D, seed=44)
+    scales = cache[3][table[0, :2].long(), 0].view(-1)  # of the sequence's blocks
+    scales[:] = torch.tensor([2.0 ** e for e in (-12, 30, 30, -12, 60, 0, 0, 0)])
+    cache[3][table[0, :2].long(), 0] = scales.view(2, -1)
+    q = rand((80, 1, D), dtype, 45)
+    for t in (table, widened(table, page)):
+        got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(t.cuda(), i32(lens), 80))
+        ref, tol = attention64(q[:16], cache, t, [16], [0, 16], D ** -0.5, 80)
+        check(got[:16], ref, tol)
+        if dtype == torch.bfloat16:  # (elsewhere the results leave the type)
+            ref, tol = attention64(q, cache, t, lens, [0, 80], D ** -0.5)
+            check(got, ref, tol)
+
+
+@pytest.mark.parametrize("most", [3, 40])
+def test_pools_beyond_32_bits(most):
+    """K and V of more than 2^32 bytes each, and tables for more keys than the last-level cache holds: the same bits as
+    from small pools and tables."""
+    ops = _ops()
+    D, page, H = 256, 1024, 8
+    pages, width = 2100, 100
+    cache = ops.paged_cache(pages, H, D, page)
+    assert cache.k.numel() > 1 << 32
+    lens = [2500, 9000]
+    table = torch.full((2, width), -1, dtype=torch.int32)
+    table[0, :3] = torch.tensor([2099, 2052, 7])
+    table[1, :9] = torch.arange(2060, 2069)
+    used = torch.cat((table[0, :3], table[1, :9])).long()
+    small = ops.paged_cache(13, H, D, page)
+    near = torch.full((2, 60), -1, dtype=torch.int32)
+    near[0, :3], near[1, :9] = torch.arange(1, 4), torch.arange(4, 13)
+    results = []
+    for c, t in ((cache, table), (small, near)):
+        g = torch.Generator(device="cuda").manual_seed(46)
+        new = torch.randn(sum(lens), H, D, device="cuda", generator=g).half()
+        ops.paged_append(c, new, new.flip(0), ops.PagedBatch(t.cuda(), i32(lens), max(lens), i32(packed(lens))), ops.rotary_plan(D))
+        q = torch.randn(2 * most, H, D, device="cuda", generator=g).half()
+        results.append(ops.attention_paged(q, c, ops.PagedBatch(t.cuda(), i32(lens), most)))
+        at = used.cuda() if c is cache else torch.arange(1, 13, device="cuda")
+        results[-1:] = [results[-1], c.k.view(torch.uint8)[at], c.v.view(torch.uint8)[at], c.k_scale[at], c.v_scale[at]]
+    assert results[0].isfinite().all() and results[0].abs().max() > 0
+    for a, b in zip(results[:5], results[5:]):
+        assert torch.equal(a, b)
+    used = set(used.tolist())
+    others = torch.tensor([i for i in range(pages) if i not in used], device="cuda")
+    assert cache.k_scale[others].abs().max() == 0 and cache.v_scale[others].abs().max() == 0
+
+
 def test_many_sequences():
     """More than 64, and more than 1024, sequences; some without a token."""
     ops = _ops()
@@ -610,6 +665,23 @@ def test_refusals_on_the_gpu():
     whole = cache.k.view(torch.float16).view(-1)[:2 * 2 * D].view(2, 2, D)  # the cache's own bytes
     with pytest.raises(ValueError, match="shares memory"):
         ops.paged_append(cache, whole, torch.zeros_like(whole), batch)
+
+
+def test_rows_of_no_sequence_in_a_long_buffer():
+    """Packed tokens that end long before the buffer does: zeros behind them in new outputs, nothing in given ones."""
+    ops = _ops()
+    D, page, T = 64, 16, 5000
+    table, pages = tables([50, 3], page, 47)
+    cache = on_gpu(empty_cache(pages, 2, page, D, seed=48))
+    q, kv, plan = rand((T, 4, D), torch.bfloat16, 49).cuda(), rand((T, 2, D), torch.bfloat16, 50).cuda(), ops.rotary_plan(D)
+    batch, exact = (ops.PagedBatch(table.cuda(), i32([50, 3]), 6, o) for o in (i32([0, 4, 5]), i32([0, 4, 5])))
+    trash = torch.full((T, 4, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    del trash  # (what a new output may be made of)
+    turned = ops.paged_append(cache, kv, kv, batch, plan, q)
+    given = ops.paged_append(cache, kv, kv, batch, plan, q, q_out=torch.full_like(q, 3.0))
+    assert (turned[5:] == 0).all() and (given[5:] == 3).all() and torch.equal(turned[:5], given[:5])
+    out = ops.attention_paged(turned, cache, batch)
+    assert (out[5:] == 0).all() and torch.equal(out[:5], ops.attention_paged(turned[:5].clone(), cache, exact))
 
 
 # together

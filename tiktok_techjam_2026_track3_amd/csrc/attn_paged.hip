@@ -617,8 +617,8 @@ MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
 // More rows: each wave has 16 NR of its own. A unit's K and V are converted once for the four of them, a quarter by
 // each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
 // buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit.
-// fp16: V's scales are taken relative to the largest so far, so that a block's V fits the type; blocks down to
-// 2^-21 of that are exact.
+// fp16: V's scales are taken relative to the largest up to their own block, so that V fits the type; blocks down to
+// 2^-21 of that are exact. (Up to their own: a later block's scale is not to touch rows that do not see it.)
 template <typename T, int DW, int NR>
 struct Many {
   using Own = Tile<T, DW, NR, 1>;
@@ -689,7 +689,7 @@ struct Many {
       st.vs[0] = w.v_factor(at);
       st.vs[1] = w.v_factor(at + BLOCK);
     };
-    float v_top = 0.0f, v_of[2] = {0.0f, 0.0f}, v_acc = 0.0f;  // RELATIVE: largest V scale so far, of the buffers, of the outputs
+    float v_top = 0.0f, v_of[2][2] = {}, v_acc = 0.0f;  // RELATIVE: largest V scale so far, of the buffers' blocks, of the outputs
     // A unit that goes into buffer `buf`, where some row does not see all of its keys: zeros for V that no row sees and for
     // NaN, whose places are noted.
     const auto sanitize = [&](Stage& st, int at, auto buffer) MI355_LAMBDA_INLINE {
@@ -725,11 +725,11 @@ struct Many {
       constexpr int buf = decltype(buffer)::value;
       float vs[2] = {st.vs[0], st.vs[1]};
       if constexpr (RELATIVE) {
-        v_top = fmaxf(v_top, fmaxf(vs[0], vs[1]));
-        v_of[buf] = v_top;
-        const float r = v_top > 0.0f ? 64.0f / v_top : 1.0f;
-        vs[0] *= r;
-        vs[1] *= r;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          v_of[buf][t] = v_top = fmaxf(v_top, vs[t]);
+          vs[t] *= v_top > 0.0f ? 64.0f / v_top : 1.0f;
+        }
       }
       for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
         constexpr int S = decltype(s)::value;
@@ -762,6 +762,15 @@ struct Many {
         __builtin_amdgcn_sched_group_barrier(0x6 | 0x200 | 0x20, decltype(others)::value, 0);  // ALU, LDS writes, loads
       });
       fence();
+    };
+    const auto relative_to = [&](float v) MI355_LAMBDA_INLINE {
+      if (v == v_acc) return;
+      const float keep = v_acc / v;
+      v_acc = v;
+#pragma unroll
+      for (int m = 0; m < NR; ++m)
+#pragma unroll
+        for (int e = 0; e < ME; ++e) own.acc[m][e] *= keep;
     };
     u32x4 operand[4 * DW];
     const auto read = [&](const u32x4 (&from)[4 * DW][64]) MI355_LAMBDA_INLINE {
@@ -803,15 +812,22 @@ struct Many {
         __builtin_amdgcn_s_setprio(0);
         own.softmax(sc, a, hi, lo);
         __builtin_amdgcn_s_setprio(1);
-        if constexpr (RELATIVE)
-          if (v_of[buf] != v_acc) {
-            const float keep = v_acc / v_of[buf];
-            v_acc = v_of[buf];
+        if constexpr (RELATIVE) {
+          if (v_of[buf][0] != v_of[buf][1]) {  // the unit's first block has another factor: it comes alone
+            relative_to(v_of[buf][0]);
+            pfrag one[NR];
 #pragma unroll
             for (int m = 0; m < NR; ++m)
 #pragma unroll
-              for (int e = 0; e < ME; ++e) own.acc[m][e] *= keep;
+              for (int r = 0; r < 8; ++r) {
+                one[m][r] = r < 4 ? hi[m][r] : T(0.0f);
+                hi[m][r] = r < 4 ? T(0.0f) : hi[m][r];
+              }
+#pragma unroll
+            for (int e = 0; e < ME; ++e) own.add(e, operand[e], one, lo);
           }
+          relative_to(v_of[buf][1]);
+        }
         fence();
 #pragma unroll
         for (int e = 0; e < ME; ++e) own.add(e, operand[e], hi, lo);
