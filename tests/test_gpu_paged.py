@@ -361,6 +361,8 @@ ATTENDS = [
     ([1] * 3, [5000, 40, 1024], 12, 3, 80, 16),
     ([200], [200], 4, 4, 48, 32),
     ([9, 1], [1100, 2080], 16, 4, 96, 256),
+    ([17, 1, 2], [900, 2000, 2], 6, 2, 256, 32),
+    ([90, 3], [90, 1400], 4, 2, 192, 16),
 ]
 
 

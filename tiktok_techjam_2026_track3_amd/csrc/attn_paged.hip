@@ -1,8 +1,8 @@
 // Attention of each sequence's newest tokens over its pages of an e4m3 cache (paged.h), heads grouped:
 //   O[i, h] = sum_j softmax_j(scale Q[i, h] · K[j, h / G]) V[j, h / G],  j <= the token's own position.
 //
-// Rows = (token, query head of a K/V head's group), 16 to a group. A wave takes its keys 32 at a time, straight from
-// memory into registers, without LDS:
+// Rows = (token, query head of a K/V head's group), 16 to a group. A wave takes its keys 32 at a time. Up to 32 rows
+// (Few) K and V go straight from memory into registers, more rows (Many) share what is converted through LDS:
 //   S^T = K · Q^T on 16x16x32 MFMAs. A lane (key l % 16, slice g = l / 16) loads 16 bytes of its key and converts them,
 //     two to an instruction, into the type of q: exact, e4m3 has 4 significant bits. The scale of the block multiplies
 //     the scores in fp32. Which dims make up an MFMA's 32 is free as long as Q is read alike: 64 c + 16 g + ..
@@ -12,6 +12,8 @@
 //     is a P^T operand as it is. For V^T a lane loads the run of dims that it has of the same eight keys; byte pairs of
 //     two keys are put together (v_perm) and converted, the block's scale applied by the conversion. Output row m of
 //     MFMA e is dim m * run + e: a free choice again.
+// Bound by the bytes of K and V up to 32 rows, by instruction issue above: two MFMAs of 8 cycles wait for an exponential, its
+// conversion and their share of the masks and operands.
 // The maximum moves only when a score exceeds it by more than 7 (log2 units), and only then do the four lanes of a row
 // exchange anything. Statistics and sums are fp32.
 //
@@ -689,7 +691,8 @@ struct Many {
       st.vs[0] = w.v_factor(at);
       st.vs[1] = w.v_factor(at + BLOCK);
     };
-    float v_top = 0.0f, v_of[2][2] = {}, v_acc = 0.0f;  // RELATIVE: largest V scale so far, of the buffers' blocks, of the outputs
+    constexpr float LEAST = 0x1p-118f;  // least scale of a block
+    float v_top = LEAST, v_of[2][2] = {}, v_acc = LEAST;  // RELATIVE: largest V scale so far, of the buffers' blocks, of the outputs
     // A unit that goes into buffer `buf`, where some row does not see all of its keys: zeros for V that no row sees and for
     // NaN, whose places are noted.
     const auto sanitize = [&](Stage& st, int at, auto buffer) MI355_LAMBDA_INLINE {
@@ -728,7 +731,7 @@ struct Many {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           v_of[buf][t] = v_top = fmaxf(v_top, vs[t]);
-          vs[t] *= v_top > 0.0f ? 64.0f / v_top : 1.0f;
+          vs[t] *= __uint_as_float((260u << 23) - __float_as_uint(v_top));  // 64 / v_top: powers of two
         }
       }
       for_each<DW>([&](auto s) MI355_LAMBDA_INLINE {
@@ -864,7 +867,7 @@ struct Many {
     }
     if (!active) return;
     if constexpr (RELATIVE) {
-      const float back = v_acc > 0.0f ? v_acc / 64.0f : 1.0f;
+      const float back = v_acc / 64.0f;
 #pragma unroll
       for (int m = 0; m < NR; ++m)
 #pragma unroll
@@ -1072,13 +1075,18 @@ Launch launch_of(const paged::Sizes& z) {
   Launch l{};
   const int64_t rows = z.most * (z.heads / z.kv_heads), dw = (z.head_dim + 63) / 64;
   l.many = rows > 32;
-  l.nr = l.many ? (dw <= 2 ? 2 : 1) : (rows > 16 && dw <= 2 ? 2 : 1);
+  // Groups of 16 rows of a wave. Few rows: as many as there are, where registers allow two. Many: two, which share each operand
+  // that is read; above head dim 128 such a wave has the SIMD for itself, and short tiles leave waves idle: only for
+  // enough rows (us of 16 sequences of 4096 keys, 32 heads of 192 / of 256, one group then two: 64 rows 92 109 / 112 177, 128
+  // rows 156 125 / 186 185, 256 rows 301 230 / 365 340; two of 1024 tokens against 8192 keys 1091 730 / 1221 1002).
+  l.nr = l.many ? (dw <= 2 || rows > 64 * (dw - 2) ? 2 : 1) : (rows > 16 && dw <= 2 ? 2 : 1);
   l.rows = 16 * l.nr * (l.many ? 4 : 1);
   l.row_tiles = (rows + l.rows - 1) / l.rows;
   const int64_t jobs = z.B * z.kv_heads * l.row_tiles;
-  // Sharing the work out evenly takes two work-groups a CU (one above head dim 128, whose registers allow no more; three
-  // or four where they do: 200000 keys of one sequence 92 us instead of 86), partial results and a second launch. A work-group for each job instead where the longest that the table allows is short, or jobs fill
-  // the GPU. Measured (us, shared out / a job each; bf16, 8 K/V heads of 128, groups of 4, K and V in the last-level cache
+  // Sharing the work out evenly takes two work-groups a CU (one above head dim 128, whose registers allow no more: with
+  // two 16 sequences of 8192 keys of 256 dims 102 us instead of 92; three or four where they are allowed: 200000 keys
+  // of one sequence 92 us instead of 86), partial results and a second launch. A work-group for each job instead where
+  // the longest that the table allows is short, or jobs fill the GPU. Measured (us, shared out / a job each; bf16, 8 K/V heads of 128, groups of 4, K and V in the last-level cache
   // but for the largest): one new token, sequences of one length, then of 10 to 100% of it: 2 sequences of 1024 keys 14.5 / 11.3, 2048
   // 17.4 / 16.7, 4096 18.6 / 27.2; 8: 2048 20.2 / 17.8 and 21.0 / 14.8, 4096 25.1 / 28.5 and 21.7 / 23.6; 16: 4096 33.7 / 29.0 and
   // 23.9 / 26.6, 8192 51.4 / 54.4 and 32.1 / 47.1; 64: 4096 110 / 98 and 56 / 59, 8192 201 / 187 and 110 / 130. Many rows: a
@@ -1089,7 +1097,8 @@ Launch launch_of(const paged::Sizes& z) {
   // as what is not kept (us, so / as what is): 64 sequences of up to 9000 keys (655 MB) 121 / 129, 200000 keys (409 MB) 79.4 / 86.0,
   // 128 sequences of 2048 keys (537 MB) 91.5 / 97.6; 1024 keys (268 MB, in that cache) 50.1 / 43.4.
   l.past = !l.many && z.B * room * z.kv_heads * z.head_dim * 2 > int64_t(320) << 20;
-  // (More than 1024 sequences fill the GPU by themselves, and each work-group would go through all their lengths.)
+  // (More than 1024 sequences fill the GPU by themselves, and each work-group would go through all their lengths: 1100 of
+  // up to 300 keys in wide tables, one K/V head, 53.1 / 21.7; 4000 of up to 4000 keys 468 / 411.)
   const bool each = z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048));
   l.groups = each ? 0 : 256 * (dw > 2 ? 1 : 2);
   l.least = 8;
@@ -1115,9 +1124,13 @@ int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
 
 template <typename T, int DW>
 int launch_rows(const PagedArgs& p, const Launch& l, hipStream_t s) {
-  if (l.many) return launch<T, DW, DW <= 2 ? 2 : 1, true>(p, l, s);
-  if constexpr (DW <= 2)
+  if constexpr (DW <= 2) {
+    if (l.many) return launch<T, DW, 2, true>(p, l, s);
     if (l.nr == 2) return launch<T, DW, 2, false>(p, l, s);
+  } else {
+    if (l.many && l.nr == 2) return launch<T, DW, 2, true>(p, l, s);
+    if (l.many) return launch<T, DW, 1, true>(p, l, s);
+  }
   return launch<T, DW, 1, false>(p, l, s);
 }
 
