@@ -886,8 +886,7 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
   const int lane = threadIdx.x & 63, kvh = p.cache.kv_heads, G = p.G;
 
   if (p.zero_tail) {  // rows that no sequence has, shared out by work-group
-    const paged::Sequence last = paged::sequence_of(p.batch, p.batch.B - 1);
-    for (int64_t t = last.first + last.n + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
+    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
       for (int i = threadIdx.x; i < p.heads * p.cache.head_dim; i += 256)
         static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
   }
@@ -1192,7 +1191,7 @@ extern "C" int mi355_attn_paged(int dtype, const void* Q, const uint8_t* cache_k
   p.row_tiles = static_cast<int32_t>(l.row_tiles);
   p.groups = static_cast<int32_t>(l.groups);
   p.least = static_cast<int32_t>(l.least);
-  p.zero_tail = zero_tail;
+  p.zero_tail = zero_tail && (offsets || z.tokens > z.B * z.most);
   p.part = static_cast<float*>(workspace);
   p.ml = p.part + l.groups * 2 * l.rows * z.head_dim;
   p.joins = reinterpret_cast<Head*>(p.ml + l.groups * 2 * l.rows * 2);

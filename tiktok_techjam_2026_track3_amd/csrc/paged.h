@@ -52,6 +52,13 @@ MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
   return s;
 }
 
+// First of the rows that no sequence has: behind the last sequence's.
+MI355_DEVINL int64_t tail_of(const Batch& p) {
+  if (p.offsets == nullptr) return static_cast<int64_t>(p.B) * p.most;
+  const int end = p.offsets[p.B];
+  return end < 0 ? 0 : end;
+}
+
 // The sizes of a call, as both entry points take them.
 struct Sizes {
   int64_t B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride;

@@ -101,8 +101,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   const int b = at / p.blocks, nth = at % p.blocks;
   const paged::Sequence s = paged::sequence_of(p.batch, b);
   if (p.zero_tail) {  // rows that no sequence has, shared out by work-group
-    const paged::Sequence last = paged::sequence_of(p.batch, p.batch.B - 1);
-    for (int64_t t = last.first + last.n + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
+    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
       for (int i = tid; i < p.heads * p.cache.head_dim; i += 256)
         static_cast<T*>(p.qo)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
   }
@@ -315,7 +314,7 @@ extern "C" int mi355_paged_append(int dtype, const void* K, const void* V, const
   p.rot = frequencies ? static_cast<int32_t>(rot_dim) : 0;
   p.interleaved = interleaved;
   p.heads = static_cast<int32_t>(z.heads);
-  p.zero_tail = Q && zero_tail && offsets;  // (without offsets every row has a sequence)
+  p.zero_tail = Q && zero_tail && (offsets || z.tokens > z.B * z.most);
   p.blocks = static_cast<int32_t>((z.most + 2 * BLOCK - 2) / BLOCK);
   // work-groups that share a block's heads: enough to have two a CU, no more than heads can use
   const int64_t groups = z.B * p.blocks;
