@@ -486,11 +486,13 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  *   cache_k, cache_v [pages, kv_heads, page, head_dim] e4m3 (no infinities), contiguous, 16-byte aligned;
  *   k_scale, v_scale [pages, kv_heads, page / 16] fp32 powers of two; an element is its byte's value times the
  *   scale of its block of 16 tokens and head. page: a power of two from 16 to 1024.
- * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32). lens [B] counts a sequence's tokens in the cache, its n new ones included, which are the
- * last. New tokens are packed: sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not
- * decreasing) of Q, K, V and the outputs, `most` at most (those behind it are ignored); offsets NULL:
- * rows b * most .. of `most` each. table, lens and offsets are read on the device, so a captured graph
- * follows their values, and checked there: no value makes an access leave the tensors.
+ *   (Of V's scales only the exponent counts.)
+ * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32). lens [B] counts
+ * a sequence's tokens in the cache, its n new ones included, which are the last. New tokens are packed:
+ * sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not decreasing) of Q, K, V and the outputs,
+ * `most` at most (those behind it are ignored); offsets NULL: rows b * most .. of `most` each. table, lens and
+ * offsets are read on the device, so a captured graph follows their values, and checked there: no value makes
+ * an access leave the tensors.
  *
  * mi355_paged_append writes the new tokens' K and V. K is rotated by its position p (mi355_rotary's formula
  * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q; with zero_tail != 0
@@ -502,10 +504,12 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * several tokens of the batch are to be written to must be one sequence's.
  *
  * mi355_attn_paged: softmax attention of the new tokens: the token at position p sees keys 0 .. p of its
- * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32, probabilities enter P·V
- * as two bf16 terms (off by 2^-16 of each at most), outputs are rounded once. A token that sees no key gives zeros; one that sees a
- * key whose page is missing gives NaN. What pages hold behind lens does not matter, nor do NaN that a
- * token does not see. bf16: |q| below 2^110, |v| below 2^100. workspace (16-byte aligned) holds
+ * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32. Probabilities
+ * enter P·V as two bf16 terms (off by 2^-16 of each at most) where most * heads / kv_heads is at most 32,
+ * rounded once to Q's type above (fp16: V there as multiples of 2^-30 of the largest scale so far). Outputs are
+ * rounded once. A token that sees no key gives zeros; one that sees a key whose page is missing gives NaN. What
+ * pages hold behind lens does not matter, nor do NaN that a token does not see. bf16: |q| below 2^110, |v|
+ * below 2^100. workspace (16-byte aligned) holds
  * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be
  * stream-ordered. Rows behind the last sequence's as above.
  *

@@ -1145,7 +1145,7 @@ PAGED_BLOCK = 16
 class PagedCache:
     """A layer's keys and values in pages, 8 bits each: ``k`` and ``v`` ``[pages, kv_heads, page, head_dim]``
     float8_e4m3fn, ``k_scale`` and ``v_scale`` ``[pages, kv_heads, page / 16]`` fp32, a power of two for each block of
-    16 tokens and head (element = scale * e4m3). All contiguous; ``page`` is a power of two from 16 to 1024."""
+    16 tokens and head (element = scale * e4m3; of V's scales only the exponent counts). All contiguous; ``page`` is a power of two from 16 to 1024."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -1362,8 +1362,8 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale
 
     A token that sees no key gives zeros, one that sees a key without a page (a table entry out of range, a position
     behind the table) NaN. What the pages hold behind ``lens`` does not matter, and a NaN in a key or value reaches
-    the tokens that see it alone. fp32 scores and statistics; probabilities are held in twice bf16's bits, outputs
-    rounded once. bf16 values are to stay below 2^110 in q and 2^100 in V. ``out`` must not share memory with the
+    the tokens that see it alone. fp32 scores and statistics; probabilities are held in twice bf16's bits where
+    ``most * heads // kv_heads`` is at most 32 and rounded once to q's type above; outputs rounded once. bf16 values are to stay below 2^110 in q and 2^100 in V. ``out`` must not share memory with the
     inputs; rows that no sequence has are left in a given ``out``, and zeros in a new one. No derivatives."""
     dev = q.get_device()
     given = out is not None
