@@ -2,8 +2,8 @@
 //   y1 = a (x1 cos t - x2 sin t),  y2 = a (x2 cos t + x1 sin t),  t = position * f_j,
 // j-th pair (x_j, x_{j + rot / 2}) or (x_2j, x_2j+1); elements behind the first rot are copied. fp32, rounded once.
 // Bound by the bytes of x and y: a thread computes the angles of its pairs once and walks over several heads with them, the
-// loads of four under way and those of the first while it computes (4096 tokens of 16 heads of 64 in fp32 9.1 -> 8.0 us). 8192 tokens of 40 heads of 128 in bf16 28.3 us, 5.9 TB/s read and written; 5 tokens 3.6 us of
-// the GPU.
+// loads of four under way and those of the first while it computes (4096 tokens of 16 heads of 64 in fp32 9.1 -> 8.0 us).
+// 8192 tokens of 40 heads of 128 in bf16 28.3 us, 5.9 TB/s read and written; 5 tokens 3.6 us of the GPU.
 #include "rotary.h"
 
 namespace {
