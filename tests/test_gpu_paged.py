@@ -686,6 +686,46 @@ def test_rows_of_no_sequence_in_a_long_buffer():
     assert (out[5:] == 0).all() and torch.equal(out[:5], ops.attention_paged(turned[:5].clone(), cache, exact))
 
 
+def test_nothing_to_do():
+    """No sequences, no rows, no new tokens, tables without columns."""
+    ops = _ops()
+    D, page = 64, 16
+    cache = on_gpu(empty_cache(4, 2, page, D, seed=51))
+    kept = cache.k.view(torch.uint8).clone(), cache.v.view(torch.uint8).clone()
+    plan = ops.rotary_plan(D)
+    none = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    for T, batch in ((0, ops.PagedBatch(none, i32([]))), (5, ops.PagedBatch(none, i32([]), 3, i32([0]))),
+                     (4, ops.PagedBatch(i32([[0], [1]]), i32([3, 9]), 2, i32([0, 0, 0]))),
+                     (0, ops.PagedBatch(i32([[0], [1]]), i32([3, 9]), 0))):
+        q, kv = rand((T, 4, D), torch.float16, 52).cuda(), rand((T, 2, D), torch.float16, 53).cuda()
+        for got in (ops.attention_paged(q, cache, batch), ops.paged_append(cache, kv, kv, batch, plan, q)):
+            assert got.shape == q.shape and not got.any()
+        given = torch.full_like(q, 2.0)
+        ops.attention_paged(q, cache, batch, out=given)
+        ops.paged_append(cache, kv, kv, batch, plan, q, q_out=given)
+        assert (given == 2).all()
+    q, kv = rand((2, 4, D), torch.float16, 54).cuda(), rand((2, 2, D), torch.float16, 55).cuda()
+    batch = ops.PagedBatch(torch.zeros(2, 0, dtype=torch.int32, device="cuda"), i32([1, 5]))
+    assert ops.attention_paged(q, cache, batch).isnan().all()
+    turned = ops.paged_append(cache, kv, kv, batch, plan, q)
+    assert torch.equal(turned, ops.rotary(q, torch.tensor([0, 4], device="cuda"), plan))
+    assert torch.equal(cache.k.view(torch.uint8), kept[0]) and torch.equal(cache.v.view(torch.uint8), kept[1])
+
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    ops = _ops()
+    cache = on_gpu(empty_cache(2, 2, 16, 64, seed=56))
+    batch = ops.PagedBatch(i32([[0], [1]]), i32([3, 4]))
+    q, kv = rand((2, 4, 64), torch.float16, 57).cuda(), rand((2, 2, 64), torch.float16, 58).cuda()
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(ValueError):
+            ops.attention_paged(dual, cache, batch)
+        with pytest.raises(ValueError):
+            ops.paged_append(cache, kv, kv, batch, ops.rotary_plan(64), dual)
+
+
 # together
 
 @pytest.mark.parametrize("wide", [False, True])
