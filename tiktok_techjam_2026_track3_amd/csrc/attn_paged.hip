@@ -994,16 +994,17 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
 }
 
 // Joins the parts of the jobs that several work-groups had: a work-group with a first part (blockIdx.x) and a row of its
-// job's tile, or WAVES = 1 four rows. A row's waves take every WAVES-th part, several requested at a time; lanes have runs
-// of four dims. Few rows have many parts, tiles of many rows few.
-template <typename T, int WAVES>
+// job's tile, or WAVES = 1 four waves of rows, LANES lanes a row. A row's waves take every WAVES-th part, several requested
+// at a time; lanes have runs of four dims. Few rows have many parts, tiles of many rows few.
+template <typename T, int WAVES, int LANES>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_tile) {
   __shared__ float lds[WAVES][256];
   __shared__ float lds_ml[4][2];
   constexpr int AHEAD = WAVES == 1 ? 4 : 8;
   const int w = blockIdx.x, hd = p.cache.head_dim, G = p.G;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int in_tile = WAVES == 1 ? blockIdx.y * 4 + wave : blockIdx.y;
+  static_assert(WAVES == 1 || LANES == 64, "");
+  const int lane = threadIdx.x & (LANES - 1), wave = threadIdx.x >> 6;
+  const int in_tile = WAVES == 1 ? blockIdx.y * (256 / LANES) + threadIdx.x / LANES : blockIdx.y;
   const Head j = p.joins[w];
   if (j.parts == 0) return;
   const Rows rows = rows_of(p, j.s);
@@ -1029,9 +1030,9 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
   };
   fetch(first);  // (under way while the maximum is made)
   float m = NEG_INF;
-  for (int k = WAVES == 1 ? lane : static_cast<int>(threadIdx.x); k < parts; k += 64 * WAVES) m = fmaxf(m, p.ml[2 * slot(k)]);
+  for (int k = WAVES == 1 ? lane : static_cast<int>(threadIdx.x); k < parts; k += LANES * WAVES) m = fmaxf(m, p.ml[2 * slot(k)]);
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  for (int off = LANES / 2; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   if constexpr (WAVES == 4) {
     if (lane == 0) lds_ml[wave][0] = m;
     __syncthreads();
@@ -1118,10 +1119,12 @@ int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
   if (!l.past) attn_paged_kernel<T, DW, NR, MANY, 0><<<grid, 256, 0, s>>>(p);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || l.groups == 0) return static_cast<int>(e);
   const int64_t rows = std::min<int64_t>(l.rows, p.batch.most * static_cast<int64_t>(p.G));
-  if constexpr (MANY)
-    attn_paged_join<T, 1><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>((rows + 3) / 4)), 256, 0, s>>>(p, l.rows);
-  else
-    attn_paged_join<T, 4><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>(rows)), 256, 0, s>>>(p, l.rows);
+  if constexpr (MANY) {
+    constexpr int LANES = DW == 1 ? 16 : DW == 2 ? 32 : 64, PER = 256 / LANES;
+    attn_paged_join<T, 1, LANES><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>((rows + PER - 1) / PER)), 256, 0, s>>>(p, l.rows);
+  } else {
+    attn_paged_join<T, 4, 64><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>(rows)), 256, 0, s>>>(p, l.rows);
+  }
   return static_cast<int>(hipGetLastError());
 }
 
