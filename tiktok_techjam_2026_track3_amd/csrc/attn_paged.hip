@@ -418,7 +418,7 @@ struct Window {
 
 // Up to 16 NR rows: the four waves have the same rows and a quarter of the keys each, and are joined through LDS. K and V
 // are waited for; a unit's bytes are requested as soon as the registers of those before it are free. 64 sequences of 0.9k to
-// 9k keys (8 K/V heads of 128, 655 MB) 116 us and 5 of the join, 5.4 TB/s in all; 200000 keys of one 71 and 7. Operands
+// 9k keys (8 K/V heads of 128, 655 MB) 116 us and 5 of the join, 5.4 TB/s in all; 200000 keys of one 71 and 5. Operands
 // through LDS or a second unit in flight gave nothing: the bytes on their way already cover the latency.
 template <typename T, int DW, int NR, int AUX>
 struct Few {
@@ -621,8 +621,8 @@ MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
 // each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
 // buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit. Each wave on its
 // own (as in Few) converted all of K and V four times: two pieces of 1024 tokens against 12000 keys (32/8 heads of 128)
-// 1039 us, so 335 and 21 of the join: 850 TFLOP/s, matrix cores busy a third of the time, exponentials and conversions
-// most of the rest. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
+// 1039 us, so 338 and 15 of the join: 860 TFLOP/s, matrix cores busy 40% of the time, exponentials and conversions most of
+// the rest. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
 // fp16: V's scales are taken relative to the largest up to their own block, so that V fits the type; blocks down to
 // 2^-21 of that are exact. (Up to their own: a later block's scale is not to touch rows that do not see it.)
 template <typename T, int DW, int NR>
@@ -994,17 +994,17 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
 }
 
 // Joins the parts of the jobs that several work-groups had: a work-group with a first part (blockIdx.x) and a row of its
-// job's tile, or WAVES = 1 four waves of rows, LANES lanes a row. A row's waves take every WAVES-th part, several requested
-// at a time; lanes have runs of four dims. Few rows have many parts, tiles of many rows few.
-template <typename T, int WAVES, int LANES>
+// job's tile, whose parts its runs of LANES lanes share (SPLIT: few rows have many parts), or a row for each run (tiles of
+// many rows have few). Several parts of a run are requested at a time; lanes have runs of four dims. 64 parts of 32 rows of
+// 128 dims 5 us, 2 of 128 rows of 450 tiles (67 MB) 15.
+template <typename T, bool SPLIT, int LANES>
 __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_tile) {
-  __shared__ float lds[WAVES][256];
-  __shared__ float lds_ml[4][2];
-  constexpr int AHEAD = WAVES == 1 ? 4 : 8;
+  constexpr int AHEAD = SPLIT ? 8 : 4, RUNS = 256 / LANES, STEP = SPLIT ? RUNS : 1;
+  __shared__ float lds[RUNS][4 * LANES];
+  __shared__ float lds_m[4], lds_z[RUNS];
   const int w = blockIdx.x, hd = p.cache.head_dim, G = p.G;
-  static_assert(WAVES == 1 || LANES == 64, "");
-  const int lane = threadIdx.x & (LANES - 1), wave = threadIdx.x >> 6;
-  const int in_tile = WAVES == 1 ? blockIdx.y * (256 / LANES) + threadIdx.x / LANES : blockIdx.y;
+  const int lane = threadIdx.x % LANES, run = threadIdx.x / LANES, wave = threadIdx.x >> 6;
+  const int in_tile = SPLIT ? blockIdx.y : blockIdx.y * RUNS + run;
   const Head j = p.joins[w];
   if (j.parts == 0) return;
   const Rows rows = rows_of(p, j.s);
@@ -1015,14 +1015,14 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
     return s * rows_of_tile + in_ws;
   };
   const int parts = (j.parts < p.groups - w ? j.parts : p.groups - 1 - w) + 1;
-  const int first = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(wave), d4 = 4 * lane < hd ? 4 * lane : 0;
+  const int first = SPLIT ? run : 0, d4 = 4 * lane < hd ? 4 * lane : 0;
   f32x4 v[AHEAD];
   float top[AHEAD], sum[AHEAD];
   const auto fetch = [&](int k0) MI355_LAMBDA_INLINE {
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x) {
-      if (k0 + WAVES * x >= parts) break;
-      const int64_t at = slot(k0 + WAVES * x);
+      if (k0 + STEP * x >= parts) break;
+      const int64_t at = slot(k0 + STEP * x);
       v[x] = *reinterpret_cast<const f32x4*>(p.part + at * hd + d4);
       top[x] = p.ml[2 * at];
       sum[x] = p.ml[2 * at + 1];
@@ -1030,36 +1030,39 @@ __global__ __launch_bounds__(256) void attn_paged_join(PagedArgs p, int rows_of_
   };
   fetch(first);  // (under way while the maximum is made)
   float m = NEG_INF;
-  for (int k = WAVES == 1 ? lane : static_cast<int>(threadIdx.x); k < parts; k += LANES * WAVES) m = fmaxf(m, p.ml[2 * slot(k)]);
+  for (int k = SPLIT ? static_cast<int>(threadIdx.x) : lane; k < parts; k += SPLIT ? 256 : LANES) m = fmaxf(m, p.ml[2 * slot(k)]);
 #pragma unroll
-  for (int off = LANES / 2; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  if constexpr (WAVES == 4) {
-    if (lane == 0) lds_ml[wave][0] = m;
+  for (int off = SPLIT ? 32 : LANES / 2; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  if constexpr (SPLIT) {
+    if ((threadIdx.x & 63) == 0) lds_m[wave] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(lds_ml[0][0], lds_ml[1][0]), fmaxf(lds_ml[2][0], lds_ml[3][0]));
+    m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
   }
   const auto factor = [&](float t) MI355_LAMBDA_INLINE { return t == NEG_INF ? 1.0f : fast_exp2(t - m); };
   float z = 0.0f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = first; k0 < parts; k0 += WAVES * AHEAD) {
+  for (int k0 = first; k0 < parts; k0 += STEP * AHEAD) {
     if (k0 != first) fetch(k0);
 #pragma unroll
     for (int x = 0; x < AHEAD; ++x) {
-      if (k0 + WAVES * x >= parts) break;
+      if (k0 + STEP * x >= parts) break;
       const float f = factor(top[x]);
       z += sum[x] * f;
       a += v[x] * f;
     }
   }
-  if constexpr (WAVES == 4) {
-    *reinterpret_cast<f32x4*>(&lds[wave][4 * lane]) = a;
-    if (lane == 0) lds_ml[wave][1] = z;
+  if constexpr (SPLIT) {
+    *reinterpret_cast<f32x4*>(&lds[run][4 * lane]) = a;
+    if (lane == 0) lds_z[run] = z;
     __syncthreads();
-    if (wave != 0) return;
-    z = lds_ml[0][1] + lds_ml[1][1] + lds_ml[2][1] + lds_ml[3][1];
+    if (run != 0) return;
+    z = 0.0f;
     a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a += *reinterpret_cast<const f32x4*>(&lds[k][4 * lane]);
+    for (int k = 0; k < RUNS; ++k) {
+      z += lds_z[k];
+      a += *reinterpret_cast<const f32x4*>(&lds[k][4 * lane]);
+    }
   }
   if (r >= rows.nrows || in_tile >= rows_of_tile || 4 * lane >= hd) return;
   const float inv = rows.inverse(z, rows.lim(r, G));
@@ -1119,12 +1122,9 @@ int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
   if (!l.past) attn_paged_kernel<T, DW, NR, MANY, 0><<<grid, 256, 0, s>>>(p);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || l.groups == 0) return static_cast<int>(e);
   const int64_t rows = std::min<int64_t>(l.rows, p.batch.most * static_cast<int64_t>(p.G));
-  if constexpr (MANY) {
-    constexpr int LANES = DW == 1 ? 16 : DW == 2 ? 32 : 64, PER = 256 / LANES;
-    attn_paged_join<T, 1, LANES><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>((rows + PER - 1) / PER)), 256, 0, s>>>(p, l.rows);
-  } else {
-    attn_paged_join<T, 4, 64><<<dim3(static_cast<uint32_t>(l.groups), static_cast<uint32_t>(rows)), 256, 0, s>>>(p, l.rows);
-  }
+  constexpr int LANES = DW == 1 ? 16 : DW == 2 ? 32 : 64, PER = MANY ? 256 / LANES : 1;
+  const dim3 grid_of_join(static_cast<uint32_t>(l.groups), static_cast<uint32_t>((rows + PER - 1) / PER));
+  attn_paged_join<T, !MANY, LANES><<<grid_of_join, 256, 0, s>>>(p, l.rows);
   return static_cast<int>(hipGetLastError());
 }
 
