@@ -621,8 +621,8 @@ MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
 // each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
 // buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit. Each wave on its
 // own (as in Few) converted all of K and V four times: two pieces of 1024 tokens against 12000 keys (32/8 heads of 128)
-// 1039 us, so 338 and 15 of the join: 860 TFLOP/s, matrix cores busy 40% of the time, exponentials and conversions most of
-// the rest. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
+// 1039 us, so 338 and 15 of the join: 860 TFLOP/s, matrix cores busy 36% of the time and the vector ALU 48%,
+// hardly at once with the two waves that a SIMD's registers hold. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
 // fp16: V's scales are taken relative to the largest up to their own block, so that V fits the type; blocks down to
 // 2^-21 of that are exact. (Up to their own: a later block's scale is not to touch rows that do not see it.)
 template <typename T, int DW, int NR>
