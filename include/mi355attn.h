@@ -501,7 +501,7 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens); elements are
  * rounded to nearest even, infinities and NaN become NaN; when the scale grows, the block's older elements are
  * rounded to it anew. Tokens whose page is none of [0, pages), or behind the table, are not written. A page that
- * several tokens of the batch are to be written to must be one sequence's.
+ * is written must be in one sequence's table, once; pages that are only read may be in many.
  *
  * mi355_attn_paged: softmax attention of the new tokens: the token at position p sees keys 0 .. p of its
  * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32. Probabilities

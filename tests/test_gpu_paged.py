@@ -686,6 +686,19 @@ def test_rows_of_no_sequence_in_a_long_buffer():
     assert (out[5:] == 0).all() and torch.equal(out[:5], ops.attention_paged(turned[:5].clone(), cache, exact))
 
 
+@pytest.mark.parametrize("most", [1, 40])
+def test_pages_in_several_tables(most):
+    """A shared beginning, and a page twice in one table."""
+    ops = _ops()
+    D, page, lens = 96, 32, [100, 130, 128]
+    table = torch.tensor([[5, 2, 7, 1, 0], [5, 2, 7, 3, 6], [4, 4, 5, 4, 9]], dtype=torch.int32)
+    cache = empty_cache(10, 2, page, D, seed=59)
+    q = rand((3 * most, 4, D), torch.bfloat16, 60)
+    ref, tol = attention64(q, cache, table, lens, [most * i for i in range(4)], D ** -0.5)
+    for t in (table, widened(table, page)):
+        check(ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(t.cuda(), i32(lens), most)), ref, tol)
+
+
 def test_nothing_to_do():
     """No sequences, no rows, no new tokens, tables without columns."""
     ops = _ops()

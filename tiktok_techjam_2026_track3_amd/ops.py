@@ -1291,8 +1291,8 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: Pag
     A block's scale is the least power of two with which its largest new element stays within e4m3's 448 (at least 2^-118),
     or the one it had where that is larger; when it grows, the block's earlier tokens are rounded to it anew.
     Elements are rounded to nearest even from fp32, once; infinities and NaN are held as NaN and leave the scale
-    alone. Tokens without a page (a table entry out of range, a position behind the table) are not written. Each page
-    that is written must be one sequence's. ``q_out`` may be ``q``; rows that no sequence has are left
+    alone. Tokens without a page (a table entry out of range, a position behind the table) are not written. A page
+    that is written must be in one sequence's table, once (pages that are only read may be in many). ``q_out`` may be ``q``; rows that no sequence has are left
     in a given ``q_out``, and zeros in a new one. No derivatives."""
     dev, held_k, given = k.get_device(), cache.k, q_out is not None
     if dev < 0 or v.get_device() != dev or held_k.get_device() != dev or batch.table.get_device() != dev or (
