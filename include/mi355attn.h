@@ -490,9 +490,9 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * Token p of sequence b is row p % page of page table[b, p / page] (table [B, width] int32). lens [B] counts
  * a sequence's tokens in the cache, its n new ones included, which are the last. New tokens are packed:
  * sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not decreasing) of Q, K, V and the outputs,
- * `most` at most (those behind it are ignored); offsets NULL: rows b * most .. of `most` each. table, lens and
- * offsets are read on the device, so a captured graph follows their values, and checked there: no value makes
- * an access leave the tensors.
+ * `most` at most (those behind it are left out, as if neither the offsets nor lens counted them); offsets NULL: rows
+ * b * most .. of `most` each. table, lens and offsets are read on the device, so a captured graph follows their
+ * values, and checked there: no value makes an access leave the tensors.
  *
  * mi355_paged_append writes the new tokens' K and V. K is rotated by its position p (mi355_rotary's formula
  * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q; with zero_tail != 0

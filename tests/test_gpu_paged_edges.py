@@ -1,0 +1,114 @@
+"""The paged cache's operators at their edges, against plain arithmetic in 64 bits (paged_reference) and themselves."""
+
+import pytest
+import torch
+
+from paged_reference import attention64, check, empty_cache, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _ops():
+    from tiktok_techjam_2026_track3_amd import ops
+    return ops
+
+
+def on_gpu(cache):
+    return _ops().PagedCache(*[t.cuda() for t in cache])
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def tables(tokens, page, seed, wide):
+    """(table, pages): every sequence has pages of its own for so many tokens, in any order; wide: with room for 2^17 tokens of
+    pages that do not exist, so that the work is shared out evenly."""
+    width = max(1, -(-max(tokens) // page))
+    pages = len(tokens) * width + 2
+    g = torch.Generator().manual_seed(seed)
+    table = torch.randperm(pages, generator=g)[:len(tokens) * width].to(torch.int32).view(len(tokens), width)
+    if wide:
+        table = torch.cat((table, torch.full((len(tokens), (1 << 17) // page - width), -1, dtype=torch.int32)), 1)
+    return table, pages
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("B", [3, 70])
+@pytest.mark.parametrize("most", [3, 40])
+def test_more_tokens_than_most(most, B, wide):
+    """Those behind the first `most` of a sequence are left out, as if neither the offsets nor the lengths counted them."""
+    ops = _ops()
+    D, page = 64, 16
+    rng = torch.Generator().manual_seed(70)
+    new = [most + 300, 2, most, 0, most + 1][:B] + [int(n) for n in torch.randint(0, most + 3, (max(0, B - 5),), generator=rng)]
+    offsets = [4]
+    for n in new:
+        offsets.append(offsets[-1] + n)
+    T = offsets[-1] + 5
+    cut = [max(0, n - most) for n in new]
+    lens = [n + 7 + 11 * (b % 4) for b, n in enumerate(new)]
+    kept_lens = [m - c for m, c in zip(lens, cut)]
+    kept = [r for a, n, c in zip(offsets, new, cut) for r in range(a, a + n - c)]
+    packed = [0]
+    for n, c in zip(new, cut):
+        packed.append(packed[-1] + n - c)
+    others = sorted(set(range(T)) - set(kept))
+    table, pages = tables(kept_lens, page, 71, wide)
+    cache = empty_cache(pages, 2, page, D, seed=72)
+    q, k, v = rand((T, 4, D), torch.bfloat16, 73).cuda(), rand((T, 2, D), torch.bfloat16, 74).cuda(), rand((T, 2, D), torch.bfloat16, 75).cuda()
+    plan = ops.rotary_plan(D)
+    batch = ops.PagedBatch(table.cuda(), i32(lens), most, i32(offsets))
+    alone = ops.PagedBatch(table.cuda(), i32(kept_lens), most, i32(packed))
+    dev, want = on_gpu(cache), on_gpu(cache)
+    ref = ops.paged_append(want, k[kept], v[kept], alone, plan, q[kept])
+    turned = ops.paged_append(dev, k, v, batch, plan, q)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(dev, name).view(torch.uint8), getattr(want, name).view(torch.uint8)), name
+    assert torch.equal(turned[kept], ref)
+    given = ops.paged_append(on_gpu(cache), k, v, batch, plan, q, q_out=torch.full_like(q, 3.0))
+    assert torch.equal(given[kept], ref) and (given[others] == 3).all()
+
+    out = ops.attention_paged(turned, dev, batch)
+    cpu = tuple(getattr(want, name).cpu() for name in ("k", "v", "k_scale", "v_scale"))
+    check(out[kept], *attention64(ref.cpu(), cpu, table, kept_lens, packed, D ** -0.5, most))
+    assert torch.equal(out[kept], ops.attention_paged(ref, want, alone))
+    given = ops.attention_paged(turned, dev, batch, out=torch.full_like(q, 3.0))
+    assert torch.equal(given[kept], out[kept]) and (given[others] == 3).all()
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("most", [3, 40])
+def test_more_tokens_than_most_in_replays(most, wide):
+    """A captured step whose offsets and lengths outgrow `most` later, and come back."""
+    ops = _ops()
+    D, page, T = 64, 16, 2 * most + 20
+    table, pages = tables([150, 150], page, 76, wide)
+    plan = ops.rotary_plan(D)
+    q, kv = rand((T, 4, D), torch.float16, 77).cuda(), rand((T, 2, D), torch.float16, 78).cuda()
+    cache = empty_cache(pages, 2, page, D, seed=79)
+    dev = on_gpu(cache)
+    lens, offsets = i32([100, 90]), i32([0, most, 2 * most])
+    batch = ops.PagedBatch(table.cuda(), lens, most, offsets)
+
+    def step(c):
+        turned = ops.paged_append(c, kv, kv, batch, plan, q)
+        return turned, ops.attention_paged(turned, c, batch)
+
+    step(dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turned, out = step(dev)
+    for at, n in (([0, most, 2 * most], [100, 90]), ([0, most + 9, 2 * most + 10], [101, 95]), ([2, 3, 2 * most + 20], [60, 120]),
+                  ([0, most, 2 * most], [100, 90]), ([0, 2 * most + 20, 2 * most + 20], [130, 5])):
+        lens.copy_(i32(n))
+        offsets.copy_(i32(at))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = turned.clone(), out.clone()
+        kept = [r for r in range(T) if any(a <= r < min(b, a + most) for a, b in zip(at, at[1:]))]
+        copy = ops.PagedCache(dev.k.clone(), dev.v.clone(), dev.k_scale.clone(), dev.v_scale.clone())
+        eager = step(copy)
+        assert torch.equal(got[0][kept], eager[0][kept])
+        assert torch.equal(got[1][kept], eager[1][kept])

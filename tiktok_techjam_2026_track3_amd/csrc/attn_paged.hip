@@ -168,7 +168,7 @@ MI355_DEVINL Rows rows_at(const PagedArgs& p, const paged::Sequence& near, int b
   if (b >= 64) return rows_of(p, paged::sequence_of(p.batch, b));
   return rows_of(p, paged::Sequence{static_cast<int32_t>(__builtin_amdgcn_readlane(near.first, b)),
                                     static_cast<int32_t>(__builtin_amdgcn_readlane(near.n, b)),
-                                    static_cast<int32_t>(__builtin_amdgcn_readlane(near.len, b))});
+                                    static_cast<int32_t>(__builtin_amdgcn_readlane(near.len, b)), 0});
 }
 
 MI355_DEVINL int64_t quotient(int64_t n, int64_t d) {  // of what is not negative, mostly of 32 bits
@@ -899,8 +899,8 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
   int b = 0, h, tile, u0, w = blockIdx.x;
   int64_t each = 0, left;
   Rows rows;
-  Head head{{0, 0, 0}, 0, 0, 0};
-  paged::Sequence near{0, 0, 0};  // lane l has sequence l
+  Head head{{0, 0, 0, 0}, 0, 0, 0};
+  paged::Sequence near{0, 0, 0, 0};  // lane l has sequence l
   if (p.groups == 0) {
     const int heads = p.batch.B * kvh;  // (later tiles see more keys: they come first)
     tile = p.row_tiles - 1 - w / heads;
@@ -916,7 +916,7 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
     // units of the sequences for one head, 64 at a time: of the lane's, and up to it
     int64_t mine = 0, upto;
     const auto scan = [&](int b0) MI355_LAMBDA_INLINE {
-      paged::Sequence s{0, 0, 0};
+      paged::Sequence s{0, 0, 0, 0};
       if (b0 + lane < p.batch.B) s = paged::sequence_of(p.batch, b0 + lane);
       mine = b0 + lane < p.batch.B ? all_units(rows_of(p, s), K::ROWS, G) : 0;
       upto = mine;

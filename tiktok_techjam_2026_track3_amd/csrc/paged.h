@@ -35,6 +35,7 @@ struct Batch {
 struct Sequence {
   int32_t first, n;  // its new tokens are first .. first + n
   int32_t len;       // tokens with them
+  int32_t cut;       // rows behind them that the offsets give it beyond `most`: left out, as if len did not count them either
 };
 
 MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
@@ -43,11 +44,14 @@ MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
   if (p.offsets == nullptr) {
     s.first = b * p.most;
     s.n = p.most;
+    s.cut = 0;
   } else {
     const int lo = p.offsets[b], hi = p.offsets[b + 1];
     s.first = lo < 0 ? 0 : (lo < p.tokens ? lo : p.tokens);
     const int end = hi < s.first ? s.first : (hi < p.tokens ? hi : p.tokens);
     s.n = end - s.first < p.most ? end - s.first : p.most;
+    s.cut = end - s.first - s.n;
+    s.len = s.len < -0x7fffffff + s.cut ? -0x7fffffff : s.len - s.cut;
   }
   return s;
 }
