@@ -491,14 +491,15 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * a sequence's tokens in the cache, its n new ones included, which are the last. New tokens are packed:
  * sequence b's are rows offsets[b] .. offsets[b + 1] ([B + 1] int32, not decreasing) of Q, K, V and the outputs,
  * `most` at most (those behind it are left out, as if neither the offsets nor lens counted them); offsets NULL: rows
- * b * most .. of `most` each. table, lens and offsets are read on the device, so a captured graph follows their
- * values, and checked there: no value makes an access leave the tensors.
+ * b * most .. of `most` each. Rows that no sequence has (behind the last one's, before the first one's, left out)
+ * become zeros in the outputs with zero_tail != 0 and are left otherwise. table, lens and offsets are read on
+ * the device, so a captured graph follows their values, and checked there: no value makes an access leave the
+ * tensors.
  *
  * mi355_paged_append writes the new tokens' K and V. K is rotated by its position p (mi355_rotary's formula
- * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q; with zero_tail != 0
- * rows behind the last sequence's become zeros, otherwise they are left). Rotated values are not rounded before
- * they are quantised: with m the largest finite magnitude of a block's new elements, the scale becomes
- * max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens); elements are
+ * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q). Rotated values
+ * are not rounded before they are quantised: with m the largest finite magnitude of a block's new elements, the
+ * scale becomes max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens); elements are
  * rounded to nearest even, infinities and NaN become NaN; when the scale grows, the block's older elements are
  * rounded to it anew. Tokens whose page is none of [0, pages), or behind the table, are not written. A page that
  * is written must be in one sequence's table, once; pages that are only read may be in many.
@@ -511,7 +512,7 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * pages hold behind lens does not matter, nor do NaN that a token does not see. bf16: |q| below 2^110, |v|
  * below 2^100. workspace (16-byte aligned) holds
  * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be
- * stream-ordered. Rows behind the last sequence's as above.
+ * stream-ordered.
  *
  * Both: dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256; rot_dim a multiple of 8.
  * sizes = {B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride}, strides = {token, head} of K,

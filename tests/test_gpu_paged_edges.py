@@ -33,11 +33,18 @@ def tables(tokens, page, seed, wide):
     return table, pages
 
 
+def poison(q):
+    """Fills and frees memory that a new output of q's size may be made of."""
+    trash = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    del trash
+
+
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("B", [3, 70])
 @pytest.mark.parametrize("most", [3, 40])
 def test_more_tokens_than_most(most, B, wide):
-    """Those behind the first `most` of a sequence are left out, as if neither the offsets nor the lengths counted them."""
+    """Those behind the first `most` of a sequence are left out, as if neither the offsets nor the lengths counted them;
+    their rows, and those before the first sequence's, are zeros in new outputs and left in given ones."""
     ops = _ops()
     D, page = 64, 16
     rng = torch.Generator().manual_seed(70)
@@ -62,14 +69,17 @@ def test_more_tokens_than_most(most, B, wide):
     alone = ops.PagedBatch(table.cuda(), i32(kept_lens), most, i32(packed))
     dev, want = on_gpu(cache), on_gpu(cache)
     ref = ops.paged_append(want, k[kept], v[kept], alone, plan, q[kept])
+    poison(q)
     turned = ops.paged_append(dev, k, v, batch, plan, q)
     for name in ("k", "v", "k_scale", "v_scale"):
         assert torch.equal(getattr(dev, name).view(torch.uint8), getattr(want, name).view(torch.uint8)), name
-    assert torch.equal(turned[kept], ref)
+    assert torch.equal(turned[kept], ref) and not turned[others].any()
     given = ops.paged_append(on_gpu(cache), k, v, batch, plan, q, q_out=torch.full_like(q, 3.0))
     assert torch.equal(given[kept], ref) and (given[others] == 3).all()
 
+    poison(q)
     out = ops.attention_paged(turned, dev, batch)
+    assert not out[others].any()
     cpu = tuple(getattr(want, name).cpu() for name in ("k", "v", "k_scale", "v_scale"))
     check(out[kept], *attention64(ref.cpu(), cpu, table, kept_lens, packed, D ** -0.5, most))
     assert torch.equal(out[kept], ops.attention_paged(ref, want, alone))
@@ -107,8 +117,9 @@ def test_more_tokens_than_most_in_replays(most, wide):
         graph.replay()
         torch.cuda.synchronize()
         got = turned.clone(), out.clone()
-        kept = [r for r in range(T) if any(a <= r < min(b, a + most) for a, b in zip(at, at[1:]))]
+        others = [r for r in range(T) if not any(a <= r < min(b, a + most) for a, b in zip(at, at[1:]))]
+        assert not got[0][others].any() and not got[1][others].any()
         copy = ops.PagedCache(dev.k.clone(), dev.v.clone(), dev.k_scale.clone(), dev.v_scale.clone())
         eager = step(copy)
-        assert torch.equal(got[0][kept], eager[0][kept])
-        assert torch.equal(got[1][kept], eager[1][kept])
+        assert torch.equal(got[0], eager[0])
+        assert torch.equal(got[1], eager[1])

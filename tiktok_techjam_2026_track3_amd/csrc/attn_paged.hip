@@ -889,11 +889,14 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
   __shared__ typename K::Lds lds;
   const int lane = threadIdx.x & 63, kvh = p.cache.kv_heads, G = p.G;
 
-  if (p.zero_tail) {  // rows that no sequence has, shared out by work-group
-    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
-      for (int i = threadIdx.x; i < p.heads * p.cache.head_dim; i += 256)
-        static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
-  }
+  // rows that no sequence has, shared out by work-group: those behind all here, others where their sequence is met
+  const auto zero = [&](int64_t t, int i0, int step) MI355_LAMBDA_INLINE {
+    for (int i = i0; i < p.heads * p.cache.head_dim; i += step)
+      static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
+  };
+  const auto of_wave = [&](int64_t t) MI355_LAMBDA_INLINE { zero(t, lane, 64); };
+  if (p.zero_tail)
+    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x) zero(t, threadIdx.x, 256);
 
   // the work-group's run of units: [x, x + left) of all, or one job whole
   int b = 0, h, tile, u0, w = blockIdx.x;
@@ -906,7 +909,13 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
     tile = p.row_tiles - 1 - w / heads;
     h = w % heads % kvh;
     b = w % heads / kvh;
-    rows = rows_of(p, paged::sequence_of(p.batch, b));
+    const paged::Sequence s = paged::sequence_of(p.batch, b);
+    if (p.zero_tail) {
+      const int worker = tile * kvh + h, workers = p.row_tiles * kvh;
+      if (b == 0 && s.first > 0) paged::zero_rows(p.batch, 0, s.first, worker, workers, of_wave);
+      if (s.cut > 0) paged::zero_rows(p.batch, s.first + s.n, static_cast<int64_t>(s.first) + s.n + s.cut, worker, workers, of_wave);
+    }
+    rows = rows_of(p, s);
     if (tile * K::ROWS >= rows.nrows) return;
     u0 = 0;
     left = rows.units((tile + 1) * K::ROWS, G);
@@ -927,11 +936,22 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
       }
       return s;
     };
+    const auto zero_between = [&](const paged::Sequence& s) MI355_LAMBDA_INLINE {  // what is cut off a lane's sequence
+      if (!p.zero_tail) return;
+      for (uint64_t left = __ballot(s.cut > 0); left; left &= left - 1) {
+        const int l = __builtin_ctzll(left);
+        const int64_t from = static_cast<int64_t>(__shfl(s.first, l)) + __shfl(s.n, l);
+        paged::zero_rows(p.batch, from, from + __shfl(s.cut, l), blockIdx.x, gridDim.x, of_wave);
+      }
+    };
     near = scan(0);
+    zero_between(near);
+    if (const int first = __builtin_amdgcn_readfirstlane(near.first); p.zero_tail && first > 0)
+      paged::zero_rows(p.batch, 0, first, blockIdx.x, gridDim.x, of_wave);
     const int64_t mine0 = mine, upto0 = upto;
     int64_t total = first_lane(__shfl(upto, 63));
     for (int b0 = 64; b0 < p.batch.B; b0 += 64) {
-      scan(b0);
+      zero_between(scan(b0));
       total += first_lane(__shfl(upto, 63));
     }
     total *= kvh;

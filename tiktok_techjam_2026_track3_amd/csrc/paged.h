@@ -56,11 +56,27 @@ MI355_DEVINL Sequence sequence_of(const Batch& p, int b) {
   return s;
 }
 
-// First of the rows that no sequence has: behind the last sequence's.
+// Rows that no sequence has, of a new output: those behind the last one's, those before the first one's, and what is cut
+// off each. First of those behind:
 MI355_DEVINL int64_t tail_of(const Batch& p) {
   if (p.offsets == nullptr) return static_cast<int64_t>(p.B) * p.most;
   const int end = p.offsets[p.B];
   return end < 0 ? 0 : end;
+}
+
+// Zeros (zero(t), by all lanes of a wave) for the rows [from, to) that no sequence has, shared out by the waves of `workers`
+// work-groups of 256. Offsets that decrease may have given them to another sequence, so each row is looked for.
+template <typename Zero>
+MI355_DEVINL void zero_rows(const Batch& p, int64_t from, int64_t to, int64_t worker, int64_t workers, Zero zero) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t t = from + 4 * worker + (threadIdx.x >> 6); t < to; t += 4 * workers) {
+    bool has = false;
+    for (int b = lane; b < p.B && !has; b += 64) {
+      const Sequence s = sequence_of(p, b);
+      has = t >= s.first && t - s.first < s.n;
+    }
+    if (__ballot(has) == 0) zero(t);
+  }
 }
 
 // The sizes of a call, as both entry points take them.

@@ -100,10 +100,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   const int slice = blockIdx.x % p.slices, at = blockIdx.x / p.slices;
   const int b = at / p.blocks, nth = at % p.blocks;
   const paged::Sequence s = paged::sequence_of(p.batch, b);
-  if (p.zero_tail) {  // rows that no sequence has, shared out by work-group
-    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x)
-      for (int i = tid; i < p.heads * p.cache.head_dim; i += 256)
+  if (p.zero_tail) {  // rows that no sequence has: those behind all by every work-group, a sequence's by its own
+    const auto zero = [&](int64_t t, int i0, int step) MI355_LAMBDA_INLINE {
+      for (int i = i0; i < p.heads * p.cache.head_dim; i += step)
         static_cast<T*>(p.qo)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
+    };
+    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x) zero(t, tid, 256);
+    const int worker = nth * p.slices + slice, workers = p.blocks * p.slices;
+    const auto of_wave = [&](int64_t t) MI355_LAMBDA_INLINE { zero(t, lane, 64); };
+    if (b == 0 && s.first > 0) paged::zero_rows(p.batch, 0, s.first, worker, workers, of_wave);
+    if (s.cut > 0) paged::zero_rows(p.batch, s.first + s.n, static_cast<int64_t>(s.first) + s.n + s.cut, worker, workers, of_wave);
   }
   const int64_t begin = static_cast<int64_t>(s.len) - s.n;  // position of the first new token
   const int64_t block = (begin >> 4) + nth;                 // (floor: positions can be negative)

@@ -1195,9 +1195,10 @@ class PagedBatch:
     a cache (``table`` int32 ``[B, width]``), ``lens[b]`` (int32) counts its tokens, the newest of this step included and
     last. The step's tokens are packed: sequence b's are rows ``offsets[b]`` to ``offsets[b + 1]`` (int32 ``[B + 1]``, from 0
     and not decreasing), ``most`` of one sequence at most; without ``offsets`` every sequence has ``most``. Tokens of a
-    sequence behind its first ``most`` are left out, as if neither ``offsets`` nor ``lens`` counted them. The same batch
-    serves all layers. The kernels read the three tensors when they run, so a captured graph follows their values; a
-    table entry that is no page is one that does not exist, whatever else it is."""
+    sequence behind its first ``most`` are left out, as if neither ``offsets`` nor ``lens`` counted them: their rows are
+    those of no sequence. The same batch serves all layers. The kernels read the three tensors when they run, so a
+    captured graph follows their values; a table entry that is no page is one that does not exist, whatever else it
+    is."""
     table: torch.Tensor
     lens: torch.Tensor
     most: int = 1
