@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from paged_reference import attention64, check, empty_cache, rand
+from paged_reference import DTYPES, attention64, check, empty_cache, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,29 @@ def test_more_tokens_than_most_in_replays(most, wide):
         eager = step(copy)
         assert torch.equal(got[0], eager[0])
         assert torch.equal(got[1], eager[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("most", [1, 3, 40])
+def test_rows_beside_far_scores_keep_their_bits(dtype, wide, most):
+    """A row's result does not depend on the scores of the other rows of its tile: neither on how far they are from 0 nor on
+    when their maximum moves (fp16 queries become infinities with the largest factor, and their rows NaN)."""
+    ops = _ops()
+    D, page, lens = 128, 64, [3000, 517]
+    table, pages = tables(lens, page, 90, wide)
+    k, v, ks, vs = empty_cache(pages, 2, page, D, seed=91)
+    cache = on_gpu((k, v, ks * 64, vs))
+    batch = ops.PagedBatch(table.cuda(), i32(lens), most)
+    q = 0.05 * rand((2 * most, 16, D), torch.float32, 92)
+    changed = [(0, 1), (0, 6), (most, 0), (most, 12), (2 * most - 1, 15)]
+    others = torch.ones(2 * most, 16, dtype=torch.bool)
+    for at in changed:
+        others[at] = False
+    want = ops.attention_paged(q.to(dtype).cuda(), cache, batch)
+    for factor in (0.1, 3.0, 30.0, 1e5, 6e5):
+        other = q.clone()
+        for at in changed:
+            other[at] *= factor
+        got = ops.attention_paged(other.to(dtype).cuda(), cache, batch)
+        assert torch.equal(got[others.cuda()], want[others.cuda()]), factor

@@ -209,7 +209,7 @@ struct Tile {
   int limit[NR];  // keys that the lane's rows see
   f32x4 acc[NR][ME];
   float top[NR], sum[NR];  // top: in log2 units
-  bool far;
+  bool far;                // a row's maximum is
 
   MI355_DEVINL void start(const PagedArgs& p, const Rows& rows, int h, int row0, int lane) {
     const int l16 = lane & 15, g = lane >> 4, hd = p.cache.head_dim;
@@ -261,31 +261,34 @@ struct Tile {
     for (int n = 0; n < NR; ++n) {
       const auto four = [&](const f32x4& x) MI355_LAMBDA_INLINE { return vmax(vmax(vmax(x[0], x[1]), x[2]), x[3]); };
       most[n] = vmax(four(sc[n][0]) * a[0], four(sc[n][1]) * a[1]);
-      moves = moves || most[n] > top[n] + SLACK;
+      moves = moves || most[n] - top[n] > SLACK;
     }
-    if (__ballot(moves)) {
+    if (__ballot(moves)) {  // (a row's statistics are its own: neither this nor `far` is another's to change)
       bool beyond = false;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const float now = vmax(top[n], row_max(most[n]));
+        const float high = row_max(most[n]);
+        const float now = high - top[n] > SLACK ? high : top[n];
         const float keep = top[n] == NEG_INF ? 0.0f : fast_exp2(top[n] - now);
         top[n] = now;
-        beyond = beyond || __builtin_fabsf(now) >= FAR;  // (rows that have seen nothing take that way too)
+        beyond = beyond || (__builtin_fabsf(now) >= FAR && now != NEG_INF);
         sum[n] *= keep;
 #pragma unroll
         for (int e = 0; e < ME; ++e) acc[n][e] *= keep;
       }
       far = __ballot(beyond) != 0;
     }
-    const auto rest = [&](auto rounded) MI355_LAMBDA_INLINE {
+    const auto rest = [&](auto some_far) MI355_LAMBDA_INLINE {
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const float ref = top[n] == NEG_INF ? 0.0f : top[n];
+        const bool rounded = decltype(some_far)::value && __builtin_fabsf(ref) >= FAR;
         float e[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          e[r] = fast_exp2(decltype(rounded)::value ? sc[n][r >> 2][r & 3] * a[r >> 2] - ref
-                                                    : __builtin_fmaf(sc[n][r >> 2][r & 3], a[r >> 2], -ref));
+        for (int r = 0; r < 8; ++r) {
+          const float s = sc[n][r >> 2][r & 3], f = a[r >> 2];
+          e[r] = fast_exp2(rounded ? s * f - ref : __builtin_fmaf(s, f, -ref));
+        }
         if constexpr (TERMS == 1) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) hi[n][r] = static_cast<TP>(e[r]);
