@@ -507,8 +507,8 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * mi355_attn_paged: softmax attention of the new tokens: the token at position p sees keys 0 .. p of its
  * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32. Probabilities
  * enter P·V as two bf16 terms (off by 2^-16 of each at most) where most * heads / kv_heads is at most 32,
- * rounded once to Q's type above (fp16: V there as multiples of 2^-30 of the largest scale so far). Outputs are
- * rounded once. A token that sees no key gives zeros; one that sees a key whose page is missing gives NaN. What
+ * rounded once to Q's type above (fp16 there: at the least to 2^-33 of the largest, V as multiples of 2^-30 of the
+ * largest scale so far). Outputs are rounded once. A token that sees no key gives zeros; one that sees a key whose page is missing gives NaN. What
  * pages hold behind lens does not matter, nor do NaN that a token does not see. bf16: |q| below 2^110, |v|
  * below 2^100. workspace (16-byte aligned) holds
  * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be

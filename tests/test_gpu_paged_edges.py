@@ -1,9 +1,11 @@
 """The paged cache's operators at their edges, against plain arithmetic in 64 bits (paged_reference) and themselves."""
 
+import math
+
 import pytest
 import torch
 
-from paged_reference import DTYPES, attention64, check, empty_cache, rand
+from paged_reference import DTYPES, UNIT, attention64, check, empty_cache, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +151,77 @@ def test_rows_beside_far_scores_keep_their_bits(dtype, wide, most):
             other[at] *= factor
         got = ops.attention_paged(other.to(dtype).cuda(), cache, batch)
         assert torch.equal(got[others.cuda()], want[others.cuda()]), factor
+
+
+def lifted(ref, tol, sees, top):
+    """attention64's bound for fp16 probabilities that are rounded once, with 2^-33 of the largest one as their smallest half
+    step (2^8 times the running maximum's is their unit, 2^-25 fp16's half step) in place of 2^-25."""
+    return ref, tol - sees * top * (2.0 ** -25 - 2.0 ** -33)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D", [64, 256])
+def test_keys_far_below_a_sink(D, wide):
+    """A key of no value 18 and 20 (in e's powers) above 12000 others: what those weigh together is not lost."""
+    ops = _ops()
+    page, keys, most = 64, 12000, 40
+    table, pages = tables([keys], page, 80, wide)
+    k, v, ks, vs = empty_cache(pages, 1, page, D)
+    ks.fill_(1.0)
+    vs.fill_(0.125)
+    k.copy_(rand(k.shape, torch.float32, 81).to(k.dtype))
+    v.copy_((2 + rand(v.shape, torch.float32, 82)).to(v.dtype))
+    k[..., 0] = torch.zeros(()).to(k.dtype)
+    sink = int(table[0, 0])
+    k[sink, 0, 0] = torch.zeros(D).to(k.dtype)
+    k[sink, 0, 0, 0] = torch.tensor(16.0).to(k.dtype)
+    v[sink, 0, 0] = torch.zeros(D).to(v.dtype)
+    q = 0.02 * rand((most, 1, D), torch.float32, 83)
+    q[::2, 0, 0], q[1::2, 0, 0] = 18.0, 20.0
+    q = q.half()
+    scale, cache = 0.0625, (k, v, ks, vs)
+    got = ops.attention_paged(q.cuda(), on_gpu(cache), ops.PagedBatch(table.cuda(), i32([keys]), most), scale=scale)
+    ref, tol = lifted(*attention64(q, cache, table, [keys], [0, most], scale), keys, float((v.float().abs().amax() * 0.125)))
+    assert (tol < 0.25 * ref.abs()).double().mean() > 0.5  # (the bound is well below what it measures)
+    check(got, ref, tol)
+    few = torch.cat([ops.attention_paged(q[i:i + 8].cuda(), on_gpu(cache), ops.PagedBatch(table.cuda(), i32([keys - most + i + 8]), 8), scale=scale)
+                     for i in range(0, most, 8)])
+    check(few, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far,step", [(0, 1), (2 ** 22, 1), (2 ** 25, 4), (-2 ** 26, 8)])
+@pytest.mark.parametrize("most", [1, 40])
+def test_scores_that_rise(dtype, far, step, most):
+    """Whole scores (2's powers) that rise by up to 16 from a unit of 32 keys to the next, near 0 and far from it: exact in fp32,
+    so that a weight is off by its exponential's 2^-20 and its own rounding, and none may overflow its type."""
+    ops = _ops()
+    D, page = 64, 32
+    rises = [0, 7, 8, 6, 14, 15, 16, 9, 1, 0, 12, 13, 15, 7, 8, 15, 16, 14, 0, 3, 15, 15, 8, 7]
+    keys = page * len(rises)
+    table, pages = tables([keys], page, 84, False)
+    k, v, ks, vs = empty_cache(pages, 1, page, D)
+    ks.fill_(1.0)
+    vs.fill_(2.0 ** -3)
+    v.copy_((448 * torch.rand(v.shape, generator=torch.Generator().manual_seed(85))).to(v.dtype))
+    at, score = 0, []  # in steps
+    for u, r in enumerate(rises):
+        at += -(-r // step)
+        row = torch.zeros(D)
+        row[0], row[1], row[2] = at // 16, at % 16, 256
+        k[table[0, u].long(), 0] = row.to(k.dtype)
+        score += [at * step] * page
+    q = torch.zeros(most, 1, D)
+    q[..., 0], q[..., 1], q[..., 2] = 16, 1, far / step / 256
+    got = ops.attention_paged(q.to(dtype).cuda(), on_gpu((k, v, ks, vs)), ops.PagedBatch(table.cuda(), i32([keys]), most),
+                              scale=math.log(2.0) * step).double().cpu()
+    score = torch.tensor(score, dtype=torch.float64)
+    values = v.double()[table[0].long(), 0].reshape(keys, D) * 2.0 ** -3
+    many = most > 32
+    for i in range(most):
+        sees = keys - most + i + 1
+        w = torch.softmax(score[:sees] * math.log(2.0), 0)
+        ref = w @ values[:sees]
+        rel = (2 * UNIT[dtype] if many else 2.0 ** -16) + 2 * 2.0 ** -20 + sees * 2.0 ** -23 + UNIT[dtype]
+        tol = rel * ref + (sees * 2.0 ** (-25 if abs(far) >= 2 ** 24 else -33) * 56 if many and dtype == torch.float16 else 0.0)
+        assert ((got[i, 0] - ref).abs() <= tol).all(), (i, got[i, 0, :4], ref[:4], tol[:4])

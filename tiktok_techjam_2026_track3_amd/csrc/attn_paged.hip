@@ -13,7 +13,7 @@
 //     two keys are put together (v_perm) and converted, the block's scale applied by the conversion. Output row m of
 //     MFMA e is dim m * run + e: a free choice again.
 // Bound by the bytes of K and V up to 32 rows, by instruction issue (matrix and vector) above.
-// The maximum moves only when a score exceeds it by more than 7 (log2 units), and only then do the four lanes of a row
+// The maximum moves only when a score exceeds it by more than 7 (log2 units; LIFT), and only then do the four lanes of a row
 // exchange anything. Statistics and sums are fp32.
 //
 // Work is dealt out evenly: the units of 32 keys of all (sequence, K/V head, tile of rows), in this order, are cut into
@@ -31,6 +31,11 @@ using paged::BLOCK;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 7.0f;
+// fp16 probabilities that are rounded once are held as 2^8 times what they are beside the running maximum, which uses the type's
+// upper range: those down to 2^-22 of it keep all their bits and 2^-33 is half the smallest step (without: 2^-14 and 2^-25, so
+// that what 10000 keys far below a sink weigh together was lost). The factor is in numerator and denominator. They stay
+// below 2^15 as the maximum moves at 2^14; a product's rounding to fp32 adds at most 1 to the exponent where it is not FAR.
+constexpr float LIFT = 8.0f, LIFTED_SLACK = 14.0f;
 // Products of scores and scale so large that fma(s, a, -top) may come out above SLACK by a factor that matters: the
 // rounding of top is 2^-24 of it. Then the product is rounded before the difference is taken, like top was.
 constexpr float FAR = 0x1p24f;
@@ -203,12 +208,14 @@ struct Tile {
   using frag = typename Mfma<T>::frag;
   using pfrag = typename Mfma<TP>::frag;
   static constexpr int KS = 2 * DW, ME = 4 * DW;  // MFMAs of S^T (32 dims each) and of O^T (16) for a group
+  static constexpr bool LIFTED = TERMS == 1 && __is_same(T, _Float16);
+  static constexpr float GATE = LIFTED ? LIFTED_SLACK : SLACK;  // a score this far above `top` moves it
   typedef T V4 __attribute__((ext_vector_type(4)));
 
   frag qf[NR][KS];
   int limit[NR];  // keys that the lane's rows see
   f32x4 acc[NR][ME];
-  float top[NR], sum[NR];  // top: in log2 units
+  float top[NR], sum[NR];  // top: what probabilities are relative to, in log2 units (the maximum then, less LIFT)
   bool far;                // a row's maximum is
 
   MI355_DEVINL void start(const PagedArgs& p, const Rows& rows, int h, int row0, int lane) {
@@ -261,14 +268,16 @@ struct Tile {
     for (int n = 0; n < NR; ++n) {
       const auto four = [&](const f32x4& x) MI355_LAMBDA_INLINE { return vmax(vmax(vmax(x[0], x[1]), x[2]), x[3]); };
       most[n] = vmax(four(sc[n][0]) * a[0], four(sc[n][1]) * a[1]);
-      moves = moves || most[n] - top[n] > SLACK;
+      moves = moves || most[n] - top[n] > GATE;
     }
     if (__ballot(moves)) {  // (a row's statistics are its own: neither this nor `far` is another's to change)
       bool beyond = false;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const float high = row_max(most[n]);
-        const float now = high - top[n] > SLACK ? high : top[n];
+        // (far ones have steps too wide to be lifted exactly)
+        const float to = LIFTED && __builtin_fabsf(high) < FAR ? high - LIFT : high;
+        const float now = high - top[n] > GATE ? to : top[n];
         const float keep = top[n] == NEG_INF ? 0.0f : fast_exp2(top[n] - now);
         top[n] = now;
         beyond = beyond || (__builtin_fabsf(now) >= FAR && now != NEG_INF);
