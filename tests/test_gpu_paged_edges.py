@@ -225,3 +225,17 @@ def test_scores_that_rise(dtype, far, step, most):
         rel = (2 * UNIT[dtype] if many else 2.0 ** -16) + 2 * 2.0 ** -20 + sees * 2.0 ** -23 + UNIT[dtype]
         tol = rel * ref + (sees * 2.0 ** (-25 if abs(far) >= 2 ** 24 else -33) * 56 if many and dtype == torch.float16 else 0.0)
         assert ((got[i, 0] - ref).abs() <= tol).all(), (i, got[i, 0, :4], ref[:4], tol[:4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("most", [2, 40])
+def test_mantissas_of_v_scales_do_not_count(dtype, most):
+    ops = _ops()
+    D, page, lens = 128, 32, [300, 77]
+    table, pages = tables(lens, page, 86, False)
+    k, v, ks, vs = empty_cache(pages, 2, page, D, seed=87)
+    q = rand((2 * most, 4, D), dtype, 88).cuda()
+    batch = ops.PagedBatch(table.cuda(), i32(lens), most)
+    want = ops.attention_paged(q, on_gpu((k, v, ks, vs)), batch)
+    factor = 1 + 0.99 * torch.rand(vs.shape, generator=torch.Generator().manual_seed(89))
+    assert torch.equal(ops.attention_paged(q, on_gpu((k, v, ks, vs * factor)), batch), want)

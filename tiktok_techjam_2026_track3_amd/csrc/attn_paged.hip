@@ -409,7 +409,8 @@ struct Window {
       const bool ok = id >= 0 && id < p.cache.pages;
       row = ((static_cast<int64_t>(ok ? id : 0) * p.cache.kv_heads + h) << shift) + (at & ((1 << shift) - 1));
       kf = ok ? p.cache.ks[row / BLOCK] * (p.scale * LOG2E) : __builtin_nanf("");
-      vf = ok ? p.cache.vs[row / BLOCK] : 0.0f;
+      // (the conversions take the exponent alone; Many divides by it)
+      vf = ok ? __uint_as_float(__float_as_uint(p.cache.vs[row / BLOCK]) & 0x7f800000u) : 0.0f;
     }
     row *= p.cache.head_dim;
     lo = static_cast<uint32_t>(row);
