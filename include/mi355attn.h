@@ -517,7 +517,8 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * Both: dtype F16 or BF16; head_dim 16, 32, 48, 64, 80, 96, 128, 192 or 256; rot_dim a multiple of 8.
  * sizes = {B, most, tokens, heads, kv_heads, head_dim, pages, page, width, table_stride}, strides = {token, head} of K,
  * V, Q and Q_out (of Q and O in the attention) in elements, multiples of 8 with 16-byte aligned bases (O: of 4, 8-byte).
- * width * page, pages, tokens, most and table_stride below 2^30, B up to 2^20, B most heads below 2^23.
+ * width * page, pages, tokens, most and table_stride below 2^30, B up to 2^20. Append: B ((most + 30) / 16) below
+ * 2^23. Attention: B most heads below 2^23, or tokens heads below 2^23 and most up to 2^20.
  */
 int mi355_paged_append(int dtype, const void* K, const void* V, const void* Q, void* Q_out,
                        uint8_t* cache_k, uint8_t* cache_v, float* k_scale, float* v_scale,

@@ -239,3 +239,31 @@ def test_mantissas_of_v_scales_do_not_count(dtype, most):
     want = ops.attention_paged(q, on_gpu((k, v, ks, vs)), batch)
     factor = 1 + 0.99 * torch.rand(vs.shape, generator=torch.Generator().manual_seed(89))
     assert torch.equal(ops.attention_paged(q, on_gpu((k, v, ks, vs * factor)), batch), want)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("B,most", [(129, 16384), (129, 1 << 20), (300, 1 << 20)])
+def test_a_large_bound_on_the_new_tokens(B, most, wide):
+    """Many sequences of which one may have a long piece: what counts is how many tokens there are."""
+    ops = _ops()
+    D, page = 32, 16
+    new = [1] * B
+    new[57] = 150
+    lens = [n + 3 + 13 * (b % 5) for b, n in enumerate(new)]
+    offsets = [0]
+    for n in new:
+        offsets.append(offsets[-1] + n)
+    table, pages = tables(lens, page, 93, False)
+    cache = empty_cache(pages, 2, page, D, seed=94)
+    if wide:
+        table = torch.cat((table, torch.full((len(lens), 200), -1, dtype=torch.int32)), 1)
+    q, k, v = (rand((offsets[-1], h, D), torch.float16, 95 + h) for h in (4, 2, 2))
+    batch = ops.PagedBatch(table.cuda(), i32(lens), most, i32(offsets))
+    dev, want, plan = on_gpu(cache), on_gpu(cache), ops.rotary_plan(D)
+    if most == 16384:
+        turned = ops.paged_append(dev, k.cuda(), v.cuda(), batch, plan, q.cuda())
+        ref = ops.paged_append(want, k.cuda(), v.cuda(), ops.PagedBatch(table.cuda(), i32(lens), 150, i32(offsets)), plan, q.cuda())
+        assert torch.equal(turned, ref) and torch.equal(dev.k.view(torch.uint8), want.k.view(torch.uint8))
+        assert torch.equal(dev.v.view(torch.uint8), want.v.view(torch.uint8))
+    cpu = tuple(t.cpu() for t in (dev.k, dev.v, dev.k_scale, dev.v_scale))
+    check(ops.attention_paged(q.cuda(), dev, batch), *attention64(q, cpu, table, lens, offsets, D ** -0.5, most))

@@ -1139,7 +1139,8 @@ Launch launch_of(const paged::Sizes& z) {
   l.past = !l.many && z.B * room * z.kv_heads * z.head_dim * 2 > int64_t(320) << 20;
   // (More than 1024 sequences fill the GPU by themselves, and each work-group would go through all their lengths: 1100 of
   // up to 300 keys in wide tables, one K/V head, 53.1 / 21.7; 4000 of up to 4000 keys 468 / 411.)
-  const bool each = z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048));
+  // (2^23 work-groups of 256 are what one launch takes.)
+  const bool each = jobs < (int64_t(1) << 23) && (z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048)));
   l.groups = each ? 0 : 256 * (dw > 2 ? 1 : 2);
   l.least = 8;
   l.grid = l.groups ? l.groups : jobs;
@@ -1183,11 +1184,13 @@ int launch_dim(const PagedArgs& p, const Launch& l, hipStream_t s) {
   }
 }
 
+// Few enough rows that 32 bits count them: by how many tokens there are, or by how many `most` allows.
 int check_all(int dtype, const paged::Sizes& z) {
   if (const int st = paged::check(dtype, z)) return st;
-  const int64_t rows = z.B * z.most;
-  if (rows >= (int64_t(1) << 30) || rows * z.heads >= (int64_t(1) << 23)) return MI355_E_BAD_SIZE;  // 2^31 threads
-  return MI355_OK;
+  constexpr int64_t MOST = int64_t(1) << 23;
+  const int64_t allowed = z.B * z.most;
+  if (allowed < MOST && allowed * z.heads < MOST) return MI355_OK;
+  return z.tokens * z.heads < MOST && z.most <= (1 << 20) ? MI355_OK : MI355_E_BAD_SIZE;
 }
 
 }  // namespace

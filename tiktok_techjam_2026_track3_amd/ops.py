@@ -1264,8 +1264,11 @@ def _paged_views(cache_shape, table_shape, table_stride, most, ragged, names, dt
         raise ValueError(f"{B} sequences of {most} new tokens need {B * most} rows, got {T}")
     if width * page >= 1 << 30 or T >= 1 << 30:
         raise ValueError("the table holds 2^30 tokens or more of a sequence, or the call has as many rows")
-    if B * most * H >= 1 << 23:
-        raise ValueError(f"{B} sequences of up to {most} new tokens in {H} heads are too many for one call")
+    if "k" in names:
+        if B * ((most + 2 * PAGED_BLOCK - 2) // PAGED_BLOCK) >= 1 << 23:
+            raise ValueError(f"{B} sequences of up to {most} new tokens are too many for one call")
+    elif B * most * H >= 1 << 23 and (T * H >= 1 << 23 or most > 1 << 20):
+        raise ValueError(f"{T} new tokens in {H} heads, or up to {most} of a sequence, are too many for one call")
     views = []
     for name, shape, st in zip(names, shapes, strides):
         views.append(_rows_strides(name, shape, st, 4 if name == "out" else 8, 0 if name in ("k", "v") else None,
