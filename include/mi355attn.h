@@ -470,7 +470,8 @@ int mi355_linear_i4(int dtype, int out_dtype, const void* X, int64_t ldx, const 
  * != 0 (x_2j, x_2j+1); the elements behind them are copied. inverse != 0 turns the other way (with
  * the same amplitude: the transposed map, which is the gradient's).
  * frequencies [rot_dim / 2] (device) are fractions of a full turn for each position, times 2^64
- * (modulo 2^64): angles are exact to 2^-31 of a turn at any position. fp32 arithmetic, rounded once.
+ * (modulo 2^64): an angle is off by 2^-32 of a turn and by what the frequency's rounding comes to at its position.
+ * fp32 arithmetic, rounded once.
  * X and Y are [n0, n1, heads, head_dim] views with a head_dim stride of 1, positions [n0, n1] int32
  * (int64 with positions_64 != 0), of any sign. sizes = {n0, n1, heads, head_dim, rot_dim}; strides = positions'
  * {batch, token}, X's {batch, token, head}, Y's, in elements. Y may be X with the same strides, and must not

@@ -1,10 +1,12 @@
 """The paged cache's operators at their edges, against plain arithmetic in 64 bits (paged_reference) and themselves."""
 
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
 
+from paged_edges_reference import pi_of
 from paged_reference import DTYPES, UNIT, attention64, check, empty_cache, rand
 
 pytestmark = pytest.mark.gpu
@@ -267,3 +269,23 @@ def test_a_large_bound_on_the_new_tokens(B, most, wide):
         assert torch.equal(dev.v.view(torch.uint8), want.v.view(torch.uint8))
     cpu = tuple(t.cpu() for t in (dev.k, dev.v, dev.k_scale, dev.v_scale))
     check(ops.attention_paged(q.cuda(), dev, batch), *attention64(q, cpu, table, lens, offsets, D ** -0.5, most))
+
+
+@pytest.mark.parametrize("base,dim", [(10000.0, 64), (500000.0, 128)])
+def test_rotary_positions_up_to_2_33(base, dim):
+    """Angles are off by 2^-31 of a turn at most: sines and cosines of their exact values, against the kernel's."""
+    ops = _ops()
+    positions = [2 ** 33, -2 ** 33, 2 ** 33 - 12345, 2 ** 31 + 7, -2 ** 31, 2 ** 26 + 1, 10 ** 6, 3]
+    x = rand((len(positions), 1, dim), torch.float32, 96)
+    pi, h = pi_of(60), dim // 2
+    with localcontext() as c:
+        c.prec = 60
+        turns = [(Decimal(base).ln() * -2 * j / dim).exp() / (2 * pi) for j in range(h)]
+        angle = torch.tensor([[float((p * t) % 1 * 2 * pi) for t in turns] for p in positions], dtype=torch.float64)
+    cos, sin = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    a, b = x[..., :h].double(), x[..., h:].double()
+    ref = torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+    # 2 pi 2^-31 of the angle; 2^-21 as in rotate64; the output's rounding
+    tol = (2.0 ** -28 + 2.0 ** -21) * (a.abs() + b.abs()).repeat(1, 1, 2) + UNIT[torch.float32] * ref.abs()
+    got = ops.rotary(x.cuda(), torch.tensor(positions).cuda(), ops.rotary_plan(dim, base))
+    check(got, ref, tol)

@@ -1,7 +1,10 @@
-"""Sizes that the paged cache's operators take and refuse, without a GPU."""
+"""Sizes that the paged cache's operators take and refuse and the frequencies of rotary plans, without a GPU."""
+from decimal import Decimal, localcontext
+
 import pytest
 import torch
 
+from paged_edges_reference import pi_of
 from tiktok_techjam_2026_track3_amd import _lib, ops
 
 BAD_SIZE = -2
@@ -37,3 +40,32 @@ def test_append_takes_what_its_launch_does(names):
     for B, most in ((1 << 20, 98), (8, (1 << 24) + 1)):
         with pytest.raises(ValueError, match="too many for one call"):
             views(names, 5, 64, B, most)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(base=10000.0), dict(base=500000.0), dict(base=1.0), dict(base=0.01), dict(base=1e300), dict(base=10000.0, scaling="linear", factor=3.0),
+    dict(base=10000.0, scaling="base", factor=16.0), dict(base=10000.0, scaling="parts", factor=8.0, original=4096),
+    dict(base=1e6, scaling="parts", factor=3.3, original=8192.5, slow=0.5, fast=7), dict(freqs=[2.5, -2.5, 1e-30, -1e-30, 0.0, 1e17, -1e17, 1e300])])
+def test_frequencies_are_rounded_once(monkeypatch, kw):
+    """The fractions of a turn times 2^64 of a plan are the nearest whole numbers, computed here with 700 digits."""
+    dim = 16
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *a, **k: seen.append(self) or self)
+    ops.rotary_plan(dim, **kw)
+    with localcontext() as c:
+        c.prec = 700
+        two_pi, base, factor = 2 * pi_of(700), Decimal(kw.get("base", 1.0)), Decimal(kw.get("factor", 1.0))
+        if kw.get("scaling") == "base":
+            base = base * (factor.ln() * dim / (dim - 2)).exp()
+        f = [Decimal(x) for x in kw["freqs"]] if "freqs" in kw else [(base.ln() * -j / 8).exp() for j in range(8)]
+        if kw.get("scaling") == "linear":
+            f = [x / factor for x in f]
+        if kw.get("scaling") == "parts":
+            slow, fast, original = Decimal(kw.get("slow", 1.0)), Decimal(kw.get("fast", 32.0)), Decimal(kw["original"])
+            for j, x in enumerate(f):
+                r = original * x / two_pi
+                g = 0 if r <= slow else 1 if r >= fast else (r - slow) / (fast - slow)
+                f[j] = x * (g + (1 - g) / factor)
+        for x, turn in zip(f, seen[0].tolist()):
+            off = abs((x / two_pi * 2 ** 64 - turn) % 2 ** 64)
+            assert min(off, 2 ** 64 - off) <= Decimal("0.5000001"), (x, turn, off)

@@ -7,11 +7,12 @@ device. Nothing here synchronises the host, so the calls are hipGraph-capturable
 from __future__ import annotations
 
 import ctypes
+import decimal
 import functools
 import math
 import operator
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -1009,6 +1010,45 @@ class RotaryPlan:
     amplitude: float
 
 
+@functools.lru_cache(maxsize=8)
+def _pi(digits: int) -> decimal.Decimal:
+    """By Machin's formula, pi / 4 = 4 arctan 1/5 - arctan 1/239."""
+    one = 10 ** (digits + 10)
+
+    def arctan_of_inverse(n):
+        power, total, k = one // n, 0, 0
+        while power:
+            total += (power if k % 2 == 0 else -power) // (2 * k + 1)
+            power, k = power // (n * n), k + 1
+        return total
+
+    with decimal.localcontext(decimal.Context(prec=digits + 10)):
+        return decimal.Decimal(4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))) / one
+
+
+def _turns(dim: int, base: float, scaling: Optional[str], factor: float, original: Optional[float], slow: float, fast: float,
+           freqs: Optional[List[float]], largest: float) -> List[int]:
+    """Each pair's fraction of a turn for a position, times 2^64 and rounded: of the frequencies that these numbers stand
+    for, not of those rounded to doubles, whose 2^-53 is 2^-24 of a turn at position 2^31. largest: of the frequencies."""
+    Dec = decimal.Decimal
+    digits = 50 + (max(0, int(math.log10(largest))) if largest else 0)  # (20 of a fraction are needed)
+    with decimal.localcontext(decimal.Context(prec=digits)):
+        if freqs is not None:
+            f = [Dec(x) for x in freqs]
+        else:
+            ln = Dec(base).ln()
+            if scaling == "base":
+                ln += Dec(factor).ln() * dim / (dim - 2)
+            f = [(ln * (-2 * j) / dim).exp() for j in range(dim // 2)]
+            if scaling == "linear":
+                f = [x / Dec(factor) for x in f]
+            elif scaling == "parts":
+                original, slow, fast = Dec(float(original)), Dec(float(slow)), Dec(float(fast))
+                kept = [min(Dec(1), max(Dec(0), (original * x / (2 * _pi(digits)) - slow) / (fast - slow))) for x in f]
+                f = [x * (g + (1 - g) / Dec(factor)) for x, g in zip(f, kept)]
+        return [int((x / (2 * _pi(digits)) % 1 * 2 ** 64).to_integral_value(decimal.ROUND_HALF_EVEN)) % (1 << 64) for x in f]
+
+
 def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: Optional[str] = None,
                 factor: float = 1.0, original: Optional[int] = None, slow: float = 1.0, fast: float = 32.0,
                 freqs: Optional[Sequence[float]] = None, amplitude: float = 1.0, device="cuda") -> RotaryPlan:
@@ -1021,14 +1061,15 @@ def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, s
       ``fast`` and more stay, those of ``slow`` and fewer become f_j / factor, and in between
       f_j (g + (1 - g) / factor), g = (r - slow) / (fast - slow).
 
-    ``freqs`` gives the radians themselves instead. ``amplitude`` multiplies the rotated elements. Host arithmetic in
-    64 bits; made once, outside a graph capture."""
+    ``freqs`` gives the radians themselves instead. ``amplitude`` multiplies the rotated elements. Frequencies are
+    rounded once, to 2^-65 of a turn; made once, outside a graph capture."""
     dim = operator.index(dim)
     if dim < 2 or dim % 2 or dim > 512:
         raise ValueError(f"dim must be even and between 2 and 512, got {dim}")
     base, factor, amplitude = float(base), float(factor), float(amplitude)
     if not 0.0 < base < math.inf or not 0.0 < factor < math.inf or not math.isfinite(amplitude):
         raise ValueError("base and factor must be positive and finite, amplitude finite")
+    own_base = base
     if freqs is not None:
         if scaling is not None:
             raise ValueError("freqs are given: nothing to scale")
@@ -1047,7 +1088,7 @@ def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, s
         if scaling == "linear":
             f = [x / factor for x in f]
         elif scaling == "parts":
-            if original is None or original <= 0 or not 0 <= slow < fast < math.inf:
+            if original is None or not original > 0 or not 0 <= slow < fast < math.inf:
                 raise ValueError("scaling 'parts' needs original > 0 and 0 <= slow < fast")
             kept = [min(1.0, max(0.0, (original * x / (2 * math.pi) - slow) / (fast - slow))) for x in f]
             f = [x * (g + (1.0 - g) / factor) for x, g in zip(f, kept)]
@@ -1058,7 +1099,7 @@ def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, s
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError(f"expected a GPU device, got {device}")
-    turns = [round(x / (2 * math.pi) % 1.0 * 2.0 ** 64) % (1 << 64) for x in f]
+    turns = _turns(dim, own_base, scaling, factor, original, slow, fast, None if freqs is None else f, max(map(abs, f)))
     turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
     return RotaryPlan(turns.to(device), dim, bool(interleaved), amplitude)
 
@@ -1105,9 +1146,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, plan: RotaryPlan, inverse: 
     of any sign and size. Elements behind the plan's ``dim`` are copied.
 
     ``inverse`` turns back: with the same amplitude it is the transposed map, so the gradient of x is
-    ``rotary(grad, positions, plan, inverse=True)``. Angles are exact to 2^-31 of a turn at any position; fp32
-    arithmetic, rounded once. ``out`` may be ``x`` itself, and must not share memory with it otherwise. No
-    derivatives."""
+    ``rotary(grad, positions, plan, inverse=True)``. Angles are exact to 2^-31 of a turn at positions up to 2^33 either
+    way, and to 2^-65 of a turn for each position beyond; fp32 arithmetic, rounded once. ``out`` may be ``x`` itself, and
+    must not share memory with it otherwise. No derivatives."""
     dev = x.get_device()
     given = out is not None
     if dev < 0 or positions.get_device() != dev or plan.turns.get_device() != dev or (given and out.get_device() != dev):
