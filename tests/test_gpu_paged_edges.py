@@ -289,3 +289,31 @@ def test_rotary_positions_up_to_2_33(base, dim):
     tol = (2.0 ** -28 + 2.0 ** -21) * (a.abs() + b.abs()).repeat(1, 1, 2) + UNIT[torch.float32] * ref.abs()
     got = ops.rotary(x.cuda(), torch.tensor(positions).cuda(), ops.rotary_plan(dim, base))
     check(got, ref, tol)
+
+
+def test_caches_that_require_gradients_are_refused():
+    ops = _ops()
+    x, kv = (torch.zeros(1, h, 64, dtype=torch.float16, device="cuda") for h in (4, 2))
+    batch, plan = ops.PagedBatch(i32([[0]]), i32([1])), ops.rotary_plan(64)
+    for at in range(4):
+        parts = [t.cuda() for t in empty_cache(2, 2, 16, 64)]
+        parts[at].requires_grad_()
+        cache = ops.PagedCache(*parts)
+        for call in (lambda: ops.attention_paged(x, cache, batch), lambda: ops.paged_append(cache, kv, kv, batch, plan, x)):
+            with pytest.raises(ValueError, match="no backward"):
+                call()
+            with torch.no_grad():
+                call()
+
+
+def test_caches_with_tangents_are_refused():
+    from torch.autograd import forward_ad
+    ops = _ops()
+    x, kv = (torch.zeros(1, h, 64, dtype=torch.float16, device="cuda") for h in (4, 2))
+    batch, plan = ops.PagedBatch(i32([[0]]), i32([1])), ops.rotary_plan(64)
+    k, v, ks, vs = (t.cuda() for t in empty_cache(2, 2, 16, 64))
+    with torch.no_grad(), forward_ad.dual_level():
+        cache = ops.PagedCache(k, v, ks, forward_ad.make_dual(vs, torch.ones_like(vs)))
+        for call in (lambda: ops.attention_paged(x, cache, batch), lambda: ops.paged_append(cache, kv, kv, batch, plan, x)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()

@@ -1346,9 +1346,9 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, batch: Pag
             given and q_out.get_device() != dev):
         _on_gpu(k, v, held_k, batch.table, None if plan is None else plan.turns, q, q_out)
     if torch.is_grad_enabled():
-        _no_backward(k, v, q, q_out)
+        _no_backward(k, v, q, q_out, held_k, cache.v, cache.k_scale, cache.v_scale)
     if forward_ad._current_level >= 0:
-        _no_tangent(k, v, q, q_out)
+        _no_tangent(k, v, q, q_out, held_k, cache.v, cache.k_scale, cache.v_scale)
     if plan is None:
         if q is not None or given:
             raise ValueError("queries are given to be rotated, but no plan")
@@ -1415,10 +1415,10 @@ def attention_paged(q: torch.Tensor, cache: PagedCache, batch: PagedBatch, scale
     given = out is not None
     if dev < 0 or cache.k.get_device() != dev or batch.table.get_device() != dev or (given and out.get_device() != dev):
         _on_gpu(q, cache.k, batch.table, out)
-    if torch.is_grad_enabled() and (q.requires_grad or (given and out.requires_grad)):
-        _no_backward(q, out)
+    if torch.is_grad_enabled():
+        _no_backward(q, out, cache.k, cache.v, cache.k_scale, cache.v_scale)
     if forward_ad._current_level >= 0:
-        _no_tangent(q, out)
+        _no_tangent(q, out, cache.k, cache.v, cache.k_scale, cache.v_scale)
     code, sizes, strides, need, _, empty, _ = _paged_views(
         cache.k.shape, batch.table.shape, batch.table.stride(), batch.most, batch.offsets is not None,
         ("q", "out") if given else ("q",), (q.dtype, out.dtype) if given else (q.dtype,),
