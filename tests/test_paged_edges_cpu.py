@@ -69,3 +69,13 @@ def test_frequencies_are_rounded_once(monkeypatch, kw):
         for x, turn in zip(f, seen[0].tolist()):
             off = abs((x / two_pi * 2 ** 64 - turn) % 2 ** 64)
             assert min(off, 2 ** 64 - off) <= Decimal("0.5000001"), (x, turn, off)
+
+
+@pytest.mark.parametrize("turns,dim", [
+    (torch.zeros(31, dtype=torch.int64), 64), (torch.zeros(0, dtype=torch.int64), 2), (torch.zeros(64, dtype=torch.int64)[::2], 64),
+    (torch.zeros(32, dtype=torch.int32), 64), (torch.zeros(32, 1, dtype=torch.int64), 64), (torch.zeros(32), 64),
+    (torch.zeros(0, dtype=torch.int64), 0), (torch.zeros(3, dtype=torch.int64), 7), (torch.zeros(257, dtype=torch.int64), 514)])
+def test_plans_that_the_kernels_would_read_beyond_are_refused(turns, dim):
+    with pytest.raises(ValueError):
+        ops.RotaryPlan(turns, dim, False, 1.0)
+    assert ops.RotaryPlan(torch.zeros(32, dtype=torch.int64), 64, False, 1.0).dim == 64

@@ -1009,6 +1009,12 @@ class RotaryPlan:
     interleaved: bool
     amplitude: float
 
+    def __post_init__(self):
+        if not 2 <= self.dim <= 512 or self.dim % 2:
+            raise ValueError(f"dim must be even and between 2 and 512, got {self.dim}")
+        if self.turns.dtype != torch.int64 or tuple(self.turns.shape) != (self.dim // 2,) or not self.turns.is_contiguous():
+            raise ValueError(f"turns must be a contiguous int64 tensor of shape ({self.dim // 2},)")
+
 
 @functools.lru_cache(maxsize=8)
 def _pi(digits: int) -> decimal.Decimal:
