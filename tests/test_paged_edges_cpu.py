@@ -79,3 +79,10 @@ def test_plans_that_the_kernels_would_read_beyond_are_refused(turns, dim):
     with pytest.raises(ValueError):
         ops.RotaryPlan(turns, dim, False, 1.0)
     assert ops.RotaryPlan(torch.zeros(32, dtype=torch.int64), 64, False, 1.0).dim == 64
+
+
+@pytest.mark.parametrize("amplitude", [1e39, -1e300, float("nan")])
+def test_amplitudes_beyond_fp32_are_refused(amplitude):
+    """(the kernels take it in fp32, where it would be an infinity)"""
+    with pytest.raises(ValueError, match="amplitude"):
+        ops.rotary_plan(64, amplitude=amplitude, device="cpu")

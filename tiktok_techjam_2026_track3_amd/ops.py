@@ -1073,8 +1073,8 @@ def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, s
     if dim < 2 or dim % 2 or dim > 512:
         raise ValueError(f"dim must be even and between 2 and 512, got {dim}")
     base, factor, amplitude = float(base), float(factor), float(amplitude)
-    if not 0.0 < base < math.inf or not 0.0 < factor < math.inf or not math.isfinite(amplitude):
-        raise ValueError("base and factor must be positive and finite, amplitude finite")
+    if not 0.0 < base < math.inf or not 0.0 < factor < math.inf or not abs(amplitude) <= torch.finfo(torch.float32).max:
+        raise ValueError("base and factor must be positive and finite, amplitude finite in fp32")
     own_base = base
     if freqs is not None:
         if scaling is not None:
