@@ -1037,22 +1037,27 @@ def _turns(dim: int, base: float, scaling: Optional[str], factor: float, origina
     """Each pair's fraction of a turn for a position, times 2^64 and rounded: of the frequencies that these numbers stand
     for, not of those rounded to doubles, whose 2^-53 is 2^-24 of a turn at position 2^31. largest: of the frequencies."""
     Dec = decimal.Decimal
-    digits = 50 + (max(0, int(math.log10(largest))) if largest else 0)  # (20 of a fraction are needed)
+    digits = 32 + (max(0, int(math.log10(largest))) if largest else 0)  # (20 of a fraction are needed)
     with decimal.localcontext(decimal.Context(prec=digits)):
+        turn = 2 * _pi(digits)
         if freqs is not None:
-            f = [Dec(x) for x in freqs]
+            f = [Dec(x) / turn for x in freqs]
         else:
             ln = Dec(base).ln()
             if scaling == "base":
                 ln += Dec(factor).ln() * dim / (dim - 2)
-            f = [(ln * (-2 * j) / dim).exp() for j in range(dim // 2)]
+            each, x, f = (ln * -2 / dim).exp(), 1 / turn, []
+            for _ in range(dim // 2):
+                f.append(x)
+                x *= each
             if scaling == "linear":
-                f = [x / Dec(factor) for x in f]
+                by = 1 / Dec(factor)
+                f = [x * by for x in f]
             elif scaling == "parts":
                 original, slow, fast = Dec(float(original)), Dec(float(slow)), Dec(float(fast))
-                kept = [min(Dec(1), max(Dec(0), (original * x / (2 * _pi(digits)) - slow) / (fast - slow))) for x in f]
+                kept = [min(Dec(1), max(Dec(0), (original * x - slow) / (fast - slow))) for x in f]
                 f = [x * (g + (1 - g) / Dec(factor)) for x, g in zip(f, kept)]
-        return [int((x / (2 * _pi(digits)) % 1 * 2 ** 64).to_integral_value(decimal.ROUND_HALF_EVEN)) % (1 << 64) for x in f]
+        return [round(x % 1 * (1 << 64)) % (1 << 64) for x in f]
 
 
 def rotary_plan(dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: Optional[str] = None,
