@@ -201,7 +201,9 @@ constexpr int per_cu(int64_t dw, int64_t nr, bool many) { return dw > 2 ? 1 : ma
 // DW: dwords that a lane has of a V row, head_dim / 64 rounded up to 1, 2, 3 or 4 (dims behind head_dim are loaded from
 // its start: Q is 0 there, and those output rows are not stored).
 // TERMS: a probability enters P·V as that many. Two bf16 terms, off by at most 2^-16 of it, where K and V are waited for
-// and they cost nothing; where rows are many enough to be matrix work, one of the type of q.
+// and they cost nothing; where rows are many enough to be matrix work, where a second term is as many MFMAs again, one of
+// the type of q: half a step of it in numerator and denominator alike (bf16 pieces of prompts 0.0023 of the output's norm off,
+// 0.0017 with its rounding alone).
 template <typename T, int DW, int NR, int TERMS>
 struct Tile {
   using TP = std::conditional_t<TERMS == 1, T, __bf16>;  // type of P and V
@@ -634,7 +636,7 @@ MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
 // each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
 // buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit. Each wave on its
 // own (as in Few) converted all of K and V four times: two pieces of 1024 tokens against 12000 keys (32/8 heads of 128)
-// 1039 us, so 338 and 15 of the join: 860 TFLOP/s, matrix cores busy 36% of the time and the vector ALU 48%,
+// 1039 us, so 353, 14 of them the join: 860 TFLOP/s, matrix cores busy 36% of the time and the vector ALU 48%,
 // hardly at once with the two waves that a SIMD's registers hold. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
 // fp16: V's scales are taken relative to the largest up to their own block, so that V fits the type; blocks down to
 // 2^-21 of that are exact. (Up to their own: a later block's scale is not to touch rows that do not see it.)
@@ -1117,8 +1119,8 @@ Launch launch_of(const paged::Sizes& z) {
   l.many = rows > 32;
   // Groups of 16 rows of a wave. Few rows: as many as there are, where registers allow two. Many: two, which share each operand
   // that is read; above head dim 128 such a wave has the SIMD for itself, and short tiles leave waves idle: only for
-  // enough rows (us of 16 sequences of 4096 keys, 32 heads of 192 / of 256, one group then two: 64 rows 92 109 / 112 177, 128
-  // rows 156 125 / 186 185, 256 rows 301 230 / 365 340; two of 1024 tokens against 8192 keys 1091 730 / 1221 1002).
+  // enough rows (us of 16 sequences of 4096 keys, 32 heads of 192 / of 256, one group then two: 64 rows 96 111 / 113 184, 128
+  // rows 156 124 / 193 196, 256 rows 300 228 / 374 352; two of 1024 tokens against 8192 keys 1087 723 / 1243 1044).
   l.nr = l.many ? (dw <= 2 || rows > 64 * (dw - 2) ? 2 : 1) : (rows > 16 && dw <= 2 ? 2 : 1);
   l.rows = 16 * l.nr * (l.many ? 4 : 1);
   l.row_tiles = (rows + l.rows - 1) / l.rows;
@@ -1141,7 +1143,8 @@ Launch launch_of(const paged::Sizes& z) {
   // up to 300 keys in wide tables, one K/V head, 53.1 / 21.7; 4000 of up to 4000 keys 468 / 411.)
   // (2^23 work-groups of 256 are what one launch takes.)
   const bool each = jobs < (int64_t(1) << 23) && (z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048)));
-  l.groups = each ? 0 : 256 * (dw > 2 ? 1 : 2);
+  constexpr int64_t CUS = 256;  // (not asked for: the workspace's size follows, which is known without a device)
+  l.groups = each ? 0 : CUS * (dw > 2 ? 1 : 2);
   l.least = 8;
   l.grid = l.groups ? l.groups : jobs;
   l.ws = l.groups * (2 * l.rows * (z.head_dim + 2) * 4 + static_cast<int64_t>(sizeof(Head)));

@@ -322,7 +322,7 @@ extern "C" int mi355_paged_append(int dtype, const void* K, const void* V, const
   p.heads = static_cast<int32_t>(z.heads);
   p.zero_tail = Q && zero_tail && (offsets || z.tokens > z.B * z.most);
   p.blocks = static_cast<int32_t>((z.most + 2 * BLOCK - 2) / BLOCK);
-  // work-groups that share a block's heads: enough to have two a CU, no more than heads can use
+  // work-groups that share a block's heads: enough for 8192 of them, 32 a CU, no more than heads can use
   const int64_t groups = z.B * p.blocks;
   const int64_t slices = (8192 + groups - 1) / groups, useful = (2 * z.kv_heads + 3) / 4;
   p.slices = static_cast<int32_t>(slices < useful ? slices : useful);

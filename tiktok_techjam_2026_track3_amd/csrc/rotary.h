@@ -1,10 +1,11 @@
 // The angle of a rotation by position, for rotary.hip and paged_append.hip.
 //
 // A pair's frequency is a fraction of a full turn a position, held as a 0.64 fixed-point number, so that position *
-// frequency modulo a turn is one 64-bit product whose overflow is the modulo: the same for positions near and far (a
-// float product loses a bit of the angle with every doubling: 2^-4 rad at a million). What is left after the nearest
-// quarter turn is within pi / 4, where the Taylor polynomials below are off by less than 2^-29 (sine, to x^9) and
-// 2^-32 (cosine, to x^10); in fp32 both come out within two of its steps.
+// frequency modulo a turn is one 64-bit product whose overflow is the modulo: off by 2^-32 of a turn, which is dropped,
+// and by position times 2^-65 of the frequency's rounding, as much again at position 2^33 (a float product loses a bit of
+// the angle with every doubling: 2^-4 rad at a million). What is left after the nearest quarter turn is within pi / 4,
+// where the Taylor polynomials below are off by less than 2^-29 (sine, to x^9) and 2^-32 (cosine, to x^10); in fp32 both
+// come out within two of its steps.
 #pragma once
 
 #include "common.h"
