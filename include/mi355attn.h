@@ -500,8 +500,8 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * mi355_paged_append writes the new tokens' K and V. K is rotated by its position p (mi355_rotary's formula
  * with these frequencies; NULL: not), and so is Q, if it is given, into Q_out (may be Q). Rotated values
  * are not rounded before they are quantised: with m the largest finite magnitude of a block's new elements, the
- * scale becomes max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens); elements are
- * rounded to nearest even, infinities and NaN become NaN; when the scale grows, the block's older elements are
+ * scale becomes max(2^-118, least power of two s with m <= 448 s, the old scale if the block has older tokens);
+ * elements are rounded to nearest even, infinities and NaN become NaN; when the scale grows, the block's older elements are
  * rounded to it anew. Tokens whose page is none of [0, pages), or behind the table, are not written. A page that
  * is written must be in one sequence's table, once; pages that are only read may be in many.
  *
@@ -509,7 +509,8 @@ int mi355_rotary(int dtype, const void* X, void* Y, const void* positions, int p
  * sequence; query head h reads K/V head h / (heads / kv_heads). Scores and statistics are fp32. Probabilities
  * enter P·V as two bf16 terms (off by 2^-16 of each at most) where most * heads / kv_heads is at most 32,
  * rounded once to Q's type above (fp16 there: at the least to 2^-33 of the largest, V as multiples of 2^-30 of the
- * largest scale so far). Outputs are rounded once. A token that sees no key gives zeros; one that sees a key whose page is missing gives NaN. What
+ * largest scale so far). Outputs are rounded once. A token that sees no key gives zeros; one that sees a key whose
+ * page is missing gives NaN. What
  * pages hold behind lens does not matter, nor do NaN that a token does not see. bf16: |q| below 2^110, |v|
  * below 2^100. workspace (16-byte aligned) holds
  * mi355_attn_paged_workspace_bytes(...) bytes (negative: that argument error); calls that share one must be

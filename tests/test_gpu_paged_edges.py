@@ -317,3 +317,27 @@ def test_caches_with_tangents_are_refused():
         for call in (lambda: ops.attention_paged(x, cache, batch), lambda: ops.paged_append(cache, kv, kv, batch, plan, x)):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+def test_an_append_of_more_rows_than_the_attention_takes():
+    """2^23 rows of queries and more in one call: the same as in two, and as the rotation alone in fp32. That one is rounded to
+    fp32 (2^-24 of it), ours to fp16 (2^-11, below 2^-14 2^-25) either from there or from the sum as it is: the compiler's
+    choice, so that fp16 results of the two kernels can be neighbours where fp32 has the middle between them."""
+    ops = _ops()
+    D, page, T, H, cut = 16, 1024, 270001, 32, 100000
+    assert T * H > 1 << 23
+    width = -(-T // page)
+    table = torch.randperm(width, generator=torch.Generator().manual_seed(97)).to(torch.int32)[None].cuda()
+    g = torch.Generator(device="cuda").manual_seed(98)
+    q, k, v = (torch.randn(T, h, D, device="cuda", generator=g).half() for h in (H, 1, 1))
+    plan, one, two = ops.rotary_plan(D), ops.paged_cache(width, 1, D, page), ops.paged_cache(width, 1, D, page)
+    turned = ops.paged_append(one, k, v, ops.PagedBatch(table, i32([T]), T), plan, q)
+    for a, b in ((0, cut), (cut, T)):
+        part = ops.paged_append(two, k[a:b], v[a:b], ops.PagedBatch(table, i32([b]), b - a), plan, q[a:b])
+        assert torch.equal(part, turned[a:b])
+    for a in range(0, T, 1 << 16):
+        part = ops.rotary(q[a:a + (1 << 16)].float(), torch.arange(a, min(T, a + (1 << 16)), device="cuda"), plan).double()
+        tol = (UNIT[torch.float16] + 2.0 ** -23) * part.abs() + 2.0 ** -25
+        assert ((turned[a:a + (1 << 16)].double() - part).abs() <= tol).all()
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(one, name).view(torch.uint8), getattr(two, name).view(torch.uint8))

@@ -1141,8 +1141,8 @@ Launch launch_of(const paged::Sizes& z) {
   l.past = !l.many && z.B * room * z.kv_heads * z.head_dim * 2 > int64_t(320) << 20;
   // (More than 1024 sequences fill the GPU by themselves, and each work-group would go through all their lengths: 1100 of
   // up to 300 keys in wide tables, one K/V head, 53.1 / 21.7; 4000 of up to 4000 keys 468 / 411.)
-  // (2^23 work-groups of 256 are what one launch takes.)
-  const bool each = jobs < (int64_t(1) << 23) && (z.B > 1024 || (l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048)));
+  const bool better = l.many ? room <= 2048 || (jobs >= 512 && jobs * 32 >= room) : room <= (jobs >= 128 ? 4096 : 2048);
+  const bool each = jobs < (int64_t(1) << 23) && (z.B > 1024 || better);  // (a launch has fewer than 2^31 threads)
   constexpr int64_t CUS = 256;  // (not asked for: the workspace's size follows, which is known without a device)
   l.groups = each ? 0 : CUS * (dw > 2 ? 1 : 2);
   l.least = 8;
