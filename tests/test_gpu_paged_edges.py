@@ -45,12 +45,12 @@ def poison(q):
 
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("B", [3, 70])
-@pytest.mark.parametrize("most", [3, 40])
-def test_more_tokens_than_most(most, B, wide):
+@pytest.mark.parametrize("most,D", [(3, 64), (40, 64), (40, 192), (40, 256), (3, 256)])
+def test_more_tokens_than_most(most, D, B, wide):
     """Those behind the first `most` of a sequence are left out, as if neither the offsets nor the lengths counted them;
     their rows, and those before the first sequence's, are zeros in new outputs and left in given ones."""
     ops = _ops()
-    D, page = 64, 16
+    page = 16
     rng = torch.Generator().manual_seed(70)
     new = [most + 300, 2, most, 0, most + 1][:B] + [int(n) for n in torch.randint(0, most + 3, (max(0, B - 5),), generator=rng)]
     offsets = [4]
@@ -92,11 +92,11 @@ def test_more_tokens_than_most(most, B, wide):
 
 
 @pytest.mark.parametrize("wide", [False, True])
-@pytest.mark.parametrize("most", [3, 40])
-def test_more_tokens_than_most_in_replays(most, wide):
+@pytest.mark.parametrize("most,D", [(3, 64), (40, 64), (40, 256)])
+def test_more_tokens_than_most_in_replays(most, D, wide):
     """A captured step whose offsets and lengths outgrow `most` later, and come back."""
     ops = _ops()
-    D, page, T = 64, 16, 2 * most + 20
+    page, T = 16, 2 * most + 20
     table, pages = tables([150, 150], page, 76, wide)
     plan = ops.rotary_plan(D)
     q, kv = rand((T, 4, D), torch.float16, 77).cuda(), rand((T, 2, D), torch.float16, 78).cuda()

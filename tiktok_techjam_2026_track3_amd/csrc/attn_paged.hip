@@ -898,20 +898,52 @@ struct Many {
   }
 };
 
+// Zeros for rows that no sequence has, shared out by work-group. i0, step: which elements are the thread's.
+template <typename T>
+MI355_DEVINL void zero_row(const PagedArgs& p, int64_t t, int i0, int step) {
+  for (int i = i0; i < p.heads * p.cache.head_dim; i += step)
+    static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
+}
+template <typename T>
+MI355_DEVINL void zero_behind(const PagedArgs& p) {
+  for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x) zero_row<T>(p, t, threadIdx.x, 256);
+}
+template <typename T>
+MI355_DEVINL void zero_between(const PagedArgs& p, int64_t from, int64_t to, int64_t worker, int64_t workers) {
+  paged::zero_rows(p.batch, from, to, worker, workers,
+                   [&](int64_t t) MI355_LAMBDA_INLINE { zero_row<T>(p, t, threadIdx.x & 63, 64); });
+}
+// ... what is before the lanes' sequences, if b0 is 0, or cut off them: sequence b0 + l is lane l's
+template <typename T>
+MI355_DEVINL void zero_of_lanes(const PagedArgs& p, const paged::Sequence& s, int b0) {
+  if (b0 == 0) zero_between<T>(p, 0, __builtin_amdgcn_readfirstlane(s.first), blockIdx.x, gridDim.x);
+  for (uint64_t left = __ballot(s.cut > 0); left; left &= left - 1) {
+    const int l = __builtin_ctzll(left);
+    const int64_t from = static_cast<int64_t>(__shfl(s.first, l)) + __shfl(s.n, l);
+    zero_between<T>(p, from, from + __shfl(s.cut, l), blockIdx.x, gridDim.x);
+  }
+}
+
+// A launch of its own for them where the kernel's registers are all taken: two groups of many rows at head dims above 192
+// spill more with it inside (two of 1024 tokens against up to 8192 keys of 256 dims, bf16 873 us, so 833).
+constexpr bool zeros_inside(int dw, bool many) { return !(many && dw > 3); }
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_paged_zero(PagedArgs p) {
+  const int lane = threadIdx.x & 63;
+  zero_behind<T>(p);
+  for (int b0 = 0; b0 < p.batch.B; b0 += 64)
+    zero_of_lanes<T>(p, b0 + lane < p.batch.B ? paged::sequence_of(p.batch, b0 + lane) : paged::Sequence{0, 0, 0, 0}, b0);
+}
+
 template <typename T, int DW, int NR, bool MANY, int AUX>
 __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel(PagedArgs p) {
   using K = std::conditional_t<MANY, Many<T, DW, NR>, Few<T, DW, NR, AUX>>;
   __shared__ typename K::Lds lds;
   const int lane = threadIdx.x & 63, kvh = p.cache.kv_heads, G = p.G;
 
-  // rows that no sequence has, shared out by work-group: those behind all here, others where their sequence is met
-  const auto zero = [&](int64_t t, int i0, int step) MI355_LAMBDA_INLINE {
-    for (int i = i0; i < p.heads * p.cache.head_dim; i += step)
-      static_cast<T*>(p.o)[t * p.ot + (i / p.cache.head_dim) * p.oh + i % p.cache.head_dim] = T(0.0f);
-  };
-  const auto of_wave = [&](int64_t t) MI355_LAMBDA_INLINE { zero(t, lane, 64); };
-  if (p.zero_tail)
-    for (int64_t t = paged::tail_of(p.batch) + blockIdx.x; t < p.batch.tokens; t += gridDim.x) zero(t, threadIdx.x, 256);
+  const bool zeros = zeros_inside(DW, MANY) && p.zero_tail;
+  if (zeros) zero_behind<T>(p);  // (others where their sequence is met)
 
   // the work-group's run of units: [x, x + left) of all, or one job whole
   int b = 0, h, tile, u0, w = blockIdx.x;
@@ -925,10 +957,11 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
     h = w % heads % kvh;
     b = w % heads / kvh;
     const paged::Sequence s = paged::sequence_of(p.batch, b);
-    if (p.zero_tail) {
+    if (zeros) {
       const int worker = tile * kvh + h, workers = p.row_tiles * kvh;
-      if (b == 0 && s.first > 0) paged::zero_rows(p.batch, 0, s.first, worker, workers, of_wave);
-      if (s.cut > 0) paged::zero_rows(p.batch, s.first + s.n, static_cast<int64_t>(s.first) + s.n + s.cut, worker, workers, of_wave);
+      if (b == 0) zero_between<T>(p, 0, s.first, worker, workers);
+      const int64_t from = static_cast<int64_t>(s.first) + s.n;
+      zero_between<T>(p, from, from + s.cut, worker, workers);
     }
     rows = rows_of(p, s);
     if (tile * K::ROWS >= rows.nrows) return;
@@ -951,22 +984,13 @@ __global__ __launch_bounds__(256, (per_cu(DW, NR, MANY))) void attn_paged_kernel
       }
       return s;
     };
-    const auto zero_between = [&](const paged::Sequence& s) MI355_LAMBDA_INLINE {  // what is cut off a lane's sequence
-      if (!p.zero_tail) return;
-      for (uint64_t left = __ballot(s.cut > 0); left; left &= left - 1) {
-        const int l = __builtin_ctzll(left);
-        const int64_t from = static_cast<int64_t>(__shfl(s.first, l)) + __shfl(s.n, l);
-        paged::zero_rows(p.batch, from, from + __shfl(s.cut, l), blockIdx.x, gridDim.x, of_wave);
-      }
-    };
     near = scan(0);
-    zero_between(near);
-    if (const int first = __builtin_amdgcn_readfirstlane(near.first); p.zero_tail && first > 0)
-      paged::zero_rows(p.batch, 0, first, blockIdx.x, gridDim.x, of_wave);
+    if (zeros) zero_of_lanes<T>(p, near, 0);
     const int64_t mine0 = mine, upto0 = upto;
     int64_t total = first_lane(__shfl(upto, 63));
     for (int b0 = 64; b0 < p.batch.B; b0 += 64) {
-      zero_between(scan(b0));
+      const paged::Sequence s = scan(b0);
+      if (zeros) zero_of_lanes<T>(p, s, b0);
       total += first_lane(__shfl(upto, 63));
     }
     total *= kvh;
@@ -1154,6 +1178,8 @@ Launch launch_of(const paged::Sizes& z) {
 template <typename T, int DW, int NR, bool MANY>
 int launch(const PagedArgs& p, const Launch& l, hipStream_t s) {
   const auto grid = static_cast<uint32_t>(l.grid);
+  if constexpr (!zeros_inside(DW, MANY))
+    if (p.zero_tail) attn_paged_zero<T><<<256, 256, 0, s>>>(p);
   if constexpr (!MANY)
     if (l.past) attn_paged_kernel<T, DW, NR, false, PAST><<<grid, 256, 0, s>>>(p);
   if (!l.past) attn_paged_kernel<T, DW, NR, MANY, 0><<<grid, 256, 0, s>>>(p);
