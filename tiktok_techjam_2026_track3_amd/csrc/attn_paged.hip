@@ -411,8 +411,7 @@ struct Window {
       const bool ok = id >= 0 && id < p.cache.pages;
       row = ((static_cast<int64_t>(ok ? id : 0) * p.cache.kv_heads + h) << shift) + (at & ((1 << shift) - 1));
       kf = ok ? p.cache.ks[row / BLOCK] * (p.scale * LOG2E) : __builtin_nanf("");
-      // (the conversions take the exponent alone; Many divides by it)
-      vf = ok ? __uint_as_float(__float_as_uint(p.cache.vs[row / BLOCK]) & 0x7f800000u) : 0.0f;
+      vf = ok ? p.cache.vs[row / BLOCK] : 0.0f;
     }
     row *= p.cache.head_dim;
     lo = static_cast<uint32_t>(row);
@@ -707,8 +706,12 @@ struct Many {
           });
         }
       });
-      st.vs[0] = w.v_factor(at);
-      st.vs[1] = w.v_factor(at + BLOCK);
+      const auto scale = [&](int k) MI355_LAMBDA_INLINE {  // as the conversions take it: the exponent alone
+        const float v = w.v_factor(k);
+        return RELATIVE ? __uint_as_float(__float_as_uint(v) & 0x7f800000u) : v;
+      };
+      st.vs[0] = scale(at);
+      st.vs[1] = scale(at + BLOCK);
     };
     constexpr float LEAST = 0x1p-118f;  // least scale of a block
     float v_top = LEAST, v_of[2][2] = {}, v_acc = LEAST;  // RELATIVE: largest V scale so far, of the buffers' blocks, of the outputs
