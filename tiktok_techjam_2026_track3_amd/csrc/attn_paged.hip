@@ -635,7 +635,7 @@ MI355_DEVINL void for_each(F f) {  // f(0) .. f(N - 1), as constants
 // each, into LDS, as the operands that the lanes read: 16 bytes each, one after the other, so without conflicts. Two
 // buffers: while unit i is worked on, unit i + 1 is converted and unit i + 3 requested; one barrier a unit. Each wave on its
 // own (as in Few) converted all of K and V four times: two pieces of 1024 tokens against 12000 keys (32/8 heads of 128)
-// 1039 us, so 353, 14 of them the join: 860 TFLOP/s, matrix cores busy 36% of the time and the vector ALU 48%,
+// 1039 us, so 350, 14 of them the join: 870 TFLOP/s, matrix cores busy 36% of the time and the vector ALU 48%,
 // hardly at once with the two waves that a SIMD's registers hold. The scores of unit i + 1 beside the softmax of unit i (more registers, one wave a SIMD) were slower.
 // fp16: V's scales are taken relative to the largest up to their own block, so that V fits the type; blocks down to
 // 2^-21 of that are exact. (Up to their own: a later block's scale is not to touch rows that do not see it.)
@@ -928,7 +928,7 @@ MI355_DEVINL void zero_of_lanes(const PagedArgs& p, const paged::Sequence& s, in
 }
 
 // A launch of its own for them where the kernel's registers are all taken: two groups of many rows at head dims above 192
-// spill more with it inside (two of 1024 tokens against up to 8192 keys of 256 dims, bf16 873 us, so 833).
+// spill more with it inside (two of 1024 tokens against up to 8192 keys of 256 dims, bf16 874 us, so 832).
 constexpr bool zeros_inside(int dw, bool many) { return !(many && dw > 3); }
 
 template <typename T>
@@ -1146,8 +1146,8 @@ Launch launch_of(const paged::Sizes& z) {
   l.many = rows > 32;
   // Groups of 16 rows of a wave. Few rows: as many as there are, where registers allow two. Many: two, which share each operand
   // that is read; above head dim 128 such a wave has the SIMD for itself, and short tiles leave waves idle: only for
-  // enough rows (us of 16 sequences of 4096 keys, 32 heads of 192 / of 256, one group then two: 64 rows 96 111 / 113 184, 128
-  // rows 156 124 / 193 196, 256 rows 300 228 / 374 352; two of 1024 tokens against 8192 keys 1087 723 / 1243 1044).
+  // enough rows (us of 16 sequences of 4096 keys, 32 heads of 192 / of 256, one group then two: 64 rows 94 112 / 112 177, 128
+  // rows 154 125 / 191 185, 256 rows 299 231 / 368 336; two of 1024 tokens against 8192 keys 1085 734 / 1229 999).
   l.nr = l.many ? (dw <= 2 || rows > 64 * (dw - 2) ? 2 : 1) : (rows > 16 && dw <= 2 ? 2 : 1);
   l.rows = 16 * l.nr * (l.many ? 4 : 1);
   l.row_tiles = (rows + l.rows - 1) / l.rows;
